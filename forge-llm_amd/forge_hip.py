@@ -196,6 +196,22 @@ class DecodeModel(ctypes.Structure):
                                                   "q", "h", "attn_part")])
 
 
+class Kv4Cache(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int) for n in ("nLayers", "nSeq", "nKvHeads", "dHead", "maxSeq")]
+                + [(n, ctypes.c_void_p) for n in ("k", "v", "kd", "vd", "len", "next", "weight", "pos")])
+
+
+class BeamState(ctypes.Structure):
+    _fields_ = [("base", ctypes.c_void_p), ("beam_stride", ctypes.c_int64), ("outer", ctypes.c_int),
+                ("outer_stride", ctypes.c_int64), ("inner", ctypes.c_int), ("inner_stride", ctypes.c_int64),
+                ("row_bytes", ctypes.c_int64), ("rows", ctypes.c_int)]
+
+
+def ref(struct):
+    """A host structure or array of them, as call() takes its address."""
+    return ctypes.byref(struct)
+
+
 class Event:
     def __init__(self):
         p = ctypes.c_void_p()

@@ -634,6 +634,122 @@ int fg_dequantize(int type, float* out, const void* q, int64_t n);
  * bit-identical to the reference (device pointers). */
 int fg_quantize(int type, void* out, const float* x, int64_t n);
 
+/* ──────────── 4-bit key-value cache of several sequences ────────────
+ * KVCache (attention.js:128-156) with its rows in Q4_0 blocks and room for
+ * nSeq sequences; no counterpart in the reference.  dHead is 32, 64, 96, 128
+ * or 256, nb = dHead / 32.  A block of 32 values is a fp16 step d and 32 codes
+ * c of 0..15 that stand for d (c - 8): with m the block's value of largest
+ * magnitude (the first of equals), d = fp16(m / -8) and
+ * c = floor(x / d + 8.5), held to 0..15 (8 where d = 0).  A block with a value
+ * that is not finite, or whose step exceeds fp16, stands for NaN.
+ *
+ * Arrays (device, 16-byte aligned), a slot being one cached token:
+ *   k, v    codes [nLayers][nSeq][nKvHeads][maxSeq][dHead / 2]: byte n nb + b of
+ *           a slot (n < 16, b < nb) has value 32 b + n in its low and value
+ *           32 b + 16 + n in its high four bits
+ *   kd, vd  steps, fp16 [nLayers][nSeq][nKvHeads][maxSeq][nb]
+ *   len     [nSeq] slots in use: the first len[s] of every layer and head.  A
+ *           length outside [0, maxSeq] counts as the nearer of the two
+ *   next    [nSeq] position of the sequence's next token
+ *   weight  [nLayers][nSeq][nKvHeads][maxSeq] attention that each cached token
+ *           has had, or NULL: not kept
+ *   pos     [nLayers][nSeq][nKvHeads][maxSeq] position of each cached token, or
+ *           NULL: not kept.  fg_kv4_evict needs both
+ * A step appends T tokens to the layers, attends, and commits once: until
+ * then len and next stand, so every layer sees the same ones.  `count` (device,
+ * [nSeq], or NULL) gives each sequence its own number of new tokens, held to
+ * 0..T.  The structure itself is host memory, read during the call. */
+typedef struct fg_kv4_cache {
+  int nLayers, nSeq, nKvHeads, dHead, maxSeq;
+  uint8_t* k;
+  uint8_t* v;
+  uint16_t* kd;
+  uint16_t* vd;
+  int32_t* len;
+  int32_t* next;
+  float* weight;
+  int32_t* pos;
+} fg_kv4_cache;
+/* KVCache.put (attention.js:137-141) of T tokens for every sequence: row
+ * s T + t of k and v (fp32, nKvHeads dHead values, row stride ld) becomes slot
+ * len[s] + t of `layer`, its weight 0 and its position next[s] + t.  Slots
+ * from maxSeq on are not written. */
+int fg_kv4_append(const fg_kv4_cache* c, int layer, const float* k, const float* v, int64_t ld, int T,
+                  const int32_t* count);
+/* sliceK / sliceV (attention.js:148-155) of T slots from `first` on: the values
+ * of slot first + t of sequence s into row s T + t of k and v, whether in use or
+ * not (0 <= first, first + T <= maxSeq). */
+int fg_kv4_read(const fg_kv4_cache* c, int layer, float* k, float* v, int64_t ld, int first, int T);
+/* Attention (attentionDecode, attention.js:31-61) of one query token a sequence
+ * over the n = len[s] + T (or + count[s]) slots of `layer`:
+ *   out[s][h] = sum_j p_j V_j,  p = softmax_j(scale q[s][h] . K_j),
+ * q and out [nSeq][nHeads][dHead], query head h on kv head h / (nHeads / nKvHeads);
+ * n = 0 gives zeros.  Where c->weight is kept, every slot j < n adds the sum of
+ * its p_j over its kv head's query heads.  Codes are exact in the products, q
+ * is held in two fp16 pieces (22 bits), sums are fp32. */
+int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
+                const int32_t* count);
+/* Ends a step: len[s] += T (or count[s]; to maxSeq at most), next[s] += the same. */
+int fg_kv4_commit(const fg_kv4_cache* c, int T, const int32_t* count);
+/* Which cached tokens a bounded cache keeps, by accumulated attention: a head
+ * [layer][seq][head] of n = len[seq] > budget slots keeps those whose position is
+ * at least next[seq] - recent, and of the others those of greatest weight (NaN
+ * below all; of equals the lowest slot), budget in all.  The kept slots from
+ * budget on (movers) belong, in order, into the dropped slots below budget
+ * (holes): moves[head] of them, listed in holes and movers
+ * [nLayers][nSeq][nHeads][max(1, min(budget, maxSeq - budget))], the rest of each
+ * list -1.  0 <= recent <= budget, 1 <= budget < maxSeq; positions of one head
+ * are distinct and below next. */
+int fg_kv_evict_select(int32_t* holes, int32_t* movers, int32_t* moves, const float* weight, const int32_t* pos,
+                       const int32_t* len, const int32_t* next, int nLayers, int nSeq, int nHeads, int maxSeq,
+                       int budget, int recent);
+/* fg_kv_evict_select over the whole cache, its moves made (codes, steps,
+ * weights and positions; the slots from budget on keep what they held) and
+ * len[s] = min(len[s], budget).  budget >= maxSeq: nothing to do. */
+int fg_kv4_evict(const fg_kv4_cache* c, int budget, int recent);
+
+/* ──────────── beam search ────────────
+ * No counterpart in the reference (its sampling.js draws one token of one
+ * sequence).  A request has W beams, rows r W .. r W + W - 1 of its arrays. */
+/* The next beams of nReq requests: of the candidates
+ *   scores[b] + logits[b][v] - log sum_u exp(logits[b][u])
+ * of its beams the W greatest, greatest first; of equals the lowest beam, then
+ * the lowest token.  A beam with done[b] != 0 has one candidate, (eos, scores[b]).
+ * score_out, token and parent (0 <= parent < W) [nReq W]; done_out = done of the
+ * parent, or token == eos.  done and done_out may be NULL (together: none done);
+ * eos < 0: none, done NULL.  Logits of -inf are masked tokens: they come after all
+ * others.  A beam of masked tokens alone has V candidates of -inf, one whose score
+ * less the log of its sum is otherwise not finite V candidates of that value; NaN
+ * comes after all others.  Candidates compare in
+ * fp64 across beams, by their logits within one.  logits rows have stride ld;
+ * 1 <= W <= 64, outputs apart from the inputs. */
+int fg_beam_select(float* score_out, int32_t* token, int32_t* parent, int32_t* done_out, const float* logits,
+                   int64_t ld, const float* scores, const int32_t* done, int eos, int nReq, int W, int V);
+/* A state of every beam: `rows` rows of row_bytes (even) for each of outer x inner
+ * parts: row i of part (a, b) of beam s at base + s beam_stride + a outer_stride +
+ * b inner_stride + i row_bytes.  base and strides are even; states and beams do
+ * not overlap. */
+typedef struct fg_beam_state {
+  void* base;
+  int64_t beam_stride;
+  int outer;
+  int64_t outer_stride;
+  int inner;
+  int64_t inner_stride;
+  int64_t row_bytes;
+  int rows;
+} fg_beam_state;
+/* Beam b of request r takes what beam parent[r W + b] of the request has, in
+ * place: the first len[r W + parent] rows of every part (len NULL or beyond: all;
+ * below 0: none), the rest left as it was.  parent outside [0, W) means b itself.
+ * Up to 8 states a call, 1 <= W <= 64. */
+#define FG_BEAM_STATES 8
+int fg_beam_reorder(const fg_beam_state* states, int count, const int32_t* parent, const int32_t* len, int nReq,
+                    int W);
+/* fg_beam_reorder of a whole cache, nSeq = requests x W: codes, steps, weights and
+ * positions of the slots in use, len and next. */
+int fg_kv4_reorder(const fg_kv4_cache* c, const int32_t* parent, int W);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,494 @@
+"""The 4-bit key-value cache on the device (fg_kv4_*, fg_kv_evict_select)
+against the plain 64-bit forms of oracle/kv4_ref.py: codes, steps, moves and
+untouched slots exactly, attention within bounds counted from the roundings."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import kv4_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [32, 64, 96, 128, 256]
+
+
+class Cache:
+    """A cache on the device with every slot filled with what must not be seen:
+    codes 0xFF, NaN steps and weights, position -7."""
+
+    def __init__(self, fh, nLayers, nSeq, nKV, dH, maxSeq, track=True, lens=None):
+        self.fh, self.dims = fh, (nLayers, nSeq, nKV, maxSeq)
+        self.nSeq, self.nKV, self.dH, self.maxSeq, self.nb = nSeq, nKV, dH, maxSeq, dH // 32
+        up = fh.DeviceArray.from_numpy
+        self.k, self.v = (up(np.full(self.dims + (dH // 2,), 0xFF, np.uint8)) for _ in range(2))
+        self.kd, self.vd = (up(np.full(self.dims + (self.nb,), np.nan, np.float16)) for _ in range(2))
+        self.len = up(np.array(lens if lens is not None else [0] * nSeq, np.int32))
+        self.next = up(np.arange(100, 100 + nSeq, dtype=np.int32))
+        self.weight = up(np.full(self.dims, np.nan, np.float32)) if track else None
+        self.pos = up(np.full(self.dims, -7, np.int32)) if track else None
+        self.arrays = [a for a in (self.k, self.v, self.kd, self.vd, self.len, self.next, self.weight, self.pos)]
+        self.struct = fh.Kv4Cache(nLayers, nSeq, nKV, dH, maxSeq, *[a.ptr if a else None for a in self.arrays])
+
+    def call(self, name, *args):
+        self.fh.call("kv4_" + name, self.fh.ref(self.struct), *args)
+
+    def host(self):
+        return [a.numpy() if a else None for a in self.arrays]
+
+    def fill(self, rng, lens):
+        """Random codes and steps, as if `lens` tokens had been stored."""
+        code = rng.integers(0, 256, self.dims + (self.dH // 2,), dtype=np.uint8), rng.integers(0, 256, self.dims + (self.dH // 2,), dtype=np.uint8)
+        step = [(rng.standard_normal(self.dims + (self.nb,)) * 0.2).astype(np.float16) for _ in range(2)]
+        for s, n in enumerate(lens):
+            for a in step:
+                a[:, s, :, n:] = np.nan
+        for d, a in zip((self.k, self.v, self.kd, self.vd), (*code, *step)):
+            d.upload(a)
+        if self.weight:
+            self.weight.upload(np.exp(rng.standard_normal(self.dims)).astype(np.float32))
+
+
+def rows(rng, *shape):
+    x = rng.standard_normal(shape).astype(np.float32)
+    return x * np.exp(rng.uniform(-3, 3, shape[-1])).astype(np.float32)
+
+
+def attend_bound(q, K, V, p, scale):
+    """Bounds of |out| and |weight| errors, term by term: q in two fp16 pieces is off by 2^-22 of
+    itself, a score's dH products and its nb block sums round at 2^-24 each (and scale, log2 e and the
+    subtraction of the maximum, 4 more of the largest score), exp2 is good to 2^-22; p's and the sums over
+    n positions round at most n / 4 + 64 times in a chain (a sum over a tile's positions stays in the
+    matrix unit's order); p d is held in two fp16 pieces, 2^-22."""
+    n, nKV, dH = K.shape
+    nH = q.shape[0]
+    out, weight = np.zeros((nH, dH)), np.zeros((nH, n))
+    for h in range(nH if n else 0):
+        z = h // (nH // nKV)
+        mass = abs(scale) * (np.abs(K[:, z]) @ np.abs(q[h].astype(np.float64)))
+        es = mass.max() * (2.0 ** -22 + (dH + 16) * 2.0 ** -24)
+        rel = 2 * es + 2.0 ** -21 + (n / 4 + 64) * 2.0 ** -24
+        out[h] = rel * (p[h] @ np.abs(V[:, z])) + 1e-30
+        weight[h] = rel * p[h] + 1e-30
+    return out, weight
+
+
+# ── store and read ────────────────────────────────────────────────────────
+@pytest.mark.parametrize("dH", HEADS)
+@pytest.mark.parametrize("nSeq,nKV,T,maxSeq,pad", [(1, 1, 1, 1, 0), (3, 2, 5, 17, 3), (2, 3, 40, 64, 0), (5, 5, 1, 9, 7)])
+def test_append_and_read(fh, dH, nSeq, nKV, T, maxSeq, pad):
+    rng = np.random.default_rng(dH + nSeq)
+    lens = rng.integers(0, maxSeq, nSeq)
+    c = Cache(fh, 2, nSeq, nKV, dH, maxSeq, lens=lens)
+    before = c.host()
+    ld = nKV * dH + pad
+    k, v = rows(rng, nSeq * T, ld), rows(rng, nSeq * T, ld)
+    count = rng.integers(-1, T + 2, nSeq).astype(np.int32)
+    up = fh.DeviceArray.from_numpy
+    dk, dv, dc = up(k), up(v), up(count)
+    c.call("append", 1, dk, dv, ld, T, dc)
+    got = c.host()
+    want = [a.copy() for a in before]
+    for s in range(nSeq):
+        for t in range(min(max(count[s], 0), T)):
+            at = lens[s] + t
+            if at >= maxSeq:
+                continue
+            for x, codes, steps in ((k, 0, 2), (v, 1, 3)):
+                q, d = ref.quantize(x[s * T + t, :nKV * dH].reshape(nKV, dH))
+                want[codes][1, s, :, at], want[steps][1, s, :, at] = ref.pack(q), d
+            want[6][1, s, :, at], want[7][1, s, :, at] = 0.0, 100 + s + t
+    for a, b in zip(got, want):
+        np.testing.assert_array_equal(a, b)
+    first, n = maxSeq // 3, maxSeq - maxSeq // 3
+    ok, ov = (fh.DeviceArray.from_numpy(np.full((nSeq * n, ld), 9.0, np.float32)) for _ in range(2))
+    c.call("read", 1, ok, ov, ld, first, n)
+    for o, codes, steps in ((ok, 0, 2), (ov, 1, 3)):
+        g = o.numpy()
+        x = ref.values(want[codes][1], want[steps][1])[:, :, first:].transpose(0, 2, 1, 3).reshape(nSeq * n, nKV * dH)
+        np.testing.assert_array_equal(g[:, :nKV * dH], x.astype(np.float32))
+        assert (g[:, nKV * dH:] == 9.0).all()
+
+
+@pytest.mark.parametrize("dH", HEADS)
+def test_append_edges(fh, dH):
+    """Zeros, equal magnitudes of both signs, borders between codes, tiny and huge blocks, what is not finite."""
+    rng = np.random.default_rng(dH)
+    T = 600
+    x = rows(rng, T, dH)
+    x[0] = 0.0
+    x[1, 3], x[1, 7], x[2, 3], x[2, 7] = 50.0, -50.0, -50.0, 50.0
+    x[3, 20], x[3, 4] = 50.0, -50.0
+    x[4, 5], x[5, 5], x[6, 5], x[7, 5] = np.nan, np.inf, -np.inf, 8 * 65519.0
+    x[8, 5], x[9, 5], x[10] = 8 * 65520.0, -3e38, x[10] * 1e-8
+    x[11], x[12], x[13] = x[11] * 1e-30, x[12] * 1e-42, -0.0
+    for r in range(14, 300):  # values on and next to the borders (c + 1/2) d
+        d = np.float16(rng.standard_normal() * np.exp(rng.uniform(-10, 6)))
+        x[r] = np.float32(d) * (rng.integers(-8, 8, dH) - np.float32(0.5))
+        x[r, ::32] = np.float32(d) * -8
+        near = rng.random(dH) < 0.4
+        x[r] = np.where(near, np.nextafter(x[r], np.float32(np.inf) * rng.choice([-1, 1], dH).astype(np.float32)), x[r])
+    c = Cache(fh, 1, 1, 1, dH, T)
+    up = fh.DeviceArray.from_numpy
+    dx = up(x)
+    c.call("append", 0, dx, dx, dH, T, None)
+    q, d = ref.quantize(x)
+    got = c.host()
+    for codes, steps in ((0, 2), (1, 3)):
+        np.testing.assert_array_equal(got[steps][0, 0, 0], d)
+        good = np.repeat(np.isfinite(d), 16, -1).reshape(T, -1, 16).transpose(0, 2, 1).reshape(T, -1)
+        np.testing.assert_array_equal(got[codes][0, 0, 0][good], ref.pack(q)[good])
+    out = fh.DeviceArray((T, dH))
+    out2 = fh.DeviceArray((T, dH))
+    c.call("read", 0, out, out2, dH, 0, T)
+    np.testing.assert_array_equal(out.numpy(), ref.values(ref.pack(q), d).astype(np.float32))
+    np.testing.assert_array_equal(out2.numpy(), out.numpy())
+
+
+# ── attention ─────────────────────────────────────────────────────────────
+def check_attend(fh, c, nH, rng, lens, T=0, count=None, scale=None, q=None, layer=0):
+    scale = 1 / np.sqrt(c.dH) if scale is None else scale
+    q = rng.standard_normal((c.nSeq, nH, c.dH)).astype(np.float32) if q is None else q
+    before = c.host()
+    up = fh.DeviceArray.from_numpy
+    dq, out = up(q), up(np.full(q.shape, 7.0, np.float32))
+    dc = up(np.array(count, np.int32)) if count is not None else None
+    c.call("attn", layer, out, dq, nH, scale, T, dc)
+    after = c.host()
+    for i, (a, b) in enumerate(zip(before, after)):
+        if i != 6 and a is not None:
+            np.testing.assert_array_equal(a, b)
+    got = out.numpy()
+    for s in range(c.nSeq):
+        n = min(max(lens[s], 0), c.maxSeq)
+        n = min(n + (T if count is None else min(max(count[s], 0), T)), c.maxSeq)
+        K = ref.values(before[0][layer, s, :, :n], before[2][layer, s, :, :n]).transpose(1, 0, 2)
+        V = ref.values(before[1][layer, s, :, :n], before[3][layer, s, :, :n]).transpose(1, 0, 2)
+        want, p = ref.attend(q[s], K, V, scale)
+        eo, ew = attend_bound(q[s], K, V, p, scale)
+        assert np.isfinite(got[s]).all(), (s, n)
+        worst = (np.abs(got[s] - want) / eo).max() if n else np.abs(got[s]).max()
+        assert worst <= (1.0 if n else 0.0), (s, n, worst)
+        if before[6] is not None:
+            group = nH // c.nKV
+            add = p.reshape(c.nKV, group, n).sum(1)
+            tol = ew.reshape(c.nKV, group, n).sum(1)
+            w0, w1 = before[6][layer, s], after[6][layer, s]
+            np.testing.assert_array_equal(w1[:, n:], w0[:, n:])
+            # the sum of the group's heads and the addition round at 2^-24 each
+            off = np.abs(w1[:, :n] - (w0[:, :n].astype(np.float64) + add))
+            assert (off <= tol + (group + 1) * 2.0 ** -24 * (np.abs(w1[:, :n]) + add)).all()
+            for other in range(c.dims[0]):
+                if other != layer:
+                    np.testing.assert_array_equal(before[6][other], after[6][other])
+
+
+@pytest.mark.parametrize("dH", HEADS)
+@pytest.mark.parametrize("nKV,group", [(1, 1), (2, 4), (3, 3), (1, 8), (2, 12)])
+def test_attend(fh, dH, nKV, group):
+    rng = np.random.default_rng(dH * 31 + nKV)
+    lens = [0, 1, 31, 32, 33, 129, 200, 517]
+    c = Cache(fh, 2, len(lens), nKV, dH, 517, lens=lens)
+    c.fill(rng, lens)
+    check_attend(fh, c, nKV * group, rng, lens, layer=1)
+
+
+@pytest.mark.parametrize("dH,group", [(32, 2), (64, 1), (96, 5), (128, 4), (256, 8)])
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 127, 128, 257, 1024, 3333])
+def test_attend_one_sequence(fh, dH, group, n):
+    rng = np.random.default_rng(n)
+    c = Cache(fh, 1, 1, 1, dH, n + rng.integers(0, 40), track=n % 2 == 0, lens=[n])
+    c.fill(rng, [n])
+    check_attend(fh, c, group, rng, [n])
+
+
+@pytest.mark.parametrize("T,count", [(3, None), (3, [0, 1, 2, 3]), (3, [9, -4, 3, 0])])
+def test_attend_new_tokens_and_bad_lengths(fh, T, count):
+    """Lengths and counts outside their ranges count as the nearest inside; new tokens are attended to before the commit."""
+    rng = np.random.default_rng(T)
+    lens = [50, 0, 39, -3]
+    c = Cache(fh, 1, 4, 2, 64, 40, lens=lens)
+    c.fill(rng, [40] * 4)
+    check_attend(fh, c, 6, rng, lens, T=T, count=count)
+
+
+@pytest.mark.parametrize("dH", HEADS)
+def test_attend_peaks_and_scales(fh, dH):
+    """One slot that takes all, large and tiny steps, a scale of zero, negative scales, a zero query."""
+    rng = np.random.default_rng(dH + 5)
+    lens = [300, 40, 77]
+    c = Cache(fh, 1, 3, 2, dH, 300, lens=lens)
+    c.fill(rng, lens)
+    kd, vd = c.kd.numpy(), c.vd.numpy()
+    kd[0, 0, :, 211] = 12.0
+    vd[0, 1] = vd[0, 1] * np.float16(2e4)
+    vd[0, 2, :, 5:] = vd[0, 2, :, 5:] * np.float16(1e-4)
+    c.kd.upload(kd)
+    c.vd.upload(vd)
+    q = rng.standard_normal((3, 4, dH)).astype(np.float32)
+    q[2, 1] = 0.0
+    q[1, 2] *= 1e-20
+    for scale in (0.1, -0.05, 0.0):
+        check_attend(fh, c, 4, rng, lens, scale=scale, q=q)
+
+
+def test_attend_steps_of_very_different_sizes(fh):
+    """Values whose steps grow and shrink by large factors along the cache: the running scale of the value products follows."""
+    rng = np.random.default_rng(8)
+    n = 2048
+    c = Cache(fh, 1, 1, 1, 128, n, lens=[n])
+    c.fill(rng, [n])
+    for factors in (np.linspace(-14, 12, n), np.linspace(12, -14, n), rng.uniform(-14, 12, n)):
+        vd = (rng.uniform(1, 2, (1, 1, 1, n, 4)) * np.exp2(factors)[None, None, None, :, None]).astype(np.float16)
+        c.vd.upload(vd)
+        check_attend(fh, c, 4, rng, [n], scale=0.02)
+
+
+def test_attend_not_finite(fh):
+    """A NaN key or value of a slot in use shows in its kv head's outputs and nowhere else."""
+    rng = np.random.default_rng(9)
+    lens = [100, 100]
+    c = Cache(fh, 1, 2, 2, 64, 128, lens=lens, track=False)
+    c.fill(rng, lens)
+    kd, vd = c.kd.numpy(), c.vd.numpy()
+    kd[0, 0, 1, 50, 1] = np.nan
+    vd[0, 1, 0, 99, 0] = np.nan
+    c.kd.upload(kd)
+    c.vd.upload(vd)
+    q = fh.DeviceArray.from_numpy(rng.standard_normal((2, 4, 64)).astype(np.float32))
+    out = fh.DeviceArray.from_numpy(np.zeros((2, 4, 64), np.float32))
+    c.call("attn", 0, out, q, 4, 0.125, 0, None)
+    bad = np.isnan(out.numpy())
+    assert bad[0, 2:].all() and not bad[0, :2].any()
+    assert bad[1, :2, :32].all() and not bad[1, :, 32:].any() and not bad[1, 2:].any()
+
+
+def test_attend_far_into_a_large_cache(fh):
+    """Codes past 2^32 bytes from the arrays' start."""
+    nLayers, maxSeq, dH, nKV = 9, 1 << 19, 256, 8
+    up = fh.DeviceArray
+    shape = (nLayers, 1, nKV, maxSeq)
+    assert np.prod(shape) * 128 > 2 ** 32
+    k, v = up(shape + (128,), np.uint8), up(shape + (128,), np.uint8)
+    kd, vd = up(shape + (8,), np.float16), up(shape + (8,), np.float16)
+    n = maxSeq - 3
+    length, nxt = up.from_numpy(np.array([n], np.int32)), up.from_numpy(np.array([n], np.int32))
+    c = fh.Kv4Cache(nLayers, 1, nKV, dH, maxSeq, k.ptr, v.ptr, kd.ptr, vd.ptr, length.ptr, nxt.ptr, None, None)
+    rng = np.random.default_rng(1)
+    row = np.zeros((1, nKV * dH), np.float32)
+    zero, one = up.from_numpy(row), up.from_numpy(rng.standard_normal((1, nKV * dH)).astype(np.float32))
+    for layer in (0, nLayers - 1):
+        fh.call("kv4_append", fh.ref(c), layer, one, one, nKV * dH, 1, None)
+    ok, ov = up((1, nKV * dH)), up((1, nKV * dH))
+    fh.call("kv4_read", fh.ref(c), nLayers - 1, ok, ov, nKV * dH, n, 1)
+    q, d = ref.quantize(one.numpy().reshape(nKV, dH))
+    np.testing.assert_array_equal(ok.numpy().reshape(nKV, dH), ref.values(ref.pack(q), d).astype(np.float32))
+    # all slots in use of the last head but the last hold zeros: uniform weights
+    for a in (kd, vd):
+        fh.check(fh.lib.fg_zero(ctypes.c_void_p(a.ptr), a.nbytes), "fg_zero")
+    fh.call("kv4_append", fh.ref(c), nLayers - 1, zero, one, nKV * dH, 1, None)
+    out = up((nKV, dH))
+    fh.call("kv4_attn", fh.ref(c), nLayers - 1, out, one, nKV, 0.1, 1, None)
+    want = ref.values(ref.pack(q), d) / (n + 1)
+    np.testing.assert_allclose(out.numpy(), want, rtol=2.0 ** -13)  # the weights' sum: 2^19 ones in fp32
+
+
+# ── eviction ──────────────────────────────────────────────────────────────
+def run_select(fh, weight, pos, lens, nxt, budget, recent):
+    nL, nS, nH, maxSeq = weight.shape
+    most = max(1, min(budget, maxSeq - budget))
+    up = fh.DeviceArray.from_numpy
+    holes, movers = (up(np.full((nL, nS, nH, most), 77, np.int32)) for _ in range(2))
+    moves = up(np.full((nL, nS, nH), 77, np.int32))
+    a = [up(x) for x in (weight, pos, np.array(lens, np.int32), np.array(nxt, np.int32))]
+    fh.call("kv_evict_select", holes, movers, moves, *a, nL, nS, nH, maxSeq, budget, recent)
+    return holes.numpy(), movers.numpy(), moves.numpy()
+
+
+def check_select(fh, weight, pos, lens, nxt, budget, recent):
+    holes, movers, moves = run_select(fh, weight, pos, lens, nxt, budget, recent)
+    maxSeq = weight.shape[-1]
+    for l, s, h in np.ndindex(weight.shape[:3]):
+        n = min(max(lens[s], 0), maxSeq)
+        wh, wm = ref.evict(weight[l, s, h], pos[l, s, h], n, nxt[s], budget, recent)
+        m = moves[l, s, h]
+        assert m == len(wh) == len(wm)
+        np.testing.assert_array_equal(holes[l, s, h], wh + [-1] * (holes.shape[-1] - m))
+        np.testing.assert_array_equal(movers[l, s, h], wm + [-1] * (holes.shape[-1] - m))
+
+
+def positions(rng, *shape):
+    return rng.permuted(np.broadcast_to(np.arange(shape[-1], dtype=np.int32), shape), axis=-1)
+
+
+@pytest.mark.parametrize("maxSeq", [2, 5, 63, 64, 65, 1000, 1024, 1025, 4097, 9000])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_select(fh, maxSeq, ties):
+    rng = np.random.default_rng(maxSeq)
+    for budget in sorted({1, maxSeq // 4 + 1, maxSeq // 2 + 1, maxSeq - 1}):
+        if not 1 <= budget < maxSeq:
+            continue
+        w = np.exp(rng.standard_normal((2, 3, 2, maxSeq)) * 2).astype(np.float32)
+        if ties:
+            w = np.floor(w).astype(np.float32)
+        lens = [maxSeq, rng.integers(0, maxSeq + 1), min(budget + 1, maxSeq)]
+        for recent in {0, budget // 2, budget}:
+            check_select(fh, w, positions(rng, 2, 3, 2, maxSeq), lens, [maxSeq] * 3, budget, recent)
+
+
+def test_evict_select_odd_weights(fh):
+    """All equal, zeros of both signs, negative, NaN and infinite weights; every slot recent; lengths out of range."""
+    rng = np.random.default_rng(4)
+    n = 300
+    w = np.zeros((1, 5, 4, n), np.float32)
+    w[0, :, 1] = rng.choice(np.array([0.0, -0.0], np.float32), n)
+    w[0, :, 2] = rng.choice(np.array([-1, np.nan, np.inf, -np.inf, 2, 1e-40, -1e-40], np.float32), n)
+    w[0, :, 3] = np.nan
+    lens = [n, n + 50, -4, 0, 151]
+    for budget, recent in ((150, 0), (150, 20), (150, 150), (1, 1), (299, 3)):
+        check_select(fh, w, positions(rng, 1, 5, 4, n), lens, [n] * 5, budget, recent)
+
+
+@pytest.mark.parametrize("dH", HEADS)
+@pytest.mark.parametrize("maxSeq,budget,recent", [(33, 32, 4), (200, 50, 10), (200, 150, 0), (2100, 2048, 256)])
+def test_evict(fh, dH, maxSeq, budget, recent):
+    rng = np.random.default_rng(dH + maxSeq)
+    lens = [maxSeq, budget, maxSeq - 1, 0]
+    c = Cache(fh, 2, 4, 2, dH, maxSeq, lens=lens)
+    c.fill(rng, [maxSeq] * 4)
+    c.pos.upload(positions(rng, *c.dims))
+    c.next.upload(np.array([maxSeq] * 4, np.int32))
+    before = c.host()
+    c.call("evict", budget, recent)
+    want = [a.copy() for a in before]
+    for l, s, h in np.ndindex(c.dims[:3]):
+        holes, movers = ref.evict(before[6][l, s, h], before[7][l, s, h], lens[s], maxSeq, budget, recent)
+        for i in (0, 1, 2, 3, 6, 7):
+            want[i][l, s, h, holes] = before[i][l, s, h, movers]
+    want[4] = np.minimum(lens, budget)
+    for a, b in zip(c.host(), want):
+        np.testing.assert_array_equal(a, b)
+    c.call("evict", budget, recent)  # nothing is over the budget any more
+    c.call("evict", maxSeq + 5, 0)
+    for a, b in zip(c.host(), want):
+        np.testing.assert_array_equal(a, b)
+
+
+def test_commit(fh):
+    c = Cache(fh, 1, 5, 1, 32, 20, lens=[0, 19, 25, -2, 7])
+    c.call("commit", 3, None)
+    np.testing.assert_array_equal(c.len.numpy(), [3, 20, 20, 3, 10])
+    np.testing.assert_array_equal(c.next.numpy(), np.arange(100, 105) + 3)
+    c.call("commit", 3, fh.DeviceArray.from_numpy(np.array([0, 1, -2, 8, 2], np.int32)))
+    np.testing.assert_array_equal(c.len.numpy(), [3, 20, 20, 6, 12])
+    np.testing.assert_array_equal(c.next.numpy(), np.arange(100, 105) + 3 + np.array([0, 1, 0, 3, 2]))
+
+
+# ── together ──────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("W", [1, 3, 4])
+def test_reorder(fh, W):
+    rng = np.random.default_rng(W)
+    lens = rng.integers(0, 38, 2 * W)
+    c = Cache(fh, 3, 2 * W, 2, 96, 37, lens=lens)
+    c.fill(rng, [37] * 2 * W)
+    c.pos.upload(positions(rng, *c.dims))
+    parent = rng.integers(-1, W + 1, 2 * W).astype(np.int32)
+    before = c.host()
+    c.call("reorder", fh.DeviceArray.from_numpy(parent), W)
+    want = [a.copy() for a in before]
+    for b in range(2 * W):
+        p = b // W * W + parent[b] if 0 <= parent[b] < W else b
+        for i in (0, 1, 2, 3, 6, 7):
+            want[i][:, b, :, :lens[p]] = before[i][:, p, :, :lens[p]]
+        want[4][b], want[5][b] = before[4][p], before[5][p]
+    for a, b in zip(c.host(), want):
+        np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("dH,nKV,group", [(32, 2, 2), (128, 1, 4)])
+def test_a_generation_under_a_budget(fh, dH, nKV, group):
+    """Prompts of their own lengths, then steps of append, attend, commit, evict, with two beams changing places."""
+    rng = np.random.default_rng(dH)
+    budget, recent, nSeq = 24, 6, 2
+    c = Cache(fh, 2, nSeq, nKV, dH, 40)
+    nH = nKV * group
+    up = fh.DeviceArray.from_numpy
+    c.next.upload(np.zeros(nSeq, np.int32))
+    lens, seen = [0, 0], [0, 0]
+    for step in range(30):
+        T, count = (9, [9, 4]) if step == 0 else (1, None)
+        per = count or [T] * nSeq
+        for layer in range(2):
+            k, v = rows(rng, nSeq * T, nKV * dH), rows(rng, nSeq * T, nKV * dH)
+            dc = up(np.array(count, np.int32)) if count else None
+            c.call("append", layer, up(k), up(v), nKV * dH, T, dc)
+            check_attend(fh, c, nH, rng, lens, T=T, count=count, layer=layer)
+        c.call("commit", T, dc)
+        lens, seen = [n + a for n, a in zip(lens, per)], [n + a for n, a in zip(seen, per)]
+        np.testing.assert_array_equal(c.len.numpy(), lens)
+        before = c.host()
+        c.call("evict", budget, recent)
+        want = [a.copy() for a in before]
+        for l, s, h in np.ndindex(c.dims[:3]):
+            holes, movers = ref.evict(before[6][l, s, h], before[7][l, s, h], lens[s], seen[s], budget, recent)
+            for i in (0, 1, 2, 3, 6, 7):
+                want[i][l, s, h, holes] = before[i][l, s, h, movers]
+        lens = [min(n, budget) for n in lens]
+        want[4] = np.array(lens, np.int32)
+        for a, b in zip(c.host(), want):
+            np.testing.assert_array_equal(a, b)
+        if step % 7 == 3:
+            c.call("reorder", up(np.array([1, 1] if step == 3 else [1, 0], np.int32)), 2)
+            lens, seen = ([lens[1]] * 2, [seen[1]] * 2) if step == 3 else (lens[::-1], seen[::-1])
+    pos = c.pos.numpy()
+    for l, s, h in np.ndindex(c.dims[:3]):  # the newest are there, once each
+        kept = pos[l, s, h, :lens[s]]
+        assert len(set(kept)) == len(kept) and set(range(seen[s] - recent, seen[s])) <= set(kept)
+
+
+def test_a_recorded_step_replays(fh):
+    """A graph of a step under a budget, replayed with eager work between, gives what the same eager steps give."""
+    rng = np.random.default_rng(2)
+    budget, nSeq, nKV, dH, nH = 60, 3, 2, 64, 4
+    up = fh.DeviceArray.from_numpy
+    k, v = (up(np.zeros((nSeq, nKV * dH), np.float32)) for _ in range(2))
+    q = up(np.zeros((nSeq, nH, dH), np.float32))
+    results = []
+    for graph in (False, True):
+        r = np.random.default_rng(6)
+        c = Cache(fh, 1, nSeq, nKV, dH, 64, lens=[60, 30, 59])
+        c.fill(np.random.default_rng(5), [60] * 3)
+        c.pos.upload(positions(np.random.default_rng(7), *c.dims))
+        out = up(np.zeros((nSeq, nH, dH), np.float32))
+        parent = up(np.array([0, 0, 2], np.int32))
+
+        def step():
+            c.call("append", 0, k, v, nKV * dH, 1, None)
+            c.call("attn", 0, out, q, nH, 0.125, 1, None)
+            c.call("commit", 1, None)
+            c.call("evict", budget, 10)
+            c.call("reorder", parent, 3)
+
+        handle = ctypes.c_void_p()
+        if graph:
+            fh.check(fh.lib.fg_graph_begin(), "begin")
+            step()
+            fh.check(fh.lib.fg_graph_end(ctypes.byref(handle)), "end")
+        got = []
+        for i in range(5):
+            for d, shape in ((k, (nSeq, nKV * dH)), (v, (nSeq, nKV * dH)), (q, (nSeq, nH, dH))):
+                d.upload(r.standard_normal(shape).astype(np.float32))
+            if graph:
+                fh.check(fh.lib.fg_graph_launch(handle), "launch")
+                junk = [up(rng.standard_normal(50000).astype(np.float32)) for _ in range(3)]
+                fh.sync()
+                del junk
+            else:
+                step()
+            got.append([a.copy() for a in c.host()] + [out.numpy()])
+        if graph:
+            fh.check(fh.lib.fg_graph_destroy(handle), "destroy")
+        results.append(got)
+    for a, b in zip(*results):
+        for x, y in zip(a, b):
+            np.testing.assert_array_equal(x, y)
