@@ -5,6 +5,7 @@
 // fp16 step d and codes c of 0..15; the codes' bytes interleave the blocks
 // (include/forge_hip.h), so 16 neighbouring lanes of nb bytes cover a slot.
 #include "common.h"
+#include "f16split.h"
 
 #include <math.h>
 
@@ -123,73 +124,445 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Cache c, int layer, 
 }
 
 // ── attention ─────────────────────────────────────────────────────────────
-// Value i of a head's slot.
-template <int NB>
-__device__ __forceinline__ float value_at(const uint8_t* codes, const _Float16* steps, int64_t slot, int i) {
-  const int b = i >> 5, n = i & 15, hi = (i >> 4) & 1;
-  const int q = (codes[slot * 16 * NB + n * NB + b] >> (4 * hi)) & 15;
-  return (float)steps[slot * NB + b] * (float)(q - 8);
+// One query token a sequence reads the cache once, 1.125 bytes a position and
+// head dim for 4 group flop: HBM-bound if decoding the codes costs few enough
+// instructions.  Both products run on the fp16 matrix pipes with the codes
+// c - 8 as operands, which fp16 holds exactly; what is not exact there is held
+// in two fp16 pieces (hi + lo, 22 bits), in rows of their own:
+//
+//   scores  16 rows (head, piece) of q x 32 values of a block x 16 positions;
+//           the block's step multiplies the sum (fp32)
+//   values  16 rows (head, piece) of w x 32 positions x 16 values of a block,
+//           w = p d with the block's step d, fp32 accumulators
+//
+// A wave takes 32 positions at a time and keeps the running maximum, sum and
+// values of its heads; p = 2^(x - ref) with ref = max - 15 + E, 2^E above every
+// step so far, so that w fills fp16's range, [0, 2^15).  max and E are only
+// raised, and the accumulators rescaled, when a score or step goes beyond
+// them: after the first positions hardly ever.  Rows beyond 2 group hold the
+// same heads again for the next blocks' steps (G heads: 8 / G blocks an
+// operand), so few heads need fewer w.
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kRound = 128;    // positions a workgroup takes at a time, 32 a wave
+constexpr int kTarget = 1024;  // workgroups that the positions are spread over
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// How the positions of all sequences are cut: pieces of `per` rounds, at least
+// one a sequence and head.  A wave works it out from the lengths (which only
+// the device knows): a lane per sequence, or several.
+struct Plan {
+  int per;
+  int s, first, pieces;  // a sequence, its first piece (of one head) and their number
+};
+__device__ __forceinline__ int attended(const Cache& c, const int32_t* count, int s, int T) {
+  return min(slots_used(c, s) + new_tokens(count, s, T), c.maxSeq);
+}
+__device__ __forceinline__ int rounds_of(int n) { return (n + kRound - 1) / kRound; }
+__device__ __forceinline__ int pieces_of(int n, int per) { return max(1, (rounds_of(n) + per - 1) / per); }
+// The sequence with the piece id / heads (by_seq false), or sequence id.  False
+// if there is no such piece.
+__device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t* count, int T, int heads, int id,
+                                         bool by_seq) {
+  const int lane = threadIdx.x & 63, each = (c.nSeq + 63) / 64, s0 = lane * each;
+  int64_t rounds = 0;
+  for (int i = 0; i < each && s0 + i < c.nSeq; ++i) rounds += rounds_of(attended(c, count, s0 + i, T));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) rounds += __shfl_xor(rounds, o, 64);
+  p.per = (int)max((int64_t)1, (rounds * heads + kTarget - 1) / kTarget);
+  int mine = 0;
+  for (int i = 0; i < each && s0 + i < c.nSeq; ++i) mine += pieces_of(attended(c, count, s0 + i, T), p.per);
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += u;
+  }
+  const unsigned long long has = __ballot(by_seq ? id < s0 + each : id < (int64_t)upto * heads);
+  if (!has) return false;
+  const int owner = __builtin_ctzll(has);
+  p.s = owner * each;
+  p.first = __shfl(upto - mine, owner, 64);
+  for (;; ++p.s) {
+    p.pieces = pieces_of(attended(c, count, p.s, T), p.per);
+    if (by_seq ? p.s == id : id < (int64_t)(p.first + p.pieces) * heads) return true;
+    p.first += p.pieces;
+  }
 }
 
-__device__ __forceinline__ float block_max(float x, float* sh) {
-  x = fg_wave_max(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-  __syncthreads();
-  for (int i = 0; i < kWaves; ++i) x = fmaxf(x, sh[i]);
-  return x;
+// The low and the high codes of a byte pair, less 8: 0x6400 | c is the fp16
+// 1024 + c, and 0x6400 | 16 c is 1024 + 16 c.
+__device__ __forceinline__ uint32_t low_codes(uint32_t x) {
+  const f16x2 y = __builtin_bit_cast(f16x2, (x & 0x000F000Fu) | 0x64006400u) + (f16x2){-1032.f, -1032.f};
+  return __builtin_bit_cast(uint32_t, y);
 }
-__device__ __forceinline__ float block_sum(float x, float* sh) {
-  x = fg_wave_sum(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = 0.f;
-  for (int i = 0; i < kWaves; ++i) x += sh[i];
-  return x;
+__device__ __forceinline__ uint32_t high_codes(uint32_t x) {
+  const f16x2 y = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (x & 0x00F000F0u) | 0x64006400u),
+                                            (f16x2){0.0625f, 0.0625f}, (f16x2){-72.f, -72.f});
+  return __builtin_bit_cast(uint32_t, y);
+}
+__device__ __forceinline__ f16x8 operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(f16x8, (u32x4){a, b, c, d});
+}
+// N bytes from p, at any alignment, as words.
+template <int N>
+__device__ __forceinline__ void load_bytes(uint32_t (&w)[(N + 3) / 4], const void* p) {
+  w[(N + 3) / 4 - 1] = 0;
+  __builtin_memcpy(w, p, N);
 }
 
-// One workgroup per (sequence, kv head), a query head after the other: scores
-// to `sc`, their maximum and sum, then a value column per thread.
+// Positions [at, at + 32) of a head's cache, as a lane of a wave holds them:
+// lane (i = lane & 15, g = lane >> 4) has values 4 g .. 4 g + 3 and 16 more on of
+// every block of positions i and 16 + i's keys, and values i and 16 + i of every
+// block of positions 8 g .. 8 g + 7.
 template <int NB>
+struct Tile {
+  uint32_t k[2][NB];                 // bytes j NB + b: value 4 g + j of block b
+  uint32_t kd[2][(NB + 1) / 2];      // the keys' steps
+  uint32_t v[8][(NB + 3) / 4];       // byte b
+  uint32_t vd[8][(NB + 1) / 2];      // the values' steps
+  uint32_t all[(NB + 3) / 4];        // all steps of the tile's values, spread over the lanes
+  __device__ __forceinline__ void load(const Cache& c, int64_t slot0, int at, int n) {
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t slot = slot0 + min(at + 16 * t + i, n - 1);
+      load_bytes<4 * NB>(k[t], c.k + slot * (16 * NB) + g * 4 * NB);
+      load_bytes<2 * NB>(kd[t], c.kd + slot * NB);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t slot = slot0 + min(at + 8 * g + e, n - 1);
+      load_bytes<NB>(v[e], c.v + slot * (16 * NB) + i * NB);
+      load_bytes<2 * NB>(vd[e], c.vd + slot * NB);
+    }
+    // half of a position's steps, or all: NB values of 2 bytes over two lanes
+    const int64_t slot = slot0 + min(at + (lane >> 1), n - 1);
+    if constexpr (NB == 1) {
+      load_bytes<2>(all, c.vd + slot);
+    } else {
+      constexpr int H = (NB + 1) / 2;  // the second half of three starts at the second
+      load_bytes<2 * H>(all, c.vd + slot * NB + (lane & 1) * (NB - H));
+    }
+  }
+};
+__device__ __forceinline__ float half_of(uint32_t w, int i) {
+  return (float)__builtin_bit_cast(f16x2, w)[i];
+}
+
+// G heads (1, 2, 4 or 8) of a kv head over one piece of a sequence.  Pieces that
+// are a whole sequence give the output, others their reference, sum and values.
+template <int NB, int G>
 __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, float* __restrict__ out,
-                                                            const float* __restrict__ q, int nH, float scale, int T,
-                                                            const int32_t* __restrict__ count,
+                                                            const float* __restrict__ q, int nH, int subs, float scale,
+                                                            int T, const int32_t* __restrict__ count,
+                                                            float2* __restrict__ part_ml, float* __restrict__ part_o,
                                                             float* __restrict__ sc) {
-  constexpr int dH = 32 * NB;
-  __shared__ float sh[kWaves], qs[dH];
-  const int s = blockIdx.y, kvh = blockIdx.x, group = nH / c.nKV;
-  const int n = min(slots_used(c, s) + new_tokens(count, s, T), c.maxSeq);
+  constexpr int dH = 32 * NB, NS = 8 / G, NA = (NB + NS - 1) / NS;
+  __shared__ __attribute__((aligned(16))) float ps[kWaves][G][32];
+  __shared__ __attribute__((aligned(16))) float os[kWaves][G][dH];
+  __shared__ float ms[kWaves][G], ls[kWaves][G];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  Plan p;
+  if (!plan_for(p, c, count, T, c.nKV * subs, blockIdx.x, false)) return;
+  const int s = p.s, in_seq = blockIdx.x - p.first * c.nKV * subs;
+  const int head = in_seq / p.pieces, piece = in_seq - head * p.pieces;  // (kv head, share of its query heads)
+  const int kvh = head / subs, sub = head - kvh * subs;
+  const int group = nH / c.nKV, share = (group + subs - 1) / subs;
+  const int h0 = kvh * group + sub * share, heads = min(share, group - sub * share);
+  const int n = attended(c, count, s, T);
+  const int begin = piece * p.per * kRound, end = min(n, begin + p.per * kRound);
   const int64_t slot0 = head_slot(c, layer, s, kvh);
-  for (int g = 0; g < group; ++g) {
-    const int h = kvh * group + g;
-    float* row = sc + ((int64_t)s * nH + h) * c.maxSeq;
-    __syncthreads();
-    if (threadIdx.x < dH) qs[threadIdx.x] = q[((int64_t)s * nH + h) * dH + threadIdx.x];
-    __syncthreads();
-    float m = -INFINITY;
-    for (int j = threadIdx.x; j < n; j += kThreads) {
-      float dot = 0.f;
-      for (int i = 0; i < dH; ++i) dot += qs[i] * value_at<NB>(c.k, c.kd, slot0 + j, i);
-      row[j] = dot * scale;
-      m = fmaxf(m, row[j]);
+
+  // q as the scores' first operand: row = lane & 15 holds head (row / 2) % G,
+  // piece row & 1; its head's factor 2^-e goes into the scores
+  f16x8 qa[NB];
+  float factor[2];
+  {
+    const int h = (i >> 1) % G;
+    const bool on = h < heads;
+    const float* qr = q + ((int64_t)s * nH + h0 + (on ? h : 0)) * dH + 4 * g;
+    float x[NB][8];
+    float m = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      __builtin_memcpy(&x[b][0], qr + 32 * b, 16);
+      __builtin_memcpy(&x[b][4], qr + 32 * b + 16, 16);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!on) x[b][e] = 0.f;
+        const float a = fabsf(x[b][e]);
+        m = a < INFINITY ? fmaxf(m, a) : m;
+      }
     }
-    m = block_max(m, sh);
-    float l = 0.f;
-    for (int j = threadIdx.x; j < n; j += kThreads) {
-      row[j] = expf(row[j] - m);
-      l += row[j];
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const int e = fg::exponent_of_max(m);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // operand pairs: values (0, 1), (16, 17), (2, 3), (18, 19) of 4 g
+        const int at = (j & 1) * 4 + (j >> 1) * 2;
+        uint32_t hi, lo;
+        fg::split2h(x[b][at], x[b][at + 1], e, hi, lo);
+        w[j] = (i & 1) ? lo : hi;
+      }
+      qa[b] = operand(w[0], w[1], w[2], w[3]);
     }
-    l = block_sum(l, sh);
-    const float inv = n > 0 ? 1.f / l : 0.f;
-    if (c.weight)
-      for (int j = threadIdx.x; j < n; j += kThreads) c.weight[slot0 + j] += row[j] * inv;
-    __syncthreads();
-    if (threadIdx.x < dH) {
-      float o = 0.f;
-      for (int j = 0; j < n; ++j) o += row[j] * value_at<NB>(c.v, c.vd, slot0 + j, threadIdx.x);
-      out[((int64_t)s * nH + h) * dH + threadIdx.x] = o * inv;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      factor[j] = __builtin_amdgcn_ldexpf(scale * kLog2e, -__shfl(e, 2 * ((2 * g + j) % G), 64));
+  }
+
+  f32x4 o[NB][2];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) o[b][0] = o[b][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float top[2] = {-INFINITY, -INFINITY}, ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+  int E = -24;
+  uint32_t limit = 0;  // the greatest fp16 below 2^E, as its bits
+  const float piece_of = (i & 1) ? 1.f : 0.f;
+  const int set = (i >> 1) / G;  // which of an operand's NS blocks this row is for
+
+  for (int at = begin + 32 * wave; at < end; at += kRound) {
+    Tile<NB> tile;
+    tile.load(c, slot0, at, n);
+    // scores x of positions i and 16 + i for heads (2 g + j) % G, in powers of two
+    float x[2][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      x[t][0] = x[t][1] = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const uint32_t* kw = tile.k[t];
+        // the words that hold byte b of values 4 g + 0, 1 and 4 g + 2, 3
+        auto pair = [&](int j0) {
+          const int a0 = j0 * NB + b, a1 = (j0 + 1) * NB + b;
+          const uint32_t w0 = kw[a0 / 4], w1 = kw[a1 / 4];
+          return __builtin_amdgcn_perm(w1, w0, 0x0c000c00u | ((4 + a1 % 4) << 16) | (a0 % 4));
+        };
+        const uint32_t lo01 = pair(0), lo23 = pair(2);
+        const f16x8 kb = operand(low_codes(lo01), high_codes(lo01), low_codes(lo23), high_codes(lo23));
+        const f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[b], kb, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        const float step = half_of(tile.kd[t][b / 2], b & 1);
+        x[t][0] += (d[0] + d[1]) * step;
+        x[t][1] += (d[2] + d[3]) * step;
+      }
+      x[t][0] *= factor[0];
+      x[t][1] *= factor[1];
+      if (at + 16 * t + i >= end) x[t][0] = x[t][1] = -INFINITY;
     }
+    // raise the maximum or the steps' power where this tile goes beyond them
+    uint32_t far = 0;
+#pragma unroll
+    for (int w = 0; w < (NB + 3) / 4; ++w) {
+      const uint32_t a = tile.all[w] & 0x7FFF7FFFu, a0 = a & 0xFFFF, a1 = a >> 16;
+      far = max(far, max(a0 < 0x7C00 ? a0 : 0u, a1 < 0x7C00 ? a1 : 0u));
+    }
+    const float here[2] = {fmaxf(x[0][0], x[1][0]), fmaxf(x[0][1], x[1][1])};
+    if (__any(here[0] > top[0] || here[1] > top[1] || far > limit)) {
+      float f = (float)__builtin_bit_cast(_Float16, (uint16_t)far);
+      f = fg_wave_max(f);
+      if (f > 0.f) E = max(E, __builtin_amdgcn_frexp_expf(f));
+      limit = E > -14 ? (uint32_t)((E + 14) << 10) | 0x3FF : (1u << (E + 24)) - 1;
+      float turn[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float m = here[j];
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 16));
+        top[j] = fmaxf(top[j], m);
+        const float r = top[j] + (float)(E - 15);
+        turn[j] = r == ref[j] ? 1.f : __builtin_amdgcn_exp2f(ref[j] - r);
+        ref[j] = r;
+        sum[j] *= turn[j];
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          o[b][u][0] *= turn[0];
+          o[b][u][1] *= turn[0];
+          o[b][u][2] *= turn[1];
+          o[b][u][3] *= turn[1];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int h = (2 * g + j) % G;
+      const bool mine = (2 * g + j) < G;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (sc && mine && h < heads && at + 16 * t + i < end)
+          sc[((int64_t)s * nH + h0 + h) * c.maxSeq + at + 16 * t + i] = x[t][j];
+        const float e = __builtin_amdgcn_exp2f(x[t][j] - ref[j]);
+        sum[j] += e;
+        if (mine) ps[wave][h][16 * t + i] = e;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float e[8];
+    {
+      const float4* pr = reinterpret_cast<const float4*>(&ps[wave][(i >> 1) % G][8 * g]);
+      const float4 a = pr[0], b = pr[1];
+      e[0] = a.x, e[1] = a.y, e[2] = a.z, e[3] = a.w, e[4] = b.x, e[5] = b.y, e[6] = b.z, e[7] = b.w;
+    }
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+      // w = p d of this row's block, the row's piece of it
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float y[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float d = 0.f;
+#pragma unroll
+          for (int z = 0; z < NS; ++z)
+            if (a * NS + z < NB && (NS == 1 || set == z)) d = half_of(tile.vd[2 * j + k][(a * NS + z) / 2], (a * NS + z) & 1);
+          y[k] = e[2 * j + k] * d;
+        }
+        const f16x2 h = __builtin_convertvector((f32x2){y[0], y[1]}, f16x2);
+        const f16x2 r = __builtin_convertvector((f32x2){y[0] - piece_of * (float)h[0], y[1] - piece_of * (float)h[1]}, f16x2);
+        w[j] = __builtin_bit_cast(uint32_t, r);
+      }
+      const f16x8 wa = operand(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int z = 0; z < NS; ++z) {
+        const int b = a * NS + z;
+        if (b >= NB) break;
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t two = __builtin_amdgcn_perm(tile.v[2 * j + 1][b / 4], tile.v[2 * j][b / 4],
+                                                     0x0c000c00u | ((4 + b % 4) << 16) | (b % 4));
+          lo[j] = low_codes(two);
+          hi[j] = high_codes(two);
+        }
+        o[b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, operand(lo[0], lo[1], lo[2], lo[3]), o[b][0], 0, 0, 0);
+        o[b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, operand(hi[0], hi[1], hi[2], hi[3]), o[b][1], 0, 0, 0);
+      }
+    }
+  }
+
+  // the waves' results joined: references to their maximum, then sums
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) sum[j] += __shfl_xor(sum[j], d, 16);
+    if (i == 0 && 2 * g + j < G) ms[wave][2 * g + j] = ref[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int h = (2 * g + j) % G;
+    float m = ms[0][h];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ms[w][h]);
+    const float turn = ref[j] == m ? 1.f : __builtin_amdgcn_exp2f(ref[j] - m);
+    if (i == 0 && 2 * g + j < G) ls[wave][h] = sum[j] * turn;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if ((2 * g + j) / G == b % NS) os[wave][h][32 * b + 16 * u + i] = (o[b][u][2 * j] + o[b][u][2 * j + 1]) * turn;
+  }
+  __syncthreads();
+  const bool whole = p.pieces == 1;
+  for (int k = threadIdx.x; k < heads * dH; k += kThreads) {
+    const int h = k / dH, d = k - h * dH;
+    float v = 0.f, l = 0.f, m = ms[0][h];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      v += os[w][h][d];
+      l += ls[w][h];
+      m = fmaxf(m, ms[w][h]);
+    }
+    if (whole) out[((int64_t)s * nH + h0 + h) * dH + d] = n > 0 ? v / l : 0.f;
+    else part_o[((int64_t)blockIdx.x * G + h) * dH + d] = v;
+    if (d == 0) part_ml[(int64_t)blockIdx.x * G + h] = make_float2(m, l);
+  }
+}
+
+// The pieces of every sequence joined: workgroups [0, nSeq nH) the output of a
+// query head, the rest (weights kept) the weights of 1024 positions of a kv head.
+constexpr int kWeightRows = 1024;
+template <int NB>
+__global__ void __launch_bounds__(kThreads) kv4_join_kernel(Cache c, int layer, float* __restrict__ out, int nH,
+                                                            int subs, int G, int T, const int32_t* __restrict__ count,
+                                                            const float2* __restrict__ part_ml,
+                                                            const float* __restrict__ part_o,
+                                                            const float* __restrict__ sc, int chunks) {
+  constexpr int dH = 32 * NB, kLanes = kThreads / dH > 0 ? kThreads / dH : 1;
+  __shared__ float red[kThreads];
+  const int group = nH / c.nKV, share = (group + subs - 1) / subs;
+  const bool weights = (int)blockIdx.x >= c.nSeq * nH;
+  const int id = weights ? blockIdx.x - c.nSeq * nH : blockIdx.x;
+  const int s = weights ? id / (c.nKV * chunks) : id / nH;
+  Plan p;
+  plan_for(p, c, count, T, c.nKV * subs, s, true);
+  const int n = attended(c, count, s, T);
+  if (weights) {
+    const int kvh = id / chunks % c.nKV, at0 = id % chunks * kWeightRows;
+    if (at0 >= n) return;
+    float add[kWeightRows / kThreads];
+#pragma unroll
+    for (int k = 0; k < kWeightRows / kThreads; ++k) add[k] = 0.f;
+    for (int h = 0; h < group; ++h) {
+      const int64_t first = ((int64_t)p.first * c.nKV * subs + (int64_t)(kvh * subs + h / share) * p.pieces) * G + h % share;
+      float m = -INFINITY;
+      for (int k = threadIdx.x & 63; k < p.pieces; k += 64) m = fmaxf(m, part_ml[first + (int64_t)k * G].x);
+      m = fg_wave_max(m);
+      float l = 0.f;
+      for (int k = threadIdx.x & 63; k < p.pieces; k += 64) {
+        const float2 ml = part_ml[first + (int64_t)k * G];
+        l += ml.y * (ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m));
+      }
+      l = 1.f / fg_wave_sum(l);
+      const float* row = sc + ((int64_t)s * nH + kvh * group + h) * c.maxSeq;
+#pragma unroll
+      for (int k = 0; k < kWeightRows / kThreads; ++k) {
+        const int at = at0 + k * kThreads + threadIdx.x;
+        if (at < n) add[k] += __builtin_amdgcn_exp2f(row[at] - m) * l;
+      }
+    }
+    float* w = c.weight + head_slot(c, layer, s, kvh);
+#pragma unroll
+    for (int k = 0; k < kWeightRows / kThreads; ++k) {
+      const int at = at0 + k * kThreads + threadIdx.x;
+      if (at < n) w[at] += add[k];
+    }
+    return;
+  }
+  if (p.pieces == 1) return;
+  const int h = id % nH, kvh = h / group, r = h - kvh * group;
+  const int64_t first = ((int64_t)p.first * c.nKV * subs + (int64_t)(kvh * subs + r / share) * p.pieces) * G + r % share;
+  float m = -INFINITY;
+  for (int k = threadIdx.x & 63; k < p.pieces; k += 64) m = fmaxf(m, part_ml[first + (int64_t)k * G].x);
+  m = fg_wave_max(m);
+  float l = 0.f;
+  for (int k = threadIdx.x & 63; k < p.pieces; k += 64) {
+    const float2 ml = part_ml[first + (int64_t)k * G];
+    l += ml.y * (ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m));
+  }
+  l = fg_wave_sum(l);
+  const int d = threadIdx.x % dH, z = threadIdx.x / dH;
+  float v = 0.f;
+  if (z < kLanes)
+    for (int k = z; k < p.pieces; k += kLanes) {
+      const float mk = part_ml[first + (int64_t)k * G].x;
+      v += part_o[(first + (int64_t)k * G) * dH + d] * (mk == m ? 1.f : __builtin_amdgcn_exp2f(mk - m));
+    }
+  red[threadIdx.x] = v;
+  __syncthreads();
+  if (z == 0) {
+    for (int k = 1; k < kLanes; ++k) v += red[k * dH + d];
+    out[((int64_t)s * nH + h) * dH + d] = v / l;
   }
 }
 
@@ -428,13 +801,37 @@ extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const f
   FG_ARG_CHECK(T >= 0, "fg_kv4_attn: T %d is negative", T);
   FG_ARG_CHECK(nHeads > 0 && nHeads % c->nKvHeads == 0, "fg_kv4_attn: %d query heads for %d kv heads", nHeads,
                c->nKvHeads);
-  FG_ARG_CHECK(c->nSeq <= 65535, "fg_kv4_attn: %d sequences are too many", c->nSeq);
   FG_REQUIRE_INIT();
   fg::KProfScope prof("kv4_attn", 0.0, (double)c->nSeq * c->maxSeq * slot_bytes(c));
+  const int group = nHeads / c->nKvHeads, subs = (group + 7) / 8, share = (group + subs - 1) / subs;
+  const int G = share > 4 ? 8 : share > 2 ? 4 : share;
+  const int64_t heads = (int64_t)c->nSeq * c->nKvHeads * subs, rounds = (c->maxSeq + kRound - 1) / kRound;
+  const int64_t grid = heads * rounds < heads + kTarget ? heads * rounds : heads + kTarget;
+  const int64_t chunks = c->weight ? (c->maxSeq + kWeightRows - 1) / kWeightRows : 0;
+  const int64_t join = (int64_t)c->nSeq * nHeads + (int64_t)c->nSeq * c->nKvHeads * chunks;
+  FG_ARG_CHECK(grid <= INT32_MAX / kThreads && join <= INT32_MAX / kThreads,
+               "fg_kv4_attn: %d sequences x %d heads x %d slots are too many", c->nSeq, nHeads, c->maxSeq);
+  // references and sums, values, and the scores where weights are kept
+  const size_t ml = (size_t)grid * G * sizeof(float2), po = rounds > 1 ? (size_t)grid * G * c->dHead * sizeof(float) : 0;
+  const size_t ps = c->weight ? (size_t)c->nSeq * nHeads * c->maxSeq * sizeof(float) : 0;
   fg::Workspace ws;
-  KV4_TRY(ws.get((size_t)c->nSeq * nHeads * c->maxSeq * sizeof(float)));
-  KV4_DISPATCH(c->dHead, FG_LAUNCH(kv4_attn_kernel<NB>, dim3(c->nKvHeads, c->nSeq), dim3(kThreads), 0, view(c), layer,
-                                   out, q, nHeads, (float)scale, T, count, (float*)ws.ptr));
+  KV4_TRY(ws.get(ml + po + ps));
+  float2* part_ml = (float2*)ws.ptr;
+  float* part_o = (float*)((uint8_t*)ws.ptr + ml);
+  float* sc = c->weight ? (float*)((uint8_t*)ws.ptr + ml + po) : nullptr;
+#define KV4_ATTN(GS)                                                                                              \
+  FG_LAUNCH((kv4_attn_kernel<NB, GS>), dim3((unsigned)grid), dim3(kThreads), 0, view(c), layer, out, q, nHeads, subs, \
+            (float)scale, T, count, part_ml, part_o, sc)
+  KV4_DISPATCH(c->dHead, {
+    if (G == 1) KV4_ATTN(1);
+    else if (G == 2) KV4_ATTN(2);
+    else if (G == 4) KV4_ATTN(4);
+    else KV4_ATTN(8);
+    if (rounds > 1 || c->weight)
+      FG_LAUNCH(kv4_join_kernel<NB>, dim3((unsigned)join), dim3(kThreads), 0, view(c), layer, out, nHeads, subs, G, T,
+                count, (const float2*)part_ml, (const float*)part_o, (const float*)sc, (int)chunks);
+  });
+#undef KV4_ATTN
   return FG_OK;
 }
 

@@ -54,12 +54,15 @@ def rows(rng, *shape):
     return x * np.exp(rng.uniform(-3, 3, shape[-1])).astype(np.float32)
 
 
-def attend_bound(q, K, V, p, scale):
+def attend_bound(q, K, V, p, scale, steps):
     """Bounds of |out| and |weight| errors, term by term: q in two fp16 pieces is off by 2^-22 of
     itself, a score's dH products and its nb block sums round at 2^-24 each (and scale, log2 e and the
     subtraction of the maximum, 4 more of the largest score), exp2 is good to 2^-22; p's and the sums over
     n positions round at most n / 4 + 64 times in a chain (a sum over a tile's positions stays in the
-    matrix unit's order); p d is held in two fp16 pieces, 2^-22."""
+    matrix unit's order); p d is held in two fp16 pieces, 2^-22.  The pieces count from the greatest
+    step: w = p d 2^(15 - E), 2^E at most twice the greatest step, has an absolute error of 2^-25 where its
+    low piece is subnormal, which is 2^-40 2^E <= 2^-39 max d of p d (and of less after the division by
+    the sum of p, 1 or more), times |c - 8| <= 8, for each of n positions."""
     n, nKV, dH = K.shape
     nH = q.shape[0]
     out, weight = np.zeros((nH, dH)), np.zeros((nH, n))
@@ -68,7 +71,7 @@ def attend_bound(q, K, V, p, scale):
         mass = abs(scale) * (np.abs(K[:, z]) @ np.abs(q[h].astype(np.float64)))
         es = mass.max() * (2.0 ** -22 + (dH + 16) * 2.0 ** -24)
         rel = 2 * es + 2.0 ** -21 + (n / 4 + 64) * 2.0 ** -24
-        out[h] = rel * (p[h] @ np.abs(V[:, z])) + 1e-30
+        out[h] = rel * (p[h] @ np.abs(V[:, z])) + n * 8 * 2.0 ** -39 * np.abs(steps[z].astype(np.float64)).max() + 1e-30
         weight[h] = rel * p[h] + 1e-30
     return out, weight
 
@@ -165,7 +168,7 @@ def check_attend(fh, c, nH, rng, lens, T=0, count=None, scale=None, q=None, laye
         K = ref.values(before[0][layer, s, :, :n], before[2][layer, s, :, :n]).transpose(1, 0, 2)
         V = ref.values(before[1][layer, s, :, :n], before[3][layer, s, :, :n]).transpose(1, 0, 2)
         want, p = ref.attend(q[s], K, V, scale)
-        eo, ew = attend_bound(q[s], K, V, p, scale)
+        eo, ew = attend_bound(q[s], K, V, p, scale, before[3][layer, s, :, :n])
         assert np.isfinite(got[s]).all(), (s, n)
         worst = (np.abs(got[s] - want) / eo).max() if n else np.abs(got[s]).max()
         assert worst <= (1.0 if n else 0.0), (s, n, worst)
