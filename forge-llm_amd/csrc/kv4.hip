@@ -8,6 +8,7 @@
 #include "f16split.h"
 
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -195,13 +196,14 @@ __device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t*
 }
 
 // The low and the high codes of a byte pair, less 8: 0x6400 | c is the fp16
-// 1024 + c, and 0x6400 | 16 c is 1024 + 16 c.
-__device__ __forceinline__ uint32_t low_codes(uint32_t x) {
-  const f16x2 y = __builtin_bit_cast(f16x2, (x & 0x000F000Fu) | 0x64006400u) + (f16x2){-1032.f, -1032.f};
+// 1024 + c, and 0x6400 | 16 c is 1024 + 16 c.  `magic` is 0x64006400 in a vector
+// register, so that mask and or are one instruction (one scalar operand each).
+__device__ __forceinline__ uint32_t low_codes(uint32_t x, uint32_t magic) {
+  const f16x2 y = __builtin_bit_cast(f16x2, (x & 0x000F000Fu) | magic) + (f16x2){-1032.f, -1032.f};
   return __builtin_bit_cast(uint32_t, y);
 }
-__device__ __forceinline__ uint32_t high_codes(uint32_t x) {
-  const f16x2 y = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (x & 0x00F000F0u) | 0x64006400u),
+__device__ __forceinline__ uint32_t high_codes(uint32_t x, uint32_t magic) {
+  const f16x2 y = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (x & 0x00F000F0u) | magic),
                                             (f16x2){0.0625f, 0.0625f}, (f16x2){-72.f, -72.f});
   return __builtin_bit_cast(uint32_t, y);
 }
@@ -214,62 +216,67 @@ __device__ __forceinline__ void load_bytes(uint32_t (&w)[(N + 3) / 4], const voi
   w[(N + 3) / 4 - 1] = 0;
   __builtin_memcpy(w, p, N);
 }
-
-// Positions [at, at + 32) of a head's cache, as a lane of a wave holds them:
-// lane (i = lane & 15, g = lane >> 4) has values 4 g .. 4 g + 3 and 16 more on of
-// every block of positions i and 16 + i's keys, and values i and 16 + i of every
-// block of positions 8 g .. 8 g + 7.
-template <int NB>
-struct Tile {
-  uint32_t k[2][NB];                 // bytes j NB + b: value 4 g + j of block b
-  uint32_t kd[2][(NB + 1) / 2];      // the keys' steps
-  uint32_t v[8][(NB + 3) / 4];       // byte b
-  uint32_t vd[8][(NB + 1) / 2];      // the values' steps
-  uint32_t all[(NB + 3) / 4];        // all steps of the tile's values, spread over the lanes
-  __device__ __forceinline__ void load(const Cache& c, int64_t slot0, int at, int n) {
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int64_t slot = slot0 + min(at + 16 * t + i, n - 1);
-      load_bytes<4 * NB>(k[t], c.k + slot * (16 * NB) + g * 4 * NB);
-      load_bytes<2 * NB>(kd[t], c.kd + slot * NB);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t slot = slot0 + min(at + 8 * g + e, n - 1);
-      load_bytes<NB>(v[e], c.v + slot * (16 * NB) + i * NB);
-      load_bytes<2 * NB>(vd[e], c.vd + slot * NB);
-    }
-    // half of a position's steps, or all: NB values of 2 bytes over two lanes
-    const int64_t slot = slot0 + min(at + (lane >> 1), n - 1);
-    if constexpr (NB == 1) {
-      load_bytes<2>(all, c.vd + slot);
-    } else {
-      constexpr int H = (NB + 1) / 2;  // the second half of three starts at the second
-      load_bytes<2 * H>(all, c.vd + slot * NB + (lane & 1) * (NB - H));
-    }
-  }
-};
 __device__ __forceinline__ float half_of(uint32_t w, int i) {
   return (float)__builtin_bit_cast(f16x2, w)[i];
 }
 
+// 32 positions of a head's cache, as a lane of a wave holds them: lane
+// (i = lane & 15, g = lane >> 4) has values 4 g .. 4 g + 3 and 16 more on of every
+// block of positions i and 16 + i's keys, and values i and 16 + i of every block
+// of positions 8 g .. 8 g + 7, with the steps of the NA blocks of its row's set.
+template <int NB, int NA>
+struct Tile {
+  uint32_t k[2][NB];             // bytes j NB + b: value 4 g + j of block b
+  uint32_t kd[2][(NB + 1) / 2];  // the keys' steps
+  uint32_t v[8][(NB + 3) / 4];   // byte b
+  uint32_t vd[8][(NA + 1) / 2];  // the values' steps
+  uint32_t all[(NB + 3) / 4];    // all steps of the values, spread over the lanes
+  // bk, bv, dk, dv: the tile's first slot (uniform); `left` of its positions exist
+  // (1 or more), the rest repeat the last
+  template <bool Whole>
+  __device__ __forceinline__ void load(const uint8_t* bk, const uint8_t* bv, const uint8_t* dk, const uint8_t* dv,
+                                       int first_block, int left) {
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    auto at = [&](int j) { return (uint32_t)(Whole ? j : min(j, left - 1)); };
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t j = Whole ? i : at(16 * t + i), imm = Whole ? 16 * t : 0;
+      load_bytes<4 * NB>(k[t], bk + (j * (16 * NB) + g * 4 * NB) + imm * (16 * NB));
+      load_bytes<2 * NB>(kd[t], dk + j * (2 * NB) + imm * (2 * NB));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t j = Whole ? 8 * g : at(8 * g + e), imm = Whole ? e : 0;
+      load_bytes<NB>(v[e], bv + (j * (16 * NB) + i * NB) + imm * (16 * NB));
+      load_bytes<2 * NA>(vd[e], dv + (j * (2 * NB) + first_block * 2) + imm * (2 * NB));
+      if constexpr (NB == 3 && NA == 2) vd[e][0] >>= 16 * first_block;  // set 1: block 2 first
+    }
+    // a lane takes half of a position's steps, of three the first or last two
+    constexpr int H = NB == 1 ? 1 : (NB + 1) / 2;
+    load_bytes<2 * H>(all, dv + at(lane >> 1) * (2 * NB) + (lane & 1) * (NB - H) * 2);
+  }
+};
+
 // G heads (1, 2, 4 or 8) of a kv head over one piece of a sequence.  Pieces that
 // are a whole sequence give the output, others their reference, sum and values.
 template <int NB, int G>
-__global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, float* __restrict__ out,
+__global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cache c, int layer, float* __restrict__ out,
                                                             const float* __restrict__ q, int nH, int subs, float scale,
                                                             int T, const int32_t* __restrict__ count,
                                                             float2* __restrict__ part_ml, float* __restrict__ part_o,
                                                             float* __restrict__ sc) {
-  constexpr int dH = 32 * NB, NS = 8 / G, NA = (NB + NS - 1) / NS;
+  constexpr int dH = 32 * NB, NS = 8 / G, NA = (NB + NS - 1) / NS;  // sets of rows, blocks of a set
   __shared__ __attribute__((aligned(16))) float ps[kWaves][G][32];
   __shared__ __attribute__((aligned(16))) float os[kWaves][G][dH];
   __shared__ float ms[kWaves][G], ls[kWaves][G];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Plan p;
   if (!plan_for(p, c, count, T, c.nKV * subs, blockIdx.x, false)) return;
-  const int s = p.s, in_seq = blockIdx.x - p.first * c.nKV * subs;
+  p.per = __builtin_amdgcn_readfirstlane(p.per);
+  p.first = __builtin_amdgcn_readfirstlane(p.first);
+  p.pieces = __builtin_amdgcn_readfirstlane(p.pieces);
+  const int s = __builtin_amdgcn_readfirstlane(p.s), in_seq = blockIdx.x - p.first * c.nKV * subs;
   const int head = in_seq / p.pieces, piece = in_seq - head * p.pieces;  // (kv head, share of its query heads)
   const int kvh = head / subs, sub = head - kvh * subs;
   const int group = nH / c.nKV, share = (group + subs - 1) / subs;
@@ -295,8 +302,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, 
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (!on) x[b][e] = 0.f;
-        const float a = fabsf(x[b][e]);
-        m = a < INFINITY ? fmaxf(m, a) : m;
+        m = fmaxf(m, fabsf(x[b][e]));
       }
     }
     m = fmaxf(m, __shfl_xor(m, 16, 64));
@@ -327,11 +333,16 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, 
   int E = -24;
   uint32_t limit = 0;  // the greatest fp16 below 2^E, as its bits
   const float piece_of = (i & 1) ? 1.f : 0.f;
-  const int set = (i >> 1) / G;  // which of an operand's NS blocks this row is for
+  const int set = (i >> 1) / G, set_block = min(set * NA, NB - NA);  // this row's blocks
+  uint32_t magic = 0x64006400u;
+  asm("" : "+v"(magic));
 
-  for (int at = begin + 32 * wave; at < end; at += kRound) {
-    Tile<NB> tile;
-    tile.load(c, slot0, at, n);
+  auto take = [&](int at, auto is_whole) __attribute__((always_inline)) {
+    constexpr bool whole = decltype(is_whole)::value;
+    Tile<NB, NA> tile;
+    const int64_t slot = slot0 + at;
+    tile.template load<whole>(c.k + slot * (16 * NB), c.v + slot * (16 * NB), (const uint8_t*)(c.kd + slot * NB),
+                              (const uint8_t*)(c.vd + slot * NB), set_block, n - at);
     // scores x of positions i and 16 + i for heads (2 g + j) % G, in powers of two
     float x[2][2];
 #pragma unroll
@@ -347,7 +358,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, 
           return __builtin_amdgcn_perm(w1, w0, 0x0c000c00u | ((4 + a1 % 4) << 16) | (a0 % 4));
         };
         const uint32_t lo01 = pair(0), lo23 = pair(2);
-        const f16x8 kb = operand(low_codes(lo01), high_codes(lo01), low_codes(lo23), high_codes(lo23));
+        const f16x8 kb = operand(low_codes(lo01, magic), high_codes(lo01, magic), low_codes(lo23, magic), high_codes(lo23, magic));
         const f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[b], kb, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
         const float step = half_of(tile.kd[t][b / 2], b & 1);
         x[t][0] += (d[0] + d[1]) * step;
@@ -355,7 +366,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, 
       }
       x[t][0] *= factor[0];
       x[t][1] *= factor[1];
-      if (at + 16 * t + i >= end) x[t][0] = x[t][1] = -INFINITY;
+      if (!whole && at + 16 * t + i >= end) x[t][0] = x[t][1] = -INFINITY;
     }
     // raise the maximum or the steps' power where this tile goes beyond them
     uint32_t far = 0;
@@ -398,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, 
       const bool mine = (2 * g + j) < G;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        if (sc && mine && h < heads && at + 16 * t + i < end)
+        if (sc && mine && h < heads && (whole || at + 16 * t + i < end))
           sc[((int64_t)s * nH + h0 + h) * c.maxSeq + at + 16 * t + i] = x[t][j];
         const float e = __builtin_amdgcn_exp2f(x[t][j] - ref[j]);
         sum[j] += e;
@@ -414,19 +425,13 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, 
     }
 #pragma unroll
     for (int a = 0; a < NA; ++a) {
-      // w = p d of this row's block, the row's piece of it
+      // w = p d of block a of this row's set, the row's piece of it
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float y[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float d = 0.f;
-#pragma unroll
-          for (int z = 0; z < NS; ++z)
-            if (a * NS + z < NB && (NS == 1 || set == z)) d = half_of(tile.vd[2 * j + k][(a * NS + z) / 2], (a * NS + z) & 1);
-          y[k] = e[2 * j + k] * d;
-        }
+        for (int k = 0; k < 2; ++k) y[k] = e[2 * j + k] * half_of(tile.vd[2 * j + k][a / 2], a & 1);
         const f16x2 h = __builtin_convertvector((f32x2){y[0], y[1]}, f16x2);
         const f16x2 r = __builtin_convertvector((f32x2){y[0] - piece_of * (float)h[0], y[1] - piece_of * (float)h[1]}, f16x2);
         w[j] = __builtin_bit_cast(uint32_t, r);
@@ -434,21 +439,24 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, 
       const f16x8 wa = operand(w[0], w[1], w[2], w[3]);
 #pragma unroll
       for (int z = 0; z < NS; ++z) {
-        const int b = a * NS + z;
+        const int b = z * NA + a;
         if (b >= NB) break;
         uint32_t lo[4], hi[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t two = __builtin_amdgcn_perm(tile.v[2 * j + 1][b / 4], tile.v[2 * j][b / 4],
                                                      0x0c000c00u | ((4 + b % 4) << 16) | (b % 4));
-          lo[j] = low_codes(two);
-          hi[j] = high_codes(two);
+          lo[j] = low_codes(two, magic);
+          hi[j] = high_codes(two, magic);
         }
         o[b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, operand(lo[0], lo[1], lo[2], lo[3]), o[b][0], 0, 0, 0);
         o[b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wa, operand(hi[0], hi[1], hi[2], hi[3]), o[b][1], 0, 0, 0);
       }
     }
-  }
+  };
+  int at = begin + 32 * wave;
+  for (; at + 32 <= end; at += kRound) take(at, std::true_type());
+  if (at < end) take(at, std::false_type());
 
   // the waves' results joined: references to their maximum, then sums
 #pragma unroll
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Cache c, int layer, 
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        if ((2 * g + j) / G == b % NS) os[wave][h][32 * b + 16 * u + i] = (o[b][u][2 * j] + o[b][u][2 * j + 1]) * turn;
+        if ((2 * g + j) / G == b / NA) os[wave][h][32 * b + 16 * u + i] = (o[b][u][2 * j] + o[b][u][2 * j + 1]) * turn;
   }
   __syncthreads();
   const bool whole = p.pieces == 1;
