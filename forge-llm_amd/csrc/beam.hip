@@ -11,128 +11,299 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxBeams = 64;
 
 // ── selection ─────────────────────────────────────────────────────────────
-// Whether (x, i) comes before (y, j): the greater value, NaN last, then the
-// lower index.
-template <typename F>
-__device__ __forceinline__ bool before(F x, int i, F y, int j) {
-  if (x > y) return true;
-  if (x < y) return false;
-  const bool nx = x != x, ny = y != y;
-  if (nx != ny) return ny;
-  return i < j;
+// Each logit is read once, so the choice is made in two launches: a workgroup
+// per segment of a row leaves the segment's maximum, sum of exponentials and W
+// first candidates, then a workgroup per request forms the rows' log sums and
+// picks among the segments' candidates, in fp64.  Both find the W first of many
+// without sorting them: the W-th greatest of the threads' own maxima bounds the
+// W-th greatest of all from below, few values reach it, and those are ranked by
+// counting.
+//
+// Values are compared as unsigned keys in the order of the values: none 0, NaN
+// 1, -inf the lowest number, -0 as +0.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.f);
+  return x != x ? 1u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __builtin_bit_cast(float, k == 1u ? 0x7FC00000u : (k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ uint64_t key_of(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
+  return x != x ? 1ull : u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double value_of(uint64_t k) {
+  return __builtin_bit_cast(double, k == 1ull ? 0x7FF8000000000000ull
+                                    : (k >> 63) ? k ^ 0x8000000000000000ull
+                                                : ~k);
 }
 
-constexpr int kNone = 0x7FFFFFFF;  // index of no candidate, after all others
-// The first of the workgroup's (x, i).
-__device__ __forceinline__ void block_first(float& x, int& i, float* shx, int* shi) {
+constexpr int kListed = 1024;  // candidates that are ranked by counting
+
+// The segment's candidates beyond kListed (ties, mostly): the W-th greatest key
+// and, among its equals, the place of the last one taken, bit by bit.
+template <int E>
+__device__ void exact_border(uint32_t& border, int& last, const uint32_t (&key)[E], int W, int* sh) {
+  const int wave = threadIdx.x >> 6;
+  auto count = [&](auto in) {
+    int n = 0;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float y = __shfl_xor(x, o, 64);
-    const int j = __shfl_xor(i, o, 64);
-    if (i == kNone || (j != kNone && before(y, j, x, i))) x = y, i = j;
+    for (int e = 0; e < E; ++e) n += __popcll(__ballot(in(e)));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[wave] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < kWaves; ++w) n += sh[w];
+    return n;
+  };
+  border = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = border | (1u << bit);
+    if (count([&](int e) { return key[e] >= t; }) >= W) border = t;
+  }
+  const int need = W - count([&](int e) { return key[e] > border; });
+  // place of element e of a thread, in the order of the row
+  auto place = [&](int e) { return (e >> 2) * 4 * kThreads + 4 * (int)threadIdx.x + (e & 3); };
+  last = 0;  // count(place < last) < need <= count(place <= last)
+  for (int bit = 14; bit >= 0; --bit) {
+    const int t = last + (1 << bit);
+    if (count([&](int e) { return key[e] == border && place(e) < t; }) < need) last = t;
+  }
+}
+
+// Segment blockIdx.x of row blockIdx.y: up to 4 P values a thread.
+template <int P>
+__global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restrict__ sums, uint2* __restrict__ cand,
+                                                                const float* __restrict__ logits, int64_t ld,
+                                                                const int32_t* __restrict__ done, int W, int V,
+                                                                int length) {
+  constexpr int E = 4 * P;
+  __shared__ uint32_t best[kThreads];
+  __shared__ uint2 list[kListed];
+  __shared__ float shm[kWaves], shs[kWaves];
+  __shared__ int shn[kWaves], listed;
+  const int64_t row = blockIdx.y;
+  if (done && done[row]) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int first = blockIdx.x * length, n = min(length, V - first);
+  const float* x = logits + row * ld + first;
+  float v[E];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int at = 4 * ((int)threadIdx.x + p * kThreads);
+    if (at + 4 <= n) {
+      __builtin_memcpy(&v[4 * p], x + at, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * p + e] = at + e < n ? x[at + e] : -INFINITY;
+    }
+  }
+  if (threadIdx.x == 0) listed = 0;
+  float m = v[0];
+#pragma unroll
+  for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
+  m = fg_wave_max(m);
+  if (lane == 0) shm[wave] = m;
+  uint32_t key[E], mine = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int at = 4 * ((int)threadIdx.x + (e >> 2) * kThreads) + (e & 3);
+    key[e] = at < n ? key_of(v[e]) : 0u;
+    mine = max(mine, key[e]);
+  }
+  best[threadIdx.x] = mine;
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, shm[w]);
+  // exp(x - m) in fp32: good to 2^-21 where it counts
+  const float from = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - from) * 1.44269504088896340736f);
+  s = fg_wave_sum(s);
+  if (lane == 0) shs[wave] = s;
+  // the W-th greatest of the threads' maxima, its low 12 bits dropped
+  uint32_t b[kWaves], border = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) b[w] = best[w * 64 + lane];
+  for (int bit = 31; bit >= 12; --bit) {
+    const uint32_t t = border | (1u << bit);
+    int c = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) c += __popcll(__ballot(b[w] >= t));
+    if (c >= W) border = t;
+  }
+  border = max(border, 1u);
+  if (mine >= border) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (key[e] >= border) {
+        const int i = atomicAdd(&listed, 1);
+        if (i < kListed) list[i] = make_uint2(key[e], 4 * (threadIdx.x + (e >> 2) * kThreads) + (e & 3));
+      }
   }
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) shx[threadIdx.x >> 6] = x, shi[threadIdx.x >> 6] = i;
-  __syncthreads();
-  x = shx[0], i = shi[0];
-  for (int w = 1; w < kWaves; ++w)
-    if (i == kNone || (shi[w] != kNone && before(shx[w], shi[w], x, i))) x = shx[w], i = shi[w];
+  int c = listed;
+  if (c > kListed) {  // the same for all threads
+    int last;
+    exact_border<E>(border, last, key, W, shn);
+    __syncthreads();
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int at = 4 * ((int)threadIdx.x + (e >> 2) * kThreads) + (e & 3);
+      if (key[e] > border || (key[e] == border && at <= last)) {
+        const int i = atomicAdd(&listed, 1);
+        if (i < kListed) list[i] = make_uint2(key[e], at);
+      }
+    }
+    __syncthreads();
+    c = min(listed, kListed);
+  }
+  const int64_t seg = row * gridDim.x + blockIdx.x;
+  cand += seg * W;
+  for (int i = threadIdx.x; i < max(c, W); i += kThreads) {
+    if (i >= c) {
+      cand[i] = make_uint2(0u, 0u);
+      continue;
+    }
+    const uint2 me = list[i];
+    int rank = 0;
+    for (int j = 0; j < c; ++j) {
+      const uint2 o = list[j];
+      rank += o.x > me.x || (o.x == me.x && o.y < me.y);
+    }
+    if (rank < W) cand[rank] = make_uint2(me.x, me.y + first);
+  }
+  if (threadIdx.x == 0) {
+    s = 0.f;
+    for (int w = 0; w < kWaves; ++w) s += shs[w];
+    sums[seg] = make_float2(m, s);
+  }
 }
 
-// One workgroup per beam: log sum exp of its logits, then its W first
-// candidates one after the other, into val / tok [beam][W].
-__global__ void __launch_bounds__(kThreads) beam_row_kernel(double* __restrict__ val, int32_t* __restrict__ tok,
-                                                            const float* __restrict__ logits, int64_t ld,
-                                                            const float* __restrict__ scores,
-                                                            const int32_t* __restrict__ done, int eos, int W, int V) {
-  __shared__ float shx[kWaves];
-  __shared__ int shi[kWaves];
-  __shared__ double shd[kWaves];
-  const int64_t b = blockIdx.x;
-  const float* x = logits + b * ld;
-  val += b * W;
-  tok += b * W;
-  if (done && done[b]) {
-    if (threadIdx.x < W) {
-      val[threadIdx.x] = scores[b];
-      tok[threadIdx.x] = threadIdx.x == 0 ? eos : kNone;
+// One workgroup per request.  A candidate's second key orders those of equal
+// value: the lower beam, within it the greater logit, then the lower token.
+constexpr int kTokenBits = 26;
+__global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__ score_out, int32_t* __restrict__ token,
+                                                             int32_t* __restrict__ parent, int32_t* __restrict__ done_out,
+                                                             const float2* __restrict__ sums,
+                                                             const uint2* __restrict__ cand,
+                                                             const float* __restrict__ scores,
+                                                             const int32_t* __restrict__ done, int eos, int W, int V,
+                                                             int S) {
+  __shared__ double base[kMaxBeams];
+  __shared__ int kind[kMaxBeams];  // 0: its candidates, 1: all equal to base, 2: done
+  __shared__ ulonglong2 list[kListed];
+  __shared__ unsigned long long border[kWaves];
+  __shared__ int listed;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t r0 = (int64_t)blockIdx.x * W;
+  for (int b = wave; b < W; b += kWaves) {
+    const bool fin = done && done[r0 + b];
+    float m = -INFINITY;
+    double s = 0.0;
+    if (!fin) {
+      const float2* row = sums + (r0 + b) * S;
+      for (int z = lane; z < S; z += 64) m = fmaxf(m, row[z].x);
+      m = fg_wave_max(m);
+      for (int z = lane; z < S; z += 64) s += (double)row[z].y * (row[z].x == m ? 1.0 : exp((double)row[z].x - (double)m));
+      s = fg_wave_sum_d(s);
+    }
+    if (lane == 0) {
+      const double score = scores[r0 + b];
+      double v = fin ? score : m == -INFINITY && s == 0.0 ? -INFINITY : score - ((double)m + log(s));
+      base[b] = v;
+      kind[b] = fin ? 2 : fabs(v) < INFINITY ? 0 : 1;
+    }
+  }
+  if (threadIdx.x == 0) listed = 0;
+  __syncthreads();
+  const int each = S * W, N = W * each;
+  auto candidate = [&](int i, ulonglong2& k) {
+    const int b = i / each, j = i - b * each;
+    uint2 c = make_uint2(1u, (uint32_t)j);  // all equal: the first W tokens
+    k = make_ulonglong2(0, 0);
+    if (kind[b] == 0) {
+      c = cand[r0 * each + i];
+      if (c.x == 0) return;
+      k.x = key_of(base[b] + (double)value_of(c.x));
+    } else if (kind[b] == 1) {
+      if (j >= W || j >= V) return;
+      k.x = key_of(base[b]);
+    } else {
+      if (j != 0) return;
+      k.x = key_of(base[b]);
+      c.y = eos;
+    }
+    k.y = ((uint64_t)(kMaxBeams - 1 - b) << (32 + kTokenBits)) | ((uint64_t)c.x << kTokenBits) |
+          ((1u << kTokenBits) - 1 - c.y);
+  };
+  auto put = [&](int rank, const ulonglong2& k) {
+    const int b = kMaxBeams - 1 - (int)(k.y >> (32 + kTokenBits));
+    const int t = (1 << kTokenBits) - 1 - (int)(k.y & ((1u << kTokenBits) - 1));
+    score_out[r0 + rank] = (float)value_of((uint64_t)k.x);
+    token[r0 + rank] = t;
+    parent[r0 + rank] = b;
+    if (done_out) done_out[r0 + rank] = kind[b] == 2 || t == eos;
+  };
+  auto above = [](const ulonglong2& a, const ulonglong2& b) { return a.x > b.x || (a.x == b.x && a.y > b.y); };
+  ulonglong2 k;
+  uint64_t mine = 0;
+  for (int i = threadIdx.x; i < N; i += kThreads) {
+    candidate(i, k);
+    mine = k.x > mine ? k.x : mine;
+  }
+  // each wave's W-th greatest of its lanes' maxima (high word); the greatest of them
+  uint32_t t32 = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = t32 | (1u << bit);
+    if (__popcll(__ballot((uint32_t)(mine >> 32) >= t)) >= W) t32 = t;
+  }
+  if (lane == 0) border[wave] = (uint64_t)t32 << 32;
+  __syncthreads();
+  uint64_t least = 1;
+  for (int w = 0; w < kWaves; ++w) least = border[w] > least ? border[w] : least;
+  if (mine >= least)
+    for (int i = threadIdx.x; i < N; i += kThreads) {
+      candidate(i, k);
+      if (k.x >= least) {
+        const int at = atomicAdd(&listed, 1);
+        if (at < kListed) list[at] = k;
+      }
+    }
+  __syncthreads();
+  const int c = listed;
+  if (c <= kListed) {
+    for (int i = threadIdx.x; i < c; i += kThreads) {
+      k = list[i];
+      int rank = 0;
+      for (int j = 0; j < c; ++j) rank += above(list[j], k);
+      if (rank < W) put(rank, k);
     }
     return;
   }
-  float m = -INFINITY;
-  int at = kNone, nan = 0;
-  for (int j = threadIdx.x; j < V; j += kThreads) {
-    if (at == kNone || before(x[j], j, m, at)) m = x[j], at = j;
-    nan |= x[j] != x[j];
-  }
-  block_first(m, at, shx, shi);
-  nan = __syncthreads_or(nan);
-  double sum = 0.0;
-  for (int j = threadIdx.x; j < V; j += kThreads) sum += exp((double)x[j] - (double)m);
-  sum = fg_wave_sum_d(sum);
-  if ((threadIdx.x & 63) == 0) shd[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  sum = 0.0;
-  for (int w = 0; w < kWaves; ++w) sum += shd[w];
-  double base = (double)scores[b] - ((double)m + log(sum));
-  if (nan || m == INFINITY) base = NAN;
-  else if (m == -INFINITY) base = -INFINITY;
-  const bool flat = !(fabs(base) < INFINITY);  // all candidates are `base`
-  float px = 0.f;
-  int pi = -1;
+  // too many equals to list: one after the other
+  ulonglong2 prev = make_ulonglong2(~0ull, ~0ull);
   for (int w = 0; w < W; ++w) {
-    float bx = 0.f;
-    int bi = kNone;
-    for (int j = threadIdx.x; j < V; j += kThreads) {
-      const float y = flat ? 0.f : x[j];
-      if (pi >= 0 && !before(px, pi, y, j)) continue;
-      if (bi == kNone || before(y, j, bx, bi)) bx = y, bi = j;
+    ulonglong2 first = make_ulonglong2(0, 0);
+    for (int i = threadIdx.x; i < N; i += kThreads) {
+      candidate(i, k);
+      if (above(prev, k) && above(k, first)) first = k;
     }
-    block_first(bx, bi, shx, shi);
-    if (threadIdx.x == 0) {
-      val[w] = flat ? base : base + (double)bx;
-      tok[w] = bi;
-    }
-    if (bi == kNone) {
-      for (int i = w + 1 + threadIdx.x; i < W; i += kThreads) tok[i] = kNone;
-      return;
-    }
-    px = bx, pi = bi;
-  }
-}
-
-// One wave per request, a lane per beam: the greatest head of the beams' sorted
-// lists, W times.
-__global__ void __launch_bounds__(64) beam_merge_kernel(float* __restrict__ score_out, int32_t* __restrict__ token,
-                                                        int32_t* __restrict__ parent, int32_t* __restrict__ done_out,
-                                                        const double* __restrict__ val, const int32_t* __restrict__ tok,
-                                                        const int32_t* __restrict__ done, int eos, int W) {
-  const int lane = threadIdx.x;
-  const int64_t r0 = (int64_t)blockIdx.x * W;
-  const bool on = lane < W;
-  const double* vs = val + (r0 + lane) * W;
-  const int32_t* ts = tok + (r0 + lane) * W;
-  const int fin = on && done ? done[r0 + lane] != 0 : 0;
-  int at = 0, mine = on ? ts[0] : kNone;
-  double v = on ? vs[0] : 0.0;
-  for (int w = 0; w < W; ++w) {
-    double best = v;
-    int beam = mine == kNone ? kNone : lane;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-      const double y = __shfl_xor(best, o, 64);
-      const int j = __shfl_xor(beam, o, 64);
-      if (beam == kNone || (j != kNone && before(y, j, best, beam))) best = y, beam = j;
+      const ulonglong2 u = make_ulonglong2(__shfl_xor(first.x, o, 64), __shfl_xor(first.y, o, 64));
+      if (above(u, first)) first = u;
     }
-    if (beam == lane) {
-      score_out[r0 + w] = (float)v;
-      token[r0 + w] = mine;
-      parent[r0 + w] = lane;
-      if (done_out) done_out[r0 + w] = fin || mine == eos;
-      ++at;
-      mine = at < W ? ts[at] : kNone;
-      v = at < W ? vs[at] : 0.0;
-    }
+    __syncthreads();
+    if (lane == 0) list[wave] = first;
+    __syncthreads();
+    first = list[0];
+    for (int z = 1; z < kWaves; ++z)
+      if (above(list[z], first)) first = list[z];
+    if (threadIdx.x == 0) put(w, first);
+    prev = first;
   }
 }
 
@@ -203,23 +374,37 @@ extern "C" int fg_beam_select(float* score_out, int32_t* token, int32_t* parent,
                               const float* logits, int64_t ld, const float* scores, const int32_t* done, int eos,
                               int nReq, int W, int V) {
   FG_ARG_CHECK(score_out && token && parent && logits && scores, "fg_beam_select: null argument");
-  FG_ARG_CHECK(nReq > 0 && V > 0 && W >= 1 && W <= kMaxBeams && nReq <= INT32_MAX / kThreads / W,
+  FG_ARG_CHECK(nReq > 0 && V > 0 && W >= 1 && W <= kMaxBeams && nReq <= 65535 / W,
                "fg_beam_select: bad dimensions: %d requests, %d beams (1 to %d), vocabulary %d", nReq, W, kMaxBeams, V);
   FG_ARG_CHECK(ld >= V, "fg_beam_select: row stride %lld is below the vocabulary %d", (long long)ld, V);
   FG_ARG_CHECK(!done == !done_out, "fg_beam_select: done and done_out go together");
   FG_ARG_CHECK(eos < V, "fg_beam_select: eos %d outside the vocabulary %d", eos, V);
   FG_ARG_CHECK(!done || eos >= 0, "fg_beam_select: done needs eos");
-  const int rows = nReq * W;
+  FG_ARG_CHECK(V <= 1 << kTokenBits, "fg_beam_select: vocabulary %d is above %d", V, 1 << kTokenBits);
   FG_REQUIRE_INIT();
+  const int rows = nReq * W;
   fg::KProfScope prof("beam_select", 0.0, 4.0 * rows * V);
+  // segments of 1024 to 8192 logits, about 1024 of them
+  int64_t S = (V + 1023) / 1024, least = (V + 8191) / 8192, want = (1024 + rows - 1) / rows;
+  if (S > want) S = want > least ? want : least;
+  const int per = (int)((V + S - 1) / S), P = per <= 1024 ? 1 : per <= 2048 ? 2 : per <= 4096 ? 4 : 8;
+  const int length = (per + 3) / 4 * 4;
+  S = (V + length - 1) / length;
   fg::Workspace ws;
-  const int rc = ws.get((size_t)rows * W * (sizeof(double) + sizeof(int32_t)));
+  const int rc = ws.get((size_t)rows * S * (sizeof(float2) + W * sizeof(uint2)));
   if (rc != FG_OK) return rc;
-  double* val = (double*)ws.ptr;
-  int32_t* tok = (int32_t*)(val + (int64_t)rows * W);
-  FG_LAUNCH(beam_row_kernel, dim3(rows), dim3(kThreads), 0, val, tok, logits, ld, scores, done, eos, W, V);
-  FG_LAUNCH(beam_merge_kernel, dim3(nReq), dim3(64), 0, score_out, token, parent, done_out, (const double*)val,
-            (const int32_t*)tok, done, eos, W);
+  float2* sums = (float2*)ws.ptr;
+  uint2* cand = (uint2*)(sums + rows * S);
+  const dim3 grid((unsigned)S, (unsigned)rows);
+#define SEGMENT(PS) \
+  FG_LAUNCH(beam_segment_kernel<PS>, grid, dim3(kThreads), 0, sums, cand, logits, ld, done, W, V, length)
+  if (P == 1) SEGMENT(1);
+  else if (P == 2) SEGMENT(2);
+  else if (P == 4) SEGMENT(4);
+  else SEGMENT(8);
+#undef SEGMENT
+  FG_LAUNCH(beam_pick_kernel, dim3(nReq), dim3(kThreads), 0, score_out, token, parent, done_out, (const float2*)sums,
+            (const uint2*)cand, scores, done, eos, W, V, (int)S);
   return FG_OK;
 }
 

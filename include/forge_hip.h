@@ -723,7 +723,7 @@ int fg_kv4_evict(const fg_kv4_cache* c, int budget, int recent);
  * less the log of its sum is otherwise not finite V candidates of that value; NaN
  * comes after all others.  Candidates compare in
  * fp64 across beams, by their logits within one.  logits rows have stride ld;
- * 1 <= W <= 64, outputs apart from the inputs. */
+ * 1 <= W <= 64, nReq W <= 65535, V <= 2^26; outputs apart from the inputs. */
 int fg_beam_select(float* score_out, int32_t* token, int32_t* parent, int32_t* done_out, const float* logits,
                    int64_t ld, const float* scores, const int32_t* done, int eos, int nReq, int W, int V);
 /* A state of every beam: `rows` rows of row_bytes (even) for each of outer x inner

@@ -105,9 +105,10 @@ def test_bad_eviction_and_beams_are_refused():
     ok = [A, A, A, A, A, 100, A, A, 2, 2, 4, 100]
     for i in (0, 1, 2, 4, 6):
         refused("beam_select", *(ok[:i] + [None] + ok[i + 1:]), says="null")
-    for i, bad in ((9, 0), (10, 0), (10, 65), (11, 0)):
+    for i, bad in ((9, 0), (10, 0), (10, 65), (11, 0), (9, 32768)):
         refused("beam_select", *(ok[:i] + [bad] + ok[i + 1:]), says="dimensions")
     refused("beam_select", *(ok[:5] + [99] + ok[6:]), says="stride")
+    refused("beam_select", *(ok[:5] + [1 << 27] + ok[6:11] + [(1 << 26) + 1]), says="vocabulary")
     refused("beam_select", *(ok[:3] + [None] + ok[4:]), says="together")
     refused("beam_select", *(ok[:7] + [None] + ok[8:]), says="together")
     refused("beam_select", *(ok[:8] + [100] + ok[9:]), says="eos")
