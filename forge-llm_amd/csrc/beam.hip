@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
                                                                 const int32_t* __restrict__ done, int W, int V,
                                                                 int length) {
   constexpr int E = 4 * P;
-  __shared__ uint32_t best[kThreads];
+  __shared__ uint32_t best[kThreads], bound;
   __shared__ uint2 list[kListed];
   __shared__ float shm[kWaves], shs[kWaves];
   __shared__ int shn[kWaves], listed;
@@ -99,21 +99,29 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
     }
   }
   if (threadIdx.x == 0) listed = 0;
-  float m = v[0];
+  float most = v[0];
 #pragma unroll
-  for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
-  m = fg_wave_max(m);
-  if (lane == 0) shm[wave] = m;
-  uint32_t key[E], mine = 0;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int at = 4 * ((int)threadIdx.x + (e >> 2) * kThreads) + (e & 3);
-    key[e] = at < n ? key_of(v[e]) : 0u;
-    mine = max(mine, key[e]);
-  }
+  for (int e = 1; e < E; ++e) most = fmaxf(most, v[e]);
+  const uint32_t mine = 4 * (int)threadIdx.x < n ? key_of(most) : 0u;
   best[threadIdx.x] = mine;
+  float m = fg_wave_max(most);
+  if (lane == 0) shm[wave] = m;
   __syncthreads();
   for (int w = 0; w < kWaves; ++w) m = fmaxf(m, shm[w]);
+  if (wave == 0) {
+    // the W-th greatest of the threads' maxima, its low bits dropped
+    uint32_t b[kWaves], t = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) b[w] = best[w * 64 + lane];
+    for (int bit = 31; bit >= 14; --bit) {
+      const uint32_t u = t | (1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) c += __popcll(__ballot(b[w] >= u));
+      if (c >= W) t = u;
+    }
+    if (lane == 0) bound = t;
+  }
   // exp(x - m) in fp32: good to 2^-21 where it counts
   const float from = m == -INFINITY ? 0.f : m;
   float s = 0.f;
@@ -121,30 +129,32 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
   for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - from) * 1.44269504088896340736f);
   s = fg_wave_sum(s);
   if (lane == 0) shs[wave] = s;
-  // the W-th greatest of the threads' maxima, its low 12 bits dropped
-  uint32_t b[kWaves], border = 0;
+  __syncthreads();
+  uint32_t border = bound;
+  const float least = value_of(border);
+  // where W threads have numbers above -inf, the values from `least` on are
+  // enough; else all of the segment are candidates
+  const bool few = border > key_of(-INFINITY);
+  if (!few || mine >= border) {
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) b[w] = best[w * 64 + lane];
-  for (int bit = 31; bit >= 12; --bit) {
-    const uint32_t t = border | (1u << bit);
-    int c = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) c += __popcll(__ballot(b[w] >= t));
-    if (c >= W) border = t;
-  }
-  border = max(border, 1u);
-  if (mine >= border) {
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (key[e] >= border) {
+    for (int e = 0; e < E; ++e) {
+      const int at = 4 * ((int)threadIdx.x + (e >> 2) * kThreads) + (e & 3);
+      if (few ? v[e] >= least : at < n) {
         const int i = atomicAdd(&listed, 1);
-        if (i < kListed) list[i] = make_uint2(key[e], 4 * (threadIdx.x + (e >> 2) * kThreads) + (e & 3));
+        if (i < kListed) list[i] = make_uint2(key_of(v[e]), at);
       }
+    }
   }
   __syncthreads();
   int c = listed;
   if (c > kListed) {  // the same for all threads
     int last;
+    uint32_t key[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int at = 4 * ((int)threadIdx.x + (e >> 2) * kThreads) + (e & 3);
+      key[e] = at < n ? key_of(v[e]) : 0u;
+    }
     exact_border<E>(border, last, key, W, shn);
     __syncthreads();
     if (threadIdx.x == 0) listed = 0;
@@ -185,7 +195,8 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
 // One workgroup per request.  A candidate's second key orders those of equal
 // value: the lower beam, within it the greater logit, then the lower token.
 constexpr int kTokenBits = 26;
-__global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__ score_out, int32_t* __restrict__ token,
+constexpr int kPick = 512, kPickWaves = kPick / 64, kHeld = 4;
+__global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ score_out, int32_t* __restrict__ token,
                                                              int32_t* __restrict__ parent, int32_t* __restrict__ done_out,
                                                              const float2* __restrict__ sums,
                                                              const uint2* __restrict__ cand,
@@ -195,11 +206,18 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__
   __shared__ double base[kMaxBeams];
   __shared__ int kind[kMaxBeams];  // 0: its candidates, 1: all equal to base, 2: done
   __shared__ ulonglong2 list[kListed];
-  __shared__ unsigned long long border[kWaves];
+  __shared__ unsigned long long border[kPickWaves];
   __shared__ int listed;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r0 = (int64_t)blockIdx.x * W;
-  for (int b = wave; b < W; b += kWaves) {
+  const int each = S * W, N = W * each;
+  uint2 held[kHeld];  // a thread's first candidates, fetched beside the sums
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h) {
+    const int i = threadIdx.x + h * kPick;
+    if (i < N) held[h] = cand[r0 * each + i];
+  }
+  for (int b = wave; b < W; b += kPickWaves) {
     const bool fin = done && done[r0 + b];
     float m = -INFINITY;
     double s = 0.0;
@@ -207,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__
       const float2* row = sums + (r0 + b) * S;
       for (int z = lane; z < S; z += 64) m = fmaxf(m, row[z].x);
       m = fg_wave_max(m);
-      for (int z = lane; z < S; z += 64) s += (double)row[z].y * (row[z].x == m ? 1.0 : exp((double)row[z].x - (double)m));
+      for (int z = lane; z < S; z += 64) s += (double)row[z].y * (row[z].x == m ? 1.f : __builtin_amdgcn_exp2f((row[z].x - m) * 1.44269504088896340736f));
       s = fg_wave_sum_d(s);
     }
     if (lane == 0) {
@@ -219,22 +237,20 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__
   }
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
-  const int each = S * W, N = W * each;
-  auto candidate = [&](int i, ulonglong2& k) {
+  auto candidate = [&](int i, uint2 c, ulonglong2& k) {
     const int b = i / each, j = i - b * each;
-    uint2 c = make_uint2(1u, (uint32_t)j);  // all equal: the first W tokens
     k = make_ulonglong2(0, 0);
     if (kind[b] == 0) {
-      c = cand[r0 * each + i];
       if (c.x == 0) return;
       k.x = key_of(base[b] + (double)value_of(c.x));
     } else if (kind[b] == 1) {
-      if (j >= W || j >= V) return;
+      if (j >= W || j >= V) return;  // all equal: the first W tokens
       k.x = key_of(base[b]);
+      c = make_uint2(1u, (uint32_t)j);
     } else {
       if (j != 0) return;
       k.x = key_of(base[b]);
-      c.y = eos;
+      c = make_uint2(1u, (uint32_t)eos);
     }
     k.y = ((uint64_t)(kMaxBeams - 1 - b) << (32 + kTokenBits)) | ((uint64_t)c.x << kTokenBits) |
           ((1u << kTokenBits) - 1 - c.y);
@@ -248,10 +264,17 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__
     if (done_out) done_out[r0 + rank] = kind[b] == 2 || t == eos;
   };
   auto above = [](const ulonglong2& a, const ulonglong2& b) { return a.x > b.x || (a.x == b.x && a.y > b.y); };
-  ulonglong2 k;
+  ulonglong2 k, kept[kHeld];
   uint64_t mine = 0;
-  for (int i = threadIdx.x; i < N; i += kThreads) {
-    candidate(i, k);
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h) {
+    const int i = threadIdx.x + h * kPick;
+    kept[h] = make_ulonglong2(0, 0);
+    if (i < N) candidate(i, held[h], kept[h]);
+    mine = kept[h].x > mine ? kept[h].x : mine;
+  }
+  for (int i = threadIdx.x + kHeld * kPick; i < N; i += kPick) {
+    candidate(i, cand[r0 * each + i], k);
     mine = k.x > mine ? k.x : mine;
   }
   // each wave's W-th greatest of its lanes' maxima (high word); the greatest of them
@@ -263,19 +286,24 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__
   if (lane == 0) border[wave] = (uint64_t)t32 << 32;
   __syncthreads();
   uint64_t least = 1;
-  for (int w = 0; w < kWaves; ++w) least = border[w] > least ? border[w] : least;
-  if (mine >= least)
-    for (int i = threadIdx.x; i < N; i += kThreads) {
-      candidate(i, k);
-      if (k.x >= least) {
-        const int at = atomicAdd(&listed, 1);
-        if (at < kListed) list[at] = k;
-      }
+  for (int w = 0; w < kPickWaves; ++w) least = border[w] > least ? border[w] : least;
+  auto note = [&](const ulonglong2& k) {
+    if (k.x < least) return;
+    const int at = atomicAdd(&listed, 1);
+    if (at < kListed) list[at] = k;
+  };
+  if (mine >= least) {
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) note(kept[h]);
+    for (int i = threadIdx.x + kHeld * kPick; i < N; i += kPick) {
+      candidate(i, cand[r0 * each + i], k);
+      note(k);
     }
+  }
   __syncthreads();
   const int c = listed;
   if (c <= kListed) {
-    for (int i = threadIdx.x; i < c; i += kThreads) {
+    for (int i = threadIdx.x; i < c; i += kPick) {
       k = list[i];
       int rank = 0;
       for (int j = 0; j < c; ++j) rank += above(list[j], k);
@@ -287,8 +315,8 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__
   ulonglong2 prev = make_ulonglong2(~0ull, ~0ull);
   for (int w = 0; w < W; ++w) {
     ulonglong2 first = make_ulonglong2(0, 0);
-    for (int i = threadIdx.x; i < N; i += kThreads) {
-      candidate(i, k);
+    for (int i = threadIdx.x; i < N; i += kPick) {
+      candidate(i, cand[r0 * each + i], k);
       if (above(prev, k) && above(k, first)) first = k;
     }
 #pragma unroll
@@ -300,7 +328,7 @@ __global__ void __launch_bounds__(kThreads) beam_pick_kernel(float* __restrict__
     if (lane == 0) list[wave] = first;
     __syncthreads();
     first = list[0];
-    for (int z = 1; z < kWaves; ++z)
+    for (int z = 1; z < kPickWaves; ++z)
       if (above(list[z], first)) first = list[z];
     if (threadIdx.x == 0) put(w, first);
     prev = first;
@@ -403,7 +431,7 @@ extern "C" int fg_beam_select(float* score_out, int32_t* token, int32_t* parent,
   else if (P == 4) SEGMENT(4);
   else SEGMENT(8);
 #undef SEGMENT
-  FG_LAUNCH(beam_pick_kernel, dim3(nReq), dim3(kThreads), 0, score_out, token, parent, done_out, (const float2*)sums,
+  FG_LAUNCH(beam_pick_kernel, dim3(nReq), dim3(kPick), 0, score_out, token, parent, done_out, (const float2*)sums,
             (const uint2*)cand, scores, done, eos, W, V, (int)S);
   return FG_OK;
 }
