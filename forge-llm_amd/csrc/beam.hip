@@ -134,12 +134,12 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
   const float least = value_of(border);
   // where W threads have numbers above -inf, the values from `least` on are
   // enough; else all of the segment are candidates
-  const bool few = border > key_of(-INFINITY);
-  if (!few || mine >= border) {
+  const bool bounded = border > key_of(-INFINITY);
+  if (!bounded || mine >= border) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int at = 4 * ((int)threadIdx.x + (e >> 2) * kThreads) + (e & 3);
-      if (few ? v[e] >= least : at < n) {
+      if (bounded ? v[e] >= least : at < n) {
         const int i = atomicAdd(&listed, 1);
         if (i < kListed) list[i] = make_uint2(key_of(v[e]), at);
       }

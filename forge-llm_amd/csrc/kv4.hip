@@ -591,7 +591,270 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelect = 1024;
+constexpr int kSelect = 1024, kSelectWaves = kSelect / 64;
+constexpr int kBins = 2 * kSelect;
+
+// The sum of x over the workgroup's later threads; `all` gets the sum of all.
+__device__ __forceinline__ int sum_after(int x, int* sh, int& all) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int s = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_down(s, o, 64);
+    if (lane + o < 64) s += u;
+  }
+  __syncthreads();
+  if (lane == 0) sh[w] = s;
+  __syncthreads();
+  s -= x;
+  all = 0;
+  for (int i = 0; i < kSelectWaves; ++i) {
+    all += sh[i];
+    if (i > w) s += sh[i];
+  }
+  return s;
+}
+__device__ __forceinline__ uint32_t block_extreme(uint32_t x, bool greatest, uint32_t* sh) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t u = __shfl_xor(x, o, 64);
+    x = greatest ? max(x, u) : min(x, u);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
+  __syncthreads();
+  for (int i = 0; i < kSelectWaves; ++i) x = greatest ? max(x, sh[i]) : min(x, sh[i]);
+  return x;
+}
+
+// One workgroup per head, its keys in registers (4 Q a thread, read once).  The
+// keys' range is cut into up to 2048 bins by their leading bits, the bin that the
+// budget ends in is found from the counts, and its keys, a few, are ranked by
+// counting; a bin of more keys is cut again, unless they are all equal.  Weights
+// spread over many powers of two, so a histogram of keys is flat where one of
+// the exponent byte piles up (256 heads of 16384 slots: four passes of 8 bits
+// took 93 us).
+template <int Q>
+__global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restrict__ holes,
+                                                               int32_t* __restrict__ movers,
+                                                               int32_t* __restrict__ moves,
+                                                               const float* __restrict__ weight,
+                                                               const int32_t* __restrict__ pos,
+                                                               const int32_t* __restrict__ len,
+                                                               const int32_t* __restrict__ next, int nSeq, int nHeads,
+                                                               int maxSeq, int budget, int recent, int most) {
+  __shared__ int bins[kBins], sh[kSelectWaves], pick[3];
+  __shared__ uint32_t shu[kSelectWaves];
+  __shared__ uint2 list[kSelect];
+  __shared__ uint64_t tab[Q * kSelectWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t head = blockIdx.x;
+  const int s = (int)(head / nHeads % nSeq);
+  const int n = min(max(len[s], 0), maxSeq);
+  const int64_t safe = (int64_t)next[s] - recent;
+  weight += head * maxSeq;
+  pos += head * maxSeq;
+  holes += head * most;
+  movers += head * most;
+  int moved = 0;
+  if (n > budget) {
+    constexpr uint32_t kSafe = 0xFFFFFFFFu;
+    uint32_t key[Q][4];
+    int safes = 0;
+    uint32_t lo = kSafe, hi = 0;
+    {
+      float w[Q][4];
+      int p[Q][4];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int at = 4 * ((int)threadIdx.x + q * kSelect);
+        if (at + 4 <= n) {
+          __builtin_memcpy(w[q], weight + at, 16);
+          __builtin_memcpy(p[q], pos + at, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[q][e] = at + e < n ? weight[at + e] : 0.f;
+            p[q][e] = at + e < n ? pos[at + e] : 0;
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = 4 * ((int)threadIdx.x + q * kSelect) + e < n;
+          const bool keep = (int64_t)p[q][e] >= safe;
+          key[q][e] = keep ? kSafe : weight_key(w[q][e]);
+          safes += in && keep;
+          if (in && !keep) {
+            lo = min(lo, key[q][e]);
+            hi = max(hi, key[q][e]);
+          }
+        }
+    }
+    int all;
+    sum_after(safes, sh, all);
+    int want = budget - all;  // of the keys in [lo, hi]
+    uint32_t border = kSafe;  // kept: above `border`, or equal to it up to slot `last`
+    int last = n;
+    if (want > 0) {
+      lo = block_extreme(lo, false, shu);
+      hi = block_extreme(hi, true, shu);
+      for (;;) {
+        if (lo == hi) {
+          border = lo;
+          last = -1;  // by rank, below
+          break;
+        }
+        const int shift = max(0, 21 - (int)__builtin_clz(hi - lo));
+        for (int i = threadIdx.x; i < kBins; i += kSelect) bins[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (4 * ((int)threadIdx.x + q * kSelect) + e < n && key[q][e] >= lo && key[q][e] <= hi)
+              atomicAdd(&bins[(key[q][e] - lo) >> shift], 1);
+        __syncthreads();
+        const int b0 = bins[2 * threadIdx.x], b1 = bins[2 * threadIdx.x + 1];
+        const int after = sum_after(b0 + b1, sh, all);
+        if (after < want && want <= after + b0 + b1) {
+          const bool upper = want <= after + b1;
+          pick[0] = 2 * threadIdx.x + upper;
+          pick[1] = want - after - (upper ? 0 : b1);
+          pick[2] = 0;
+        }
+        __syncthreads();
+        const uint32_t from = lo + ((uint32_t)pick[0] << shift);
+        const uint32_t to = min(hi, from + ((1u << shift) - 1));
+        want = pick[1];
+        lo = kSafe;
+        hi = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = 4 * ((int)threadIdx.x + q * kSelect) + e;
+            if (at < n && key[q][e] >= from && key[q][e] <= to) {
+              const int i = atomicAdd(&pick[2], 1);
+              if (i < kSelect) list[i] = make_uint2(key[q][e], (uint32_t)at);
+              lo = min(lo, key[q][e]);
+              hi = max(hi, key[q][e]);
+            }
+          }
+        __syncthreads();
+        const int c = pick[2];
+        if (c <= kSelect) {
+          if ((int)threadIdx.x < c) {
+            const uint2 me = list[threadIdx.x];
+            int rank = 0;
+            for (int i = 0; i < c; ++i) {
+              const uint2 o = list[i];
+              rank += o.x > me.x || (o.x == me.x && o.y < me.y);
+            }
+            if (rank == want - 1) {
+              pick[0] = (int)me.x;
+              pick[1] = (int)me.y;
+            }
+          }
+          __syncthreads();
+          border = (uint32_t)pick[0];
+          last = pick[1];
+          break;
+        }
+        lo = block_extreme(lo, false, shu);
+        hi = block_extreme(hi, true, shu);
+      }
+    }
+    // the number of flagged slots before each of a thread's, by slot order: counts
+    // of (group of 4 Q, wave) summed up in a table, two flags at a time
+    uint64_t before[Q];
+    auto rank_flags = [&](auto flags) {  // flags(q, e): bit 0 and bit 1
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        int mine0 = 0, mine1 = 0, all0 = 0, all1 = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int f = flags(q, e);
+          const unsigned long long b0 = __ballot(f & 1), b1 = __ballot(f & 2), low = (1ull << lane) - 1;
+          mine0 += __popcll(b0 & low);
+          mine1 += __popcll(b1 & low);
+          all0 += __popcll(b0);
+          all1 += __popcll(b1);
+        }
+        before[q] = (uint64_t)mine0 | (uint64_t)mine1 << 32;
+        if (lane == 0) tab[q * kSelectWaves + wave] = (uint64_t)all0 | (uint64_t)all1 << 32;
+      }
+      __syncthreads();
+      if (wave == 0) {
+        constexpr int each = (Q * kSelectWaves + 63) / 64;
+        uint64_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < each; ++i) {
+          const int k = lane * each + i;
+          if (k < Q * kSelectWaves) mine += tab[k];
+        }
+        uint64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const uint64_t u = __shfl_up((unsigned long long)upto, o, 64);
+          if (lane >= o) upto += u;
+        }
+        upto -= mine;
+#pragma unroll
+        for (int i = 0; i < each; ++i) {
+          const int k = lane * each + i;
+          if (k < Q * kSelectWaves) {
+            const uint64_t t = tab[k];
+            tab[k] = upto;
+            upto += t;
+          }
+        }
+        if (lane == 63) pick[2] = (int)(uint32_t)upto;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < Q; ++q) before[q] += tab[q * kSelectWaves + wave];
+    };
+    if (last < 0) {  // the want-th of the equals, in slot order
+      auto equal = [&](int q, int e) {
+        return 4 * ((int)threadIdx.x + q * kSelect) + e < n && key[q][e] == border ? 1 : 0;
+      };
+      rank_flags(equal);
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        int rank = (int)(uint32_t)before[q];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (equal(q, e) && ++rank == want) pick[1] = 4 * ((int)threadIdx.x + q * kSelect) + e;
+      }
+      __syncthreads();
+      last = pick[1];
+    }
+    auto place = [&](int q, int e) {  // 1: a hole, 2: a mover
+      const int at = 4 * ((int)threadIdx.x + q * kSelect) + e;
+      const bool kept = key[q][e] > border || (key[q][e] == border && at <= last);
+      return at >= n ? 0 : at < budget ? (kept ? 0 : 1) : kept ? 2 : 0;
+    };
+    rank_flags(place);
+    moved = pick[2];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      int h = (int)(uint32_t)before[q], m = (int)(before[q] >> 32);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int f = place(q, e), at = 4 * ((int)threadIdx.x + q * kSelect) + e;
+        if (f == 1 && h < most) holes[h++] = at;
+        if (f == 2 && m < most) movers[m++] = at;
+      }
+    }
+  }
+  for (int i = moved + (int)threadIdx.x; i < most; i += kSelect) holes[i] = movers[i] = -1;
+  if (threadIdx.x == 0) moves[head] = moved;
+}
+
 // The number of `in` flags of the workgroup's earlier threads; `all` gets the
 // number of all.
 __device__ __forceinline__ int block_rank(bool in, int* sh, int& all) {
@@ -609,9 +872,9 @@ __device__ __forceinline__ int block_rank(bool in, int* sh, int& all) {
   return before;
 }
 
-// One workgroup per head: the budget-th greatest key by four passes of 8 bits
+// The same for heads of more slots than the registers hold: four passes of 8 bits
 // over the keys, then the lists in slot order.
-__global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restrict__ holes,
+__global__ void __launch_bounds__(kSelect) evict_select_long_kernel(int32_t* __restrict__ holes,
                                                                int32_t* __restrict__ movers,
                                                                int32_t* __restrict__ moves,
                                                                const float* __restrict__ weight,
@@ -641,11 +904,11 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
         if (shift == 24 || (u >> (shift + 8)) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1);
       }
       __syncthreads();
-      if (threadIdx.x == 0) {
-        int i = 255, left = want;
-        while (i > 0 && hist[i] < left) left -= hist[i--];
-        pick[0] = i;
-        pick[1] = left;
+      int all;
+      const int mine = threadIdx.x < 256 ? hist[threadIdx.x] : 0, after = sum_after(mine, sh, all);
+      if (after < want && want <= after + mine) {
+        pick[0] = threadIdx.x;
+        pick[1] = want - after;
       }
       __syncthreads();
       prefix = (prefix << 8) | (uint32_t)pick[0];
@@ -673,33 +936,44 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
   if (threadIdx.x == 0) moves[head] = nm;
 }
 
+// The moves, sixteen lanes each, and the new lengths (which the selection has
+// read by now).
+template <int NB>
 __global__ void __launch_bounds__(kThreads) kv4_move_kernel(Cache c, const int32_t* __restrict__ holes,
                                                             const int32_t* __restrict__ movers,
-                                                            const int32_t* __restrict__ moves, int most, int row,
-                                                            int nb) {
+                                                            const int32_t* __restrict__ moves, int most, int budget) {
   const int64_t head = blockIdx.x;
+  if (blockIdx.y == 0 && head < c.nSeq && threadIdx.x == 0) c.len[head] = min(slots_used(c, head), budget);
+  const int n = moves[head], l = threadIdx.x & 15;
   const int64_t slot0 = head * c.maxSeq;
-  const int n = moves[head];
-  for (int i = threadIdx.x >> 6; i < n; i += kWaves) {
+  uint4 *k = reinterpret_cast<uint4*>(c.k), *v = reinterpret_cast<uint4*>(c.v);
+  for (int i = blockIdx.y * (kThreads / 16) + (threadIdx.x >> 4); i < n; i += gridDim.y * (kThreads / 16)) {
     const int64_t to = slot0 + holes[head * most + i], from = slot0 + movers[head * most + i];
-    for (int b = threadIdx.x & 63; b < row; b += 64) {
-      c.k[to * row + b] = c.k[from * row + b];
-      c.v[to * row + b] = c.v[from * row + b];
+    uint4 row;
+    if (l < NB) row = k[from * NB + l];
+    else if (l < 2 * NB) row = v[from * NB + l - NB];
+    _Float16 a, b;
+    if (l < NB) {
+      a = c.kd[from * NB + l];
+      b = c.vd[from * NB + l];
     }
-    for (int b = threadIdx.x & 63; b < nb; b += 64) {
-      c.kd[to * nb + b] = c.kd[from * nb + b];
-      c.vd[to * nb + b] = c.vd[from * nb + b];
+    float w;
+    int p;
+    if (l == 0) {
+      w = c.weight[from];
+      p = c.pos[from];
     }
-    if ((threadIdx.x & 63) == 0) {
-      c.weight[to] = c.weight[from];
-      c.pos[to] = c.pos[from];
+    if (l < NB) k[to * NB + l] = row;
+    else if (l < 2 * NB) v[to * NB + l - NB] = row;
+    if (l < NB) {
+      c.kd[to * NB + l] = a;
+      c.vd[to * NB + l] = b;
+    }
+    if (l == 0) {
+      c.weight[to] = w;
+      c.pos[to] = p;
     }
   }
-}
-
-__global__ void kv4_cut_kernel(Cache c, int budget) {
-  const int s = blockIdx.x * kThreads + threadIdx.x;
-  if (s < c.nSeq) c.len[s] = min(slots_used(c, s), budget);
 }
 
 __global__ void kv4_follow_kernel(int32_t* __restrict__ len, int32_t* __restrict__ next,
@@ -865,8 +1139,15 @@ extern "C" int fg_kv_evict_select(int32_t* holes, int32_t* movers, int32_t* move
   const int heads = nLayers * nSeq * nHeads, most = budget < maxSeq - budget ? budget : maxSeq - budget;
   FG_REQUIRE_INIT();
   fg::KProfScope prof("kv_evict_select", 0.0, (double)heads * (8.0 * maxSeq + 8.0 * most));
-  FG_LAUNCH(evict_select_kernel, dim3(heads), dim3(kSelect), 0, holes, movers, moves, weight, pos, len, next, nSeq,
-            nHeads, maxSeq, budget, recent, most);
+#define EVICT_SELECT(kernel)                                                                                    \
+  FG_LAUNCH((kernel), dim3(heads), dim3(kSelect), 0, holes, movers, moves, weight, pos, len, next, nSeq, nHeads, \
+            maxSeq, budget, recent, most)
+  if (maxSeq <= 4 * kSelect) EVICT_SELECT(evict_select_kernel<1>);
+  else if (maxSeq <= 8 * kSelect) EVICT_SELECT(evict_select_kernel<2>);
+  else if (maxSeq <= 16 * kSelect) EVICT_SELECT(evict_select_kernel<4>);
+  else if (maxSeq <= 32 * kSelect) EVICT_SELECT(evict_select_kernel<8>);
+  else EVICT_SELECT(evict_select_long_kernel);
+#undef EVICT_SELECT
   return FG_OK;
 }
 
@@ -884,9 +1165,10 @@ extern "C" int fg_kv4_evict(const fg_kv4_cache* c, int budget, int recent) {
   KV4_TRY(fg_kv_evict_select(holes, movers, moves, c->weight, c->pos, c->len, c->next, c->nLayers, c->nSeq, c->nKvHeads,
                              c->maxSeq, budget, recent));
   fg::KProfScope prof("kv4_evict", 0.0, (double)c->nLayers * c->nSeq * most * 2 * slot_bytes(c));
-  FG_LAUNCH(kv4_move_kernel, dim3(heads), dim3(kThreads), 0, view(c), (const int32_t*)holes, (const int32_t*)movers,
-            (const int32_t*)moves, most, c->dHead / 2, c->dHead / 32);
-  FG_LAUNCH(kv4_cut_kernel, dim3((c->nSeq + kThreads - 1) / kThreads), dim3(kThreads), 0, view(c), budget);
+  const int want = (most + kThreads / 16 - 1) / (kThreads / 16), fit = (4096 + heads - 1) / heads;
+  const dim3 grid(heads, want < fit ? want : fit);
+  KV4_DISPATCH(c->dHead, FG_LAUNCH(kv4_move_kernel<NB>, grid, dim3(kThreads), 0, view(c), (const int32_t*)holes,
+                                   (const int32_t*)movers, (const int32_t*)moves, most, budget));
   return FG_OK;
 }
 
