@@ -628,9 +628,9 @@ __device__ __forceinline__ uint32_t block_extreme(uint32_t x, bool greatest, uin
 }
 
 // One workgroup per head, its keys in registers (4 Q a thread, read once).  The
-// keys' range is cut into up to 2048 bins by their leading bits, the bin that the
-// budget ends in is found from the counts, and its keys, a few, are ranked by
-// counting; a bin of more keys is cut again, unless they are all equal.  Weights
+// keys' range is cut into up to 2048 bins by their leading bits and the bin that
+// the budget ends in is found from the counts; its keys, one a thread when they
+// are few enough, are cut again until they are equal.  Weights
 // spread over many powers of two, so a histogram of keys is flat where one of
 // the exponent byte piles up (256 heads of 16384 slots: four passes of 8 bits
 // took 93 us).
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
                                                                int maxSeq, int budget, int recent, int most) {
   __shared__ int bins[kBins], sh[kSelectWaves], pick[3];
   __shared__ uint32_t shu[kSelectWaves];
-  __shared__ uint2 list[kSelect];
+  __shared__ uint32_t list[kSelect];
   __shared__ uint64_t tab[Q * kSelectWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t head = blockIdx.x;
@@ -701,21 +701,15 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
     if (want > 0) {
       lo = block_extreme(lo, false, shu);
       hi = block_extreme(hi, true, shu);
-      for (;;) {
-        if (lo == hi) {
-          border = lo;
-          last = -1;  // by rank, below
-          break;
-        }
+      // the bin of [lo, hi] that the want-th greatest of its keys is in becomes
+      // [lo, hi], `want` counts inside it
+      auto narrow = [&](auto each_key) {
         const int shift = max(0, 21 - (int)__builtin_clz(hi - lo));
         for (int i = threadIdx.x; i < kBins; i += kSelect) bins[i] = 0;
         __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (4 * ((int)threadIdx.x + q * kSelect) + e < n && key[q][e] >= lo && key[q][e] <= hi)
-              atomicAdd(&bins[(key[q][e] - lo) >> shift], 1);
+        each_key([&](uint32_t u) {
+          if (u >= lo && u <= hi) atomicAdd(&bins[(u - lo) >> shift], 1);
+        });
         __syncthreads();
         const int b0 = bins[2 * threadIdx.x], b1 = bins[2 * threadIdx.x + 1];
         const int after = sum_after(b0 + b1, sh, all);
@@ -723,49 +717,45 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
           const bool upper = want <= after + b1;
           pick[0] = 2 * threadIdx.x + upper;
           pick[1] = want - after - (upper ? 0 : b1);
-          pick[2] = 0;
+          pick[2] = upper ? b1 : b0;
         }
         __syncthreads();
-        const uint32_t from = lo + ((uint32_t)pick[0] << shift);
-        const uint32_t to = min(hi, from + ((1u << shift) - 1));
+        lo += (uint32_t)pick[0] << shift;
+        hi = min(hi, lo + ((1u << shift) - 1));
         want = pick[1];
-        lo = kSafe;
-        hi = 0;
+        return pick[2];
+      };
+      int c = n;
+      while (lo != hi && c > kSelect)
+        c = narrow([&](auto take) {
+#pragma unroll
+          for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (4 * ((int)threadIdx.x + q * kSelect) + e < n) take(key[q][e]);
+        });
+      if (lo != hi) {
+        // few enough to hold one a thread
+        __syncthreads();
+        if (threadIdx.x == 0) pick[2] = 0;
+        __syncthreads();
 #pragma unroll
         for (int q = 0; q < Q; ++q)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int at = 4 * ((int)threadIdx.x + q * kSelect) + e;
-            if (at < n && key[q][e] >= from && key[q][e] <= to) {
-              const int i = atomicAdd(&pick[2], 1);
-              if (i < kSelect) list[i] = make_uint2(key[q][e], (uint32_t)at);
-              lo = min(lo, key[q][e]);
-              hi = max(hi, key[q][e]);
-            }
-          }
+          for (int e = 0; e < 4; ++e)
+            if (4 * ((int)threadIdx.x + q * kSelect) + e < n && key[q][e] >= lo && key[q][e] <= hi)
+              list[atomicAdd(&pick[2], 1) & (kSelect - 1)] = key[q][e];
         __syncthreads();
-        const int c = pick[2];
-        if (c <= kSelect) {
-          if ((int)threadIdx.x < c) {
-            const uint2 me = list[threadIdx.x];
-            int rank = 0;
-            for (int i = 0; i < c; ++i) {
-              const uint2 o = list[i];
-              rank += o.x > me.x || (o.x == me.x && o.y < me.y);
-            }
-            if (rank == want - 1) {
-              pick[0] = (int)me.x;
-              pick[1] = (int)me.y;
-            }
-          }
-          __syncthreads();
-          border = (uint32_t)pick[0];
-          last = pick[1];
-          break;
-        }
-        lo = block_extreme(lo, false, shu);
-        hi = block_extreme(hi, true, shu);
+        c = pick[2];
+        const uint32_t mine = (int)threadIdx.x < c ? list[threadIdx.x] : kSafe;
+        const int held = c;
+        while (lo != hi)
+          c = narrow([&](auto take) {
+            if ((int)threadIdx.x < held) take(mine);
+          });
       }
+      border = lo;
+      if (c != want) last = -1;  // not all of the equals: by rank, below
     }
     // the number of flagged slots before each of a thread's, by slot order: counts
     // of (group of 4 Q, wave) summed up in a table, two flags at a time
