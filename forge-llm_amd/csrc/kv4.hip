@@ -140,9 +140,10 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Cache c, int layer, 
 // values of its heads; p = 2^(x - ref) with ref = max - 15 + E, 2^E above every
 // step so far, so that w fills fp16's range, [0, 2^15).  max and E are only
 // raised, and the accumulators rescaled, when a score or step goes beyond
-// them: after the first positions hardly ever.  Rows beyond 2 group hold the
-// same heads again for the next blocks' steps (G heads: 8 / G blocks an
-// operand), so few heads need fewer w.
+// them: after the first positions hardly ever.  There are eight slots of two rows:
+// up to four heads (G) repeat, so that the scores of positions 0 .. 15 come out in
+// the lower eight rows and those of 16 .. 31 in the upper, one lane each, and
+// 8 / G blocks' steps share an operand of w.
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -169,6 +170,13 @@ __device__ __forceinline__ int pieces_of(int n, int per) { return max(1, (rounds
 // if there is no such piece.
 __device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t* count, int T, int heads, int id,
                                          bool by_seq) {
+  if (c.nSeq == 1) {
+    const int r = rounds_of(attended(c, count, 0, T));
+    p.per = (int)max((int64_t)1, ((int64_t)r * heads + kTarget - 1) / kTarget);
+    p.s = p.first = 0;
+    p.pieces = max(1, (r + p.per - 1) / p.per);
+    return by_seq || id < (int64_t)p.pieces * heads;
+  }
   const int lane = threadIdx.x & 63, each = (c.nSeq + 63) / 64, s0 = lane * each;
   int64_t rounds = 0;
   for (int i = 0; i < each && s0 + i < c.nSeq; ++i) rounds += rounds_of(attended(c, count, s0 + i, T));
@@ -223,52 +231,97 @@ __device__ __forceinline__ float half_of(uint32_t w, int i) {
 // 32 positions of a head's cache, as a lane of a wave holds them: lane
 // (i = lane & 15, g = lane >> 4) has values 4 g .. 4 g + 3 and 16 more on of every
 // block of positions i and 16 + i's keys, and values i and 16 + i of every block
-// of positions 8 g .. 8 g + 7, with the steps of the NA blocks of its row's set.
-template <int NB, int NA>
-struct Tile {
-  uint32_t k[2][NB];             // bytes j NB + b: value 4 g + j of block b
-  uint32_t kd[2][(NB + 1) / 2];  // the keys' steps
-  uint32_t v[8][(NB + 3) / 4];   // byte b
-  uint32_t vd[8][(NA + 1) / 2];  // the values' steps
-  uint32_t all[(NB + 3) / 4];    // all steps of the values, spread over the lanes
-  // bk, bv, dk, dv: the tile's first slot (uniform); `left` of its positions exist
-  // (1 or more), the rest repeat the last
+// of positions 4 e + g, e < 8: a load of the wave is a run of the array.  The
+// values' steps come in once, half a position's a lane.  Loads start at the tile's first slot (uniform); `left` of its positions exist
+// (1 or more), the rest repeat the last.
+template <bool Whole>
+__device__ __forceinline__ uint32_t tile_slot(int j, int left) {
+  return (uint32_t)(Whole ? j : min(j, left - 1));
+}
+template <int NB, bool Halves>
+struct KeyTile {
+  uint32_t k[2][NB];                          // bytes j NB + b: value 4 g + j of block b
+  uint32_t kd[Halves ? 1 : 2][(NB + 1) / 2];  // steps, of position 16 (g / 2) + i where halved
   template <bool Whole>
-  __device__ __forceinline__ void load(const uint8_t* bk, const uint8_t* bv, const uint8_t* dk, const uint8_t* dv,
-                                       int first_block, int left) {
+  __device__ __forceinline__ void load(const Cache& c, int64_t slot, int left) {
+    const uint8_t *bk = c.k + slot * (16 * NB), *dk = (const uint8_t*)(c.kd + slot * NB);
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    auto at = [&](int j) { return (uint32_t)(Whole ? j : min(j, left - 1)); };
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint32_t j = Whole ? i : at(16 * t + i), imm = Whole ? 16 * t : 0;
+      const uint32_t j = tile_slot<Whole>(Whole ? i : 16 * t + i, left), imm = Whole ? 16 * t : 0;
       load_bytes<4 * NB>(k[t], bk + (j * (16 * NB) + g * 4 * NB) + imm * (16 * NB));
-      load_bytes<2 * NB>(kd[t], dk + j * (2 * NB) + imm * (2 * NB));
+      if constexpr (!Halves) load_bytes<2 * NB>(kd[t], dk + j * (2 * NB) + imm * (2 * NB));
     }
+    if constexpr (Halves) load_bytes<2 * NB>(kd[0], dk + tile_slot<Whole>(16 * (g >> 1) + i, left) * (2 * NB));
+  }
+};
+template <int NB>
+struct ValueTile {
+  uint32_t v[8][(NB + 3) / 4];       // byte b
+  uint32_t d[NB == 8 ? 2 : 1];       // steps
+  template <bool Whole>
+  __device__ __forceinline__ void load(const Cache& c, int64_t slot, int left) {
+    const uint8_t *bv = c.v + slot * (16 * NB), *dv = (const uint8_t*)(c.vd + slot * NB);
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t j = Whole ? 8 * g : at(8 * g + e), imm = Whole ? e : 0;
+      const uint32_t j = tile_slot<Whole>(Whole ? g : 4 * e + g, left), imm = Whole ? 4 * e : 0;
       load_bytes<NB>(v[e], bv + (j * (16 * NB) + i * NB) + imm * (16 * NB));
-      load_bytes<2 * NA>(vd[e], dv + (j * (2 * NB) + first_block * 2) + imm * (2 * NB));
-      if constexpr (NB == 3 && NA == 2) vd[e][0] >>= 16 * first_block;  // set 1: block 2 first
     }
     // a lane takes half of a position's steps, of three the first or last two
     constexpr int H = NB == 1 ? 1 : (NB + 1) / 2;
-    load_bytes<2 * H>(all, dv + at(lane >> 1) * (2 * NB) + (lane & 1) * (NB - H) * 2);
+    load_bytes<2 * H>(d, dv + tile_slot<Whole>(lane >> 1, left) * (2 * NB) + (lane & 1) * (NB - H) * 2);
   }
 };
+
+// Maximum and sum over the 16 lanes of a row, by rotation.
+template <int N>
+__device__ __forceinline__ float row_turned(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, row_turned<8>(x));
+  x = fmaxf(x, row_turned<4>(x));
+  x = fmaxf(x, row_turned<2>(x));
+  return fmaxf(x, row_turned<1>(x));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  x += row_turned<8>(x);
+  x += row_turned<4>(x);
+  x += row_turned<2>(x);
+  return x + row_turned<1>(x);
+}
+// The same over the wave.
+__device__ __forceinline__ float lane_value(float x, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = row_max(x);
+  return fmaxf(fmaxf(lane_value(x, 0), lane_value(x, 16)), fmaxf(lane_value(x, 32), lane_value(x, 48)));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = row_sum(x);
+  return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
+}
 
 // G heads (1, 2, 4 or 8) of a kv head over one piece of a sequence.  Pieces that
 // are a whole sequence give the output, others their reference, sum and values.
 template <int NB, int G>
-__global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cache c, int layer, float* __restrict__ out,
+__global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : NB > 2 ? 3 : 4) kv4_attn_kernel(Cache c, int layer, float* __restrict__ out,
                                                             const float* __restrict__ q, int nH, int subs, float scale,
                                                             int T, const int32_t* __restrict__ count,
                                                             float2* __restrict__ part_ml, float* __restrict__ part_o,
                                                             float* __restrict__ sc) {
   constexpr int dH = 32 * NB, NS = 8 / G, NA = (NB + NS - 1) / NS;  // sets of rows, blocks of a set
+  constexpr int kHalves = G <= 4 ? 2 : 1, kScores = 2 / kHalves;     // a lane's positions of a tile
   __shared__ __attribute__((aligned(16))) float ps[kWaves][G][32];
-  __shared__ __attribute__((aligned(16))) float os[kWaves][G][dH];
-  __shared__ float ms[kWaves][G], ls[kWaves][G];
+  __shared__ __attribute__((aligned(16))) _Float16 ds[kWaves][4][NB][8];
+  // q's operand at first, the waves' values at the end
+  constexpr int kShared = kWaves * G * dH > NB * 64 * 4 ? kWaves * G * dH : NB * 64 * 4;
+  __shared__ __attribute__((aligned(16))) float shared[kShared];
+  float(*const os)[G][dH] = reinterpret_cast<float(*)[G][dH]>(shared);  // [kWaves]
+  u32x4(*const qs)[64] = reinterpret_cast<u32x4(*)[64]>(shared);        // [NB]
+  __shared__ float ms[kWaves][G], ls[kWaves][G], qm[kWaves][16];
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Plan p;
@@ -285,41 +338,65 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cach
   const int begin = piece * p.per * kRound, end = min(n, begin + p.per * kRound);
   const int64_t slot0 = head_slot(c, layer, s, kvh);
 
-  // q as the scores' first operand: row = lane & 15 holds head (row / 2) % G,
-  // piece row & 1; its head's factor 2^-e goes into the scores
-  f16x8 qa[NB];
+  const int set = (i >> 1) / G;  // this row's blocks: set NA ..
+  KeyTile<NB, kHalves == 2> keys;
+  ValueTile<NB> vals;
+  int at = begin + 32 * wave;
+  if (at + 32 <= end) {
+    keys.template load<true>(c, slot0 + at, 32);
+    vals.template load<true>(c, slot0 + at, 32);
+  }
+
+  // q as the scores' first operand: row = lane & 15 holds slot row / 2, that is
+  // head (row / 2) % G, piece row & 1; its head's power 2^-e goes into the scores.
+  // The waves share the blocks out.
+  f16x8 qa[kHalves][NB];
   float factor[2];
   {
+    constexpr int mine = (NB + kWaves - 1) / kWaves;
     const int h = (i >> 1) % G;
-    const bool on = h < heads;
-    const float* qr = q + ((int64_t)s * nH + h0 + (on ? h : 0)) * dH + 4 * g;
-    float x[NB][8];
+    const float* qr = q + ((int64_t)s * nH + h0 + min(h, heads - 1)) * dH + 4 * g;
+    float x[mine][8];
     float m = 0.f;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      __builtin_memcpy(&x[b][0], qr + 32 * b, 16);
-      __builtin_memcpy(&x[b][4], qr + 32 * b + 16, 16);
+    for (int k = 0; k < mine; ++k) {
+      const int b = min(wave + k * kWaves, NB - 1);
+      __builtin_memcpy(&x[k][0], qr + 32 * b, 16);
+      __builtin_memcpy(&x[k][4], qr + 32 * b + 16, 16);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (!on) x[b][e] = 0.f;
-        m = fmaxf(m, fabsf(x[b][e]));
-      }
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[k][e]));
     }
     m = fmaxf(m, __shfl_xor(m, 16, 64));
     m = fmaxf(m, __shfl_xor(m, 32, 64));
+    if (lane < 16) qm[wave][i] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, qm[w][i]);
     const int e = fg::exponent_of_max(m);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      uint32_t w[4];
+    for (int k = 0; k < mine; ++k) {
+      const int b = wave + k * kWaves;
+      u32x4 w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // operand pairs: values (0, 1), (16, 17), (2, 3), (18, 19) of 4 g
         const int at = (j & 1) * 4 + (j >> 1) * 2;
         uint32_t hi, lo;
-        fg::split2h(x[b][at], x[b][at + 1], e, hi, lo);
+        fg::split2h(x[k][at], x[k][at + 1], e, hi, lo);
         w[j] = (i & 1) ? lo : hi;
       }
-      qa[b] = operand(w[0], w[1], w[2], w[3]);
+      if (b < NB) qs[b][lane] = w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const u32x4 w = qs[b][lane], none = {0u, 0u, 0u, 0u};
+      if constexpr (kHalves == 2) {
+        qa[0][b] = __builtin_bit_cast(f16x8, i < 8 ? w : none);
+        qa[1][b] = __builtin_bit_cast(f16x8, i < 8 ? none : w);
+      } else {
+        qa[0][b] = __builtin_bit_cast(f16x8, w);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -333,60 +410,66 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cach
   int E = -24;
   uint32_t limit = 0;  // the greatest fp16 below 2^E, as its bits
   const float piece_of = (i & 1) ? 1.f : 0.f;
-  const int set = (i >> 1) / G, set_block = min(set * NA, NB - NA);  // this row's blocks
   uint32_t magic = 0x64006400u;
   asm("" : "+v"(magic));
 
-  auto take = [&](int at, auto is_whole) __attribute__((always_inline)) {
+  // scores of positions 16 t + i (of four heads or fewer: 16 (g / 2) + i) for heads
+  // (2 g + j) % G, in powers of two
+  float x[kScores][2];
+  const int i0 = kHalves == 2 ? 16 * (g >> 1) + i : i;
+  const bool owns[2] = {(kHalves == 2 ? 2 * (g & 1) : 2 * g) < G, (kHalves == 2 ? 2 * (g & 1) + 1 : 2 * g + 1) < G};
+  auto score = [&](int at, auto is_whole) __attribute__((always_inline)) {
     constexpr bool whole = decltype(is_whole)::value;
-    Tile<NB, NA> tile;
-    const int64_t slot = slot0 + at;
-    tile.template load<whole>(c.k + slot * (16 * NB), c.v + slot * (16 * NB), (const uint8_t*)(c.kd + slot * NB),
-                              (const uint8_t*)(c.vd + slot * NB), set_block, n - at);
-    // scores x of positions i and 16 + i for heads (2 g + j) % G, in powers of two
-    float x[2][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      x[t][0] = x[t][1] = 0.f;
+    for (int u = 0; u < kScores; ++u) x[u][0] = x[u][1] = 0.f;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const uint32_t* kw = tile.k[t];
+    for (int b = 0; b < NB; ++b) {
+      f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         // the words that hold byte b of values 4 g + 0, 1 and 4 g + 2, 3
         auto pair = [&](int j0) {
           const int a0 = j0 * NB + b, a1 = (j0 + 1) * NB + b;
-          const uint32_t w0 = kw[a0 / 4], w1 = kw[a1 / 4];
-          return __builtin_amdgcn_perm(w1, w0, 0x0c000c00u | ((4 + a1 % 4) << 16) | (a0 % 4));
+          return __builtin_amdgcn_perm(keys.k[t][a1 / 4], keys.k[t][a0 / 4], 0x0c000c00u | ((4 + a1 % 4) << 16) | (a0 % 4));
         };
-        const uint32_t lo01 = pair(0), lo23 = pair(2);
-        const f16x8 kb = operand(low_codes(lo01, magic), high_codes(lo01, magic), low_codes(lo23, magic), high_codes(lo23, magic));
-        const f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[b], kb, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-        const float step = half_of(tile.kd[t][b / 2], b & 1);
-        x[t][0] += (d[0] + d[1]) * step;
-        x[t][1] += (d[2] + d[3]) * step;
+        const uint32_t k01 = pair(0), k23 = pair(2);
+        const f16x8 kb = operand(low_codes(k01, magic), high_codes(k01, magic), low_codes(k23, magic), high_codes(k23, magic));
+        if (kHalves == 1 && t == 1) d = (f32x4){0.f, 0.f, 0.f, 0.f};
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(qa[kHalves == 2 ? t : 0][b], kb, d, 0, 0, 0);
+        if (kHalves == 2 && t == 0) continue;
+        const int u = kHalves == 2 ? 0 : t;
+        const float step = half_of(keys.kd[u][b / 2], b & 1);
+        x[u][0] += (d[0] + d[1]) * step;
+        x[u][1] += (d[2] + d[3]) * step;
       }
-      x[t][0] *= factor[0];
-      x[t][1] *= factor[1];
-      if (!whole && at + 16 * t + i >= end) x[t][0] = x[t][1] = -INFINITY;
     }
+#pragma unroll
+    for (int u = 0; u < kScores; ++u) {
+      x[u][0] *= factor[0];
+      x[u][1] *= factor[1];
+      if (!whole && at + 16 * u + i0 >= end) x[u][0] = x[u][1] = -INFINITY;
+    }
+  };
+  auto add = [&](int at, auto is_whole) __attribute__((always_inline)) {
+    constexpr bool whole = decltype(is_whole)::value;
     // raise the maximum or the steps' power where this tile goes beyond them
     uint32_t far = 0;
 #pragma unroll
-    for (int w = 0; w < (NB + 3) / 4; ++w) {
-      const uint32_t a = tile.all[w] & 0x7FFF7FFFu, a0 = a & 0xFFFF, a1 = a >> 16;
+    for (int w = 0; w < (NB == 8 ? 2 : 1); ++w) {
+      const uint32_t a = vals.d[w] & 0x7FFF7FFFu, a0 = a & 0xFFFF, a1 = a >> 16;
       far = max(far, max(a0 < 0x7C00 ? a0 : 0u, a1 < 0x7C00 ? a1 : 0u));
     }
-    const float here[2] = {fmaxf(x[0][0], x[1][0]), fmaxf(x[0][1], x[1][1])};
+    const float here[2] = {fmaxf(x[0][0], x[kScores - 1][0]), fmaxf(x[0][1], x[kScores - 1][1])};
     if (__any(here[0] > top[0] || here[1] > top[1] || far > limit)) {
       float f = (float)__builtin_bit_cast(_Float16, (uint16_t)far);
-      f = fg_wave_max(f);
+      f = wave_max(f);
       if (f > 0.f) E = max(E, __builtin_amdgcn_frexp_expf(f));
       limit = E > -14 ? (uint32_t)((E + 14) << 10) | 0x3FF : (1u << (E + 24)) - 1;
       float turn[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float m = here[j];
-#pragma unroll
-        for (int d = 8; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 16));
+        float m = row_max(here[j]);
+        if constexpr (kHalves == 2) m = fmaxf(m, __shfl_xor(m, 32, 64));
         top[j] = fmaxf(top[j], m);
         const float r = top[j] + (float)(E - 15);
         turn[j] = r == ref[j] ? 1.f : __builtin_amdgcn_exp2f(ref[j] - r);
@@ -406,15 +489,22 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cach
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int h = (2 * g + j) % G;
-      const bool mine = (2 * g + j) < G;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (sc && mine && h < heads && (whole || at + 16 * t + i < end))
-          sc[((int64_t)s * nH + h0 + h) * c.maxSeq + at + 16 * t + i] = x[t][j];
-        const float e = __builtin_amdgcn_exp2f(x[t][j] - ref[j]);
+      for (int u = 0; u < kScores; ++u) {
+        if (sc && owns[j] && h < heads && (whole || at + 16 * u + i0 < end))
+          sc[((int64_t)s * nH + h0 + h) * c.maxSeq + at + 16 * u + i0] = x[u][j];
+        const float e = __builtin_amdgcn_exp2f(x[u][j] - ref[j]);
         sum[j] += e;
-        if (mine) ps[wave][h][16 * t + i] = e;
+        if (owns[j]) ps[wave][h][8 * (i0 & 3) + 4 * u + (i0 >> 2)] = e;
       }
+    }
+    // the steps by (position & 3, block, position / 4)
+    {
+      constexpr int H = NB == 1 ? 1 : (NB + 1) / 2;
+      const int at = lane >> 1, first = (lane & 1) * (NB - H);
+#pragma unroll
+      for (int k = 0; k < H; ++k)
+        ds[wave][at & 3][first + k][at >> 2] = __builtin_bit_cast(f16x2, vals.d[k / 2])[k & 1];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     float e[8];
@@ -426,12 +516,13 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cach
 #pragma unroll
     for (int a = 0; a < NA; ++a) {
       // w = p d of block a of this row's set, the row's piece of it
+      const f16x8 step = *reinterpret_cast<const f16x8*>(&ds[wave][g][min(set * NA + a, NB - 1)][0]);
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float y[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) y[k] = e[2 * j + k] * half_of(tile.vd[2 * j + k][a / 2], a & 1);
+        for (int k = 0; k < 2; ++k) y[k] = e[2 * j + k] * (float)step[2 * j + k];
         const f16x2 h = __builtin_convertvector((f32x2){y[0], y[1]}, f16x2);
         const f16x2 r = __builtin_convertvector((f32x2){y[0] - piece_of * (float)h[0], y[1] - piece_of * (float)h[1]}, f16x2);
         w[j] = __builtin_bit_cast(uint32_t, r);
@@ -444,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cach
         uint32_t lo[4], hi[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t two = __builtin_amdgcn_perm(tile.v[2 * j + 1][b / 4], tile.v[2 * j][b / 4],
+          const uint32_t two = __builtin_amdgcn_perm(vals.v[2 * j + 1][b / 4], vals.v[2 * j][b / 4],
                                                      0x0c000c00u | ((4 + b % 4) << 16) | (b % 4));
           lo[j] = low_codes(two, magic);
           hi[j] = high_codes(two, magic);
@@ -454,15 +545,29 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cach
       }
     }
   };
-  int at = begin + 32 * wave;
-  for (; at + 32 <= end; at += kRound) take(at, std::true_type());
-  if (at < end) take(at, std::false_type());
+  // the next tile's keys are fetched once this one's scores are there, its values
+  // once this one's are added
+  const std::true_type whole;
+  const std::false_type part;
+  for (; at + 32 <= end; at += kRound) {
+    const bool more = at + kRound + 32 <= end;
+    score(at, whole);
+    if (more) keys.template load<true>(c, slot0 + at + kRound, 32);
+    add(at, whole);
+    if (more) vals.template load<true>(c, slot0 + at + kRound, 32);
+  }
+  if (at < end) {
+    keys.template load<false>(c, slot0 + at, n - at);
+    vals.template load<false>(c, slot0 + at, n - at);
+    score(at, part);
+    add(at, part);
+  }
 
   // the waves' results joined: references to their maximum, then sums
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-#pragma unroll
-    for (int d = 8; d > 0; d >>= 1) sum[j] += __shfl_xor(sum[j], d, 16);
+    sum[j] = row_sum(sum[j]);
+    if constexpr (kHalves == 2) sum[j] += __shfl_xor(sum[j], 32, 64);
     if (i == 0 && 2 * g + j < G) ms[wave][2 * g + j] = ref[j];
   }
   __syncthreads();
@@ -481,7 +586,6 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cach
         if ((2 * g + j) / G == b / NA) os[wave][h][32 * b + 16 * u + i] = (o[b][u][2 * j] + o[b][u][2 * j + 1]) * turn;
   }
   __syncthreads();
-  const bool whole = p.pieces == 1;
   for (int k = threadIdx.x; k < heads * dH; k += kThreads) {
     const int h = k / dH, d = k - h * dH;
     float v = 0.f, l = 0.f, m = ms[0][h];
@@ -491,86 +595,137 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : 4) kv4_attn_kernel(Cach
       l += ls[w][h];
       m = fmaxf(m, ms[w][h]);
     }
-    if (whole) out[((int64_t)s * nH + h0 + h) * dH + d] = n > 0 ? v / l : 0.f;
+    if (p.pieces == 1) out[((int64_t)s * nH + h0 + h) * dH + d] = n > 0 ? v / l : 0.f;
     else part_o[((int64_t)blockIdx.x * G + h) * dH + d] = v;
     if (d == 0) part_ml[(int64_t)blockIdx.x * G + h] = make_float2(m, l);
   }
 }
 
 // The pieces of every sequence joined: workgroups [0, nSeq nH) the output of a
-// query head, the rest (weights kept) the weights of 1024 positions of a kv head.
-constexpr int kWeightRows = 1024;
+// query head, the rest (weights kept) the weights of 512 positions of a kv head.
+// Short launches, so loads that do not depend on each other go first: a head's
+// values of its first pieces beside its references, the scores beside them.
+constexpr int kWeightRows = 512;
+constexpr int kJoinPieces = 512;  // pieces whose factors are kept in LDS
+// Reference and 1 / sum of a head over its pieces, by one wave; w gets the
+// pieces' factors.
+__device__ __forceinline__ float2 join_head(const float2* __restrict__ ml, int G, int pieces, float* w) {
+  const int lane = threadIdx.x & 63;
+  float2 first = make_float2(-INFINITY, 0.f);
+  if (lane < pieces) first = ml[(int64_t)lane * G];
+  float m = first.x;
+  for (int k = lane + 64; k < pieces; k += 64) m = fmaxf(m, ml[(int64_t)k * G].x);
+  m = wave_max(m);
+  float l = 0.f;
+  for (int k = lane; k < pieces; k += 64) {
+    const float2 v = k == lane ? first : ml[(int64_t)k * G];
+    const float f = v.x == m ? 1.f : __builtin_amdgcn_exp2f(v.x - m);
+    if (w && k < kJoinPieces) w[k] = f;
+    l += v.y * f;
+  }
+  return make_float2(m, wave_sum(l));
+}
+
 template <int NB>
 __global__ void __launch_bounds__(kThreads) kv4_join_kernel(Cache c, int layer, float* __restrict__ out, int nH,
                                                             int subs, int G, int T, const int32_t* __restrict__ count,
                                                             const float2* __restrict__ part_ml,
                                                             const float* __restrict__ part_o,
                                                             const float* __restrict__ sc, int chunks) {
-  constexpr int dH = 32 * NB, kLanes = kThreads / dH > 0 ? kThreads / dH : 1;
-  __shared__ float red[kThreads];
+  constexpr int dH = 32 * NB, kLanes = kThreads / dH > 0 ? kThreads / dH : 1, kAhead = 8;
+  __shared__ float red[kThreads], factor[kJoinPieces], shm[64], shl[64];
   const int group = nH / c.nKV, share = (group + subs - 1) / subs;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool weights = (int)blockIdx.x >= c.nSeq * nH;
   const int id = weights ? blockIdx.x - c.nSeq * nH : blockIdx.x;
   const int s = weights ? id / (c.nKV * chunks) : id / nH;
   Plan p;
   plan_for(p, c, count, T, c.nKV * subs, s, true);
-  const int n = attended(c, count, s, T);
+  auto first_of = [&](int kvh, int r) {  // of query head r of its group
+    return ((int64_t)p.first * c.nKV * subs + (int64_t)(kvh * subs + r / share) * p.pieces) * G + r % share;
+  };
   if (weights) {
-    const int kvh = id / chunks % c.nKV, at0 = id % chunks * kWeightRows;
+    const int n = attended(c, count, s, T), kvh = id / chunks % c.nKV, at0 = id % chunks * kWeightRows;
     if (at0 >= n) return;
-    float add[kWeightRows / kThreads];
-#pragma unroll
-    for (int k = 0; k < kWeightRows / kThreads; ++k) add[k] = 0.f;
-    for (int h = 0; h < group; ++h) {
-      const int64_t first = ((int64_t)p.first * c.nKV * subs + (int64_t)(kvh * subs + h / share) * p.pieces) * G + h % share;
-      float m = -INFINITY;
-      for (int k = threadIdx.x & 63; k < p.pieces; k += 64) m = fmaxf(m, part_ml[first + (int64_t)k * G].x);
-      m = fg_wave_max(m);
-      float l = 0.f;
-      for (int k = threadIdx.x & 63; k < p.pieces; k += 64) {
-        const float2 ml = part_ml[first + (int64_t)k * G];
-        l += ml.y * (ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m));
-      }
-      l = 1.f / fg_wave_sum(l);
-      const float* row = sc + ((int64_t)s * nH + kvh * group + h) * c.maxSeq;
-#pragma unroll
-      for (int k = 0; k < kWeightRows / kThreads; ++k) {
-        const int at = at0 + k * kThreads + threadIdx.x;
-        if (at < n) add[k] += __builtin_amdgcn_exp2f(row[at] - m) * l;
-      }
-    }
+    constexpr int R = kWeightRows / kThreads;
     float* w = c.weight + head_slot(c, layer, s, kvh);
+    float sum[R];
 #pragma unroll
-    for (int k = 0; k < kWeightRows / kThreads; ++k) {
+    for (int k = 0; k < R; ++k) sum[k] = 0.f;
+    for (int h0 = 0; h0 < group; h0 += 4) {
+      float x[4][R];
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const int at = at0 + k * kThreads + threadIdx.x;
+          x[h][k] = h0 + h < group && at < n ? sc[((int64_t)s * nH + kvh * group + h0 + h) * c.maxSeq + at] : 0.f;
+        }
+      __syncthreads();
+      if (h0 + wave < group) {
+        const float2 v = join_head(part_ml + first_of(kvh, h0 + wave), G, p.pieces, nullptr);
+        shm[wave] = v.x;
+        shl[wave] = 1.f / v.y;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        if (h0 + h < group) {
+#pragma unroll
+          for (int k = 0; k < R; ++k) sum[k] += __builtin_amdgcn_exp2f(x[h][k] - shm[h]) * shl[h];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
       const int at = at0 + k * kThreads + threadIdx.x;
-      if (at < n) w[at] += add[k];
+      if (at < n) w[at] += sum[k];
     }
     return;
   }
   if (p.pieces == 1) return;
-  const int h = id % nH, kvh = h / group, r = h - kvh * group;
-  const int64_t first = ((int64_t)p.first * c.nKV * subs + (int64_t)(kvh * subs + r / share) * p.pieces) * G + r % share;
-  float m = -INFINITY;
-  for (int k = threadIdx.x & 63; k < p.pieces; k += 64) m = fmaxf(m, part_ml[first + (int64_t)k * G].x);
-  m = fg_wave_max(m);
-  float l = 0.f;
-  for (int k = threadIdx.x & 63; k < p.pieces; k += 64) {
-    const float2 ml = part_ml[first + (int64_t)k * G];
-    l += ml.y * (ml.x == m ? 1.f : __builtin_amdgcn_exp2f(ml.x - m));
-  }
-  l = fg_wave_sum(l);
+  const int h = id % nH, kvh = h / group;
+  const int64_t first = first_of(kvh, h - kvh * group);
   const int d = threadIdx.x % dH, z = threadIdx.x / dH;
+  const float* po = part_o + first * dH + d;
+  const int64_t step = (int64_t)G * dH;
+  float ahead[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const int k = z + u * kLanes;
+    ahead[u] = z < kLanes && k < p.pieces ? po[k * step] : 0.f;
+  }
+  float2 ml = make_float2(0.f, 0.f);
+  if (wave == 0) {
+    ml = join_head(part_ml + first, G, p.pieces, factor);
+    shm[0] = ml.x;
+    shl[0] = ml.y;
+  }
+  __syncthreads();
+  const float m = shm[0];
+  auto turn = [&](int k) {
+    if (k < kJoinPieces) return factor[k];
+    const float mk = part_ml[first + (int64_t)k * G].x;
+    return mk == m ? 1.f : __builtin_amdgcn_exp2f(mk - m);
+  };
   float v = 0.f;
-  if (z < kLanes)
-    for (int k = z; k < p.pieces; k += kLanes) {
-      const float mk = part_ml[first + (int64_t)k * G].x;
-      v += part_o[(first + (int64_t)k * G) * dH + d] * (mk == m ? 1.f : __builtin_amdgcn_exp2f(mk - m));
+  if (z < kLanes) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (z + u * kLanes < p.pieces) v += ahead[u] * turn(z + u * kLanes);
+    int k = z + kAhead * kLanes;
+    for (; k + 7 * kLanes < p.pieces; k += 8 * kLanes) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) ahead[u] = po[(k + u * kLanes) * step];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += ahead[u] * turn(k + u * kLanes);
     }
+    for (; k < p.pieces; k += kLanes) v += po[k * step] * turn(k);
+  }
   red[threadIdx.x] = v;
   __syncthreads();
   if (z == 0) {
     for (int k = 1; k < kLanes; ++k) v += red[k * dH + d];
-    out[((int64_t)s * nH + h) * dH + d] = v / l;
+    out[((int64_t)s * nH + h) * dH + d] = v / shl[0];
   }
 }
 
