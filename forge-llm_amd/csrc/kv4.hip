@@ -137,10 +137,12 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Cache c, int layer, 
 //           w = p d with the block's step d, fp32 accumulators
 //
 // A wave takes 32 positions at a time and keeps the running maximum, sum and
-// values of its heads; p = 2^(x - ref) with ref = max - 15 + E, 2^E above every
-// step so far, so that w fills fp16's range, [0, 2^15).  max and E are only
-// raised, and the accumulators rescaled, when a score or step goes beyond
-// them: after the first positions hardly ever.  There are eight slots of two rows:
+// values of its heads; p = 2^(x - ref) with ref = top + kRoom - 15 + E, 2^E above
+// every step so far, so that w stays below 2^15 for scores x up to top + kRoom.
+// top (the greatest score) and E are only raised, and the accumulators
+// rescaled, when a score or step goes beyond that: with room for a factor of 64
+// hardly ever after the first tile (without, four heads of even scores raise
+// one's maximum in six of the first ten).  There are eight slots of two rows:
 // up to four heads (G) repeat, so that the scores of positions 0 .. 15 come out in
 // the lower eight rows and those of 16 .. 31 in the upper, one lane each, and
 // 8 / G blocks' steps share an operand of w.
@@ -153,6 +155,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kRound = 128;    // positions a workgroup takes at a time, 32 a wave
 constexpr int kTarget = 1024;  // workgroups that the positions are spread over
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kRoom = 6.f;   // powers of two that a score may pass the maximum by
 
 // How the positions of all sequences are cut: pieces of `per` rounds, at least
 // one a sequence and head.  A wave works it out from the lengths (which only
@@ -406,7 +409,8 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : NB > 2 ? 3 : 4) kv4_att
   f32x4 o[NB][2];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b][0] = o[b][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float top[2] = {-INFINITY, -INFINITY}, ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+  float top[2] = {-INFINITY, -INFINITY}, roof[2] = {-INFINITY, -INFINITY}, ref[2] = {-INFINITY, -INFINITY};
+  float sum[2] = {0.f, 0.f};
   int E = -24;
   uint32_t limit = 0;  // the greatest fp16 below 2^E, as its bits
   const float piece_of = (i & 1) ? 1.f : 0.f;
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : NB > 2 ? 3 : 4) kv4_att
       far = max(far, max(a0 < 0x7C00 ? a0 : 0u, a1 < 0x7C00 ? a1 : 0u));
     }
     const float here[2] = {fmaxf(x[0][0], x[kScores - 1][0]), fmaxf(x[0][1], x[kScores - 1][1])};
-    if (__any(here[0] > top[0] || here[1] > top[1] || far > limit)) {
+    if (__any(here[0] > roof[0] || here[1] > roof[1] || far > limit)) {
       float f = (float)__builtin_bit_cast(_Float16, (uint16_t)far);
       f = wave_max(f);
       if (f > 0.f) E = max(E, __builtin_amdgcn_frexp_expf(f));
@@ -471,7 +475,8 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : NB > 2 ? 3 : 4) kv4_att
         float m = row_max(here[j]);
         if constexpr (kHalves == 2) m = fmaxf(m, __shfl_xor(m, 32, 64));
         top[j] = fmaxf(top[j], m);
-        const float r = top[j] + (float)(E - 15);
+        roof[j] = top[j] + kRoom;
+        const float r = roof[j] + (float)(E - 15);
         turn[j] = r == ref[j] ? 1.f : __builtin_amdgcn_exp2f(ref[j] - r);
         ref[j] = r;
         sum[j] *= turn[j];
@@ -522,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : NB > 2 ? 3 : 4) kv4_att
       for (int j = 0; j < 4; ++j) {
         float y[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) y[k] = e[2 * j + k] * (float)step[2 * j + k];
+        for (int k = 0; k < 2; ++k) y[k] = __builtin_fmaf(e[2 * j + k], (float)step[2 * j + k], 0.f);
         const f16x2 h = __builtin_convertvector((f32x2){y[0], y[1]}, f16x2);
         const f16x2 r = __builtin_convertvector((f32x2){y[0] - piece_of * (float)h[0], y[1] - piece_of * (float)h[1]}, f16x2);
         w[j] = __builtin_bit_cast(uint32_t, r);

@@ -687,7 +687,7 @@ int fg_kv4_read(const fg_kv4_cache* c, int layer, float* k, float* v, int64_t ld
  * n = 0 gives zeros.  Where c->weight is kept, every slot j < n adds the sum of
  * its p_j over its kv head's query heads.  Codes are exact in the products; q and
  * p_j d (d the step of a block of V_j) are held in two fp16 pieces (22 bits, the
- * latter to 2^-40 of the greatest step at least), sums are fp32. */
+ * latter to 2^-33 of the greatest step at least), sums are fp32. */
 int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
                 const int32_t* count);
 /* Ends a step: len[s] += T (or count[s]; to maxSeq at most), next[s] += the same. */

@@ -60,9 +60,10 @@ def attend_bound(q, K, V, p, scale, steps):
     subtraction of the maximum, 4 more of the largest score), exp2 is good to 2^-22; p's and the sums over
     n positions round at most n / 4 + 64 times in a chain (a sum over a tile's positions stays in the
     matrix unit's order); p d is held in two fp16 pieces, 2^-22.  The pieces count from the greatest
-    step: w = p d 2^(15 - E), 2^E at most twice the greatest step, has an absolute error of 2^-25 where its
-    low piece is subnormal, which is 2^-40 2^E <= 2^-39 max d of p d (and of less after the division by
-    the sum of p, 1 or more), times |c - 8| <= 8, for each of n positions."""
+    step and from a reference that the maximum may pass by 2^6 (and lies above 2^-6 of it): w = p d 2^(9 - E),
+    2^E at most twice the greatest step, has an absolute error of 2^-25 where its low piece is subnormal,
+    which is 2^-34 2^E <= 2^-33 max d of p d (and of less after the division by the sum of p, 1 or more),
+    times |c - 8| <= 8, for each of n positions."""
     n, nKV, dH = K.shape
     nH = q.shape[0]
     out, weight = np.zeros((nH, dH)), np.zeros((nH, n))
@@ -71,7 +72,7 @@ def attend_bound(q, K, V, p, scale, steps):
         mass = abs(scale) * (np.abs(K[:, z]) @ np.abs(q[h].astype(np.float64)))
         es = mass.max() * (2.0 ** -22 + (dH + 16) * 2.0 ** -24)
         rel = 2 * es + 2.0 ** -21 + (n / 4 + 64) * 2.0 ** -24
-        out[h] = rel * (p[h] @ np.abs(V[:, z])) + n * 8 * 2.0 ** -39 * np.abs(steps[z].astype(np.float64)).max() + 1e-30
+        out[h] = rel * (p[h] @ np.abs(V[:, z])) + n * 8 * 2.0 ** -33 * np.abs(steps[z].astype(np.float64)).max() + 1e-30
         weight[h] = rel * p[h] + 1e-30
     return out, weight
 
