@@ -34,12 +34,33 @@ __device__ __forceinline__ int new_tokens(const int32_t* count, int s, int T) {
 }
 __device__ __forceinline__ int slots_used(const Cache& c, int s) { return min(max(c.len[s], 0), c.maxSeq); }
 
+// Maximum, minimum and sum over the 16 lanes of a row, by rotation.
+template <int N>
+__device__ __forceinline__ float row_turned(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, row_turned<8>(x));
+  x = fmaxf(x, row_turned<4>(x));
+  x = fmaxf(x, row_turned<2>(x));
+  return fmaxf(x, row_turned<1>(x));
+}
+__device__ __forceinline__ float row_sum(float x) {
+  x += row_turned<8>(x);
+  x += row_turned<4>(x);
+  x += row_turned<2>(x);
+  return x + row_turned<1>(x);
+}
+
 // ── store ─────────────────────────────────────────────────────────────────
 // Sixteen lanes take a head's slot: lane n holds values 32 b + n and 32 b + 16 + n
-// of every block, so a block's maximum is a reduction over 16 lanes and the
-// lane's nb bytes are its share of the slot.  floor(x / d + 8.5) is found from
-// an approximate quotient and the exact borders (c - 8.5) d: 5 bits times 11
-// bits, no rounding in fp32.
+// of every block, so a block's extremes are reductions over 16 lanes and the
+// lane's nb bytes are its share of the slot.  HBM-bound (7.1 B read for 1 written)
+// as long as a block costs few instructions.
+
+// A block by its definition: the first of the greatest magnitudes by ballots, and
+// floor(x / d + 8.5) from an approximate quotient and the exact borders (c - 8.5) d:
+// 5 bits times 11 bits, no rounding in fp32.
 __device__ __forceinline__ int code_of(float x, float inv, float d) {
   const float y = d < 0.f ? -x : x, s = fabsf(d);
   float q = floorf(y * inv + 8.5f);
@@ -47,18 +68,55 @@ __device__ __forceinline__ int code_of(float x, float inv, float d) {
   else if (y >= (q - 7.5f) * s) q += 1.f;
   return (int)fminf(fmaxf(q, 0.f), 15.f);
 }
+__device__ __noinline__ uint32_t exact_block(float lo, float hi) {  // step << 16 | codes
+  const int lane0 = threadIdx.x & 48;
+  const float a = row_max(fmaxf(fabsf(lo), fabsf(hi)));
+  const uint32_t in_lo = (uint32_t)(__ballot(fabsf(lo) == a) >> lane0) & 0xFFFF;
+  const uint32_t in_hi = (uint32_t)(__ballot(fabsf(hi) == a) >> lane0) & 0xFFFF;
+  const uint32_t neg_lo = (uint32_t)(__ballot(lo < 0.f) >> lane0) & 0xFFFF;
+  const uint32_t neg_hi = (uint32_t)(__ballot(hi < 0.f) >> lane0) & 0xFFFF;
+  const bool nan = ((uint32_t)(__ballot(lo != lo || hi != hi) >> lane0) & 0xFFFF) != 0;
+  const bool neg = in_lo ? (neg_lo >> __builtin_ctz(in_lo)) & 1 : (neg_hi >> __builtin_ctz(in_hi | 0x10000)) & 1;
+  _Float16 d = (_Float16)((neg ? a : -a) * 0.125f);  // m / -8
+  const float df = (float)d;
+  const bool bad = nan || !(fabsf(df) < INFINITY);
+  if (bad) d = (_Float16)NAN;
+  int q0 = 8, q1 = 8;
+  if (!bad && df != 0.f) {
+    const float inv = 1.f / fabsf(df);
+    q0 = code_of(lo, inv, df);
+    q1 = code_of(hi, inv, df);
+  }
+  return (uint32_t)__builtin_bit_cast(uint16_t, d) << 16 | (uint32_t)(q0 | (q1 << 4));
+}
+// The same where no value is NaN, the step is finite and not 0, the extremes differ
+// in size and no quotient is near a border; `sure` is false for lanes that this
+// cannot tell for.
+__device__ __forceinline__ uint32_t quick_block(float lo, float hi, bool& sure) {
+  const float most = row_max(fmaxf(lo, hi)), least = -row_max(fmaxf(-lo, -hi));
+  const _Float16 d = (_Float16)((most > -least ? most : least) * -0.125f);
+  const float inv = __builtin_amdgcn_rcpf((float)d);
+  // quotients up to 8.5 (12 for the smallest steps) are off by less than 2^-18
+  const float t0 = __builtin_fmaf(lo, inv, 8.5f), t1 = __builtin_fmaf(hi, inv, 8.5f);
+  const float f0 = __builtin_amdgcn_fractf(t0), f1 = __builtin_amdgcn_fractf(t1);
+  sure = most != -least && inv != 0.f && fmaxf(fabsf(f0 - 0.5f), fabsf(f1 - 0.5f)) < 0.5f - 0x1p-16f &&
+         fmaxf(fabsf(t0), fabsf(t1)) < 32.f && lo == lo && hi == hi;
+  const uint32_t q0 = (uint32_t)__builtin_amdgcn_fmed3f(t0 - f0, 0.f, 15.f);
+  const uint32_t q1 = (uint32_t)__builtin_amdgcn_fmed3f(t1 - f1, 0.f, 15.f);
+  return (uint32_t)__builtin_bit_cast(uint16_t, d) << 16 | (q0 | q1 << 4);
+}
 
 template <int NB>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(Cache c, int layer, const float* __restrict__ k,
                                                               const float* __restrict__ v, int64_t ld, int T,
-                                                              const int32_t* __restrict__ count, int64_t rows) {
+                                                              const int32_t* __restrict__ count, uint32_t rows) {
   constexpr int dH = 32 * NB;
-  const int n = threadIdx.x & 15, lane0 = threadIdx.x & 48;
-  const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
-  const bool on = item < rows * c.nKV;
-  const int64_t row = on ? item / c.nKV : 0;
-  const int h = on ? (int)(item - row * c.nKV) : 0;
-  const int s = (int)(row / T), t = (int)(row - (int64_t)s * T);
+  const int n = threadIdx.x & 15;
+  const uint32_t item = (blockIdx.x * kThreads + threadIdx.x) >> 4;
+  const bool on = item < rows * (uint32_t)c.nKV;
+  const uint32_t row = on ? item / (uint32_t)c.nKV : 0;
+  const int h = on ? (int)(item - row * (uint32_t)c.nKV) : 0;
+  const int s = (int)(row / (uint32_t)T), t = (int)(row - (uint32_t)s * (uint32_t)T);
   const int64_t at = (int64_t)slots_used(c, s) + t;
   if (!on || t >= new_tokens(count, s, T) || at >= c.maxSeq) return;  // whole groups of 16 lanes
   const float* x = (blockIdx.y ? v : k) + row * ld + (int64_t)h * dH;
@@ -69,48 +127,37 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(Cache c, int layer
     lo[b] = x[32 * b + n];
     hi[b] = x[32 * b + 16 + n];
   }
-  uint8_t* bytes = (blockIdx.y ? c.v : c.k) + slot * (dH / 2) + n * NB;
-  _Float16* steps = (blockIdx.y ? c.vd : c.kd) + slot * NB;
+  uint8_t bytes[NB];
+  uint16_t steps[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    float a = fmaxf(fabsf(lo[b]), fabsf(hi[b]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 16));
-    const uint32_t in_lo = (uint32_t)(__ballot(fabsf(lo[b]) == a) >> lane0) & 0xFFFF;
-    const uint32_t in_hi = (uint32_t)(__ballot(fabsf(hi[b]) == a) >> lane0) & 0xFFFF;
-    const uint32_t neg_lo = (uint32_t)(__ballot(lo[b] < 0.f) >> lane0) & 0xFFFF;
-    const uint32_t neg_hi = (uint32_t)(__ballot(hi[b] < 0.f) >> lane0) & 0xFFFF;
-    const bool nan = ((uint32_t)(__ballot(lo[b] != lo[b] || hi[b] != hi[b]) >> lane0) & 0xFFFF) != 0;
-    const bool neg = in_lo ? (neg_lo >> __builtin_ctz(in_lo)) & 1 : (neg_hi >> __builtin_ctz(in_hi | 0x10000)) & 1;
-    _Float16 d = (_Float16)((neg ? a : -a) * 0.125f);  // m / -8
-    const float df = (float)d;
-    const bool bad = nan || !(fabsf(df) < INFINITY);
-    int q0 = 8, q1 = 8;
-    if (!bad && df != 0.f) {
-      const float inv = 1.f / fabsf(df);
-      q0 = code_of(lo[b], inv, df);
-      q1 = code_of(hi[b], inv, df);
-    }
-    bytes[b] = (uint8_t)(q0 | (q1 << 4));
-    if (n == 0) steps[b] = bad ? (_Float16)NAN : d;
+    bool sure;
+    uint32_t w = quick_block(lo[b], hi[b], sure);
+    if (!__all(sure)) w = exact_block(lo[b], hi[b]);
+    bytes[b] = (uint8_t)w;
+    steps[b] = (uint16_t)(w >> 16);
   }
-  if (n == 0 && blockIdx.y == 0) {
-    if (c.weight) c.weight[slot] = 0.f;
-    if (c.pos) c.pos[slot] = c.next[s] + t;
+  __builtin_memcpy((blockIdx.y ? c.v : c.k) + slot * (dH / 2) + n * NB, bytes, NB);
+  if (n == 0) {
+    __builtin_memcpy((blockIdx.y ? c.vd : c.kd) + slot * NB, steps, 2 * NB);
+    if (blockIdx.y == 0) {
+      if (c.weight) c.weight[slot] = 0.f;
+      if (c.pos) c.pos[slot] = c.next[s] + t;
+    }
   }
 }
 
 template <int NB>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Cache c, int layer, float* __restrict__ k,
                                                             float* __restrict__ v, int64_t ld, int first, int T,
-                                                            int64_t rows) {
+                                                            uint32_t rows) {
   constexpr int dH = 32 * NB;
   const int n = threadIdx.x & 15;
-  const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4;
-  if (item >= rows * c.nKV) return;
-  const int64_t row = item / c.nKV;
-  const int h = (int)(item - row * c.nKV);
-  const int s = (int)(row / T), t = (int)(row - (int64_t)s * T);
+  const uint32_t item = (blockIdx.x * kThreads + threadIdx.x) >> 4;
+  if (item >= rows * (uint32_t)c.nKV) return;
+  const uint32_t row = item / (uint32_t)c.nKV;
+  const int h = (int)(item - row * (uint32_t)c.nKV);
+  const int s = (int)(row / (uint32_t)T), t = (int)(row - (uint32_t)s * (uint32_t)T);
   const int64_t slot = head_slot(c, layer, s, h) + first + t;
   const uint8_t* bytes = (blockIdx.y ? c.v : c.k) + slot * (dH / 2) + n * NB;
   const _Float16* steps = (blockIdx.y ? c.vd : c.kd) + slot * NB;
@@ -152,14 +199,17 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kRound = 128;    // positions a workgroup takes at a time, 32 a wave
-constexpr int kTarget = 1024;  // workgroups that the positions are spread over
+constexpr int kRound = 128;  // positions a workgroup takes at a time, 32 a wave
+// Workgroups a CU, by registers.
+template <int NB>
+constexpr int kResident = NB > 4 ? 2 : NB > 2 ? 3 : 4;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kRoom = 6.f;   // powers of two that a score may pass the maximum by
 
 // How the positions of all sequences are cut: pieces of `per` rounds, at least
-// one a sequence and head.  A wave works it out from the lengths (which only
-// the device knows): a lane per sequence, or several.
+// one a sequence and head, `target` of them beside the sequences' last ones.  A
+// wave works it out from the lengths (which only the device knows): a lane per
+// sequence, or several.
 struct Plan {
   int per;
   int s, first, pieces;  // a sequence, its first piece (of one head) and their number
@@ -171,11 +221,11 @@ __device__ __forceinline__ int rounds_of(int n) { return (n + kRound - 1) / kRou
 __device__ __forceinline__ int pieces_of(int n, int per) { return max(1, (rounds_of(n) + per - 1) / per); }
 // The sequence with the piece id / heads (by_seq false), or sequence id.  False
 // if there is no such piece.
-__device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t* count, int T, int heads, int id,
-                                         bool by_seq) {
+__device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t* count, int T, int heads, int target,
+                                         int id, bool by_seq) {
   if (c.nSeq == 1) {
     const int r = rounds_of(attended(c, count, 0, T));
-    p.per = (int)max((int64_t)1, ((int64_t)r * heads + kTarget - 1) / kTarget);
+    p.per = (int)max((int64_t)1, ((int64_t)r * heads + target - 1) / target);
     p.s = p.first = 0;
     p.pieces = max(1, (r + p.per - 1) / p.per);
     return by_seq || id < (int64_t)p.pieces * heads;
@@ -185,7 +235,7 @@ __device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t*
   for (int i = 0; i < each && s0 + i < c.nSeq; ++i) rounds += rounds_of(attended(c, count, s0 + i, T));
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) rounds += __shfl_xor(rounds, o, 64);
-  p.per = (int)max((int64_t)1, (rounds * heads + kTarget - 1) / kTarget);
+  p.per = (int)max((int64_t)1, (rounds * heads + target - 1) / target);
   int mine = 0;
   for (int i = 0; i < each && s0 + i < c.nSeq; ++i) mine += pieces_of(attended(c, count, s0 + i, T), p.per);
   int upto = mine;
@@ -277,24 +327,7 @@ struct ValueTile {
   }
 };
 
-// Maximum and sum over the 16 lanes of a row, by rotation.
-template <int N>
-__device__ __forceinline__ float row_turned(float x) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + N, 0xF, 0xF, false));
-}
-__device__ __forceinline__ float row_max(float x) {
-  x = fmaxf(x, row_turned<8>(x));
-  x = fmaxf(x, row_turned<4>(x));
-  x = fmaxf(x, row_turned<2>(x));
-  return fmaxf(x, row_turned<1>(x));
-}
-__device__ __forceinline__ float row_sum(float x) {
-  x += row_turned<8>(x);
-  x += row_turned<4>(x);
-  x += row_turned<2>(x);
-  return x + row_turned<1>(x);
-}
-// The same over the wave.
+// Over the wave.
 __device__ __forceinline__ float lane_value(float x, int l) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
 }
@@ -310,9 +343,9 @@ __device__ __forceinline__ float wave_sum(float x) {
 // G heads (1, 2, 4 or 8) of a kv head over one piece of a sequence.  Pieces that
 // are a whole sequence give the output, others their reference, sum and values.
 template <int NB, int G>
-__global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : NB > 2 ? 3 : 4) kv4_attn_kernel(Cache c, int layer, float* __restrict__ out,
+__global__ void __launch_bounds__(kThreads, kResident<NB>) kv4_attn_kernel(Cache c, int layer, float* __restrict__ out,
                                                             const float* __restrict__ q, int nH, int subs, float scale,
-                                                            int T, const int32_t* __restrict__ count,
+                                                            int T, const int32_t* __restrict__ count, int target,
                                                             float2* __restrict__ part_ml, float* __restrict__ part_o,
                                                             float* __restrict__ sc) {
   constexpr int dH = 32 * NB, NS = 8 / G, NA = (NB + NS - 1) / NS;  // sets of rows, blocks of a set
@@ -328,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : NB > 2 ? 3 : 4) kv4_att
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Plan p;
-  if (!plan_for(p, c, count, T, c.nKV * subs, blockIdx.x, false)) return;
+  if (!plan_for(p, c, count, T, c.nKV * subs, target, blockIdx.x, false)) return;
   p.per = __builtin_amdgcn_readfirstlane(p.per);
   p.first = __builtin_amdgcn_readfirstlane(p.first);
   p.pieces = __builtin_amdgcn_readfirstlane(p.pieces);
@@ -606,14 +639,13 @@ __global__ void __launch_bounds__(kThreads, NB > 4 ? 2 : NB > 2 ? 3 : 4) kv4_att
   }
 }
 
-// The pieces of every sequence joined: workgroups [0, nSeq nH) the output of a
-// query head, the rest (weights kept) the weights of 512 positions of a kv head.
+// The pieces of every sequence joined: workgroups [0, nSeq nH) the output of a query
+// head, the rest (weights kept) the weights of kJoin positions of a kv head.
 // Short launches, so loads that do not depend on each other go first: a head's
 // values of its first pieces beside its references, the scores beside them.
-constexpr int kWeightRows = 512;
-constexpr int kJoinPieces = 512;  // pieces whose factors are kept in LDS
-// Reference and 1 / sum of a head over its pieces, by one wave; w gets the
-// pieces' factors.
+constexpr int kJoinPieces = 1024;  // pieces whose factors are kept in LDS
+// Reference and sum of a head over its pieces, by one wave; w gets the pieces'
+// factors.
 __device__ __forceinline__ float2 join_head(const float2* __restrict__ ml, int G, int pieces, float* w) {
   const int lane = threadIdx.x & 63;
   float2 first = make_float2(-INFINITY, 0.f);
@@ -631,43 +663,35 @@ __device__ __forceinline__ float2 join_head(const float2* __restrict__ ml, int G
   return make_float2(m, wave_sum(l));
 }
 
-template <int NB>
-__global__ void __launch_bounds__(kThreads) kv4_join_kernel(Cache c, int layer, float* __restrict__ out, int nH,
-                                                            int subs, int G, int T, const int32_t* __restrict__ count,
-                                                            const float2* __restrict__ part_ml,
-                                                            const float* __restrict__ part_o,
-                                                            const float* __restrict__ sc, int chunks) {
-  constexpr int dH = 32 * NB, kLanes = kThreads / dH > 0 ? kThreads / dH : 1, kAhead = 8;
-  __shared__ float red[kThreads], factor[kJoinPieces], shm[64], shl[64];
+template <int NB, int kJoin>  // threads, and positions of a weights' workgroup
+__global__ void __launch_bounds__(kJoin) kv4_join_kernel(Cache c, int layer, float* __restrict__ out, int nH, int subs,
+                                                         int G, int T, const int32_t* __restrict__ count, int target,
+                                                         const float2* __restrict__ part_ml,
+                                                         const float* __restrict__ part_o,
+                                                         const float* __restrict__ sc, int chunks) {
+  constexpr int dH = 32 * NB, kLanes = kJoin / dH, kAhead = 4096 / kJoin, kJoinWaves = kJoin / 64;
+  __shared__ float red[kJoin], factor[kJoinPieces], shm[kJoinWaves], shl[kJoinWaves];
   const int group = nH / c.nKV, share = (group + subs - 1) / subs;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool weights = (int)blockIdx.x >= c.nSeq * nH;
   const int id = weights ? blockIdx.x - c.nSeq * nH : blockIdx.x;
   const int s = weights ? id / (c.nKV * chunks) : id / nH;
   Plan p;
-  plan_for(p, c, count, T, c.nKV * subs, s, true);
+  plan_for(p, c, count, T, c.nKV * subs, target, s, true);
   auto first_of = [&](int kvh, int r) {  // of query head r of its group
     return ((int64_t)p.first * c.nKV * subs + (int64_t)(kvh * subs + r / share) * p.pieces) * G + r % share;
   };
   if (weights) {
-    const int n = attended(c, count, s, T), kvh = id / chunks % c.nKV, at0 = id % chunks * kWeightRows;
-    if (at0 >= n) return;
-    constexpr int R = kWeightRows / kThreads;
-    float* w = c.weight + head_slot(c, layer, s, kvh);
-    float sum[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k) sum[k] = 0.f;
+    const int n = attended(c, count, s, T), kvh = id / chunks % c.nKV, at = id % chunks * kJoin + (int)threadIdx.x;
+    if (id % chunks * kJoin >= n) return;
+    float sum = 0.f;
     for (int h0 = 0; h0 < group; h0 += 4) {
-      float x[4][R];
+      float x[4];
 #pragma unroll
       for (int h = 0; h < 4; ++h)
-#pragma unroll
-        for (int k = 0; k < R; ++k) {
-          const int at = at0 + k * kThreads + threadIdx.x;
-          x[h][k] = h0 + h < group && at < n ? sc[((int64_t)s * nH + kvh * group + h0 + h) * c.maxSeq + at] : 0.f;
-        }
+        x[h] = h0 + h < group && at < n ? sc[((int64_t)s * nH + kvh * group + h0 + h) * c.maxSeq + at] : 0.f;
       __syncthreads();
-      if (h0 + wave < group) {
+      if (wave < 4 && h0 + wave < group) {
         const float2 v = join_head(part_ml + first_of(kvh, h0 + wave), G, p.pieces, nullptr);
         shm[wave] = v.x;
         shl[wave] = 1.f / v.y;
@@ -675,16 +699,9 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(Cache c, int layer, 
       __syncthreads();
 #pragma unroll
       for (int h = 0; h < 4; ++h)
-        if (h0 + h < group) {
-#pragma unroll
-          for (int k = 0; k < R; ++k) sum[k] += __builtin_amdgcn_exp2f(x[h][k] - shm[h]) * shl[h];
-        }
+        if (h0 + h < group) sum += __builtin_amdgcn_exp2f(x[h] - shm[h]) * shl[h];
     }
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int at = at0 + k * kThreads + threadIdx.x;
-      if (at < n) w[at] += sum[k];
-    }
+    if (at < n) c.weight[head_slot(c, layer, s, kvh) + at] += sum;
     return;
   }
   if (p.pieces == 1) return;
@@ -699,9 +716,8 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(Cache c, int layer, 
     const int k = z + u * kLanes;
     ahead[u] = z < kLanes && k < p.pieces ? po[k * step] : 0.f;
   }
-  float2 ml = make_float2(0.f, 0.f);
   if (wave == 0) {
-    ml = join_head(part_ml + first, G, p.pieces, factor);
+    const float2 ml = join_head(part_ml + first, G, p.pieces, factor);
     shm[0] = ml.x;
     shl[0] = ml.y;
   }
@@ -714,17 +730,16 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(Cache c, int layer, 
   };
   float v = 0.f;
   if (z < kLanes) {
+    for (int k0 = z; k0 < p.pieces; k0 += kAhead * kLanes) {
+      if (k0 != z) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (z + u * kLanes < p.pieces) v += ahead[u] * turn(z + u * kLanes);
-    int k = z + kAhead * kLanes;
-    for (; k + 7 * kLanes < p.pieces; k += 8 * kLanes) {
+        for (int u = 0; u < kAhead; ++u)
+          ahead[u] = k0 + u * kLanes < p.pieces ? po[(k0 + u * kLanes) * step] : 0.f;
+      }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) ahead[u] = po[(k + u * kLanes) * step];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v += ahead[u] * turn(k + u * kLanes);
+      for (int u = 0; u < kAhead; ++u)
+        if (k0 + u * kLanes < p.pieces) v += ahead[u] * turn(k0 + u * kLanes);
     }
-    for (; k < p.pieces; k += kLanes) v += po[k * step] * turn(k);
   }
   red[threadIdx.x] = v;
   __syncthreads();
@@ -1203,7 +1218,7 @@ extern "C" int fg_kv4_append(const fg_kv4_cache* c, int layer, const float* k, c
   if (T == 0) return FG_OK;
   fg::KProfScope prof("kv4_append", 0.0, rows * (8.0 * c->nKvHeads * c->dHead + slot_bytes(c)));
   KV4_DISPATCH(c->dHead, FG_LAUNCH(kv4_append_kernel<NB>, dim3((unsigned)blocks, 2), dim3(kThreads), 0, view(c), layer,
-                                   k, v, ld, T, count, rows));
+                                   k, v, ld, T, count, (uint32_t)rows));
   return FG_OK;
 }
 
@@ -1221,7 +1236,7 @@ extern "C" int fg_kv4_read(const fg_kv4_cache* c, int layer, float* k, float* v,
   if (T == 0) return FG_OK;
   fg::KProfScope prof("kv4_read", 0.0, rows * (8.0 * c->nKvHeads * c->dHead + slot_bytes(c)));
   KV4_DISPATCH(c->dHead, FG_LAUNCH(kv4_read_kernel<NB>, dim3((unsigned)blocks, 2), dim3(kThreads), 0, view(c), layer, k,
-                                   v, ld, first, T, rows));
+                                   v, ld, first, T, (uint32_t)rows));
   return FG_OK;
 }
 
@@ -1238,10 +1253,22 @@ extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const f
   const int group = nHeads / c->nKvHeads, subs = (group + 7) / 8, share = (group + subs - 1) / subs;
   const int G = share > 4 ? 8 : share > 2 ? 4 : share;
   const int64_t heads = (int64_t)c->nSeq * c->nKvHeads * subs, rounds = (c->maxSeq + kRound - 1) / kRound;
-  const int64_t grid = heads * rounds < heads + kTarget ? heads * rounds : heads + kTarget;
-  const int64_t chunks = c->weight ? (c->maxSeq + kWeightRows - 1) / kWeightRows : 0;
+  // One sequence: equal pieces, all resident at once (130001 positions of 8 heads
+  // 32.6 us, in pieces of half the size 37.4).  Several: their last pieces are
+  // shorter, pieces of half the size even that out (32 sequences up to 8192
+  // 40.6 us, else 47.6).
+  const int cus = fg::device_cu_count() > 0 ? fg::device_cu_count() : 256;
+  int target = 0;
+  KV4_DISPATCH(c->dHead, target = kResident<NB> * cus);
+  if (c->nSeq > 1) target *= 2;
+  const int64_t grid = heads * rounds < heads + target ? heads * rounds : heads + target;
+  // Few heads of many pieces each are fetched by many threads (32 heads of 96
+  // pieces 5.4 us, with 256 threads 9.0); others by small workgroups (1024 heads of
+  // up to 11 pieces 6.4 us, with 1024 threads 12.4; 96 heads of up to 8 4.1 and 5.5).
+  const int kJoin = rounds > 64 && (int64_t)c->nSeq * nHeads <= 256 ? 1024 : 256;
+  const int64_t chunks = c->weight ? (c->maxSeq + kJoin - 1) / kJoin : 0;
   const int64_t join = (int64_t)c->nSeq * nHeads + (int64_t)c->nSeq * c->nKvHeads * chunks;
-  FG_ARG_CHECK(grid <= INT32_MAX / kThreads && join <= INT32_MAX / kThreads,
+  FG_ARG_CHECK(grid <= INT32_MAX / kThreads && join <= INT32_MAX / kJoin,
                "fg_kv4_attn: %d sequences x %d heads x %d slots are too many", c->nSeq, nHeads, c->maxSeq);
   // references and sums, values, and the scores where weights are kept
   const size_t ml = (size_t)grid * G * sizeof(float2), po = rounds > 1 ? (size_t)grid * G * c->dHead * sizeof(float) : 0;
@@ -1253,16 +1280,21 @@ extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const f
   float* sc = c->weight ? (float*)((uint8_t*)ws.ptr + ml + po) : nullptr;
 #define KV4_ATTN(GS)                                                                                              \
   FG_LAUNCH((kv4_attn_kernel<NB, GS>), dim3((unsigned)grid), dim3(kThreads), 0, view(c), layer, out, q, nHeads, subs, \
-            (float)scale, T, count, part_ml, part_o, sc)
+            (float)scale, T, count, target, part_ml, part_o, sc)
+#define KV4_JOIN(J)                                                                                               \
+  FG_LAUNCH((kv4_join_kernel<NB, J>), dim3((unsigned)join), dim3(J), 0, view(c), layer, out, nHeads, subs, G, T, count, \
+            target, (const float2*)part_ml, (const float*)part_o, (const float*)sc, (int)chunks)
   KV4_DISPATCH(c->dHead, {
     if (G == 1) KV4_ATTN(1);
     else if (G == 2) KV4_ATTN(2);
     else if (G == 4) KV4_ATTN(4);
     else KV4_ATTN(8);
-    if (rounds > 1 || c->weight)
-      FG_LAUNCH(kv4_join_kernel<NB>, dim3((unsigned)join), dim3(kThreads), 0, view(c), layer, out, nHeads, subs, G, T,
-                count, (const float2*)part_ml, (const float*)part_o, (const float*)sc, (int)chunks);
+    if (rounds > 1 || c->weight) {
+      if (kJoin == 1024) KV4_JOIN(1024);
+      else KV4_JOIN(256);
+    }
   });
+#undef KV4_JOIN
 #undef KV4_ATTN
   return FG_OK;
 }

@@ -149,6 +149,34 @@ def test_append_edges(fh, dH):
     np.testing.assert_array_equal(out2.numpy(), out.numpy())
 
 
+@pytest.mark.parametrize("kind", ["zero", "tie", "overflow", "almost", "inf", "nan", "tiny", "one"])
+def test_append_edges_alone(fh, kind):
+    """Every row of the same kind, so that none takes its neighbours' path."""
+    rng = np.random.default_rng(3)
+    T, dH = 64, 64
+    x = rows(rng, T, dH)
+    far = x.reshape(T, 2, 32)
+    if kind == "zero":
+        x[:] = 0.0
+    elif kind == "one":
+        x[:] = 0.0
+        far[:, :, 5] = rng.standard_normal((T, 2))
+    elif kind == "tie":
+        far[:, :, 30], far[:, :, 2] = 99.0, -99.0
+    elif kind == "tiny":
+        x *= 1e-7
+    else:
+        far[:, :, 9] = {"overflow": -8 * 65520.0, "almost": 8 * 65519.0, "inf": -np.inf, "nan": np.nan}[kind]
+    c = Cache(fh, 1, 1, 1, dH, T)
+    d = fh.DeviceArray.from_numpy(x)
+    c.call("append", 0, d, d, dH, T, None)
+    ok, ov = fh.DeviceArray((T, dH)), fh.DeviceArray((T, dH))
+    c.call("read", 0, ok, ov, dH, 0, T)
+    codes, steps = ref.quantize(x)
+    np.testing.assert_array_equal(ok.numpy(), ref.values(ref.pack(codes), steps).astype(np.float32))
+    np.testing.assert_array_equal(ov.numpy(), ok.numpy())
+
+
 # ── attention ─────────────────────────────────────────────────────────────
 def check_attend(fh, c, nH, rng, lens, T=0, count=None, scale=None, q=None, layer=0):
     scale = 1 / np.sqrt(c.dH) if scale is None else scale
