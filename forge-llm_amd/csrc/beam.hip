@@ -336,62 +336,111 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
 }
 
 // ── states ────────────────────────────────────────────────────────────────
-// A thread holds one place of a part, `U` bytes of it, in every beam of the
-// request: it reads what the beams take, then writes, so no second buffer and
-// no order between threads is needed.
+// A thread holds one place of a part, sizeof(U) bytes of it, in every beam of the
+// request: it reads what the beams take, then writes, so no second buffer and no
+// order between threads is needed, and a beam that goes on from itself costs
+// nothing.  HBM-bound: a parent that several beams take is fetched once and read
+// again from the caches.  States of one unit size share a launch.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+struct State {
+  uint8_t* base;
+  int64_t beam_stride, outer_stride, inner_stride, row_bytes;
+  int inner, rows, first;  // first: the first of its parts among all
+};
+struct States {
+  State s[FG_BEAM_STATES];
+  int count;
+};
 template <typename U, int WM>
-__global__ void __launch_bounds__(kThreads) beam_reorder_kernel(uint8_t* __restrict__ base, int64_t beam_stride,
-                                                                int64_t outer_stride, int inner, int64_t inner_stride,
-                                                                int64_t row_bytes, int rows,
-                                                                const int32_t* __restrict__ parent,
+__global__ void __launch_bounds__(kThreads) beam_reorder_kernel(States all, const int32_t* __restrict__ parent,
                                                                 const int32_t* __restrict__ len, int W) {
-  __shared__ int from[WM];
-  __shared__ int64_t end[WM];
+  __shared__ int64_t from[WM], end[WM], most;  // where a beam's bytes come from, how many
+  int k = 0;
+  while (k + 1 < all.count && (int)blockIdx.y >= all.s[k + 1].first) ++k;
+  const State& s = all.s[k];
   const int64_t r0 = (int64_t)blockIdx.z * W;
-  if (threadIdx.x < WM) {
-    int p = threadIdx.x;
+  if (threadIdx.x < 64) {
+    const int b = threadIdx.x;
+    int p = b;
     int64_t e = 0;
-    if (p < W) {
-      const int q = parent[r0 + p];
-      if (q >= 0 && q < W && q != p) {
+    if (b < W) {
+      const int q = parent[r0 + b];
+      if (q >= 0 && q < W && q != b) {
         p = q;
-        e = (len ? min(max(len[r0 + p], 0), rows) : rows) * row_bytes;
+        e = (len ? min(max(len[r0 + p], 0), s.rows) : s.rows) * s.row_bytes;
       }
     }
-    from[threadIdx.x] = p;
-    end[threadIdx.x] = e;
+    if (b < WM) {
+      from[b] = p * s.beam_stride;
+      end[b] = e;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const int64_t u = __shfl_xor((long long)e, o, 64);
+      e = u > e ? u : e;
+    }
+    if (b == 0) most = e;
   }
   __syncthreads();
-  uint8_t* part = base + r0 * beam_stride + (blockIdx.y / inner) * outer_stride + (blockIdx.y % inner) * inner_stride;
-  int64_t most = 0;
-  for (int b = 0; b < W; ++b) most = end[b] > most ? end[b] : most;
-  for (int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * sizeof(U); at < most;
-       at += (int64_t)gridDim.x * kThreads * sizeof(U)) {
+  const int part_of = blockIdx.y - s.first;
+  uint8_t* part = s.base + r0 * s.beam_stride + (part_of / s.inner) * s.outer_stride +
+                  (part_of % s.inner) * s.inner_stride;
+  constexpr int64_t step = sizeof(U);
+  for (int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * step; at < most;
+       at += (int64_t)gridDim.x * kThreads * step) {
     U v[WM];
+    bool cut = false;
+#pragma unroll
+    for (int b = 0; b < WM; ++b) {
+      if (at + step <= end[b]) v[b] = *reinterpret_cast<const U*>(part + from[b] + at);
+      else cut |= at < end[b];
+    }
+    if (step > 2 && cut) {
+      // a beam's last bytes, less than a unit, two at a time: nothing of this unit
+      // has been written yet, and these two bytes of it are read before they are
+      for (int64_t e = at; e < at + step; e += 2) {
+        uint16_t t[WM];
+#pragma unroll
+        for (int b = 0; b < WM; ++b)
+          if (at + step > end[b] && e < end[b]) t[b] = *reinterpret_cast<const uint16_t*>(part + from[b] + e);
+#pragma unroll
+        for (int b = 0; b < WM; ++b)
+          if (at + step > end[b] && e < end[b])
+            *reinterpret_cast<uint16_t*>(part + b * s.beam_stride + e) = t[b];
+      }
+    }
 #pragma unroll
     for (int b = 0; b < WM; ++b)
-      if (at < end[b]) v[b] = *reinterpret_cast<const U*>(part + from[b] * beam_stride + at);
-#pragma unroll
-    for (int b = 0; b < WM; ++b)
-      if (at < end[b]) *reinterpret_cast<U*>(part + b * beam_stride + at) = v[b];
+      if (at + step <= end[b]) *reinterpret_cast<U*>(part + b * s.beam_stride + at) = v[b];
   }
 }
 
+// The states of unit size U among all (units[i] of each).
 template <typename U>
-int launch_reorder(const fg_beam_state& s, const int32_t* parent, const int32_t* len, int nReq, int W) {
-  const int64_t units = s.row_bytes * s.rows / (int64_t)sizeof(U);
-  const int64_t parts = (int64_t)s.outer * s.inner;
-  int64_t gx = (units + kThreads - 1) / kThreads;
+int launch_reorder(const fg_beam_state* states, int count, const int* units, const int32_t* parent, const int32_t* len,
+                   int nReq, int W) {
+  States all{};
+  int64_t parts = 0, longest = 0;
+  for (int i = 0; i < count; ++i) {
+    const fg_beam_state& s = states[i];
+    if (units[i] != (int)sizeof(U) || s.rows == 0) continue;
+    all.s[all.count++] = {(uint8_t*)s.base, s.beam_stride, s.outer_stride, s.inner_stride, s.row_bytes, s.inner, s.rows,
+                          (int)parts};
+    parts += (int64_t)s.outer * s.inner;
+    const int64_t n = (s.row_bytes * s.rows + sizeof(U) - 1) / sizeof(U);
+    longest = n > longest ? n : longest;
+  }
+  if (!all.count) return FG_OK;
+  int64_t gx = (longest + kThreads - 1) / kThreads;
   if (gx > 4096) gx = 4096;
-#define REORDER(WM)                                                                                                   \
-  FG_LAUNCH((beam_reorder_kernel<U, WM>), dim3((unsigned)gx, (unsigned)parts, (unsigned)nReq), dim3(kThreads), 0,     \
-            (uint8_t*)s.base, s.beam_stride, s.outer_stride, s.inner, s.inner_stride, s.row_bytes, s.rows, parent, len, \
-            W)
+  const dim3 grid((unsigned)gx, (unsigned)parts, (unsigned)nReq);
+#define REORDER(WM) FG_LAUNCH((beam_reorder_kernel<U, WM>), grid, dim3(kThreads), 0, all, parent, len, W)
   if (W <= 4) REORDER(4);
   else if (W <= 8) REORDER(8);
   else if (W <= 16) REORDER(16);
   else if (W <= 32) REORDER(32);
-  else REORDER(64);
+  else if constexpr (sizeof(U) <= 8) REORDER(64);  // more beams than 32 in units of up to 8 bytes
 #undef REORDER
   return FG_OK;
 }
@@ -447,7 +496,8 @@ extern "C" int fg_beam_reorder(const fg_beam_state* states, int count, const int
   for (int i = 0; i < count; ++i) {
     const fg_beam_state& s = states[i];
     FG_ARG_CHECK(s.base, "fg_beam_reorder: state %d is null", i);
-    FG_ARG_CHECK(s.outer > 0 && s.inner > 0 && (int64_t)s.outer * s.inner <= 65535 && s.rows >= 0 && s.row_bytes >= 2,
+    FG_ARG_CHECK(s.outer > 0 && s.inner > 0 && (int64_t)s.outer * s.inner <= 65535 / FG_BEAM_STATES && s.rows >= 0 &&
+                     s.row_bytes >= 2,
                  "fg_beam_reorder: state %d: %d x %d parts of %d rows of %lld bytes", i, s.outer, s.inner, s.rows,
                  (long long)s.row_bytes);
     FG_ARG_CHECK((((uintptr_t)s.base | s.beam_stride | s.outer_stride | s.inner_stride | s.row_bytes) & 1) == 0,
@@ -458,15 +508,18 @@ extern "C" int fg_beam_reorder(const fg_beam_state* states, int count, const int
   }
   FG_REQUIRE_INIT();
   fg::KProfScope prof("beam_reorder", 0.0, bytes);
+  if (W == 1) return FG_OK;
+  int units[FG_BEAM_STATES];
   for (int i = 0; i < count; ++i) {
     const fg_beam_state& s = states[i];
-    if (s.rows == 0 || W == 1) continue;
-    const uintptr_t all = (uintptr_t)s.base | s.beam_stride | s.outer_stride | s.inner_stride | s.row_bytes;
-    const int rc = all % 16 == 0 && W <= 32 ? launch_reorder<uint4>(s, parent, len, nReq, W)
-                   : all % 8 == 0           ? launch_reorder<uint2>(s, parent, len, nReq, W)
-                   : all % 4 == 0           ? launch_reorder<uint32_t>(s, parent, len, nReq, W)
-                                            : launch_reorder<uint16_t>(s, parent, len, nReq, W);
-    if (rc != FG_OK) return rc;
+    const uintptr_t all = (uintptr_t)s.base | s.beam_stride | s.outer_stride | s.inner_stride;
+    units[i] = all % 16 == 0 && W <= 32 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
   }
-  return FG_OK;
+  const int rc = launch_reorder<u32x4>(states, count, units, parent, len, nReq, W);
+  if (rc != FG_OK) return rc;
+  const int rc8 = launch_reorder<u32x2>(states, count, units, parent, len, nReq, W);
+  if (rc8 != FG_OK) return rc8;
+  const int rc4 = launch_reorder<uint32_t>(states, count, units, parent, len, nReq, W);
+  if (rc4 != FG_OK) return rc4;
+  return launch_reorder<uint16_t>(states, count, units, parent, len, nReq, W);
 }

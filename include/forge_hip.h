@@ -743,7 +743,7 @@ typedef struct fg_beam_state {
 /* Beam b of request r takes what beam parent[r W + b] of the request has, in
  * place: the first len[r W + parent] rows of every part (len NULL or beyond: all;
  * below 0: none), the rest left as it was.  parent outside [0, W) means b itself.
- * Up to 8 states a call, 1 <= W <= 64. */
+ * Up to 8 states a call, each of up to 8191 parts; 1 <= W <= 64, nReq <= 65535. */
 #define FG_BEAM_STATES 8
 int fg_beam_reorder(const fg_beam_state* states, int count, const int32_t* parent, const int32_t* len, int nReq,
                     int W);
