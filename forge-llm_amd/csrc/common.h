@@ -86,6 +86,9 @@ struct XpSpec {
 constexpr int kMaxXpSpecs = 8;
 int absmax_parts(const XpSpec* specs, int count, const char* prof_name);
 
+// What every entry point over a 4-bit cache checks of it; `fn` names the caller.
+int check_kv4_cache(const fg_kv4_cache* c, const char* fn);
+
 }  // namespace fg
 
 #define FG_HIP_CHECK(expr)                                                          \

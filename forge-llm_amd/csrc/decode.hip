@@ -191,7 +191,9 @@ __global__ void __launch_bounds__(kThreads) dec_embed_kernel(float* __restrict__
 // Row pairs (n, n+1) per wave: RoPE rotates adjacent pairs, so a pair's two
 // dot products are all its rotation needs.  With emb (layer 0) the input
 // vector is the token's embedding row (NaN for a token outside [0,V)), which
-// workgroup 0 also stores into x for the residual stream.
+// workgroup 0 also stores into x for the residual stream.  Position p's K and V go to
+// row p of the cache, pos_stride apart (0: the one row of a caller that stores them
+// itself).
 template <int QT>
 __global__ void __launch_bounds__(kThreads) dec_qkv_kernel(float* __restrict__ q, float* __restrict__ kc,
                                                            float* __restrict__ vc, float* __restrict__ x,
@@ -201,7 +203,8 @@ __global__ void __launch_bounds__(kThreads) dec_qkv_kernel(float* __restrict__ q
                                                            const float* __restrict__ rcos,
                                                            const float* __restrict__ rsin,
                                                            const int32_t* __restrict__ state, int D, int qD, int kvD,
-                                                           int dH, int maxSeq, int64_t layer_off) {
+                                                           int dH, int maxSeq, int64_t layer_off,
+                                                           int pos_stride) {
 #pragma clang fp contract(off)
   extern __shared__ __attribute__((aligned(16))) float xn[];
   __shared__ double sh[kWaves];
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) dec_qkv_kernel(float* __restrict__ q
   const int pos = state[1];
   if (pos < 0 || pos >= maxSeq) return;  // the host rejects such positions
   const int half = dH >> 1;
-  const int64_t cache_off = layer_off + (int64_t)pos * kvD;
+  const int64_t cache_off = layer_off + (int64_t)pos * pos_stride;
   for (bool first = true; pr < pairs; pr += stride, first = false) {
     const int n = 2 * pr;
     if (!first) {
@@ -760,6 +763,7 @@ struct QkvOp {
   const int32_t* state;
   int D, qD, kvD, dH, maxSeq;
   int64_t layer_off;
+  int pos_stride;
   __device__ int rows() const { return qD + 2 * kvD; }
   __device__ const uint8_t* row(int n) const { return W + min(n, rows() - 1) * rb; }
   template <int QT>
@@ -774,7 +778,7 @@ struct QkvOp {
     const int pos = state[1];
     if (pos < 0 || pos >= maxSeq) return;  // the host rejects such positions
     const int half = dH >> 1;
-    const int64_t cache_off = layer_off + (int64_t)pos * kvD;
+    const int64_t cache_off = layer_off + (int64_t)pos * pos_stride;
 #pragma unroll
     for (int r = 0; r < kUnitRows; r += 2) {  // rows() is even: whole pairs
       const int n = n0 + r;
@@ -1019,6 +1023,150 @@ unsigned grid_for_waves(int64_t waves) {
   return (unsigned)(g < 1 ? 1 : g);
 }
 
+// The launches of one step that f32 and 4-bit caches share, for one token: x, q, h
+// and logits are its vectors, state its {token, position}.
+struct Step {
+  const fg_decode_model* m;
+  int D, H, V, nH, nKV, dH, qD, kvD;
+  size_t lds_qkv;
+  bool emb_f32, vec;  // vec: the unit kernels read the vectors as float4
+};
+int check_model(const fg_decode_model* m, const char* fn, Step& st, double& wbytes) {
+  FG_ARG_CHECK(m, "%s: null argument", fn);
+  const int D = m->dim, H = m->hidden, L = m->nLayers, nH = m->nHeads, nKV = m->nKvHeads, V = m->vocab;
+  FG_ARG_CHECK(D > 0 && H > 0 && L > 0 && nH > 0 && nKV > 0 && V > 0 && m->maxSeq > 0, "%s: bad dimensions", fn);
+  FG_ARG_CHECK(nH % nKV == 0 && D % nH == 0, "%s: nHeads %d must divide dim %d and be a multiple of "
+               "nKvHeads %d", fn, nH, D, nKV);
+  const int dH = D / nH, qD = nH * dH, kvD = nKV * dH;
+  FG_ARG_CHECK(dH % 2 == 0 && dH <= 1024, "%s: head dim %d must be even and <= 1024", fn, dH);
+  st = {m, D, H, V, nH, nKV, dH, qD, kvD, 2 * (size_t)D * sizeof(float), m->emb_type == fgq::kF32, false};
+  FG_ARG_CHECK(m->layers && m->tok_emb && m->ln_f && m->wcls && m->rope_cos && m->rope_sin && m->x && m->q && m->h,
+               "%s: null model pointer", fn);
+  // Every matrix: a known ggml type whose blocks tile its rows (K = dim, or hidden for down).
+  auto type_ok = [](int t, int K) { return fgq::known_type(t) && K % fgq::block_elems(t) == 0; };
+  FG_ARG_CHECK(type_ok(m->emb_type, D) && type_ok(m->cls_type, D),
+               "%s: tok_emb type %d / wcls type %d is unsupported or does not tile dim %d", fn, m->emb_type,
+               m->cls_type, D);
+  int64_t bytes = fgq::row_bytes(m->cls_type, D) * (int64_t)V;
+  for (int l = 0; l < L; ++l) {
+    const fg_decode_layer& ly = m->layers[l];
+    FG_ARG_CHECK(ly.ln1 && ly.wqkv && ly.wo && ly.ln2 && ly.gate && ly.up && ly.down,
+                 "%s: layer %d has a null weight", fn, l);
+    FG_ARG_CHECK(type_ok(ly.wqkv_type, D) && type_ok(ly.wo_type, D) && type_ok(ly.gate_type, D) &&
+                     type_ok(ly.down_type, H) && ly.up_type == ly.gate_type,
+                 "%s: layer %d: weight types wqkv %d wo %d gate %d up %d down %d (gate and up must "
+                 "match; each type must tile its rows of %d / %d)", fn, l, ly.wqkv_type, ly.wo_type, ly.gate_type,
+                 ly.up_type, ly.down_type, D, H);
+    bytes += fgq::row_bytes(ly.wqkv_type, D) * (qD + 2 * kvD) + fgq::row_bytes(ly.wo_type, D) * D +
+             2 * fgq::row_bytes(ly.gate_type, D) * H + fgq::row_bytes(ly.down_type, H) * D;
+  }
+  wbytes = (double)bytes;
+  return FG_OK;
+}
+
+int step_embed(const Step& st, float* x, const int32_t* state) {
+  if (st.emb_f32) return FG_OK;  // the first layer reads it
+  const uint8_t* emb = static_cast<const uint8_t*>(st.m->tok_emb);
+  const int64_t erb = fgq::row_bytes(st.m->emb_type, st.D);
+  const unsigned g = (unsigned)((st.D + kThreads - 1) / kThreads);
+  FGQ_DISPATCH(st.m->emb_type, {
+    FG_LAUNCH(dec_embed_kernel<QT>, dim3(g), dim3(kThreads), 0, x, emb, erb, st.V, state, st.D);
+  });
+  return FG_OK;
+}
+
+int step_qkv(const Step& st, int l, float* x, float* q, float* kcache, float* vcache, const int32_t* state,
+             int64_t layer_off, int pos_stride) {
+  const fg_decode_model* m = st.m;
+  const fg_decode_layer& ly = m->layers[l];
+  const int D = st.D, qD = st.qD, kvD = st.kvD, dH = st.dH, V = st.V;
+  const float* emb0 = (l == 0 && st.emb_f32) ? static_cast<const float*>(m->tok_emb) : nullptr;
+  const uint8_t* W = static_cast<const uint8_t*>(ly.wqkv);
+  const int64_t rb = fgq::row_bytes(ly.wqkv_type, D);
+  if (st.vec && aligned16(ly.ln1) && use_units(kAfterNorm, ly.wqkv_type, W, D, qD + 2 * kvD)) {
+    const QkvOp op{q, kcache, vcache, x, emb0, V, ly.ln1, m->normEps, W, rb, m->rope_cos, m->rope_sin, state,
+                   D, qD, kvD, dH, m->maxSeq, layer_off, pos_stride};
+    FGQ_DISPATCH(ly.wqkv_type, {
+      const int rc = launch_unit<QT>(op, qD + 2 * kvD, D);
+      if (rc) return rc;
+    });
+  } else FGQ_DISPATCH(ly.wqkv_type, {
+    FG_LAUNCH(dec_qkv_kernel<QT>, dim3(grid_for_waves((qD + 2 * kvD) / 2)), dim3(kThreads), st.lds_qkv, q, kcache,
+              vcache, x, emb0, V, ly.ln1, m->normEps, W, rb, m->rope_cos, m->rope_sin, state, D, qD, kvD, dH, m->maxSeq,
+              layer_off, pos_stride);
+  });
+  return FG_OK;
+}
+
+// x += W in (the down projection, or the output projection of an attention that
+// is whole): N rows of K.
+int step_residual(const Step& st, UnitAt at, float* x, const float* in, const void* weight, int type, int N, int K) {
+  const uint8_t* W = static_cast<const uint8_t*>(weight);
+  const int64_t rb = fgq::row_bytes(type, K);
+  if (st.vec && use_units(at, type, W, K, N)) {
+    const ResidOp op{x, in, W, rb, N, K};
+    FGQ_DISPATCH(type, {
+      const int rc = launch_unit<QT>(op, N, K);
+      if (rc) return rc;
+    });
+  } else FGQ_DISPATCH(type, {
+    FG_LAUNCH(dec_down_kernel<QT>, dim3(grid_for_waves(N)), dim3(kThreads), K * sizeof(float), x, in, W, rb, N, K);
+  });
+  return FG_OK;
+}
+
+int step_ffn(const Step& st, int l, float* x, float* h) {
+  const fg_decode_layer& ly = st.m->layers[l];
+  const int D = st.D, H = st.H;
+  const uint8_t* Wg = static_cast<const uint8_t*>(ly.gate);
+  const uint8_t* Wu = static_cast<const uint8_t*>(ly.up);
+  const int64_t rb = fgq::row_bytes(ly.gate_type, D);
+  const double eps = st.m->normEps;
+  if (st.vec && aligned16(ly.ln2) && use_units(kAfterNorm, ly.gate_type, Wg, D, 2 * H) && aligned16(Wu)) {
+    const GateUpOp op{h, x, ly.ln2, eps, Wg, Wu, rb, H, D};
+    FGQ_DISPATCH(ly.gate_type, {
+      const int rc = launch_unit<QT>(op, 2 * H, D);
+      if (rc) return rc;
+    });
+  } else FGQ_DISPATCH(ly.gate_type, {
+    FG_LAUNCH(dec_gateup_kernel<QT>, dim3(grid_for_waves(H)), dim3(kThreads), D * sizeof(float), h, x, ly.ln2, eps, Wg,
+              Wu, rb, H, D);
+  });
+  return step_residual(st, kDown, x, h, ly.down, ly.down_type, D, H);
+}
+
+int step_head(const Step& st, float* logits, const float* x) {
+  const fg_decode_model* m = st.m;
+  const uint8_t* W = static_cast<const uint8_t*>(m->wcls);
+  const int D = st.D, V = st.V;
+  const int64_t rb = fgq::row_bytes(m->cls_type, D);
+  if (st.vec && use_units(kAfterNorm, m->cls_type, W, D, V)) {
+    const HeadOp op{logits, x, m->ln_f, m->normEps, W, rb, V, D};
+    FGQ_DISPATCH(m->cls_type, {
+      const int rc = launch_unit<QT>(op, V, D);
+      if (rc) return rc;
+    });
+  } else FGQ_DISPATCH(m->cls_type, {
+    FG_LAUNCH(dec_head_kernel<QT>, dim3(grid_for_waves((V + 1) / 2)), dim3(kThreads), D * sizeof(float), logits, x,
+              m->ln_f, m->normEps, W, rb, V, D);
+  });
+  return FG_OK;
+}
+
+// Sequence s's {token, position} and whether it takes part: a token of the
+// vocabulary, a position of the RoPE table and a free slot; else {-1, 0}.
+__global__ void kv4_states_kernel(int32_t* __restrict__ state, int32_t* __restrict__ count,
+                                  const int32_t* __restrict__ tokens, const int32_t* __restrict__ len,
+                                  const int32_t* __restrict__ next, int nSeq, int V, int maxPos, int maxSeq) {
+  const int s = blockIdx.x * kThreads + threadIdx.x;
+  if (s >= nSeq) return;
+  const int t = tokens[s], p = next[s];
+  const bool on = t >= 0 && t < V && p >= 0 && p < maxPos && len[s] < maxSeq;
+  state[2 * s] = on ? t : -1;
+  state[2 * s + 1] = on ? p : 0;
+  count[s] = on;
+}
+
 template <int LP, int C = 1>
 int launch_attn(const fg_decode_model* m, float* kcache, float* vcache, const int32_t* state, int dH,
                 int64_t layer_off, double scale, int S) {
@@ -1033,77 +1181,31 @@ extern "C" int fg_decode_step(const fg_decode_model* m, float* kcache, float* vc
                               float* logits) {
   FG_REQUIRE_INIT();
   FG_ARG_CHECK(m && kcache && vcache && state && logits, "fg_decode_step: null argument");
-  const int D = m->dim, H = m->hidden, L = m->nLayers, nH = m->nHeads, nKV = m->nKvHeads, V = m->vocab;
-  FG_ARG_CHECK(D > 0 && H > 0 && L > 0 && nH > 0 && nKV > 0 && V > 0 && m->maxSeq > 0,
-               "fg_decode_step: bad dimensions");
-  FG_ARG_CHECK(nH % nKV == 0 && D % nH == 0, "fg_decode_step: nHeads %d must divide dim %d and be a multiple of "
-               "nKvHeads %d", nH, D, nKV);
-  const int dH = D / nH, qD = nH * dH, kvD = nKV * dH;
-  FG_ARG_CHECK(dH % 2 == 0 && dH <= 1024, "fg_decode_step: head dim %d must be even and <= 1024", dH);
+  Step st;
+  double wbytes;
+  const int rc0 = check_model(m, "fg_decode_step", st, wbytes);
+  if (rc0) return rc0;
+  const int D = st.D, H = st.H, L = m->nLayers, nH = st.nH, nKV = st.nKV, dH = st.dH, kvD = st.kvD;
   const int S = (m->maxSeq + kChunk - 1) / kChunk;
-  const size_t lds_qkv = 2 * (size_t)D * sizeof(float);
   const size_t lds_wo = (size_t)((D + 3) & ~3) * sizeof(float) + ((size_t)nH * S + 2 * nH) * sizeof(double);
-  FG_ARG_CHECK(lds_qkv <= 64 * 1024 && lds_wo <= 64 * 1024 && (size_t)H * sizeof(float) <= 64 * 1024,
+  FG_ARG_CHECK(st.lds_qkv <= 64 * 1024 && lds_wo <= 64 * 1024 && (size_t)H * sizeof(float) <= 64 * 1024,
                "fg_decode_step: dim %d / hidden %d / %d heads x %d chunks exceed the 64 KiB LDS of a launch", D, H,
                nH, S);
-  FG_ARG_CHECK(m->layers && m->tok_emb && m->ln_f && m->wcls && m->rope_cos && m->rope_sin && m->x && m->q &&
-                   m->h && m->attn_part,
-               "fg_decode_step: null model pointer");
-  // Every matrix: a known ggml type whose blocks tile its rows (K = dim, or hidden for down).
-  auto type_ok = [](int t, int K) { return fgq::known_type(t) && K % fgq::block_elems(t) == 0; };
-  FG_ARG_CHECK(type_ok(m->emb_type, D) && type_ok(m->cls_type, D),
-               "fg_decode_step: tok_emb type %d / wcls type %d is unsupported or does not tile dim %d", m->emb_type,
-               m->cls_type, D);
-  int64_t wbytes = fgq::row_bytes(m->cls_type, D) * (int64_t)V;
-  for (int l = 0; l < L; ++l) {
-    const fg_decode_layer& ly = m->layers[l];
-    FG_ARG_CHECK(ly.ln1 && ly.wqkv && ly.wo && ly.ln2 && ly.gate && ly.up && ly.down,
-                 "fg_decode_step: layer %d has a null weight", l);
-    FG_ARG_CHECK(type_ok(ly.wqkv_type, D) && type_ok(ly.wo_type, D) && type_ok(ly.gate_type, D) &&
-                     type_ok(ly.down_type, H) && ly.up_type == ly.gate_type,
-                 "fg_decode_step: layer %d: weight types wqkv %d wo %d gate %d up %d down %d (gate and up must "
-                 "match; each type must tile its rows of %d / %d)", l, ly.wqkv_type, ly.wo_type, ly.gate_type,
-                 ly.up_type, ly.down_type, D, H);
-    wbytes += fgq::row_bytes(ly.wqkv_type, D) * (qD + 2 * kvD) + fgq::row_bytes(ly.wo_type, D) * D +
-              2 * fgq::row_bytes(ly.gate_type, D) * H + fgq::row_bytes(ly.down_type, H) * D;
-  }
-  const double eps = m->normEps;
+  FG_ARG_CHECK(m->attn_part, "fg_decode_step: null model pointer");
   const double scale = 1.0 / sqrt((double)dH);
   int LP = 1;
   while (4 * LP < dH && LP < 64) LP <<= 1;
-  fg::KProfScope prof("decode_step", 0.0, (double)wbytes);
-  const bool emb_f32 = m->emb_type == fgq::kF32;
+  fg::KProfScope prof("decode_step", 0.0, wbytes);
   // the unit kernels read the vectors as float4
   const bool vec = aligned16(m->x) && aligned16(m->q) && aligned16(m->h) && aligned16(m->tok_emb) && aligned16(m->ln_f);
-  if (!emb_f32) {
-    const uint8_t* emb = static_cast<const uint8_t*>(m->tok_emb);
-    const int64_t erb = fgq::row_bytes(m->emb_type, D);
-    const unsigned g = (unsigned)((D + kThreads - 1) / kThreads);
-    FGQ_DISPATCH(m->emb_type, {
-      FG_LAUNCH(dec_embed_kernel<QT>, dim3(g), dim3(kThreads), 0, m->x, emb, erb, V, state, D);
-    });
-  }
+  st.vec = vec;
+  int rc = step_embed(st, m->x, state);
+  if (rc) return rc;
   for (int l = 0; l < L; ++l) {
     const fg_decode_layer& ly = m->layers[l];
     const int64_t layer_off = (int64_t)l * m->maxSeq * kvD;
-    const float* emb0 = (l == 0 && emb_f32) ? static_cast<const float*>(m->tok_emb) : nullptr;
-    {
-      const uint8_t* W = static_cast<const uint8_t*>(ly.wqkv);
-      const int64_t rb = fgq::row_bytes(ly.wqkv_type, D);
-      if (vec && aligned16(ly.ln1) && use_units(kAfterNorm, ly.wqkv_type, W, D, qD + 2 * kvD)) {
-        const QkvOp op{m->q, kcache, vcache, m->x, emb0, V, ly.ln1, eps, W, rb, m->rope_cos, m->rope_sin, state,
-                       D, qD, kvD, dH, m->maxSeq, layer_off};
-        FGQ_DISPATCH(ly.wqkv_type, {
-          const int rc = launch_unit<QT>(op, qD + 2 * kvD, D);
-          if (rc) return rc;
-        });
-      } else FGQ_DISPATCH(ly.wqkv_type, {
-        FG_LAUNCH(dec_qkv_kernel<QT>, dim3(grid_for_waves((qD + 2 * kvD) / 2)), dim3(kThreads), lds_qkv, m->q,
-                  kcache, vcache, m->x, emb0, V, ly.ln1, eps, W, rb, m->rope_cos, m->rope_sin, state, D, qD, kvD,
-                  dH, m->maxSeq, layer_off);
-      });
-    }
-    int rc;
+    rc = step_qkv(st, l, m->x, m->q, kcache, vcache, state, layer_off, kvD);
+    if (rc) return rc;
     const bool chunk = dH % 4 == 0 && dH > 16 && dH <= 256 && aligned16(m->q) && aligned16(kcache) && aligned16(vcache);
     const dim3 agrid(nH, S), ablock(kThreads);
 #define FG_CHUNK(LPS)                                                                                              \
@@ -1157,51 +1259,66 @@ extern "C" int fg_decode_step(const fg_decode_model* m, float* kcache, float* vc
                   (const double*)m->attn_part, state, W, rb, D, nH, dH, m->maxSeq, S);
       });
     }
-    {
-      const uint8_t* Wg = static_cast<const uint8_t*>(ly.gate);
-      const uint8_t* Wu = static_cast<const uint8_t*>(ly.up);
-      const int64_t rb = fgq::row_bytes(ly.gate_type, D);
-      if (vec && aligned16(ly.ln2) && use_units(kAfterNorm, ly.gate_type, Wg, D, 2 * H) && aligned16(Wu)) {
-        const GateUpOp op{m->h, m->x, ly.ln2, eps, Wg, Wu, rb, H, D};
-        FGQ_DISPATCH(ly.gate_type, {
-          const int rc = launch_unit<QT>(op, 2 * H, D);
-          if (rc) return rc;
-        });
-      } else FGQ_DISPATCH(ly.gate_type, {
-        FG_LAUNCH(dec_gateup_kernel<QT>, dim3(grid_for_waves(H)), dim3(kThreads), D * sizeof(float), m->h, m->x,
-                  ly.ln2, eps, Wg, Wu, rb, H, D);
-      });
+    rc = step_ffn(st, l, m->x, m->h);
+    if (rc) return rc;
+  }
+  return step_head(st, logits, m->x);
+}
+
+extern "C" int fg_decode_step_kv4(const fg_decode_model* m, const fg_kv4_cache* c, const int32_t* tokens,
+                                  float* logits) {
+  FG_ARG_CHECK(tokens && logits, "fg_decode_step_kv4: null argument");
+  Step st;
+  double wbytes;
+  int rc = check_model(m, "fg_decode_step_kv4", st, wbytes);
+  if (rc) return rc;
+  rc = fg::check_kv4_cache(c, "fg_decode_step_kv4");
+  if (rc) return rc;
+  FG_ARG_CHECK(c->nLayers == m->nLayers && c->nKvHeads == m->nKvHeads && c->dHead == st.dH,
+               "fg_decode_step_kv4: a cache of %d layers, %d kv heads of %d, %d sequences of %d for a model of %d, %d of "
+               "%d", c->nLayers, c->nKvHeads, c->dHead, c->nSeq, c->maxSeq, m->nLayers, m->nKvHeads, st.dH);
+  const int D = st.D, kvD = st.kvD, N = c->nSeq;
+  FG_ARG_CHECK(st.lds_qkv <= 64 * 1024 && (size_t)st.H * sizeof(float) <= 64 * 1024,
+               "fg_decode_step_kv4: dim %d / hidden %d exceed the 64 KiB LDS of a launch", D, st.H);
+  FG_REQUIRE_INIT();
+  fg::KProfScope prof("decode_step_kv4", 0.0, wbytes);
+  st.vec = aligned16(m->x) && aligned16(m->q) && aligned16(m->h) && aligned16(m->tok_emb) && aligned16(m->ln_f) &&
+           D % 4 == 0 && st.H % 4 == 0;
+  // new keys and values, attention, states and counts
+  fg::Workspace ws;
+  rc = ws.get((size_t)N * ((2 * (size_t)kvD + D) * sizeof(float) + 3 * sizeof(int32_t)));
+  if (rc) return rc;
+  float *k = (float*)ws.ptr, *v = k + (int64_t)N * kvD, *att = v + (int64_t)N * kvD;
+  int32_t *state = (int32_t*)(att + (int64_t)N * D), *count = state + 2 * N;
+  FG_LAUNCH(kv4_states_kernel, dim3((N + kThreads - 1) / kThreads), dim3(kThreads), 0, state, count, tokens,
+            (const int32_t*)c->len, (const int32_t*)c->next, N, st.V, m->maxSeq, c->maxSeq);
+  auto x = [&](int s) { return m->x + (int64_t)s * D; };
+  for (int s = 0; s < N; ++s) {
+    rc = step_embed(st, x(s), state + 2 * s);
+    if (rc) return rc;
+  }
+  for (int l = 0; l < m->nLayers; ++l) {
+    const fg_decode_layer& ly = m->layers[l];
+    for (int s = 0; s < N; ++s) {
+      rc = step_qkv(st, l, x(s), m->q + (int64_t)s * D, k + (int64_t)s * kvD, v + (int64_t)s * kvD, state + 2 * s, 0, 0);
+      if (rc) return rc;
     }
-    {
-      const uint8_t* W = static_cast<const uint8_t*>(ly.down);
-      const int64_t rb = fgq::row_bytes(ly.down_type, H);
-      if (vec && use_units(kDown, ly.down_type, W, H, D)) {
-        const ResidOp op{m->x, m->h, W, rb, D, H};
-        FGQ_DISPATCH(ly.down_type, {
-          const int rc = launch_unit<QT>(op, D, H);
-          if (rc) return rc;
-        });
-      } else FGQ_DISPATCH(ly.down_type, {
-        FG_LAUNCH(dec_down_kernel<QT>, dim3(grid_for_waves(D)), dim3(kThreads), H * sizeof(float), m->x,
-                  m->h, W, rb, D, H);
-      });
+    rc = fg_kv4_append(c, l, k, v, kvD, 1, count);
+    if (rc) return rc;
+    rc = fg_kv4_attn(c, l, att, m->q, st.nH, 1.0 / sqrt((double)st.dH), 1, count);
+    if (rc) return rc;
+    for (int s = 0; s < N; ++s) {
+      rc = step_residual(st, kWoCombined, x(s), att + (int64_t)s * D, ly.wo, ly.wo_type, D, D);
+      if (rc) return rc;
+      rc = step_ffn(st, l, x(s), m->h + (int64_t)s * st.H);
+      if (rc) return rc;
     }
   }
-  {
-    const uint8_t* W = static_cast<const uint8_t*>(m->wcls);
-    const int64_t rb = fgq::row_bytes(m->cls_type, D);
-    if (vec && use_units(kAfterNorm, m->cls_type, W, D, V)) {
-      const HeadOp op{logits, m->x, m->ln_f, eps, W, rb, V, D};
-      FGQ_DISPATCH(m->cls_type, {
-        const int rc = launch_unit<QT>(op, V, D);
-        if (rc) return rc;
-      });
-    } else FGQ_DISPATCH(m->cls_type, {
-      FG_LAUNCH(dec_head_kernel<QT>, dim3(grid_for_waves((V + 1) / 2)), dim3(kThreads), D * sizeof(float), logits,
-                m->x, m->ln_f, eps, W, rb, V, D);
-    });
+  for (int s = 0; s < N; ++s) {
+    rc = step_head(st, logits + (int64_t)s * st.V, x(s));
+    if (rc) return rc;
   }
-  return FG_OK;
+  return fg_kv4_commit(c, 1, count);
 }
 
 extern "C" int fg_decode_part_len(int nHeads, int dHead, int maxSeq, int64_t* doubles) {

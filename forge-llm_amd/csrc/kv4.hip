@@ -1162,22 +1162,6 @@ __global__ void kv4_follow_kernel(int32_t* __restrict__ len, int32_t* __restrict
 constexpr int kMaxHeads = 1 << 21;  // heads x sequences x layers: a workgroup of 1024 threads each
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
-int check_cache(const fg_kv4_cache* c, const char* fn) {
-  FG_ARG_CHECK(c, "%s: null cache", fn);
-  FG_ARG_CHECK(c->nLayers > 0 && c->nSeq > 0 && c->nKvHeads > 0 && c->maxSeq > 0,
-               "%s: bad dimensions: %d layers, %d sequences, %d kv heads, %d slots", fn, c->nLayers, c->nSeq,
-               c->nKvHeads, c->maxSeq);
-  const int d = c->dHead;
-  FG_ARG_CHECK(d == 32 || d == 64 || d == 96 || d == 128 || d == 256,
-               "%s: head size %d is not one of 32, 64, 96, 128, 256", fn, d);
-  FG_ARG_CHECK((int64_t)c->nLayers * c->nSeq < kMaxHeads / c->nKvHeads, "%s: %d x %d x %d heads are too many", fn,
-               c->nLayers, c->nSeq, c->nKvHeads);
-  FG_ARG_CHECK(c->k && c->v && c->kd && c->vd && c->len && c->next, "%s: null array", fn);
-  FG_ARG_CHECK(aligned16(c->k) && aligned16(c->v) && aligned16(c->kd) && aligned16(c->vd) && aligned16(c->weight) &&
-                   aligned16(c->pos),
-               "%s: the cache's arrays must be 16-byte aligned", fn);
-  return FG_OK;
-}
 int check_layer(const fg_kv4_cache* c, int layer, const char* fn) {
   FG_ARG_CHECK(layer >= 0 && layer < c->nLayers, "%s: layer %d outside [0, %d)", fn, layer, c->nLayers);
   return FG_OK;
@@ -1198,6 +1182,23 @@ double slot_bytes(const fg_kv4_cache* c) { return (double)c->nKvHeads * (c->dHea
 
 }  // namespace
 
+int fg::check_kv4_cache(const fg_kv4_cache* c, const char* fn) {
+  FG_ARG_CHECK(c, "%s: null cache", fn);
+  FG_ARG_CHECK(c->nLayers > 0 && c->nSeq > 0 && c->nKvHeads > 0 && c->maxSeq > 0,
+               "%s: bad dimensions: %d layers, %d sequences, %d kv heads, %d slots", fn, c->nLayers, c->nSeq,
+               c->nKvHeads, c->maxSeq);
+  const int d = c->dHead;
+  FG_ARG_CHECK(d == 32 || d == 64 || d == 96 || d == 128 || d == 256,
+               "%s: head size %d is not one of 32, 64, 96, 128, 256", fn, d);
+  FG_ARG_CHECK((int64_t)c->nLayers * c->nSeq < kMaxHeads / c->nKvHeads, "%s: %d x %d x %d heads are too many", fn,
+               c->nLayers, c->nSeq, c->nKvHeads);
+  FG_ARG_CHECK(c->k && c->v && c->kd && c->vd && c->len && c->next, "%s: null array", fn);
+  FG_ARG_CHECK(aligned16(c->k) && aligned16(c->v) && aligned16(c->kd) && aligned16(c->vd) && aligned16(c->weight) &&
+                   aligned16(c->pos),
+               "%s: the cache's arrays must be 16-byte aligned", fn);
+  return FG_OK;
+}
+
 #define KV4_TRY(expr)                 \
   do {                                \
     const int rc_ = (expr);           \
@@ -1206,7 +1207,7 @@ double slot_bytes(const fg_kv4_cache* c) { return (double)c->nKvHeads * (c->dHea
 
 extern "C" int fg_kv4_append(const fg_kv4_cache* c, int layer, const float* k, const float* v, int64_t ld, int T,
                              const int32_t* count) {
-  KV4_TRY(check_cache(c, "fg_kv4_append"));
+  KV4_TRY(fg::check_kv4_cache(c, "fg_kv4_append"));
   KV4_TRY(check_layer(c, layer, "fg_kv4_append"));
   FG_ARG_CHECK(T >= 0, "fg_kv4_append: T %d is negative", T);
   FG_ARG_CHECK(T == 0 || (k && v), "fg_kv4_append: null argument");
@@ -1223,7 +1224,7 @@ extern "C" int fg_kv4_append(const fg_kv4_cache* c, int layer, const float* k, c
 }
 
 extern "C" int fg_kv4_read(const fg_kv4_cache* c, int layer, float* k, float* v, int64_t ld, int first, int T) {
-  KV4_TRY(check_cache(c, "fg_kv4_read"));
+  KV4_TRY(fg::check_kv4_cache(c, "fg_kv4_read"));
   KV4_TRY(check_layer(c, layer, "fg_kv4_read"));
   FG_ARG_CHECK(first >= 0 && T >= 0 && (int64_t)first + T <= c->maxSeq, "fg_kv4_read: slots [%d, %lld) outside [0, %d)",
                first, (long long)first + T, c->maxSeq);
@@ -1242,7 +1243,7 @@ extern "C" int fg_kv4_read(const fg_kv4_cache* c, int layer, float* k, float* v,
 
 extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, int nHeads, double scale,
                            int T, const int32_t* count) {
-  KV4_TRY(check_cache(c, "fg_kv4_attn"));
+  KV4_TRY(fg::check_kv4_cache(c, "fg_kv4_attn"));
   KV4_TRY(check_layer(c, layer, "fg_kv4_attn"));
   FG_ARG_CHECK(out && q, "fg_kv4_attn: null argument");
   FG_ARG_CHECK(T >= 0, "fg_kv4_attn: T %d is negative", T);
@@ -1300,7 +1301,7 @@ extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const f
 }
 
 extern "C" int fg_kv4_commit(const fg_kv4_cache* c, int T, const int32_t* count) {
-  KV4_TRY(check_cache(c, "fg_kv4_commit"));
+  KV4_TRY(fg::check_kv4_cache(c, "fg_kv4_commit"));
   FG_ARG_CHECK(T >= 0, "fg_kv4_commit: T %d is negative", T);
   FG_REQUIRE_INIT();
   fg::KProfScope prof("kv4_commit", 0.0, 16.0 * c->nSeq);
@@ -1334,7 +1335,7 @@ extern "C" int fg_kv_evict_select(int32_t* holes, int32_t* movers, int32_t* move
 }
 
 extern "C" int fg_kv4_evict(const fg_kv4_cache* c, int budget, int recent) {
-  KV4_TRY(check_cache(c, "fg_kv4_evict"));
+  KV4_TRY(fg::check_kv4_cache(c, "fg_kv4_evict"));
   FG_ARG_CHECK(c->weight && c->pos, "fg_kv4_evict: the cache keeps no weights or positions");
   FG_ARG_CHECK(budget >= 1, "fg_kv4_evict: budget %d is below 1", budget);
   FG_ARG_CHECK(recent >= 0 && recent <= budget, "fg_kv4_evict: recent %d outside [0, %d]", recent, budget);
@@ -1355,7 +1356,7 @@ extern "C" int fg_kv4_evict(const fg_kv4_cache* c, int budget, int recent) {
 }
 
 extern "C" int fg_kv4_reorder(const fg_kv4_cache* c, const int32_t* parent, int W) {
-  KV4_TRY(check_cache(c, "fg_kv4_reorder"));
+  KV4_TRY(fg::check_kv4_cache(c, "fg_kv4_reorder"));
   FG_ARG_CHECK(parent, "fg_kv4_reorder: null argument");
   FG_ARG_CHECK(W >= 1 && W <= 64 && c->nSeq % W == 0, "fg_kv4_reorder: %d sequences are not groups of %d beams "
                "(1 to 64)", c->nSeq, W);

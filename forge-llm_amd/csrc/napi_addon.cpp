@@ -1058,6 +1058,90 @@ FN(js_decode_step) {  // decodeStep(model, kcache, vcache, state, logits)
   CALL(fg_decode_step(&static_cast<DecodeHolder*>(d)->m, a.f(1), a.f(2), a.i32p(3), a.f(4)), "fg_decode_step");
 }
 
+// ── 4-bit cache and beam search ─────────────────────────────────────────
+constexpr uint32_t kKv4Tag = 0x46474b34u;  // 4-bit cache
+struct Kv4Holder {
+  uint32_t tag;
+  fg_kv4_cache c;
+};
+void kv4_finalize(napi_env, void* data, void*) { delete static_cast<Kv4Holder*>(data); }
+const fg_kv4_cache* kv4_of(Args& a, size_t i) {
+  void* d = nullptr;
+  if (napi_get_value_external(a.env, a.argv[i], &d) != napi_ok || !d || static_cast<Kv4Holder*>(d)->tag != kKv4Tag) {
+    a.ok = false;
+    throw_err(a.env, "expected a 4-bit cache handle");
+    return nullptr;
+  }
+  return &static_cast<Kv4Holder*>(d)->c;
+}
+// kv4Cache(nLayers, nSeq, nKvHeads, dHead, maxSeq, k, v, kd, vd, len, next, weight|null, pos|null) -> handle
+// (the caller keeps the buffers for as long as the handle is used)
+FN(js_kv4_cache) {
+  Args a(env, info, 13);
+  if (!a.ok) return nullptr;
+  Kv4Holder* h = new Kv4Holder();
+  h->tag = kKv4Tag;
+  h->c = {a.i32(0), a.i32(1), a.i32(2), a.i32(3), a.i32(4), (uint8_t*)a.ptr(5), (uint8_t*)a.ptr(6), (uint16_t*)a.ptr(7),
+          (uint16_t*)a.ptr(8), a.i32p(9), a.i32p(10), a.f(11), a.i32p(12)};
+  napi_value ext;
+  if (!a.ok || napi_create_external(env, h, kv4_finalize, nullptr, &ext) != napi_ok) {
+    delete h;
+    return a.ok ? throw_err(env, "napi_create_external failed") : nullptr;
+  }
+  return ext;
+}
+FN(js_kv4_append) {  // kv4Append(cache, layer, k, v, ld, T, count|null)
+  Args a(env, info, 7);
+  if (!a.ok) return nullptr;
+  const fg_kv4_cache* c = kv4_of(a, 0);
+  CALL(fg_kv4_append(c, a.i32(1), a.f(2), a.f(3), a.i64(4), a.i32(5), a.i32p(6)), "fg_kv4_append");
+}
+FN(js_kv4_read) {  // kv4Read(cache, layer, k, v, ld, first, T)
+  Args a(env, info, 7);
+  if (!a.ok) return nullptr;
+  const fg_kv4_cache* c = kv4_of(a, 0);
+  CALL(fg_kv4_read(c, a.i32(1), a.f(2), a.f(3), a.i64(4), a.i32(5), a.i32(6)), "fg_kv4_read");
+}
+FN(js_kv4_attn) {  // kv4Attn(cache, layer, out, q, nHeads, scale, T, count|null)
+  Args a(env, info, 8);
+  if (!a.ok) return nullptr;
+  const fg_kv4_cache* c = kv4_of(a, 0);
+  CALL(fg_kv4_attn(c, a.i32(1), a.f(2), a.f(3), a.i32(4), a.f64(5), a.i32(6), a.i32p(7)), "fg_kv4_attn");
+}
+FN(js_kv4_commit) {  // kv4Commit(cache, T, count|null)
+  Args a(env, info, 3);
+  if (!a.ok) return nullptr;
+  const fg_kv4_cache* c = kv4_of(a, 0);
+  CALL(fg_kv4_commit(c, a.i32(1), a.i32p(2)), "fg_kv4_commit");
+}
+FN(js_kv4_evict) {  // kv4Evict(cache, budget, recent)
+  Args a(env, info, 3);
+  if (!a.ok) return nullptr;
+  const fg_kv4_cache* c = kv4_of(a, 0);
+  CALL(fg_kv4_evict(c, a.i32(1), a.i32(2)), "fg_kv4_evict");
+}
+FN(js_kv4_reorder) {  // kv4Reorder(cache, parent, W)
+  Args a(env, info, 3);
+  if (!a.ok) return nullptr;
+  const fg_kv4_cache* c = kv4_of(a, 0);
+  CALL(fg_kv4_reorder(c, a.i32p(1), a.i32(2)), "fg_kv4_reorder");
+}
+FN(js_decode_step_kv4) {  // decodeStepKv4(model, cache, tokens, logits)
+  Args a(env, info, 4);
+  if (!a.ok) return nullptr;
+  void* d = nullptr;
+  if (napi_get_value_external(env, a.argv[0], &d) != napi_ok || !d) return throw_err(env, "decodeStepKv4: bad model");
+  const fg_kv4_cache* c = kv4_of(a, 1);
+  CALL(fg_decode_step_kv4(&static_cast<DecodeHolder*>(d)->m, c, a.i32p(2), a.f(3)), "fg_decode_step_kv4");
+}
+// beamSelect(scoreOut, token, parent, doneOut|null, logits, ld, scores, done|null, eos, nReq, W, V)
+FN(js_beam_select) {
+  Args a(env, info, 12);
+  if (!a.ok) return nullptr;
+  CALL(fg_beam_select(a.f(0), a.i32p(1), a.i32p(2), a.i32p(3), a.f(4), a.i64(5), a.f(6), a.i32p(7), a.i32(8), a.i32(9),
+                      a.i32(10), a.i32(11)), "fg_beam_select");
+}
+
 napi_value Init(napi_env env, napi_value exports) {
   struct {
     const char* name;
@@ -1096,6 +1180,9 @@ napi_value Init(napi_env env, napi_value exports) {
       {"graphDestroy", js_graph_destroy}, {"graphAbort", js_graph_abort}, {"decodeModel", js_decode_model},
       {"qrowBytes", js_qrow_bytes}, {"qmatvec", js_qmatvec}, {"qmatvecF64", js_qmatvec_f64}, {"siluMul", js_silu_mul}, {"dequantize", js_dequantize}, {"quantize", js_quantize},
       {"decodeStep", js_decode_step}, {"decodePartLen", js_decode_part_len},
+      {"kv4Cache", js_kv4_cache}, {"kv4Append", js_kv4_append}, {"kv4Read", js_kv4_read}, {"kv4Attn", js_kv4_attn},
+      {"kv4Commit", js_kv4_commit}, {"kv4Evict", js_kv4_evict}, {"kv4Reorder", js_kv4_reorder},
+      {"decodeStepKv4", js_decode_step_kv4}, {"beamSelect", js_beam_select},
   };
   for (auto& f : fns) {
     napi_value fn;

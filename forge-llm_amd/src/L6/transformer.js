@@ -5,7 +5,7 @@
  * Transformer is its inference forward (:69-184) on the device.
  */
 import { hip } from "../L2/device.js";
-import { KVCache } from "../L5/attention.js";
+import { KVCache, KV4Cache } from "../L5/attention.js";
 import { info, rowBytes } from "../L3/quant.js";
 
 function pick(o, k, d) { return o[k] === undefined || o[k] === null ? d : o[k]; }
@@ -97,7 +97,9 @@ const GRAPHS_KEPT = 4;
  * cache runs op by op; the second is recorded as a HIP graph that later
  * steps with that cache replay (token and position are read from device
  * memory); `opts.graph = false` issues every step op by op.  `cache` must be
- * this package's device KVCache.
+ * this package's device KVCache, or its KV4Cache: `forward` takes one of one
+ * sequence, at the sequence's next position, `forwardAll(tokens, cache)` one token
+ * of every sequence (fg_decode_step_kv4).
  */
 export class Transformer {
   constructor(config, opts = {}) {
@@ -106,7 +108,7 @@ export class Transformer {
     const c = this.cfg;
     if (c.dim % c.nHeads !== 0) throw new Error(`Transformer: dim ${c.dim} must be a multiple of nHeads ${c.nHeads}`);
     this.logits = new Float32Array(c.vocabSize);
-    this._w = null; this._model = null; this._graphs = [];
+    this._w = null; this._model = null; this._graphs = []; this._kv4 = null;
   }
 
   loadWeights(w) {
@@ -166,8 +168,86 @@ export class Transformer {
     return this._model;
   }
 
+  // The model over vectors of every sequence of a 4-bit cache, kept for the last
+  // cache used.
+  _kv4For(cache) {
+    const c = this.cfg, W = this._w, a = hip();
+    if (this._kv4 && this._kv4.cache === cache) return this._kv4;
+    this._dropKv4();
+    const N = cache.sequences, bufs = [];
+    const scratch = (n) => { const h = a.alloc(n * 4); bufs.push(h); return h; };
+    const x = scratch(N * c.dim);
+    const model = a.decodeModel({
+      dim: c.dim, hidden: c.hidden, nLayers: c.nLayers, nHeads: c.nHeads, nKvHeads: c.nKvHeads,
+      vocab: c.vocabSize, maxSeq: c.maxSeq, normEps: c.normEps, tok_emb: W.tok, ln_f: W.ln_f, wcls: W.wcls,
+      emb_type: W.emb_type, cls_type: W.cls_type,
+      rope_cos: W.rope_cos, rope_sin: W.rope_sin, x, q: scratch(N * c.dim), h: scratch(N * c.hidden), attn_part: x,
+      layers: W.layers,
+    });
+    this._kv4 = { cache, model, bufs, tokens: scratch(N), logits: scratch(N * c.vocabSize), graph: null, steps: 0 };
+    return this._kv4;
+  }
+  _dropKv4() {
+    if (!this._kv4) return;
+    const a = hip();
+    if (this._kv4.graph) a.graphDestroy(this._kv4.graph);
+    for (const h of this._kv4.bufs) a.free(h);
+    this._kv4 = null;
+  }
+
+  /** Queues one token of every sequence of a 4-bit cache (logits stay in device
+   *  memory, `_kv4.logits`); a token outside the vocabulary leaves its sequence idle. */
+  _stepAll(tokens, cache) {
+    const c = this.cfg, a = hip();
+    if (!this._w) throw new Error("Transformer.forward: call loadWeights first");
+    if (!(cache instanceof KV4Cache)) throw new TypeError("Transformer.forwardAll: cache must be a KV4Cache");
+    const handle = cache.handle;
+    if (cache.nLayers !== c.nLayers || cache.nKvHeads !== c.nKvHeads || cache.dHead !== c.dHead)
+      throw new RangeError("Transformer.forwardAll: cache shape does not match the Config");
+    if (!tokens || tokens.length !== cache.sequences) throw new RangeError(`Transformer.forwardAll: ${cache.sequences} tokens expected`);
+    const ids = Int32Array.from(tokens, (t) => (Number.isInteger(t) && t >= 0 && t < c.vocabSize ? t : -1));
+    ids.forEach((t, s) => {
+      if (t < 0) return;
+      if (cache.lens[s] >= cache.maxSeq) throw new RangeError(`Transformer.forwardAll: sequence ${s} fills the cache (${cache.maxSeq})`);
+      if (cache.nexts[s] >= c.maxSeq) throw new RangeError(`Transformer.forwardAll: sequence ${s} is at position ${cache.nexts[s]} of ${c.maxSeq}`);
+    });
+    const e = this._kv4For(cache);
+    const step = () => a.decodeStepKv4(e.model, handle, e.tokens, e.logits);
+    a.h2d(e.tokens, ids);
+    if (this._graphOn && e.steps > 0 && !e.graph) {
+      a.graphBegin();
+      try {
+        step();
+        e.graph = a.graphEnd();
+      } catch (err) {
+        a.graphAbort();
+        throw err;
+      }
+    }
+    if (e.graph) a.graphLaunch(e.graph);
+    else step();
+    e.steps++;
+    cache._advance(ids.map((t) => (t >= 0 ? 1 : 0)));
+    return e;
+  }
+
+  /** One token of every sequence of a KV4Cache: logits [sequences][vocabSize] (NaN
+   *  for idle sequences, whose token is outside the vocabulary). */
+  forwardAll(tokens, cache) {
+    const e = this._stepAll(tokens, cache);
+    const out = new Float32Array(cache.sequences * this.cfg.vocabSize);
+    hip().d2h(e.logits, out);
+    return out;
+  }
+
   /** One decode step: logits of `token` at position `pos`, K/V appended to `cache`. */
   forward(token, pos, cache) {
+    if (cache instanceof KV4Cache) {
+      if (cache.sequences !== 1) throw new TypeError("Transformer.forward: a cache of several sequences goes to forwardAll");
+      if (pos !== cache.nexts[0]) throw new RangeError(`Transformer.forward: position ${pos}, the 4-bit cache is at ${cache.nexts[0]}`);
+      hip().d2h(this._stepAll([token], cache).logits, this.logits);
+      return this.logits;
+    }
     this._step(token, pos, cache);
     hip().d2h(this._w.logits, this.logits);
     return this.logits;
@@ -223,6 +303,7 @@ export class Transformer {
     if (!this._w) return;
     const a = hip();
     this._dropGraphs();
+    this._dropKv4();
     for (const h of this._w.bufs) a.free(h);
     if (this._w.part) a.free(this._w.part);
     this._w = null; this._model = null;

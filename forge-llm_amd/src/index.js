@@ -14,7 +14,8 @@ export {
   packPair, DeviceIds,
 } from "./L2/tensor.js";
 export { Config, Transformer } from "./L6/transformer.js";
-export { KVCache, attentionDecode, attentionNaive, flashAttention } from "./L5/attention.js";
+export { KVCache, KV4Cache, attentionDecode, attentionNaive, flashAttention } from "./L5/attention.js";
+export { beamSelect, beamSearch } from "./L8/beam.js";
 export { TrainableTransformer, initWeights, toParams, train, DeviceTrainLoop } from "./L6/train.js";
 export { hip } from "./L2/device.js";
 export {

@@ -708,6 +708,17 @@ int fg_kv_evict_select(int32_t* holes, int32_t* movers, int32_t* moves, const fl
  * weights and positions; the slots from budget on keep what they held) and
  * len[s] = min(len[s], budget).  budget >= maxSeq: nothing to do. */
 int fg_kv4_evict(const fg_kv4_cache* c, int budget, int recent);
+/* Transformer.forward (transformer.js:134-184) of one token for every sequence of a
+ * 4-bit cache: tokens[nSeq] (device), logits [nSeq][vocab].  Sequence s's token
+ * stands at position next[s]; its keys and values are appended to every layer,
+ * attended to from the cache, and committed at the end, so nothing else changes
+ * from step to step and a recorded graph of one serves them all.  A sequence
+ * whose token is outside [0, vocab), whose position is outside the model's RoPE
+ * table (m->maxSeq) or whose cache is full gets NaN logits and stays as it was.
+ * m->x, m->q and m->h hold nSeq vectors each; m->attn_part is not used.  The
+ * limits of fg_decode_step on dim and hidden hold, the head size is one of the
+ * cache's. */
+int fg_decode_step_kv4(const fg_decode_model* m, const fg_kv4_cache* c, const int32_t* tokens, float* logits);
 
 /* ──────────── beam search ────────────
  * No counterpart in the reference (its sampling.js draws one token of one
