@@ -340,38 +340,55 @@ __device__ __forceinline__ float wave_sum(float x) {
   return (lane_value(x, 0) + lane_value(x, 16)) + (lane_value(x, 32) + lane_value(x, 48));
 }
 
-// G heads (1, 2, 4 or 8) of a kv head over one piece of a sequence.  Pieces that
-// are a whole sequence give the output, others their reference, sum and values.
+// Waves of a workgroup that has all of a head, as many as the LDS takes.
 template <int NB, int G>
-__global__ void __launch_bounds__(kThreads, kResident<NB>) kv4_attn_kernel(Cache c, int layer, float* __restrict__ out,
-                                                            const float* __restrict__ q, int nH, int subs, float scale,
-                                                            int T, const int32_t* __restrict__ count, int target,
-                                                            float2* __restrict__ part_ml, float* __restrict__ part_o,
-                                                            float* __restrict__ sc) {
+constexpr int kWholeWaves = NB * G > 32 ? 4 : 8;
+
+// G heads (1, 2, 4 or 8) of a kv head, or of a share of its query heads, over one
+// piece of a sequence.  Pieces that are a whole sequence give the output, others
+// their reference, sum and values.  Whole: one workgroup a sequence and head, no
+// plan, no pieces; it adds the weights, too (sc != NULL), from the scores that it
+// has left in sc.
+template <int NB, int G, bool Whole>
+__global__ void __launch_bounds__((Whole ? 64 * kWholeWaves<NB, G> : kThreads), (Whole ? 2 : kResident<NB>)) kv4_attn_kernel(
+    Cache c, int layer, float* __restrict__ out, const float* __restrict__ q, int nH, int subs, float scale, int T,
+    const int32_t* __restrict__ count, int target, float2* __restrict__ part_ml, float* __restrict__ part_o,
+    float* __restrict__ sc) {
   constexpr int dH = 32 * NB, NS = 8 / G, NA = (NB + NS - 1) / NS;  // sets of rows, blocks of a set
   constexpr int kHalves = G <= 4 ? 2 : 1, kScores = 2 / kHalves;     // a lane's positions of a tile
-  __shared__ __attribute__((aligned(16))) float ps[kWaves][G][32];
-  __shared__ __attribute__((aligned(16))) _Float16 ds[kWaves][4][NB][8];
+  constexpr int kW = Whole ? kWholeWaves<NB, G> : kWaves, kStep = 32 * kW;
+  __shared__ __attribute__((aligned(16))) float ps[kW][G][32];
+  __shared__ __attribute__((aligned(16))) _Float16 ds[kW][4][NB][8];
   // q's operand at first, the waves' values at the end
-  constexpr int kShared = kWaves * G * dH > NB * 64 * 4 ? kWaves * G * dH : NB * 64 * 4;
+  constexpr int kShared = kW * G * dH > NB * 64 * 4 ? kW * G * dH : NB * 64 * 4;
   __shared__ __attribute__((aligned(16))) float shared[kShared];
-  float(*const os)[G][dH] = reinterpret_cast<float(*)[G][dH]>(shared);  // [kWaves]
+  float(*const os)[G][dH] = reinterpret_cast<float(*)[G][dH]>(shared);  // [kW]
   u32x4(*const qs)[64] = reinterpret_cast<u32x4(*)[64]>(shared);        // [NB]
-  __shared__ float ms[kWaves][G], ls[kWaves][G], qm[kWaves][16];
+  __shared__ float ms[kW][G], ls[kW][G], qm[kW][16];
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Plan p;
-  if (!plan_for(p, c, count, T, c.nKV * subs, target, blockIdx.x, false)) return;
-  p.per = __builtin_amdgcn_readfirstlane(p.per);
-  p.first = __builtin_amdgcn_readfirstlane(p.first);
-  p.pieces = __builtin_amdgcn_readfirstlane(p.pieces);
-  const int s = __builtin_amdgcn_readfirstlane(p.s), in_seq = blockIdx.x - p.first * c.nKV * subs;
-  const int head = in_seq / p.pieces, piece = in_seq - head * p.pieces;  // (kv head, share of its query heads)
+  int s, head, begin, n, end, pieces;  // head: (kv head, share of its query heads)
+  if constexpr (Whole) {
+    s = blockIdx.x / (c.nKV * subs);
+    head = blockIdx.x - s * (c.nKV * subs);
+    n = end = attended(c, count, s, T);
+    begin = 0;
+    pieces = 1;
+  } else {
+    Plan p;
+    if (!plan_for(p, c, count, T, c.nKV * subs, target, blockIdx.x, false)) return;
+    const int per = __builtin_amdgcn_readfirstlane(p.per);
+    pieces = __builtin_amdgcn_readfirstlane(p.pieces);
+    s = __builtin_amdgcn_readfirstlane(p.s);
+    const int in_seq = blockIdx.x - __builtin_amdgcn_readfirstlane(p.first) * c.nKV * subs;
+    head = in_seq / pieces;
+    n = attended(c, count, s, T);
+    begin = (in_seq - head * pieces) * per * kRound;
+    end = min(n, begin + per * kRound);
+  }
   const int kvh = head / subs, sub = head - kvh * subs;
   const int group = nH / c.nKV, share = (group + subs - 1) / subs;
   const int h0 = kvh * group + sub * share, heads = min(share, group - sub * share);
-  const int n = attended(c, count, s, T);
-  const int begin = piece * p.per * kRound, end = min(n, begin + p.per * kRound);
   const int64_t slot0 = head_slot(c, layer, s, kvh);
 
   const int set = (i >> 1) / G;  // this row's blocks: set NA ..
@@ -389,14 +406,14 @@ __global__ void __launch_bounds__(kThreads, kResident<NB>) kv4_attn_kernel(Cache
   f16x8 qa[kHalves][NB];
   float factor[2];
   {
-    constexpr int mine = (NB + kWaves - 1) / kWaves;
+    constexpr int mine = (NB + kW - 1) / kW;
     const int h = (i >> 1) % G;
     const float* qr = q + ((int64_t)s * nH + h0 + min(h, heads - 1)) * dH + 4 * g;
     float x[mine][8];
     float m = 0.f;
 #pragma unroll
     for (int k = 0; k < mine; ++k) {
-      const int b = min(wave + k * kWaves, NB - 1);
+      const int b = min(wave + k * kW, NB - 1);
       __builtin_memcpy(&x[k][0], qr + 32 * b, 16);
       __builtin_memcpy(&x[k][4], qr + 32 * b + 16, 16);
 #pragma unroll
@@ -407,11 +424,11 @@ __global__ void __launch_bounds__(kThreads, kResident<NB>) kv4_attn_kernel(Cache
     if (lane < 16) qm[wave][i] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, qm[w][i]);
+    for (int w = 0; w < kW; ++w) m = fmaxf(m, qm[w][i]);
     const int e = fg::exponent_of_max(m);
 #pragma unroll
     for (int k = 0; k < mine; ++k) {
-      const int b = wave + k * kWaves;
+      const int b = wave + k * kW;
       u32x4 w;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -587,12 +604,12 @@ __global__ void __launch_bounds__(kThreads, kResident<NB>) kv4_attn_kernel(Cache
   // once this one's are added
   const std::true_type whole;
   const std::false_type part;
-  for (; at + 32 <= end; at += kRound) {
-    const bool more = at + kRound + 32 <= end;
+  for (; at + 32 <= end; at += kStep) {
+    const bool more = at + kStep + 32 <= end;
     score(at, whole);
-    if (more) keys.template load<true>(c, slot0 + at + kRound, 32);
+    if (more) keys.template load<true>(c, slot0 + at + kStep, 32);
     add(at, whole);
-    if (more) vals.template load<true>(c, slot0 + at + kRound, 32);
+    if (more) vals.template load<true>(c, slot0 + at + kStep, 32);
   }
   if (at < end) {
     keys.template load<false>(c, slot0 + at, n - at);
@@ -614,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, kResident<NB>) kv4_attn_kernel(Cache
     const int h = (2 * g + j) % G;
     float m = ms[0][h];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ms[w][h]);
+    for (int w = 1; w < kW; ++w) m = fmaxf(m, ms[w][h]);
     const float turn = ref[j] == m ? 1.f : __builtin_amdgcn_exp2f(ref[j] - m);
     if (i == 0 && 2 * g + j < G) ls[wave][h] = sum[j] * turn;
 #pragma unroll
@@ -624,18 +641,42 @@ __global__ void __launch_bounds__(kThreads, kResident<NB>) kv4_attn_kernel(Cache
         if ((2 * g + j) / G == b / NA) os[wave][h][32 * b + 16 * u + i] = (o[b][u][2 * j] + o[b][u][2 * j + 1]) * turn;
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < heads * dH; k += kThreads) {
+  for (int k = threadIdx.x; k < heads * dH; k += 64 * kW) {
     const int h = k / dH, d = k - h * dH;
     float v = 0.f, l = 0.f, m = ms[0][h];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kW; ++w) {
       v += os[w][h][d];
       l += ls[w][h];
       m = fmaxf(m, ms[w][h]);
     }
-    if (p.pieces == 1) out[((int64_t)s * nH + h0 + h) * dH + d] = n > 0 ? v / l : 0.f;
+    if (pieces == 1) out[((int64_t)s * nH + h0 + h) * dH + d] = n > 0 ? v / l : 0.f;
     else part_o[((int64_t)blockIdx.x * G + h) * dH + d] = v;
-    if (d == 0) part_ml[(int64_t)blockIdx.x * G + h] = make_float2(m, l);
+    if constexpr (!Whole) {
+      if (d == 0 && part_ml) part_ml[(int64_t)blockIdx.x * G + h] = make_float2(m, l);
+    }
+  }
+  if constexpr (Whole) {
+    if (!sc) return;
+    float m[G], inv[G];
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      m[h] = ms[0][h];
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+        m[h] = fmaxf(m[h], ms[w][h]);
+        l += ls[w][h];
+      }
+      inv[h] = 1.f / l;
+    }
+    for (int j = threadIdx.x; j < n; j += 64 * kW) {
+      float add = 0.f;
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+        if (h < heads) add += __builtin_amdgcn_exp2f(sc[((int64_t)s * nH + h0 + h) * c.maxSeq + j] - m[h]) * inv[h];
+      c.weight[slot0 + j] += add;
+    }
   }
 }
 
@@ -1254,6 +1295,20 @@ extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const f
   const int group = nHeads / c->nKvHeads, subs = (group + 7) / 8, share = (group + subs - 1) / subs;
   const int G = share > 4 ? 8 : share > 2 ? 4 : share;
   const int64_t heads = (int64_t)c->nSeq * c->nKvHeads * subs, rounds = (c->maxSeq + kRound - 1) / kRound;
+  // Short caches, of more slots the more heads there are to fill the chip: a
+  // workgroup a head, no second launch (but where shares of a head's query heads
+  // would add to the same weights).  us, a workgroup a head against pieces:
+  //                     256 slots    1024          2048          4096
+  //   12 heads of 64    4.7  8.1     7.0  8.2      10.0  8.4
+  //    8 heads of 128   5.9  8.8     9.6  9.2      14.6  9.9
+  //    8 heads of 256   9.8 11.5    19.6 11.8
+  //   96 heads of 64    4.7 10.6     7.1 12.0      10.2 16.5     18.2 18.2
+  //   64 heads of 128   6.0 11.4     9.6 12.9      15.9 18.4     26.8 21.7
+  //  256 heads of 128   6.2 14.2    11.5 22.0      17.2 29.7     28.8 39.8
+  // (at 8192 slots 256 heads still take 55 against 64, but only as long as the
+  // sequences are: of all lengths, 55 against 45)
+  const int few = c->dHead == 32 ? 1536 : c->dHead == 64 ? 1280 : c->dHead == 96 ? 1024 : c->dHead == 128 ? 896 : 384;
+  const bool whole = c->maxSeq <= few * (heads < 64 ? 1 : heads < 192 ? 2 : 5) && !(c->weight && subs > 1);
   // One sequence: equal pieces, all resident at once (130001 positions of 8 heads
   // 32.6 us, in pieces of half the size 37.4).  Several: their last pieces are
   // shorter, pieces of half the size even that out (32 sequences up to 8192
@@ -1262,35 +1317,46 @@ extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const f
   int target = 0;
   KV4_DISPATCH(c->dHead, target = kResident<NB> * cus);
   if (c->nSeq > 1) target *= 2;
-  const int64_t grid = heads * rounds < heads + target ? heads * rounds : heads + target;
+  const int64_t grid = whole ? heads : heads * rounds < heads + target ? heads * rounds : heads + target;
   // Few heads of many pieces each are fetched by many threads (32 heads of 96
   // pieces 5.4 us, with 256 threads 9.0); others by small workgroups (1024 heads of
-  // up to 11 pieces 6.4 us, with 1024 threads 12.4; 96 heads of up to 8 4.1 and 5.5).
+  // up to 11 pieces 6.4 us, with 1024 threads 12.4).
   const int kJoin = rounds > 64 && (int64_t)c->nSeq * nHeads <= 256 ? 1024 : 256;
   const int64_t chunks = c->weight ? (c->maxSeq + kJoin - 1) / kJoin : 0;
   const int64_t join = (int64_t)c->nSeq * nHeads + (int64_t)c->nSeq * c->nKvHeads * chunks;
-  FG_ARG_CHECK(grid <= INT32_MAX / kThreads && join <= INT32_MAX / kJoin,
+  FG_ARG_CHECK(grid <= INT32_MAX / 512 && join <= INT32_MAX / kJoin,
                "fg_kv4_attn: %d sequences x %d heads x %d slots are too many", c->nSeq, nHeads, c->maxSeq);
   // references and sums, values, and the scores where weights are kept
-  const size_t ml = (size_t)grid * G * sizeof(float2), po = rounds > 1 ? (size_t)grid * G * c->dHead * sizeof(float) : 0;
+  const bool pieces = !whole && (rounds > 1 || c->weight);
+  const size_t ml = pieces ? (size_t)grid * G * sizeof(float2) : 0;
+  const size_t po = pieces && rounds > 1 ? (size_t)grid * G * c->dHead * sizeof(float) : 0;
   const size_t ps = c->weight ? (size_t)c->nSeq * nHeads * c->maxSeq * sizeof(float) : 0;
   fg::Workspace ws;
-  KV4_TRY(ws.get(ml + po + ps));
+  if (ml + po + ps > 0) KV4_TRY(ws.get(ml + po + ps));
   float2* part_ml = (float2*)ws.ptr;
   float* part_o = (float*)((uint8_t*)ws.ptr + ml);
   float* sc = c->weight ? (float*)((uint8_t*)ws.ptr + ml + po) : nullptr;
-#define KV4_ATTN(GS)                                                                                              \
-  FG_LAUNCH((kv4_attn_kernel<NB, GS>), dim3((unsigned)grid), dim3(kThreads), 0, view(c), layer, out, q, nHeads, subs, \
-            (float)scale, T, count, target, part_ml, part_o, sc)
+#define KV4_ATTN(GS)                                                                                                   \
+  if (whole)                                                                                                           \
+    FG_LAUNCH((kv4_attn_kernel<NB, GS, true>), dim3((unsigned)grid), dim3(64 * kWholeWaves<NB, GS>), 0, view(c), layer, \
+              out, q, nHeads, subs, (float)scale, T, count, target, part_ml, part_o, sc);                              \
+  else                                                                                                                 \
+    FG_LAUNCH((kv4_attn_kernel<NB, GS, false>), dim3((unsigned)grid), dim3(kThreads), 0, view(c), layer, out, q,       \
+              nHeads, subs, (float)scale, T, count, target, part_ml, part_o, sc)
 #define KV4_JOIN(J)                                                                                               \
   FG_LAUNCH((kv4_join_kernel<NB, J>), dim3((unsigned)join), dim3(J), 0, view(c), layer, out, nHeads, subs, G, T, count, \
             target, (const float2*)part_ml, (const float*)part_o, (const float*)sc, (int)chunks)
   KV4_DISPATCH(c->dHead, {
-    if (G == 1) KV4_ATTN(1);
-    else if (G == 2) KV4_ATTN(2);
-    else if (G == 4) KV4_ATTN(4);
-    else KV4_ATTN(8);
-    if (rounds > 1 || c->weight) {
+    if (G == 1) {
+      KV4_ATTN(1);
+    } else if (G == 2) {
+      KV4_ATTN(2);
+    } else if (G == 4) {
+      KV4_ATTN(4);
+    } else {
+      KV4_ATTN(8);
+    }
+    if (pieces) {
       if (kJoin == 1024) KV4_JOIN(1024);
       else KV4_JOIN(256);
     }

@@ -83,9 +83,9 @@ def check(rc, what=""):
 
 def call(name, *args):
     """Call fg_<name>(*args); DeviceArray arguments are passed by pointer."""
-    conv = [a.ptr if isinstance(a, DeviceArray) else a for a in args]
-    rc = getattr(lib, "fg_" + name)(*conv)
-    check(rc, "fg_" + name)
+    rc = getattr(lib, "fg_" + name)(*args)
+    if rc != 0:
+        check(rc, "fg_" + name)
 
 
 def device_count():
@@ -117,6 +117,10 @@ class DeviceArray:
         p = ctypes.c_void_p()
         check(lib.fg_malloc(ctypes.byref(p), max(self.nbytes, 1)), "fg_malloc")
         self.ptr = p.value
+
+    @property
+    def _as_parameter_(self):  # how ctypes passes it
+        return ctypes.c_void_p(self.ptr)
 
     @classmethod
     def from_numpy(cls, a):

@@ -234,6 +234,28 @@ def test_attend_one_sequence(fh, dH, group, n):
     check_attend(fh, c, group, rng, [n])
 
 
+@pytest.mark.parametrize("dH", HEADS)
+@pytest.mark.parametrize("nKV,group,track", [(1, 1, True), (2, 4, False), (2, 3, True), (1, 12, True), (1, 20, False)])
+def test_attend_in_pieces(fh, dH, nKV, group, track):
+    """Room for far more slots than are in use: the cache is read in pieces whose sizes come from the lengths on the device."""
+    rng = np.random.default_rng(dH * 7 + group)
+    lens = [0, 1, 32, 127, 128, 129, 700, 1500]
+    c = Cache(fh, 1, len(lens), nKV, dH, 9000 // group * 2, lens=lens, track=track)
+    c.fill(rng, lens)
+    check_attend(fh, c, nKV * group, rng, lens)
+
+
+@pytest.mark.parametrize("nSeq,maxSeq", [(65, 40), (70, 6000), (130, 9000), (200, 3)])
+def test_attend_many_sequences(fh, nSeq, maxSeq):
+    """More sequences than a wave has lanes, most of them short, some empty."""
+    rng = np.random.default_rng(nSeq)
+    lens = [int(n) for n in rng.choice([0, 1, 5, 33, 140, 300], nSeq) % (maxSeq + 1)]
+    lens[nSeq // 2] = min(maxSeq, 2000)
+    c = Cache(fh, 1, nSeq, 1, 32, maxSeq, lens=lens, track=nSeq != 70)
+    c.fill(rng, lens)
+    check_attend(fh, c, 2, rng, lens)
+
+
 @pytest.mark.parametrize("T,count", [(3, None), (3, [0, 1, 2, 3]), (3, [9, -4, 3, 0])])
 def test_attend_new_tokens_and_bad_lengths(fh, T, count):
     """Lengths and counts outside their ranges count as the nearest inside; new tokens are attended to before the commit."""
