@@ -830,24 +830,11 @@ __device__ __forceinline__ int sum_after(int x, int* sh, int& all) {
   }
   return s;
 }
-__device__ __forceinline__ uint32_t block_extreme(uint32_t x, bool greatest, uint32_t* sh) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t u = __shfl_xor(x, o, 64);
-    x = greatest ? max(x, u) : min(x, u);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-  __syncthreads();
-  for (int i = 0; i < kSelectWaves; ++i) x = greatest ? max(x, sh[i]) : min(x, sh[i]);
-  return x;
-}
-
 // One workgroup per head, its keys in registers (4 Q a thread, read once).  The
-// keys' range is cut into up to 2048 bins by their leading bits and the bin that
-// the budget ends in is found from the counts; its keys, one a thread when they
-// are few enough, are cut again until they are equal.  Weights
-// spread over many powers of two, so a histogram of keys is flat where one of
+// keys are cut into 2048 bins by their leading bits, quarters of a power of two, and
+// the bin that the budget ends in is found from the counts; its keys, one a thread
+// when they are few enough, are cut again until all or equals of them are kept.
+// Weights spread over many powers of two, so a histogram of keys is flat where one of
 // the exponent byte piles up (256 heads of 16384 slots: four passes of 8 bits
 // took 93 us).
 template <int Q>
@@ -859,8 +846,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
                                                                const int32_t* __restrict__ len,
                                                                const int32_t* __restrict__ next, int nSeq, int nHeads,
                                                                int maxSeq, int budget, int recent, int most) {
-  __shared__ int bins[kBins], sh[kSelectWaves], pick[3];
-  __shared__ uint32_t shu[kSelectWaves];
+  __shared__ int bins[kBins], sh[kSelectWaves], kept_by_wave[kSelectWaves], pick[3];
   __shared__ uint32_t list[kSelect];
   __shared__ uint64_t tab[Q * kSelectWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -877,7 +863,6 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
     constexpr uint32_t kSafe = 0xFFFFFFFFu;
     uint32_t key[Q][4];
     int safes = 0;
-    uint32_t lo = kSafe, hi = 0;
     {
       float w[Q][4];
       int p[Q][4];
@@ -903,75 +888,75 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
           const bool keep = (int64_t)p[q][e] >= safe;
           key[q][e] = keep ? kSafe : weight_key(w[q][e]);
           safes += in && keep;
-          if (in && !keep) {
-            lo = min(lo, key[q][e]);
-            hi = max(hi, key[q][e]);
-          }
         }
     }
-    int all;
-    sum_after(safes, sh, all);
-    int want = budget - all;  // of the keys in [lo, hi]
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) safes += __shfl_xor(safes, o, 64);
+    if (lane == 0) kept_by_wave[wave] = safes;
+    int want = 0;             // of the keys in [lo, hi]
     uint32_t border = kSafe;  // kept: above `border`, or equal to it up to slot `last`
     int last = n;
-    if (want > 0) {
-      lo = block_extreme(lo, false, shu);
-      hi = block_extreme(hi, true, shu);
-      // the bin of [lo, hi] that the want-th greatest of its keys is in becomes
-      // [lo, hi], `want` counts inside it
-      auto narrow = [&](auto each_key) {
-        const int shift = max(0, 21 - (int)__builtin_clz(hi - lo));
-        for (int i = threadIdx.x; i < kBins; i += kSelect) bins[i] = 0;
-        __syncthreads();
-        each_key([&](uint32_t u) {
-          if (u >= lo && u <= hi) atomicAdd(&bins[(u - lo) >> shift], 1);
-        });
-        __syncthreads();
-        const int b0 = bins[2 * threadIdx.x], b1 = bins[2 * threadIdx.x + 1];
-        const int after = sum_after(b0 + b1, sh, all);
-        if (after < want && want <= after + b0 + b1) {
-          const bool upper = want <= after + b1;
-          pick[0] = 2 * threadIdx.x + upper;
-          pick[1] = want - after - (upper ? 0 : b1);
-          pick[2] = upper ? b1 : b0;
-        }
-        __syncthreads();
-        lo += (uint32_t)pick[0] << shift;
-        hi = min(hi, lo + ((1u << shift) - 1));
-        want = pick[1];
-        return pick[2];
-      };
-      int c = n;
-      while (lo != hi && c > kSelect)
-        c = narrow([&](auto take) {
-#pragma unroll
-          for (int q = 0; q < Q; ++q)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (4 * ((int)threadIdx.x + q * kSelect) + e < n) take(key[q][e]);
-        });
-      if (lo != hi) {
-        // few enough to hold one a thread
-        __syncthreads();
-        if (threadIdx.x == 0) pick[2] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (4 * ((int)threadIdx.x + q * kSelect) + e < n && key[q][e] >= lo && key[q][e] <= hi)
-              list[atomicAdd(&pick[2], 1) & (kSelect - 1)] = key[q][e];
-        __syncthreads();
-        c = pick[2];
-        const uint32_t mine = (int)threadIdx.x < c ? list[threadIdx.x] : kSafe;
-        const int held = c;
-        while (lo != hi)
-          c = narrow([&](auto take) {
-            if ((int)threadIdx.x < held) take(mine);
-          });
+    bool by_rank = false;
+    uint32_t lo = 0, hi = kSafe - 1;
+    // the bin of [lo, hi] that the want-th greatest of its keys is in becomes
+    // [lo, hi], `want` counts inside it; its number of keys
+    auto narrow = [&](bool first, auto each_key) {
+      const int shift = max(0, 21 - (int)__builtin_clz(hi - lo));
+      for (int i = threadIdx.x; i < kBins; i += kSelect) bins[i] = 0;
+      __syncthreads();
+      each_key([&](uint32_t u) {
+        if (u >= lo && u <= hi) atomicAdd(&bins[(u - lo) >> shift], 1);
+      });
+      __syncthreads();
+      if (first) {
+        want = budget;
+        for (int w = 0; w < kSelectWaves; ++w) want -= kept_by_wave[w];
+        if (want == 0) return 0;
       }
-      border = lo;
-      if (c != want) last = -1;  // not all of the equals: by rank, below
+      const int b0 = bins[2 * threadIdx.x], b1 = bins[2 * threadIdx.x + 1];
+      int all;
+      const int after = sum_after(b0 + b1, sh, all);
+      if (after < want && want <= after + b0 + b1) {
+        const bool upper = want <= after + b1;
+        pick[0] = 2 * threadIdx.x + upper;
+        pick[1] = want - after - (upper ? 0 : b1);
+        pick[2] = upper ? b1 : b0;
+      }
+      __syncthreads();
+      lo += (uint32_t)pick[0] << shift;
+      hi = min(hi, lo + ((1u << shift) - 1));
+      want = pick[1];
+      return pick[2];
+    };
+    auto all_keys = [&](auto take) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * ((int)threadIdx.x + q * kSelect) + e < n) take(key[q][e]);
+    };
+    int c = narrow(true, all_keys);
+    while (lo != hi && c != want && c > kSelect) c = narrow(false, all_keys);
+    if (want > 0 && lo != hi && c != want) {
+      // few enough to hold one a thread
+      __syncthreads();
+      if (threadIdx.x == 0) pick[2] = 0;
+      __syncthreads();
+      all_keys([&](uint32_t u) {
+        if (u >= lo && u <= hi) list[atomicAdd(&pick[2], 1) & (kSelect - 1)] = u;
+      });
+      __syncthreads();
+      const int held = c;
+      const uint32_t mine = (int)threadIdx.x < held ? list[threadIdx.x] : kSafe;
+      while (lo != hi && c != want)
+        c = narrow(false, [&](auto take) {
+          if ((int)threadIdx.x < held) take(mine);
+        });
+    }
+    if (want > 0) {
+      by_rank = c != want;  // lo == hi, and not all of the equals
+      border = by_rank || lo == 0 ? lo : lo - 1;
+      if (border < lo) last = -1;  // all from lo on
     }
     // the number of flagged slots before each of a thread's, by slot order: counts
     // of (group of 4 Q, wave) summed up in a table, two flags at a time
@@ -1024,7 +1009,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
 #pragma unroll
       for (int q = 0; q < Q; ++q) before[q] += tab[q * kSelectWaves + wave];
     };
-    if (last < 0) {  // the want-th of the equals, in slot order
+    if (by_rank) {  // up to the want-th of the equals, in slot order
       auto equal = [&](int q, int e) {
         return 4 * ((int)threadIdx.x + q * kSelect) + e < n && key[q][e] == border ? 1 : 0;
       };
