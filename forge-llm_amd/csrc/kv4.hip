@@ -808,7 +808,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr int kSelect = 1024, kSelectWaves = kSelect / 64;
-constexpr int kBins = 2 * kSelect;
+constexpr int kBinBits = 11, kBins = 1 << kBinBits;  // two bins a thread
+static_assert(kBins == 2 * kSelect, "every bin has a thread");
 
 // The sum of x over the workgroup's later threads; `all` gets the sum of all.
 __device__ __forceinline__ int sum_after(int x, int* sh, int& all) {
@@ -901,7 +902,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
     // the bin of [lo, hi] that the want-th greatest of its keys is in becomes
     // [lo, hi], `want` counts inside it; its number of keys
     auto narrow = [&](bool first, auto each_key) {
-      const int shift = max(0, 21 - (int)__builtin_clz(hi - lo));
+      const int shift = max(0, 32 - kBinBits - (int)__builtin_clz(hi - lo));
       for (int i = threadIdx.x; i < kBins; i += kSelect) bins[i] = 0;
       __syncthreads();
       each_key([&](uint32_t u) {
@@ -911,7 +912,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
       if (first) {
         want = budget;
         for (int w = 0; w < kSelectWaves; ++w) want -= kept_by_wave[w];
-        if (want == 0) return 0;
+        if (want <= 0) return want;
       }
       const int b0 = bins[2 * threadIdx.x], b1 = bins[2 * threadIdx.x + 1];
       int all;
@@ -936,7 +937,8 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
           if (4 * ((int)threadIdx.x + q * kSelect) + e < n) take(key[q][e]);
     };
     int c = narrow(true, all_keys);
-    while (lo != hi && c != want && c > kSelect) c = narrow(false, all_keys);
+    // three levels of 11 bits make lo == hi
+    for (int level = 1; level < 3 && lo != hi && c != want && c > kSelect; ++level) c = narrow(false, all_keys);
     if (want > 0 && lo != hi && c != want) {
       // few enough to hold one a thread
       __syncthreads();
@@ -948,12 +950,15 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
       __syncthreads();
       const int held = c;
       const uint32_t mine = (int)threadIdx.x < held ? list[threadIdx.x] : kSafe;
-      while (lo != hi && c != want)
+      for (int level = 1; level < 3 && lo != hi && c != want; ++level)
         c = narrow(false, [&](auto take) {
           if ((int)threadIdx.x < held) take(mine);
         });
     }
-    if (want > 0) {
+    if (want < 0) {  // more recent slots than the budget: the lowest
+      by_rank = true;
+      want = budget;
+    } else if (want > 0) {
       by_rank = c != want;  // lo == hi, and not all of the equals
       border = by_rank || lo == 0 ? lo : lo - 1;
       if (border < lo) last = -1;  // all from lo on
@@ -1185,6 +1190,7 @@ __global__ void kv4_follow_kernel(int32_t* __restrict__ len, int32_t* __restrict
 }
 
 // ── entry points ──────────────────────────────────────────────────────────
+constexpr int kMaxSlots = 1 << 30;
 constexpr int kMaxHeads = 1 << 21;  // heads x sequences x layers: a workgroup of 1024 threads each
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
@@ -1216,6 +1222,7 @@ int fg::check_kv4_cache(const fg_kv4_cache* c, const char* fn) {
   const int d = c->dHead;
   FG_ARG_CHECK(d == 32 || d == 64 || d == 96 || d == 128 || d == 256,
                "%s: head size %d is not one of 32, 64, 96, 128, 256", fn, d);
+  FG_ARG_CHECK(c->maxSeq <= kMaxSlots, "%s: %d slots are above %d", fn, c->maxSeq, kMaxSlots);
   FG_ARG_CHECK((int64_t)c->nLayers * c->nSeq < kMaxHeads / c->nKvHeads, "%s: %d x %d x %d heads are too many", fn,
                c->nLayers, c->nSeq, c->nKvHeads);
   FG_ARG_CHECK(c->k && c->v && c->kd && c->vd && c->len && c->next, "%s: null array", fn);
@@ -1364,7 +1371,7 @@ extern "C" int fg_kv_evict_select(int32_t* holes, int32_t* movers, int32_t* move
                                   const int32_t* pos, const int32_t* len, const int32_t* next, int nLayers, int nSeq,
                                   int nHeads, int maxSeq, int budget, int recent) {
   FG_ARG_CHECK(holes && movers && moves && weight && pos && len && next, "fg_kv_evict_select: null argument");
-  FG_ARG_CHECK(nLayers > 0 && nSeq > 0 && nHeads > 0 && maxSeq > 0 &&
+  FG_ARG_CHECK(nLayers > 0 && nSeq > 0 && nHeads > 0 && maxSeq > 0 && maxSeq <= kMaxSlots &&
                    (int64_t)nLayers * nSeq < kMaxHeads / nHeads,
                "fg_kv_evict_select: bad dimensions: %d layers, %d sequences, %d heads, %d slots", nLayers, nSeq, nHeads,
                maxSeq);

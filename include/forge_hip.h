@@ -637,7 +637,7 @@ int fg_quantize(int type, void* out, const float* x, int64_t n);
 /* ──────────── 4-bit key-value cache of several sequences ────────────
  * KVCache (attention.js:128-156) with its rows in Q4_0 blocks and room for
  * nSeq sequences; no counterpart in the reference.  dHead is 32, 64, 96, 128
- * or 256, nb = dHead / 32.  A block of 32 values is a fp16 step d and 32 codes
+ * or 256, nb = dHead / 32; maxSeq <= 2^30.  A block of 32 values is a fp16 step d and 32 codes
  * c of 0..15 that stand for d (c - 8): with m the block's value of largest
  * magnitude (the first of equals), d = fp16(m / -8) and
  * c = floor(x / d + 8.5), held to 0..15 (8 where d = 0).  A block with a value
@@ -699,8 +699,9 @@ int fg_kv4_commit(const fg_kv4_cache* c, int T, const int32_t* count);
  * budget on (movers) belong, in order, into the dropped slots below budget
  * (holes): moves[head] of them, listed in holes and movers
  * [nLayers][nSeq][nHeads][max(1, min(budget, maxSeq - budget))], the rest of each
- * list -1.  0 <= recent <= budget, 1 <= budget < maxSeq; positions of one head
- * are distinct and below next. */
+ * list -1.  0 <= recent <= budget, 1 <= budget < maxSeq <= 2^30; positions of one
+ * head are distinct and below next (else, of more than budget recent slots the
+ * lowest are kept). */
 int fg_kv_evict_select(int32_t* holes, int32_t* movers, int32_t* moves, const float* weight, const int32_t* pos,
                        const int32_t* len, const int32_t* next, int nLayers, int nSeq, int nHeads, int maxSeq,
                        int budget, int recent);

@@ -375,7 +375,7 @@ def positions(rng, *shape):
     return rng.permuted(np.broadcast_to(np.arange(shape[-1], dtype=np.int32), shape), axis=-1)
 
 
-@pytest.mark.parametrize("maxSeq", [2, 5, 63, 64, 65, 1000, 1024, 1025, 4097, 9000])
+@pytest.mark.parametrize("maxSeq", [2, 5, 63, 64, 65, 1000, 1024, 1025, 4096, 4097, 9000, 17000, 33000])
 @pytest.mark.parametrize("ties", [False, True])
 def test_evict_select(fh, maxSeq, ties):
     rng = np.random.default_rng(maxSeq)
@@ -401,6 +401,17 @@ def test_evict_select_odd_weights(fh):
     lens = [n, n + 50, -4, 0, 151]
     for budget, recent in ((150, 0), (150, 20), (150, 150), (1, 1), (299, 3)):
         check_select(fh, w, positions(rng, 1, 5, 4, n), lens, [n] * 5, budget, recent)
+
+
+@pytest.mark.parametrize("maxSeq", [100, 5000, 20000, 40000])
+def test_evict_select_more_recent_than_the_budget(fh, maxSeq):
+    """Positions that say so against the rules: the lowest of those slots are kept, and nothing waits for more."""
+    rng = np.random.default_rng(maxSeq)
+    w = np.exp(rng.standard_normal((1, 2, 1, maxSeq))).astype(np.float32)
+    pos = np.full(w.shape, maxSeq, np.int32)
+    pos[0, 1, 0, ::3] = 0
+    for budget in (1, maxSeq // 3, maxSeq - 1):
+        check_select(fh, w, pos, [maxSeq, maxSeq - 1], [maxSeq] * 2, budget, budget // 2)
 
 
 @pytest.mark.parametrize("dH", HEADS)

@@ -62,6 +62,7 @@ def test_bad_caches_are_refused(name):
     for p in ("k", "v", "kd", "vd", "weight", "pos"):
         refused(name, *args(fh.ref(cache(**{p: A + 8}))), says="aligned")
     refused(name, *args(fh.ref(cache(nLayers=1 << 20, nSeq=1 << 10))), says="too many")
+    refused(name, *args(fh.ref(cache(maxSeq=(1 << 30) + 1))), says="slots")
 
 
 def test_bad_arguments_are_refused():
@@ -100,6 +101,7 @@ def test_bad_eviction_and_beams_are_refused():
         refused("kv_evict_select", *(ok[:i] + [None] + ok[i + 1:]), says="null")
     for i in (7, 8, 9, 10):
         refused("kv_evict_select", *(ok[:i] + [0] + ok[i + 1:]), says="dimensions|budget")
+    refused("kv_evict_select", *(ok[:10] + [(1 << 30) + 1] + ok[11:]), says="dimensions")
     for budget, recent in ((0, 0), (40, 1), (8, 9), (8, -1)):
         refused("kv_evict_select", *(ok[:11] + [budget, recent]), says="budget|recent")
     ok = [A, A, A, A, A, 100, A, A, 2, 2, 4, 100]
