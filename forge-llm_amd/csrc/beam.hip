@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
 // One workgroup per request.  A candidate's second key orders those of equal
 // value: the lower beam, within it the greater logit, then the lower token.
 constexpr int kTokenBits = 26;
-constexpr int kPick = 512, kPickWaves = kPick / 64, kHeld = 4;
+constexpr int kPick = 512, kPickWaves = kPick / 64;
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ score_out, int32_t* __restrict__ token,
                                                              int32_t* __restrict__ parent, int32_t* __restrict__ done_out,
                                                              const float2* __restrict__ sums,
@@ -207,16 +207,16 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
   __shared__ int kind[kMaxBeams];  // 0: its candidates, 1: all equal to base, 2: done
   __shared__ ulonglong2 list[kListed];
   __shared__ unsigned long long border[kPickWaves];
+  __shared__ uint32_t best[kPick];
   __shared__ int listed;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t r0 = (int64_t)blockIdx.x * W;
-  const int each = S * W, N = W * each;
-  uint2 held[kHeld];  // a thread's first candidates, fetched beside the sums
-#pragma unroll
-  for (int h = 0; h < kHeld; ++h) {
-    const int i = threadIdx.x + h * kPick;
-    if (i < N) held[h] = cand[r0 * each + i];
-  }
+  // W S sorted lists of W candidates, each dealt out to `m` threads (its candidates
+  // r, r + m, ...), as many as there are
+  const int lists = W * S, m = min(W, max(1, kPick / lists)), parts = lists * m;
+  const uint2* mine = cand + r0 * lists;
+  uint2 held = make_uint2(0u, 0u);  // a thread's first candidate, fetched beside the sums
+  if ((int)threadIdx.x < parts) held = mine[threadIdx.x / m * W + threadIdx.x % m];
   for (int b = wave; b < W; b += kPickWaves) {
     const bool fin = done && done[r0 + b];
     float m = -INFINITY;
@@ -225,7 +225,8 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
       const float2* row = sums + (r0 + b) * S;
       for (int z = lane; z < S; z += 64) m = fmaxf(m, row[z].x);
       m = fg_wave_max(m);
-      for (int z = lane; z < S; z += 64) s += (double)row[z].y * (row[z].x == m ? 1.f : __builtin_amdgcn_exp2f((row[z].x - m) * 1.44269504088896340736f));
+      for (int z = lane; z < S; z += 64)
+        s += (double)row[z].y * (row[z].x == m ? 1.f : __builtin_amdgcn_exp2f((row[z].x - m) * 1.44269504088896340736f));
       s = fg_wave_sum_d(s);
     }
     if (lane == 0) {
@@ -237,18 +238,18 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
   }
   if (threadIdx.x == 0) listed = 0;
   __syncthreads();
-  auto candidate = [&](int i, uint2 c, ulonglong2& k) {
-    const int b = i / each, j = i - b * each;
+  auto candidate = [&](int l, int j, uint2 c, ulonglong2& k) {  // j of list l
+    const int b = l / S, z = l - b * S;
     k = make_ulonglong2(0, 0);
     if (kind[b] == 0) {
       if (c.x == 0) return;
       k.x = key_of(base[b] + (double)value_of(c.x));
     } else if (kind[b] == 1) {
-      if (j >= W || j >= V) return;  // all equal: the first W tokens
+      if (z != 0 || j >= V) return;  // all equal: the first W tokens
       k.x = key_of(base[b]);
       c = make_uint2(1u, (uint32_t)j);
     } else {
-      if (j != 0) return;
+      if (z != 0 || j != 0) return;
       k.x = key_of(base[b]);
       c = make_uint2(1u, (uint32_t)eos);
     }
@@ -264,40 +265,55 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
     if (done_out) done_out[r0 + rank] = kind[b] == 2 || t == eos;
   };
   auto above = [](const ulonglong2& a, const ulonglong2& b) { return a.x > b.x || (a.x == b.x && a.y > b.y); };
-  ulonglong2 k, kept[kHeld];
-  uint64_t mine = 0;
+  ulonglong2 k, first = make_ulonglong2(0, 0);
+  uint64_t greatest = 0;
+  if ((int)threadIdx.x < parts) {
+    candidate(threadIdx.x / m, threadIdx.x % m, held, first);
+    greatest = first.x;
+  }
+  for (int u = threadIdx.x + kPick; u < parts; u += kPick) {
+    candidate(u / m, u % m, mine[u / m * W + u % m], k);
+    greatest = k.x > greatest ? k.x : greatest;
+  }
+  // a bound that W candidates reach: for few beams the W-th greatest of a wave's
+  // first candidates (the greatest of these), for more that of all threads' (their
+  // high words)
+  const uint32_t high = (uint32_t)(greatest >> 32);
+  uint32_t bound = 0;
+  if (W <= 8) {
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t t = bound | (1u << bit);
+      if (__popcll(__ballot(high >= t)) >= W) bound = t;
+    }
+  } else {
+    best[threadIdx.x] = high;
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t v[kPickWaves];
 #pragma unroll
-  for (int h = 0; h < kHeld; ++h) {
-    const int i = threadIdx.x + h * kPick;
-    kept[h] = make_ulonglong2(0, 0);
-    if (i < N) candidate(i, held[h], kept[h]);
-    mine = kept[h].x > mine ? kept[h].x : mine;
+      for (int w = 0; w < kPickWaves; ++w) v[w] = best[w * 64 + lane];
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t t = bound | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) c += __popcll(__ballot(v[w] >= t));
+        if (c >= W) bound = t;
+      }
+    }
   }
-  for (int i = threadIdx.x + kHeld * kPick; i < N; i += kPick) {
-    candidate(i, cand[r0 * each + i], k);
-    mine = k.x > mine ? k.x : mine;
-  }
-  // each wave's W-th greatest of its lanes' maxima (high word); the greatest of them
-  uint32_t t32 = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t t = t32 | (1u << bit);
-    if (__popcll(__ballot((uint32_t)(mine >> 32) >= t)) >= W) t32 = t;
-  }
-  if (lane == 0) border[wave] = (uint64_t)t32 << 32;
+  if (lane == 0) border[wave] = (uint64_t)bound << 32;
   __syncthreads();
   uint64_t least = 1;
   for (int w = 0; w < kPickWaves; ++w) least = border[w] > least ? border[w] : least;
-  auto note = [&](const ulonglong2& k) {
-    if (k.x < least) return;
-    const int at = atomicAdd(&listed, 1);
-    if (at < kListed) list[at] = k;
-  };
-  if (mine >= least) {
-#pragma unroll
-    for (int h = 0; h < kHeld; ++h) note(kept[h]);
-    for (int i = threadIdx.x + kHeld * kPick; i < N; i += kPick) {
-      candidate(i, cand[r0 * each + i], k);
-      note(k);
+  // every part from its greatest on, as long as it reaches the bound
+  for (int u = threadIdx.x; u < parts; u += kPick) {
+    const int l = u / m;
+    for (int j = u % m; j < W; j += m) {
+      if (u == (int)threadIdx.x && j == u % m) k = first;
+      else candidate(l, j, mine[l * W + j], k);
+      if (k.x < least) break;
+      const int at = atomicAdd(&listed, 1);
+      if (at < kListed) list[at] = k;
     }
   }
   __syncthreads();
@@ -314,9 +330,9 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
   // too many equals to list: one after the other
   ulonglong2 prev = make_ulonglong2(~0ull, ~0ull);
   for (int w = 0; w < W; ++w) {
-    ulonglong2 first = make_ulonglong2(0, 0);
-    for (int i = threadIdx.x; i < N; i += kPick) {
-      candidate(i, cand[r0 * each + i], k);
+    first = make_ulonglong2(0, 0);
+    for (int i = threadIdx.x; i < lists * W; i += kPick) {
+      candidate(i / W, i % W, mine[i], k);
       if (above(prev, k) && above(k, first)) first = k;
     }
 #pragma unroll
