@@ -33,6 +33,10 @@ __device__ __forceinline__ int new_tokens(const int32_t* count, int s, int T) {
   return count ? min(max(count[s], 0), T) : T;
 }
 __device__ __forceinline__ int slots_used(const Cache& c, int s) { return min(max(c.len[s], 0), c.maxSeq); }
+__device__ __forceinline__ int slots_after(const Cache& c, const int32_t* count, int s, int T) {
+  const int used = slots_used(c, s);
+  return used + min(new_tokens(count, s, T), c.maxSeq - used);
+}
 
 // Maximum, minimum and sum over the 16 lanes of a row, by rotation.
 template <int N>
@@ -214,9 +218,6 @@ struct Plan {
   int per;
   int s, first, pieces;  // a sequence, its first piece (of one head) and their number
 };
-__device__ __forceinline__ int attended(const Cache& c, const int32_t* count, int s, int T) {
-  return min(slots_used(c, s) + new_tokens(count, s, T), c.maxSeq);
-}
 __device__ __forceinline__ int rounds_of(int n) { return (n + kRound - 1) / kRound; }
 __device__ __forceinline__ int pieces_of(int n, int per) { return max(1, (rounds_of(n) + per - 1) / per); }
 // The sequence with the piece id / heads (by_seq false), or sequence id.  False
@@ -224,7 +225,7 @@ __device__ __forceinline__ int pieces_of(int n, int per) { return max(1, (rounds
 __device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t* count, int T, int heads, int target,
                                          int id, bool by_seq) {
   if (c.nSeq == 1) {
-    const int r = rounds_of(attended(c, count, 0, T));
+    const int r = rounds_of(slots_after(c, count, 0, T));
     p.per = (int)max((int64_t)1, ((int64_t)r * heads + target - 1) / target);
     p.s = p.first = 0;
     p.pieces = max(1, (r + p.per - 1) / p.per);
@@ -232,12 +233,12 @@ __device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t*
   }
   const int lane = threadIdx.x & 63, each = (c.nSeq + 63) / 64, s0 = lane * each;
   int64_t rounds = 0;
-  for (int i = 0; i < each && s0 + i < c.nSeq; ++i) rounds += rounds_of(attended(c, count, s0 + i, T));
+  for (int i = 0; i < each && s0 + i < c.nSeq; ++i) rounds += rounds_of(slots_after(c, count, s0 + i, T));
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) rounds += __shfl_xor(rounds, o, 64);
   p.per = (int)max((int64_t)1, (rounds * heads + target - 1) / target);
   int mine = 0;
-  for (int i = 0; i < each && s0 + i < c.nSeq; ++i) mine += pieces_of(attended(c, count, s0 + i, T), p.per);
+  for (int i = 0; i < each && s0 + i < c.nSeq; ++i) mine += pieces_of(slots_after(c, count, s0 + i, T), p.per);
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -250,7 +251,7 @@ __device__ __forceinline__ bool plan_for(Plan& p, const Cache& c, const int32_t*
   p.s = owner * each;
   p.first = __shfl(upto - mine, owner, 64);
   for (;; ++p.s) {
-    p.pieces = pieces_of(attended(c, count, p.s, T), p.per);
+    p.pieces = pieces_of(slots_after(c, count, p.s, T), p.per);
     if (by_seq ? p.s == id : id < (int64_t)(p.first + p.pieces) * heads) return true;
     p.first += p.pieces;
   }
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__((Whole ? 64 * kWholeWaves<NB, G> : kThreads), 
   if constexpr (Whole) {
     s = blockIdx.x / (c.nKV * subs);
     head = blockIdx.x - s * (c.nKV * subs);
-    n = end = attended(c, count, s, T);
+    n = end = slots_after(c, count, s, T);
     begin = 0;
     pieces = 1;
   } else {
@@ -382,7 +383,7 @@ __global__ void __launch_bounds__((Whole ? 64 * kWholeWaves<NB, G> : kThreads), 
     s = __builtin_amdgcn_readfirstlane(p.s);
     const int in_seq = blockIdx.x - __builtin_amdgcn_readfirstlane(p.first) * c.nKV * subs;
     head = in_seq / pieces;
-    n = attended(c, count, s, T);
+    n = slots_after(c, count, s, T);
     begin = (in_seq - head * pieces) * per * kRound;
     end = min(n, begin + per * kRound);
   }
@@ -723,7 +724,7 @@ __global__ void __launch_bounds__(kJoin) kv4_join_kernel(Cache c, int layer, flo
     return ((int64_t)p.first * c.nKV * subs + (int64_t)(kvh * subs + r / share) * p.pieces) * G + r % share;
   };
   if (weights) {
-    const int n = attended(c, count, s, T), kvh = id / chunks % c.nKV, at = id % chunks * kJoin + (int)threadIdx.x;
+    const int n = slots_after(c, count, s, T), kvh = id / chunks % c.nKV, at = id % chunks * kJoin + (int)threadIdx.x;
     if (id % chunks * kJoin >= n) return;
     float sum = 0.f;
     for (int h0 = 0; h0 < group; h0 += 4) {
@@ -793,9 +794,8 @@ __global__ void __launch_bounds__(kJoin) kv4_join_kernel(Cache c, int layer, flo
 __global__ void kv4_commit_kernel(Cache c, int T, const int32_t* __restrict__ count) {
   const int s = blockIdx.x * kThreads + threadIdx.x;
   if (s >= c.nSeq) return;
-  const int add = new_tokens(count, s, T);
-  c.len[s] = min(slots_used(c, s) + add, c.maxSeq);
-  c.next[s] += add;
+  c.len[s] = slots_after(c, count, s, T);
+  c.next[s] += new_tokens(count, s, T);
 }
 
 // ── eviction ──────────────────────────────────────────────────────────────

@@ -449,6 +449,22 @@ def test_commit(fh):
     np.testing.assert_array_equal(c.next.numpy(), np.arange(100, 105) + 3 + np.array([0, 1, 0, 3, 2]))
 
 
+@pytest.mark.parametrize("maxSeq", [40, 9000])
+def test_more_new_tokens_than_32_bits_add_up(fh, maxSeq):
+    """A step of as many tokens as an int holds fills the sequences; nothing wraps round."""
+    most = 2 ** 31 - 1
+    rng = np.random.default_rng(maxSeq)
+    lens = [0, 7, maxSeq]
+    c = Cache(fh, 1, 3, 1, 64, maxSeq, lens=lens)
+    c.fill(rng, [maxSeq] * 3)
+    check_attend(fh, c, 2, rng, lens, T=most)
+    check_attend(fh, c, 2, rng, lens, T=most, count=[most, 0, -most - 1])
+    c.next.upload(np.array([0, -5, 0], np.int32))
+    c.call("commit", most, fh.DeviceArray.from_numpy(np.array([most, most, 1], np.int32)))
+    np.testing.assert_array_equal(c.len.numpy(), [maxSeq] * 3)
+    np.testing.assert_array_equal(c.next.numpy(), [most, most - 5, 1])
+
+
 # ── together ──────────────────────────────────────────────────────────────
 @pytest.mark.parametrize("W", [1, 3, 4])
 def test_reorder(fh, W):
@@ -557,3 +573,52 @@ def test_a_recorded_step_replays(fh):
     for a, b in zip(*results):
         for x, y in zip(a, b):
             np.testing.assert_array_equal(x, y)
+
+
+def test_two_recorded_steps_take_turns(fh):
+    """Graphs over two caches, and a beam choice in one of them, launched in turn without a wait between:
+    neither's working memory is the other's."""
+    up = fh.DeviceArray.from_numpy
+    sizes = [(9000, 2, 64, 4, 300), (2500, 4, 128, 8, 700)]  # slots, kv heads, head size, query heads, budget
+    results = []
+    for graphs in (False, True):
+        r = np.random.default_rng(3)
+        parts, steps = [], []
+        for maxSeq, nKV, dH, nH, budget in sizes:
+            c = Cache(fh, 1, 4, nKV, dH, maxSeq, lens=[2000, 10, 1999, 700])
+            c.fill(np.random.default_rng(dH), [maxSeq] * 4)
+            c.pos.upload(positions(np.random.default_rng(nH), *c.dims))
+            c.next.upload(np.full(4, maxSeq, np.int32))
+            kv = [up(r.standard_normal((4, nKV * dH)).astype(np.float32)) for _ in range(2)]
+            q, out = up(r.standard_normal((4, nH, dH)).astype(np.float32)), up(np.zeros((4, nH, dH), np.float32))
+            logits, scores = up(r.standard_normal((4, 20000)).astype(np.float32)), up(np.zeros(4, np.float32))
+            picked = [up(np.zeros(4, d)) for d in (np.float32, np.int32, np.int32)]
+            parts.append((c, out, picked))
+
+            def step(c=c, kv=kv, q=q, out=out, logits=logits, scores=scores, picked=picked, nH=nH, dH=dH, nKV=nKV, budget=budget):
+                c.call("append", 0, *kv, nKV * dH, 1, None)
+                c.call("attn", 0, out, q, nH, 0.125, 1, None)
+                c.call("commit", 1, None)
+                fh.call("beam_select", *picked, None, logits, 20000, scores, None, -1, 1, 4, 20000)
+                c.call("reorder", picked[2], 4)
+                c.call("evict", budget, 10)
+
+            steps.append(step)
+        handles = []
+        if graphs:
+            for step in steps:
+                h = ctypes.c_void_p()
+                fh.check(fh.lib.fg_graph_begin(), "begin")
+                step()
+                fh.check(fh.lib.fg_graph_end(ctypes.byref(h)), "end")
+                handles.append(h)
+        for turn in (0, 1, 0, 1, 1, 0):
+            if graphs:
+                fh.check(fh.lib.fg_graph_launch(handles[turn]), "launch")
+            else:
+                steps[turn]()
+        results.append([x for c, out, picked in parts for x in c.host() + [out.numpy()] + [p.numpy() for p in picked]])
+        for h in handles:
+            fh.check(fh.lib.fg_graph_destroy(h), "destroy")
+    for x, y in zip(*results):
+        np.testing.assert_array_equal(x, y)
