@@ -187,7 +187,8 @@ export class KV4Cache {
   _perSlot(buf, Type, layer, seq, head) {
     this._layer(layer);
     if (!buf) throw new Error("KV4Cache: the cache was made without trackWeights");
-    if (!(seq >= 0 && seq < this.sequences && head >= 0 && head < this.nKvHeads)) throw new RangeError(`KV4Cache: sequence ${seq}, head ${head}`);
+    if (!Number.isInteger(seq) || seq < 0 || seq >= this.sequences || !Number.isInteger(head) || head < 0 || head >= this.nKvHeads)
+      throw new RangeError(`KV4Cache: sequence ${seq}, head ${head}`);
     const out = new Type(this.lens[seq]);
     this.handle;
     if (out.length) hip().d2h(buf, out, (((layer * this.sequences + seq) * this.nKvHeads + head) * this.maxSeq) * 4);

@@ -188,6 +188,7 @@ rec("errors", () => {
     throws(() => c.append(0, new Float32Array(63), new Float32Array(64)), RangeError),
     throws(() => c.append(0, new Float32Array(64 * 9), new Float32Array(64 * 9), 9), RangeError),
     throws(() => c2.reorder([0, 2]), RangeError), throws(() => c2.reorder([0]), RangeError), throws(() => c2.reorder([0, 1], 3), RangeError),
+    throws(() => cacheFor(cfg, 8, { trackWeights: true }).weights(0, 0.5), RangeError),
     throws(() => c.kView(0, 9), RangeError), throws(() => c.weights(0), Error), throws(() => c.attend(0, new Float32Array(96), 3), Error),
     throws(() => beamSearch(tr, []), RangeError), throws(() => beamSearch(tr, [1], { beams: 0 }), RangeError),
     throws(() => beamSearch(tr, [400]), RangeError), throws(() => beamSelect(new Float32Array(4), [0], { beams: 1, vocab: 5 }), RangeError),
