@@ -831,13 +831,103 @@ __device__ __forceinline__ int sum_after(int x, int* sh, int& all) {
   }
   return s;
 }
-// One workgroup per head, its keys in registers (4 Q a thread, read once).  The
-// keys are cut into 2048 bins by their leading bits, quarters of a power of two, and
-// the bin that the budget ends in is found from the counts; its keys, one a thread
-// when they are few enough, are cut again until all or equals of them are kept.
-// Weights spread over many powers of two, so a histogram of keys is flat where one of
-// the exponent byte piles up (256 heads of 16384 slots: four passes of 8 bits
-// took 93 us).
+
+// One workgroup per head.  The keys are cut into 2048 bins by their leading bits,
+// quarters of a power of two, and the bin that the budget ends in is found from the
+// counts; its keys, one a thread when they are few enough, are cut again until all or
+// equals of them are kept.  Weights spread over many powers of two, so a histogram of
+// keys is flat where one of the exponent byte piles up (256 heads of 16384 slots:
+// four passes of 8 bits took 93 us).
+//
+// Kept: keys above `border`, and the first `take` of those equal to it.
+constexpr uint32_t kSafe = 0xFFFFFFFFu;
+struct Search {
+  int bins[kBins], sh[kSelectWaves], kept_by_wave[kSelectWaves], pick[3];
+  uint32_t list[kSelect];
+};
+template <class AllKeys>  // all_keys(take): take(u) for every key of this thread
+__device__ __forceinline__ void find_border(AllKeys all_keys, int budget, Search& f, uint32_t& border, int& take) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int want = 0;  // of the keys in [lo, hi]
+  uint32_t lo = 0, hi = kSafe - 1;
+  // the bin of [lo, hi] that the want-th greatest of its keys is in becomes
+  // [lo, hi], `want` counts inside it; its number of keys
+  auto narrow = [&](auto first, auto each_key) {
+    const int shift = max(0, 32 - kBinBits - (int)__builtin_clz(hi - lo));
+    for (int i = threadIdx.x; i < kBins; i += kSelect) f.bins[i] = 0;
+    __syncthreads();
+    int safes = 0;
+    each_key([&](uint32_t u) {
+      if (decltype(first)::value) safes += u == kSafe;
+      if (u >= lo && u <= hi) atomicAdd(&f.bins[(u - lo) >> shift], 1);
+    });
+    if constexpr (decltype(first)::value) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) safes += __shfl_xor(safes, o, 64);
+      if (lane == 0) f.kept_by_wave[wave] = safes;
+    }
+    __syncthreads();
+    if constexpr (decltype(first)::value) {
+      want = budget;
+      for (int w = 0; w < kSelectWaves; ++w) want -= f.kept_by_wave[w];
+      if (want <= 0) return want;
+    }
+    const int b0 = f.bins[2 * threadIdx.x], b1 = f.bins[2 * threadIdx.x + 1];
+    int all;
+    const int after = sum_after(b0 + b1, f.sh, all);
+    if (after < want && want <= after + b0 + b1) {
+      const bool upper = want <= after + b1;
+      f.pick[0] = 2 * threadIdx.x + upper;
+      f.pick[1] = want - after - (upper ? 0 : b1);
+      f.pick[2] = upper ? b1 : b0;
+    }
+    __syncthreads();
+    lo += (uint32_t)f.pick[0] << shift;
+    hi = min(hi, lo + ((1u << shift) - 1));
+    want = f.pick[1];
+    return f.pick[2];
+  };
+  const std::true_type first;
+  const std::false_type later;
+  int c = narrow(first, all_keys);
+  // three levels of 11 bits make lo == hi
+  for (int level = 1; level < 3 && want > 0 && lo != hi && c != want && c > kSelect; ++level) c = narrow(later, all_keys);
+  if (want > 0 && lo != hi && c != want) {
+    // few enough to hold one a thread
+    __syncthreads();
+    if (threadIdx.x == 0) f.pick[2] = 0;
+    __syncthreads();
+    all_keys([&](uint32_t u) {
+      if (u >= lo && u <= hi) f.list[atomicAdd(&f.pick[2], 1) & (kSelect - 1)] = u;
+    });
+    __syncthreads();
+    const int held = c;
+    const uint32_t mine = (int)threadIdx.x < held ? f.list[threadIdx.x] : kSafe;
+    for (int level = 1; level < 3 && lo != hi && c != want; ++level)
+      c = narrow(later, [&](auto count) {
+        if ((int)threadIdx.x < held) count(mine);
+      });
+  }
+  border = kSafe;
+  take = INT32_MAX;
+  if (want < 0) {  // more recent slots than the budget: the lowest
+    take = budget;
+  } else if (want > 0) {
+    if (c != want) {  // lo == hi, and not all of the equals
+      border = lo;
+      take = want;
+    } else if (lo == 0) {
+      border = 0;
+    } else {  // all from lo on
+      border = lo - 1;
+      take = 0;
+    }
+  }
+}
+
+// Keys in registers (4 Q a thread), read once.  256 heads of 16384 slots 23.6 us, of
+// which reading is 9 to 10.7, the bins 6.5, the ranks 3.3, the lists 5: a workgroup
+// fills a CU, so they do not overlap.
 template <int Q>
 __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restrict__ holes,
                                                                int32_t* __restrict__ movers,
@@ -847,9 +937,8 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
                                                                const int32_t* __restrict__ len,
                                                                const int32_t* __restrict__ next, int nSeq, int nHeads,
                                                                int maxSeq, int budget, int recent, int most) {
-  __shared__ int bins[kBins], sh[kSelectWaves], kept_by_wave[kSelectWaves], pick[3];
-  __shared__ uint32_t list[kSelect];
-  __shared__ uint64_t tab[Q * kSelectWaves];
+  __shared__ Search f;
+  __shared__ uint32_t tab[Q * kSelectWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t head = blockIdx.x;
   const int s = (int)(head / nHeads % nSeq);
@@ -861,111 +950,49 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
   movers += head * most;
   int moved = 0;
   if (n > budget) {
-    constexpr uint32_t kSafe = 0xFFFFFFFFu;
     uint32_t key[Q][4];
-    int safes = 0;
     {
-      float w[Q][4];
-      int p[Q][4];
+      constexpr int kLoads = Q < 8 ? Q : 4;  // in flight, of both arrays
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int at = 4 * ((int)threadIdx.x + q * kSelect);
-        if (at + 4 <= n) {
-          __builtin_memcpy(w[q], weight + at, 16);
-          __builtin_memcpy(p[q], pos + at, 16);
-        } else {
+      for (int q0 = 0; q0 < Q; q0 += kLoads) {
+        float w[kLoads][4];
+        int p[kLoads][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            w[q][e] = at + e < n ? weight[at + e] : 0.f;
-            p[q][e] = at + e < n ? pos[at + e] : 0;
+        for (int q = 0; q < kLoads; ++q) {
+          const int at = 4 * ((int)threadIdx.x + (q0 + q) * kSelect);
+          if (at + 4 <= n) {
+            __builtin_memcpy(w[q], weight + at, 16);
+            __builtin_memcpy(p[q], pos + at, 16);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[q][e] = at + e < n ? weight[at + e] : 0.f;
+              p[q][e] = at + e < n ? pos[at + e] : 0;
+            }
           }
         }
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            key[q0 + q][e] = (int64_t)p[q][e] >= safe ? kSafe : weight_key(w[q][e]);
       }
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool in = 4 * ((int)threadIdx.x + q * kSelect) + e < n;
-          const bool keep = (int64_t)p[q][e] >= safe;
-          key[q][e] = keep ? kSafe : weight_key(w[q][e]);
-          safes += in && keep;
-        }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) safes += __shfl_xor(safes, o, 64);
-    if (lane == 0) kept_by_wave[wave] = safes;
-    int want = 0;             // of the keys in [lo, hi]
-    uint32_t border = kSafe;  // kept: above `border`, or equal to it up to slot `last`
-    int last = n;
-    bool by_rank = false;
-    uint32_t lo = 0, hi = kSafe - 1;
-    // the bin of [lo, hi] that the want-th greatest of its keys is in becomes
-    // [lo, hi], `want` counts inside it; its number of keys
-    auto narrow = [&](bool first, auto each_key) {
-      const int shift = max(0, 32 - kBinBits - (int)__builtin_clz(hi - lo));
-      for (int i = threadIdx.x; i < kBins; i += kSelect) bins[i] = 0;
-      __syncthreads();
-      each_key([&](uint32_t u) {
-        if (u >= lo && u <= hi) atomicAdd(&bins[(u - lo) >> shift], 1);
-      });
-      __syncthreads();
-      if (first) {
-        want = budget;
-        for (int w = 0; w < kSelectWaves; ++w) want -= kept_by_wave[w];
-        if (want <= 0) return want;
-      }
-      const int b0 = bins[2 * threadIdx.x], b1 = bins[2 * threadIdx.x + 1];
-      int all;
-      const int after = sum_after(b0 + b1, sh, all);
-      if (after < want && want <= after + b0 + b1) {
-        const bool upper = want <= after + b1;
-        pick[0] = 2 * threadIdx.x + upper;
-        pick[1] = want - after - (upper ? 0 : b1);
-        pick[2] = upper ? b1 : b0;
-      }
-      __syncthreads();
-      lo += (uint32_t)pick[0] << shift;
-      hi = min(hi, lo + ((1u << shift) - 1));
-      want = pick[1];
-      return pick[2];
-    };
-    auto all_keys = [&](auto take) {
+    auto all_keys = [&](auto use) {
 #pragma unroll
       for (int q = 0; q < Q; ++q)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (4 * ((int)threadIdx.x + q * kSelect) + e < n) take(key[q][e]);
+          if (4 * ((int)threadIdx.x + q * kSelect) + e < n) use(key[q][e]);
     };
-    int c = narrow(true, all_keys);
-    // three levels of 11 bits make lo == hi
-    for (int level = 1; level < 3 && lo != hi && c != want && c > kSelect; ++level) c = narrow(false, all_keys);
-    if (want > 0 && lo != hi && c != want) {
-      // few enough to hold one a thread
-      __syncthreads();
-      if (threadIdx.x == 0) pick[2] = 0;
-      __syncthreads();
-      all_keys([&](uint32_t u) {
-        if (u >= lo && u <= hi) list[atomicAdd(&pick[2], 1) & (kSelect - 1)] = u;
-      });
-      __syncthreads();
-      const int held = c;
-      const uint32_t mine = (int)threadIdx.x < held ? list[threadIdx.x] : kSafe;
-      for (int level = 1; level < 3 && lo != hi && c != want; ++level)
-        c = narrow(false, [&](auto take) {
-          if ((int)threadIdx.x < held) take(mine);
-        });
-    }
-    if (want < 0) {  // more recent slots than the budget: the lowest
-      by_rank = true;
-      want = budget;
-    } else if (want > 0) {
-      by_rank = c != want;  // lo == hi, and not all of the equals
-      border = by_rank || lo == 0 ? lo : lo - 1;
-      if (border < lo) last = -1;  // all from lo on
-    }
+    uint32_t border;
+    int take;
+    find_border(all_keys, budget, f, border, take);
+    int last = take == 0 ? -1 : n;  // the last slot whose key may be `border`
     // the number of flagged slots before each of a thread's, by slot order: counts
-    // of (group of 4 Q, wave) summed up in a table, two flags at a time
-    uint64_t before[Q];
+    // of (group of 4 Q, wave) summed up in a table, two flags at a time in halves of
+    // 16 bits (at most 32767 slots are before one)
+    uint32_t before[Q];
     auto rank_flags = [&](auto flags) {  // flags(q, e): bit 0 and bit 1
       __syncthreads();
 #pragma unroll
@@ -980,22 +1007,22 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
           all0 += __popcll(b0);
           all1 += __popcll(b1);
         }
-        before[q] = (uint64_t)mine0 | (uint64_t)mine1 << 32;
-        if (lane == 0) tab[q * kSelectWaves + wave] = (uint64_t)all0 | (uint64_t)all1 << 32;
+        before[q] = (uint32_t)mine0 | (uint32_t)mine1 << 16;
+        if (lane == 0) tab[q * kSelectWaves + wave] = (uint32_t)all0 | (uint32_t)all1 << 16;
       }
       __syncthreads();
       if (wave == 0) {
         constexpr int each = (Q * kSelectWaves + 63) / 64;
-        uint64_t mine = 0;
+        uint32_t mine = 0;
 #pragma unroll
         for (int i = 0; i < each; ++i) {
           const int k = lane * each + i;
           if (k < Q * kSelectWaves) mine += tab[k];
         }
-        uint64_t upto = mine;
+        uint32_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-          const uint64_t u = __shfl_up((unsigned long long)upto, o, 64);
+          const uint32_t u = __shfl_up(upto, o, 64);
           if (lane >= o) upto += u;
         }
         upto -= mine;
@@ -1003,31 +1030,31 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
         for (int i = 0; i < each; ++i) {
           const int k = lane * each + i;
           if (k < Q * kSelectWaves) {
-            const uint64_t t = tab[k];
+            const uint32_t t = tab[k];
             tab[k] = upto;
             upto += t;
           }
         }
-        if (lane == 63) pick[2] = (int)(uint32_t)upto;
+        if (lane == 63) f.pick[2] = (int)(upto & 0xFFFF);
       }
       __syncthreads();
 #pragma unroll
       for (int q = 0; q < Q; ++q) before[q] += tab[q * kSelectWaves + wave];
     };
-    if (by_rank) {  // up to the want-th of the equals, in slot order
+    if (take > 0 && take < INT32_MAX) {  // up to that of the equals, in slot order
       auto equal = [&](int q, int e) {
         return 4 * ((int)threadIdx.x + q * kSelect) + e < n && key[q][e] == border ? 1 : 0;
       };
       rank_flags(equal);
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
-        int rank = (int)(uint32_t)before[q];
+        int rank = (int)before[q];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (equal(q, e) && ++rank == want) pick[1] = 4 * ((int)threadIdx.x + q * kSelect) + e;
+          if (equal(q, e) && ++rank == take) f.pick[1] = 4 * ((int)threadIdx.x + q * kSelect) + e;
       }
       __syncthreads();
-      last = pick[1];
+      last = f.pick[1];
     }
     auto place = [&](int q, int e) {  // 1: a hole, 2: a mover
       const int at = 4 * ((int)threadIdx.x + q * kSelect) + e;
@@ -1035,10 +1062,10 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
       return at >= n ? 0 : at < budget ? (kept ? 0 : 1) : kept ? 2 : 0;
     };
     rank_flags(place);
-    moved = pick[2];
+    moved = f.pick[2];
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      int h = (int)(uint32_t)before[q], m = (int)(before[q] >> 32);
+      int h = (int)(before[q] & 0xFFFF), m = (int)(before[q] >> 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int f = place(q, e), at = 4 * ((int)threadIdx.x + q * kSelect) + e;
@@ -1051,25 +1078,34 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restri
   if (threadIdx.x == 0) moves[head] = moved;
 }
 
-// The number of `in` flags of the workgroup's earlier threads; `all` gets the
-// number of all.
-__device__ __forceinline__ int block_rank(bool in, int* sh, int& all) {
-  const unsigned long long b = __ballot(in);
-  const int w = threadIdx.x >> 6;
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[w] = __popcll(b);
-  __syncthreads();
-  int before = __popcll(b & ((1ull << (threadIdx.x & 63)) - 1));
-  all = 0;
-  for (int i = 0; i < kSelect / 64; ++i) {
-    if (i < w) before += sh[i];
-    all += sh[i];
+// The sum of x, two numbers in halves of 16 bits, over the workgroup's earlier
+// threads; `all` gets the sum of all.
+__device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* sh, uint32_t& all) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  uint32_t s = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t u = __shfl_up(s, o, 64);
+    if (lane >= o) s += u;
   }
-  return before;
+  __syncthreads();
+  if (lane == 63) sh[w] = s;
+  __syncthreads();
+  s -= x;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < kSelectWaves; ++i) {
+    const uint32_t u = sh[i];
+    all += u;
+    s += i < w ? u : 0;
+  }
+  return s;
 }
 
-// The same for heads of more slots than the registers hold: four passes of 8 bits
-// over the keys, then the lists in slot order.
+// The same for heads of more slots than the registers hold: their keys are read for
+// every level, then for the lists in slot order,
+// four slots a thread at a time.  One head of 65536 slots 61 us, 64 heads 76, bound by
+// the LDS counts and the lists' barriers (loads further ahead change nothing).
 __global__ void __launch_bounds__(kSelect) evict_select_long_kernel(int32_t* __restrict__ holes,
                                                                int32_t* __restrict__ movers,
                                                                int32_t* __restrict__ moves,
@@ -1078,7 +1114,8 @@ __global__ void __launch_bounds__(kSelect) evict_select_long_kernel(int32_t* __r
                                                                const int32_t* __restrict__ len,
                                                                const int32_t* __restrict__ next, int nSeq, int nHeads,
                                                                int maxSeq, int budget, int recent, int most) {
-  __shared__ int hist[256], sh[kSelect / 64], pick[2];
+  __shared__ Search f;
+  __shared__ uint32_t halves[kSelectWaves];
   const int64_t head = blockIdx.x;
   const int s = (int)(head / nHeads % nSeq);
   const int n = min(max(len[s], 0), maxSeq);
@@ -1089,43 +1126,61 @@ __global__ void __launch_bounds__(kSelect) evict_select_long_kernel(int32_t* __r
   movers += head * most;
   int nh = 0, nm = 0;
   if (n > budget) {
-    auto key = [&](int j) { return (int64_t)pos[j] >= safe ? 0xFFFFFFFFu : weight_key(weight[j]); };
-    uint32_t prefix = 0;
-    int want = budget;  // of the keys that share the prefix so far
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = threadIdx.x; i < 256; i += kSelect) hist[i] = 0;
-      __syncthreads();
-      for (int j = threadIdx.x; j < n; j += kSelect) {
-        const uint32_t u = key(j);
-        if (shift == 24 || (u >> (shift + 8)) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1);
+    auto keys = [&](uint32_t (&u)[4], int j) {
+      float w[4];
+      int p[4];
+      if (j + 4 <= n) {
+        __builtin_memcpy(w, weight + j, 16);
+        __builtin_memcpy(p, pos + j, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = j + e < n ? weight[j + e] : 0.f;
+          p[e] = j + e < n ? pos[j + e] : 0;
+        }
       }
-      __syncthreads();
-      int all;
-      const int mine = threadIdx.x < 256 ? hist[threadIdx.x] : 0, after = sum_after(mine, sh, all);
-      if (after < want && want <= after + mine) {
-        pick[0] = threadIdx.x;
-        pick[1] = want - after;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = (int64_t)p[e] >= safe ? kSafe : weight_key(w[e]);
+    };
+    auto all_keys = [&](auto use) {
+      for (int j = 4 * (int)threadIdx.x; j < n; j += 4 * kSelect) {
+        uint32_t u[4];
+        keys(u, j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e < n) use(u[e]);
       }
-      __syncthreads();
-      prefix = (prefix << 8) | (uint32_t)pick[0];
-      want = pick[1];
-      __syncthreads();
-    }
+    };
+    uint32_t border;
+    int take;
+    find_border(all_keys, budget, f, border, take);
     int equals = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelect) {
-      const int j = j0 + (int)threadIdx.x;
-      const uint32_t u = j < n ? key(j) : 0;
-      int all;
-      const int rank = equals + block_rank(j < n && u == prefix, sh, all);
-      equals += all;
-      const bool kept = j < n && (u > prefix || (u == prefix && rank < want));
-      const bool hole = j < n && j < budget && !kept, mover = kept && j >= budget;
-      const int ih = nh + block_rank(hole, sh, all);
-      nh += all;
-      const int im = nm + block_rank(mover, sh, all);
-      nm += all;
-      if (hole && ih < most) holes[ih] = j;
-      if (mover && im < most) movers[im] = j;
+    for (int j0 = 0; j0 < n; j0 += 4 * kSelect) {
+      const int j = j0 + 4 * (int)threadIdx.x;
+      uint32_t u[4], all, mine = 0;
+      keys(u, j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine += j + e < n && u[e] == border;
+      int rank = equals + (int)sum_before(mine, halves, all);
+      equals += (int)all;
+      int place[4];  // 1: a hole, 2: a mover
+      mine = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool kept = u[e] > border || (u[e] == border && rank < take);
+        rank += u[e] == border;
+        place[e] = j + e >= n ? 0 : j + e < budget ? (kept ? 0 : 1) : kept ? 2 : 0;
+        mine += place[e] == 1 ? 1u : place[e] == 2 ? 0x10000u : 0u;
+      }
+      const uint32_t before = sum_before(mine, halves, all);
+      int ih = nh + (int)(before & 0xFFFF), im = nm + (int)(before >> 16);
+      nh += (int)(all & 0xFFFF);
+      nm += (int)(all >> 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (place[e] == 1 && ih < most) holes[ih++] = j + e;
+        if (place[e] == 2 && im < most) movers[im++] = j + e;
+      }
     }
   }
   for (int i = nm + (int)threadIdx.x; i < most; i += kSelect) holes[i] = movers[i] = -1;
@@ -1380,6 +1435,9 @@ extern "C" int fg_kv_evict_select(int32_t* holes, int32_t* movers, int32_t* move
   const int heads = nLayers * nSeq * nHeads, most = budget < maxSeq - budget ? budget : maxSeq - budget;
   FG_REQUIRE_INIT();
   fg::KProfScope prof("kv_evict_select", 0.0, (double)heads * (8.0 * maxSeq + 8.0 * most));
+  // Keys in registers up to 32768 slots: 128 heads of 32768 35.2 us, read from memory
+  // for every level 42.2; 256 of 16384 23.6 and 26.2.  At 65536 they would not fit:
+  // 64 heads 76 us from memory, 91 from registers that spill.
 #define EVICT_SELECT(kernel)                                                                                    \
   FG_LAUNCH((kernel), dim3(heads), dim3(kSelect), 0, holes, movers, moves, weight, pos, len, next, nSeq, nHeads, \
             maxSeq, budget, recent, most)

@@ -390,6 +390,18 @@ def test_evict_select(fh, maxSeq, ties):
             check_select(fh, w, positions(rng, 2, 3, 2, maxSeq), lens, [maxSeq] * 3, budget, recent)
 
 
+@pytest.mark.parametrize("maxSeq", [32769, 65535, 65536, 65537, 70001, 150000])
+def test_evict_select_long(fh, maxSeq):
+    """Long heads: spread and even weights, all equal, all slots recent; budgets at either end."""
+    rng = np.random.default_rng(maxSeq)
+    w = np.exp(rng.standard_normal((1, 2, 3, maxSeq)) * 2).astype(np.float32)
+    w[0, :, 1] = np.floor(w[0, :, 1])
+    w[0, :, 2] = 1.5
+    pos = positions(rng, 1, 2, 3, maxSeq)
+    for budget, recent in ((1, 1), (maxSeq // 2 + 1, 1000), (maxSeq // 2, maxSeq // 2), (maxSeq - 1, 0)):
+        check_select(fh, w, pos, [maxSeq, maxSeq - 77], [maxSeq] * 2, budget, recent)
+
+
 def test_evict_select_odd_weights(fh):
     """All equal, zeros of both signs, negative, NaN and infinite weights; every slot recent; lengths out of range."""
     rng = np.random.default_rng(4)
