@@ -176,14 +176,18 @@ struct WRows {
   }
 };
 
+// Every kernel of a step but the attention takes one sequence a blockIdx.y, its
+// vectors behind those of the sequences before (fg_decode_step has one).
+
 // x = the embedding row of the token (a quantized tok_emb, decoded as
 // Transformer._embed does, transformer.js:121-131); NaN for a token outside [0,V).
 template <int QT>
 __global__ void __launch_bounds__(kThreads) dec_embed_kernel(float* __restrict__ x, const uint8_t* __restrict__ emb,
                                                              int64_t rb, int V, const int32_t* __restrict__ state,
                                                              int D) {
-  const int tok = state[0];
+  const int tok = state[2 * blockIdx.y];
   const bool ok = tok >= 0 && tok < V;
+  x += (int64_t)blockIdx.y * D;
   for (int i = blockIdx.x * kThreads + threadIdx.x; i < D; i += gridDim.x * kThreads)
     x[i] = ok ? fgq::dq_elem<QT>(emb + (int64_t)tok * rb, i) : NAN;
 }
@@ -208,6 +212,9 @@ __global__ void __launch_bounds__(kThreads) dec_qkv_kernel(float* __restrict__ q
 #pragma clang fp contract(off)
   extern __shared__ __attribute__((aligned(16))) float xn[];
   __shared__ double sh[kWaves];
+  x += (int64_t)blockIdx.y * D;
+  q += (int64_t)blockIdx.y * qD;
+  state += 2 * blockIdx.y;
   const int pairs = (qD + 2 * kvD) >> 1;
   const int stride = gridDim.x * kWaves;
   int pr = blockIdx.x * kWaves + (threadIdx.x >> 6);
@@ -234,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) dec_qkv_kernel(float* __restrict__ q
   const int pos = state[1];
   if (pos < 0 || pos >= maxSeq) return;  // the host rejects such positions
   const int half = dH >> 1;
-  const int64_t cache_off = layer_off + (int64_t)pos * pos_stride;
+  const int64_t cache_off = layer_off + (int64_t)pos * pos_stride + (int64_t)blockIdx.y * kvD;
   for (bool first = true; pr < pairs; pr += stride, first = false) {
     const int n = 2 * pr;
     if (!first) {
@@ -609,6 +616,8 @@ template <int QT>
 __global__ void __launch_bounds__(kThreads) dec_down_kernel(float* __restrict__ x, const float* __restrict__ in,
                                                             const uint8_t* __restrict__ W, int64_t rb, int N, int K) {
   extern __shared__ __attribute__((aligned(16))) float xs[];
+  x += (int64_t)blockIdx.y * N;
+  in += (int64_t)blockIdx.y * K;
   const int stride = gridDim.x * kWaves;
   int r = blockIdx.x * kWaves + (threadIdx.x >> 6);
   WRows<QT, 1, kPFDown> rw;
@@ -639,6 +648,8 @@ __global__ void __launch_bounds__(kThreads) dec_gateup_kernel(float* __restrict_
 #pragma clang fp contract(off)
   extern __shared__ __attribute__((aligned(16))) float xn[];
   __shared__ double sh[kWaves];
+  x += (int64_t)blockIdx.y * D;
+  hout += (int64_t)blockIdx.y * H;
   const int stride = gridDim.x * kWaves;
   int r = blockIdx.x * kWaves + (threadIdx.x >> 6);
   WRows<QT, 2> rw;
@@ -670,6 +681,8 @@ __global__ void __launch_bounds__(kThreads) dec_head_kernel(float* __restrict__ 
                                                             const uint8_t* __restrict__ W, int64_t rb, int V, int D) {
   extern __shared__ __attribute__((aligned(16))) float xn[];
   __shared__ double sh[kWaves];
+  x += (int64_t)blockIdx.y * D;
+  logits += (int64_t)blockIdx.y * V;
   const int pairs = (V + 1) >> 1;
   const int stride = gridDim.x * kWaves;
   int pr = blockIdx.x * kWaves + (threadIdx.x >> 6);
@@ -764,6 +777,12 @@ struct QkvOp {
   int D, qD, kvD, dH, maxSeq;
   int64_t layer_off;
   int pos_stride;
+  __device__ void sequence(int s) {
+    x += (int64_t)s * D;
+    q += (int64_t)s * qD;
+    state += 2 * s;
+    layer_off += (int64_t)s * kvD;
+  }
   __device__ int rows() const { return qD + 2 * kvD; }
   __device__ const uint8_t* row(int n) const { return W + min(n, rows() - 1) * rb; }
   template <int QT>
@@ -807,6 +826,10 @@ struct ResidOp {
   const uint8_t* W;
   int64_t rb;
   int N, K;
+  __device__ void sequence(int s) {
+    x += (int64_t)s * N;
+    in += (int64_t)s * K;
+  }
   __device__ int rows() const { return N; }
   __device__ const uint8_t* row(int n) const { return W + min(n, N - 1) * rb; }
   template <int QT>
@@ -826,6 +849,7 @@ struct WoOp {
   const uint8_t* W;
   int64_t rb;
   int D, nH, dH, maxSeq, S;
+  __device__ void sequence(int) {}  // one
   __device__ int rows() const { return D; }
   __device__ const uint8_t* row(int n) const { return W + min(n, D - 1) * rb; }
   template <int QT>
@@ -849,6 +873,10 @@ struct GateUpOp {
   const uint8_t *Wg, *Wu;
   int64_t rb;
   int H, D;
+  __device__ void sequence(int s) {
+    h += (int64_t)s * H;
+    x += (int64_t)s * D;
+  }
   __device__ int rows() const { return 2 * H; }
   __device__ const uint8_t* row(int n) const { return ((n & 1) ? Wu : Wg) + min(n >> 1, H - 1) * rb; }
   template <int QT>
@@ -874,6 +902,10 @@ struct HeadOp {
   const uint8_t* W;
   int64_t rb;
   int V, D;
+  __device__ void sequence(int s) {
+    logits += (int64_t)s * V;
+    x += (int64_t)s * D;
+  }
   __device__ int rows() const { return V; }
   __device__ const uint8_t* row(int n) const { return W + (int64_t)min(n, V - 1) * rb; }
   template <int QT>
@@ -895,6 +927,7 @@ __global__ void __launch_bounds__(fgq::kUnitThreads, 3) dec_unit_kernel(Op op, i
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = wave & (P - 1), slots = fgq::kUnitWaves / P, groups = (op.rows() + kUnitRows - 1) / kUnitRows;
   int g = blockIdx.x * slots + wave / P;
+  op.sequence(blockIdx.y);
   fgq::UnitRows<QT, kUnitRows> rw;
   auto start = [&]() {
     if (g >= groups) return;
@@ -960,7 +993,7 @@ inline bool use_units(UnitAt at, int type, const void* W, int K, int rows) {
   return K >= least[at][i] || (rows >= 16384 && (i != 4 || K >= 1280));
 }
 template <int QT, typename Op>
-int launch_unit(const Op& op, int rows, int K, size_t more_lds = 0) {
+int launch_unit(const Op& op, int rows, int K, size_t more_lds = 0, int seqs = 1) {
   if constexpr (fgq::has_units(QT)) {
     const int U = K / fgq::unit_elems(QT), P = fgq::unit_parts(U), slots = fgq::kUnitWaves / P;
     const int groups = (rows + kUnitRows - 1) / kUnitRows;
@@ -968,7 +1001,7 @@ int launch_unit(const Op& op, int rows, int K, size_t more_lds = 0) {
     // second round would repeat the prologue
     const int per_cu = min(3, (int)((160 * 1024) / ((size_t)K * sizeof(float) + more_lds + 512)));
     const int cap = per_cu * (fg::device_cu_count() > 0 ? fg::device_cu_count() : 256);
-    FG_LAUNCH((dec_unit_kernel<QT, Op>), dim3((unsigned)min((groups + slots - 1) / slots, cap)),
+    FG_LAUNCH((dec_unit_kernel<QT, Op>), dim3((unsigned)min((groups + slots - 1) / slots, max(1, cap / seqs)), seqs),
               dim3(fgq::kUnitThreads), (size_t)K * sizeof(float) + more_lds, op, U, P);
   }
   return FG_OK;
@@ -1023,8 +1056,9 @@ unsigned grid_for_waves(int64_t waves) {
   return (unsigned)(g < 1 ? 1 : g);
 }
 
-// The launches of one step that f32 and 4-bit caches share, for one token: x, q, h
-// and logits are its vectors, state its {token, position}.
+// The launches of one step that f32 and 4-bit caches share, for one token of each of
+// `seqs` sequences: x, q, h
+// and logits are their vectors, state their {token, position}.
 struct Step {
   const fg_decode_model* m;
   int D, H, V, nH, nKV, dH, qD, kvD;
@@ -1064,19 +1098,19 @@ int check_model(const fg_decode_model* m, const char* fn, Step& st, double& wbyt
   return FG_OK;
 }
 
-int step_embed(const Step& st, float* x, const int32_t* state) {
+int step_embed(const Step& st, float* x, const int32_t* state, int seqs = 1) {
   if (st.emb_f32) return FG_OK;  // the first layer reads it
   const uint8_t* emb = static_cast<const uint8_t*>(st.m->tok_emb);
   const int64_t erb = fgq::row_bytes(st.m->emb_type, st.D);
   const unsigned g = (unsigned)((st.D + kThreads - 1) / kThreads);
   FGQ_DISPATCH(st.m->emb_type, {
-    FG_LAUNCH(dec_embed_kernel<QT>, dim3(g), dim3(kThreads), 0, x, emb, erb, st.V, state, st.D);
+    FG_LAUNCH(dec_embed_kernel<QT>, dim3(g, seqs), dim3(kThreads), 0, x, emb, erb, st.V, state, st.D);
   });
   return FG_OK;
 }
 
 int step_qkv(const Step& st, int l, float* x, float* q, float* kcache, float* vcache, const int32_t* state,
-             int64_t layer_off, int pos_stride) {
+             int64_t layer_off, int pos_stride, int seqs = 1) {
   const fg_decode_model* m = st.m;
   const fg_decode_layer& ly = m->layers[l];
   const int D = st.D, qD = st.qD, kvD = st.kvD, dH = st.dH, V = st.V;
@@ -1087,11 +1121,11 @@ int step_qkv(const Step& st, int l, float* x, float* q, float* kcache, float* vc
     const QkvOp op{q, kcache, vcache, x, emb0, V, ly.ln1, m->normEps, W, rb, m->rope_cos, m->rope_sin, state,
                    D, qD, kvD, dH, m->maxSeq, layer_off, pos_stride};
     FGQ_DISPATCH(ly.wqkv_type, {
-      const int rc = launch_unit<QT>(op, qD + 2 * kvD, D);
+      const int rc = launch_unit<QT>(op, qD + 2 * kvD, D, 0, seqs);
       if (rc) return rc;
     });
   } else FGQ_DISPATCH(ly.wqkv_type, {
-    FG_LAUNCH(dec_qkv_kernel<QT>, dim3(grid_for_waves((qD + 2 * kvD) / 2)), dim3(kThreads), st.lds_qkv, q, kcache,
+    FG_LAUNCH(dec_qkv_kernel<QT>, dim3(grid_for_waves((qD + 2 * kvD) / 2), seqs), dim3(kThreads), st.lds_qkv, q, kcache,
               vcache, x, emb0, V, ly.ln1, m->normEps, W, rb, m->rope_cos, m->rope_sin, state, D, qD, kvD, dH, m->maxSeq,
               layer_off, pos_stride);
   });
@@ -1100,22 +1134,23 @@ int step_qkv(const Step& st, int l, float* x, float* q, float* kcache, float* vc
 
 // x += W in (the down projection, or the output projection of an attention that
 // is whole): N rows of K.
-int step_residual(const Step& st, UnitAt at, float* x, const float* in, const void* weight, int type, int N, int K) {
+int step_residual(const Step& st, UnitAt at, float* x, const float* in, const void* weight, int type, int N, int K,
+                  int seqs = 1) {
   const uint8_t* W = static_cast<const uint8_t*>(weight);
   const int64_t rb = fgq::row_bytes(type, K);
   if (st.vec && use_units(at, type, W, K, N)) {
     const ResidOp op{x, in, W, rb, N, K};
     FGQ_DISPATCH(type, {
-      const int rc = launch_unit<QT>(op, N, K);
+      const int rc = launch_unit<QT>(op, N, K, 0, seqs);
       if (rc) return rc;
     });
   } else FGQ_DISPATCH(type, {
-    FG_LAUNCH(dec_down_kernel<QT>, dim3(grid_for_waves(N)), dim3(kThreads), K * sizeof(float), x, in, W, rb, N, K);
+    FG_LAUNCH(dec_down_kernel<QT>, dim3(grid_for_waves(N), seqs), dim3(kThreads), K * sizeof(float), x, in, W, rb, N, K);
   });
   return FG_OK;
 }
 
-int step_ffn(const Step& st, int l, float* x, float* h) {
+int step_ffn(const Step& st, int l, float* x, float* h, int seqs = 1) {
   const fg_decode_layer& ly = st.m->layers[l];
   const int D = st.D, H = st.H;
   const uint8_t* Wg = static_cast<const uint8_t*>(ly.gate);
@@ -1125,17 +1160,17 @@ int step_ffn(const Step& st, int l, float* x, float* h) {
   if (st.vec && aligned16(ly.ln2) && use_units(kAfterNorm, ly.gate_type, Wg, D, 2 * H) && aligned16(Wu)) {
     const GateUpOp op{h, x, ly.ln2, eps, Wg, Wu, rb, H, D};
     FGQ_DISPATCH(ly.gate_type, {
-      const int rc = launch_unit<QT>(op, 2 * H, D);
+      const int rc = launch_unit<QT>(op, 2 * H, D, 0, seqs);
       if (rc) return rc;
     });
   } else FGQ_DISPATCH(ly.gate_type, {
-    FG_LAUNCH(dec_gateup_kernel<QT>, dim3(grid_for_waves(H)), dim3(kThreads), D * sizeof(float), h, x, ly.ln2, eps, Wg,
+    FG_LAUNCH(dec_gateup_kernel<QT>, dim3(grid_for_waves(H), seqs), dim3(kThreads), D * sizeof(float), h, x, ly.ln2, eps, Wg,
               Wu, rb, H, D);
   });
-  return step_residual(st, kDown, x, h, ly.down, ly.down_type, D, H);
+  return step_residual(st, kDown, x, h, ly.down, ly.down_type, D, H, seqs);
 }
 
-int step_head(const Step& st, float* logits, const float* x) {
+int step_head(const Step& st, float* logits, const float* x, int seqs = 1) {
   const fg_decode_model* m = st.m;
   const uint8_t* W = static_cast<const uint8_t*>(m->wcls);
   const int D = st.D, V = st.V;
@@ -1143,11 +1178,11 @@ int step_head(const Step& st, float* logits, const float* x) {
   if (st.vec && use_units(kAfterNorm, m->cls_type, W, D, V)) {
     const HeadOp op{logits, x, m->ln_f, m->normEps, W, rb, V, D};
     FGQ_DISPATCH(m->cls_type, {
-      const int rc = launch_unit<QT>(op, V, D);
+      const int rc = launch_unit<QT>(op, V, D, 0, seqs);
       if (rc) return rc;
     });
   } else FGQ_DISPATCH(m->cls_type, {
-    FG_LAUNCH(dec_head_kernel<QT>, dim3(grid_for_waves((V + 1) / 2)), dim3(kThreads), D * sizeof(float), logits, x,
+    FG_LAUNCH(dec_head_kernel<QT>, dim3(grid_for_waves((V + 1) / 2), seqs), dim3(kThreads), D * sizeof(float), logits, x,
               m->ln_f, m->normEps, W, rb, V, D);
   });
   return FG_OK;
@@ -1278,6 +1313,7 @@ extern "C" int fg_decode_step_kv4(const fg_decode_model* m, const fg_kv4_cache* 
                "fg_decode_step_kv4: a cache of %d layers, %d kv heads of %d, %d sequences of %d for a model of %d, %d of "
                "%d", c->nLayers, c->nKvHeads, c->dHead, c->nSeq, c->maxSeq, m->nLayers, m->nKvHeads, st.dH);
   const int D = st.D, kvD = st.kvD, N = c->nSeq;
+  FG_ARG_CHECK(N <= 65535, "fg_decode_step_kv4: %d sequences are above 65535", N);
   FG_ARG_CHECK(st.lds_qkv <= 64 * 1024 && (size_t)st.H * sizeof(float) <= 64 * 1024,
                "fg_decode_step_kv4: dim %d / hidden %d exceed the 64 KiB LDS of a launch", D, st.H);
   FG_REQUIRE_INIT();
@@ -1292,32 +1328,23 @@ extern "C" int fg_decode_step_kv4(const fg_decode_model* m, const fg_kv4_cache* 
   int32_t *state = (int32_t*)(att + (int64_t)N * D), *count = state + 2 * N;
   FG_LAUNCH(kv4_states_kernel, dim3((N + kThreads - 1) / kThreads), dim3(kThreads), 0, state, count, tokens,
             (const int32_t*)c->len, (const int32_t*)c->next, N, st.V, m->maxSeq, c->maxSeq);
-  auto x = [&](int s) { return m->x + (int64_t)s * D; };
-  for (int s = 0; s < N; ++s) {
-    rc = step_embed(st, x(s), state + 2 * s);
-    if (rc) return rc;
-  }
+  rc = step_embed(st, m->x, state, N);
+  if (rc) return rc;
   for (int l = 0; l < m->nLayers; ++l) {
     const fg_decode_layer& ly = m->layers[l];
-    for (int s = 0; s < N; ++s) {
-      rc = step_qkv(st, l, x(s), m->q + (int64_t)s * D, k + (int64_t)s * kvD, v + (int64_t)s * kvD, state + 2 * s, 0, 0);
-      if (rc) return rc;
-    }
+    rc = step_qkv(st, l, m->x, m->q, k, v, state, 0, 0, N);
+    if (rc) return rc;
     rc = fg_kv4_append(c, l, k, v, kvD, 1, count);
     if (rc) return rc;
     rc = fg_kv4_attn(c, l, att, m->q, st.nH, 1.0 / sqrt((double)st.dH), 1, count);
     if (rc) return rc;
-    for (int s = 0; s < N; ++s) {
-      rc = step_residual(st, kWoCombined, x(s), att + (int64_t)s * D, ly.wo, ly.wo_type, D, D);
-      if (rc) return rc;
-      rc = step_ffn(st, l, x(s), m->h + (int64_t)s * st.H);
-      if (rc) return rc;
-    }
-  }
-  for (int s = 0; s < N; ++s) {
-    rc = step_head(st, logits + (int64_t)s * st.V, x(s));
+    rc = step_residual(st, kWoCombined, m->x, att, ly.wo, ly.wo_type, D, D, N);
+    if (rc) return rc;
+    rc = step_ffn(st, l, m->x, m->h, N);
     if (rc) return rc;
   }
+  rc = step_head(st, logits, m->x, N);
+  if (rc) return rc;
   return fg_kv4_commit(c, 1, count);
 }
 

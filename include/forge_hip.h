@@ -718,7 +718,7 @@ int fg_kv4_evict(const fg_kv4_cache* c, int budget, int recent);
  * table (m->maxSeq) or whose cache is full gets NaN logits and stays as it was.
  * m->x, m->q and m->h hold nSeq vectors each; m->attn_part is not used.  The
  * limits of fg_decode_step on dim and hidden hold, the head size is one of the
- * cache's. */
+ * cache's; nSeq <= 65535. */
 int fg_decode_step_kv4(const fg_decode_model* m, const fg_kv4_cache* c, const int32_t* tokens, float* logits);
 
 /* ──────────── beam search ────────────

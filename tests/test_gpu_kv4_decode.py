@@ -137,6 +137,30 @@ def test_step_against_the_reference_forward(fh, name):
         np.testing.assert_array_equal(m.next.numpy(), at)
 
 
+@pytest.mark.parametrize("name", ["dh64_gqa", "dh96", "units"])
+def test_many_sequences_are_each_as_alone(fh, name):
+    """One launch serves all sequences: each one's logits are those of a cache of its own, idle ones between them."""
+    kw, types = CASES[name]
+    N, steps = 37, 4
+    rng = np.random.default_rng(8)
+    m = Model(fh, kw, 5, N, 6, 16, types=types)
+    tokens = rng.integers(0, m.cfg.vocab, (steps, N))
+    tokens[rng.random((steps, N)) < 0.2] = -1
+    got = [m.step(x) for x in tokens]
+    for s in (0, 1, 17, N - 1):
+        one = Model(fh, kw, 5, 1, 6, 16, types=types)
+        for t in range(steps):
+            want = one.step(tokens[t, s:s + 1])[0]
+            if tokens[t, s] < 0:
+                assert np.isnan(got[t][s]).all() and np.isnan(want).all()
+            else:
+                assert rel_l2(got[t][s], want) <= TOL_FWD, (s, t)
+    np.testing.assert_array_equal(m.len.numpy(), (tokens >= 0).sum(0))
+    m.cache.nSeq = 65536  # refused before anything is launched
+    with pytest.raises(fh.ForgeError, match="above 65535"):
+        m.step(tokens[0])
+
+
 def test_full_caches_and_far_positions_stay_as_they_were(fh):
     kw = CASES["dh32"][0]
     m = Model(fh, kw, 6, 2, 3, 5, track=True)
