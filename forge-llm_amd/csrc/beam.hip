@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
 // value: the lower beam, within it the greater logit, then the lower token.
 constexpr int kTokenBits = 26;
 constexpr int kPick = 512, kPickWaves = kPick / 64;
+static_assert(kPick >= 8 * kMaxBeams, "every beam has lanes");
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ score_out, int32_t* __restrict__ token,
                                                              int32_t* __restrict__ parent, int32_t* __restrict__ done_out,
                                                              const float2* __restrict__ sums,
@@ -217,23 +218,28 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
   const uint2* mine = cand + r0 * lists;
   uint2 held = make_uint2(0u, 0u);  // a thread's first candidate, fetched beside the sums
   if ((int)threadIdx.x < parts) held = mine[threadIdx.x / m * W + threadIdx.x % m];
-  for (int b = wave; b < W; b += kPickWaves) {
-    const bool fin = done && done[r0 + b];
-    float m = -INFINITY;
-    double s = 0.0;
-    if (!fin) {
-      const float2* row = sums + (r0 + b) * S;
-      for (int z = lane; z < S; z += 64) m = fmaxf(m, row[z].x);
-      m = fg_wave_max(m);
-      for (int z = lane; z < S; z += 64)
-        s += (double)row[z].y * (row[z].x == m ? 1.f : __builtin_amdgcn_exp2f((row[z].x - m) * 1.44269504088896340736f));
-      s = fg_wave_sum_d(s);
-    }
-    if (lane == 0) {
+  {  // the beams' log sums, all at once: L lanes each
+    const int L = W <= 8 ? 64 : W <= 16 ? 32 : W <= 32 ? 16 : 8;
+    const int b = threadIdx.x / L, l = threadIdx.x & (L - 1);
+    if (b < W) {
+      const bool fin = done && done[r0 + b];
       const double score = scores[r0 + b];
-      double v = fin ? score : m == -INFINITY && s == 0.0 ? -INFINITY : score - ((double)m + log(s));
-      base[b] = v;
-      kind[b] = fin ? 2 : fabs(v) < INFINITY ? 0 : 1;
+      float most = -INFINITY;
+      double s = 0.0;
+      if (!fin) {
+        const float2* row = sums + (r0 + b) * S;
+        for (int z = l; z < S; z += L) most = fmaxf(most, row[z].x);
+        for (int o = L / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+        for (int z = l; z < S; z += L)
+          s += (double)row[z].y *
+               (row[z].x == most ? 1.f : __builtin_amdgcn_exp2f((row[z].x - most) * 1.44269504088896340736f));
+        for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+      }
+      if (l == 0) {
+        const double v = fin ? score : most == -INFINITY && s == 0.0 ? -INFINITY : score - ((double)most + log(s));
+        base[b] = v;
+        kind[b] = fin ? 2 : fabs(v) < INFINITY ? 0 : 1;
+      }
     }
   }
   if (threadIdx.x == 0) listed = 0;
