@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
                                                                 int length) {
   constexpr int E = 4 * P;
   __shared__ uint32_t best[kThreads], bound;
-  __shared__ uint2 list[kListed];
+  __shared__ uint64_t list[kListed];  // key << 32 | ~place: one comparison ranks two
   __shared__ float shm[kWaves], shs[kWaves];
   __shared__ int shn[kWaves], listed;
   const int64_t row = blockIdx.y;
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
       const int at = 4 * ((int)threadIdx.x + (e >> 2) * kThreads) + (e & 3);
       if (bounded ? v[e] >= least : at < n) {
         const int i = atomicAdd(&listed, 1);
-        if (i < kListed) list[i] = make_uint2(key_of(v[e]), at);
+        if (i < kListed) list[i] = (uint64_t)key_of(v[e]) << 32 | ~(uint32_t)at;
       }
     }
   }
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
       const int at = 4 * ((int)threadIdx.x + (e >> 2) * kThreads) + (e & 3);
       if (key[e] > border || (key[e] == border && at <= last)) {
         const int i = atomicAdd(&listed, 1);
-        if (i < kListed) list[i] = make_uint2(key[e], at);
+        if (i < kListed) list[i] = (uint64_t)key[e] << 32 | ~(uint32_t)at;
       }
     }
     __syncthreads();
@@ -177,13 +177,11 @@ __global__ void __launch_bounds__(kThreads) beam_segment_kernel(float2* __restri
       cand[i] = make_uint2(0u, 0u);
       continue;
     }
-    const uint2 me = list[i];
+    const uint64_t me = list[i];
     int rank = 0;
-    for (int j = 0; j < c; ++j) {
-      const uint2 o = list[j];
-      rank += o.x > me.x || (o.x == me.x && o.y < me.y);
-    }
-    if (rank < W) cand[rank] = make_uint2(me.x, me.y + first);
+#pragma unroll 8
+    for (int j = 0; j < c; ++j) rank += list[j] > me;
+    if (rank < W) cand[rank] = make_uint2((uint32_t)(me >> 32), ~(uint32_t)me + first);
   }
   if (threadIdx.x == 0) {
     s = 0.f;
@@ -270,7 +268,8 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
     parent[r0 + rank] = b;
     if (done_out) done_out[r0 + rank] = kind[b] == 2 || t == eos;
   };
-  auto above = [](const ulonglong2& a, const ulonglong2& b) { return a.x > b.x || (a.x == b.x && a.y > b.y); };
+  // (both halves compared, without a branch between their loads)
+  auto above = [](const ulonglong2& a, const ulonglong2& b) { return (a.x > b.x) | ((a.x == b.x) & (a.y > b.y)); };
   ulonglong2 k, first = make_ulonglong2(0, 0);
   uint64_t greatest = 0;
   if ((int)threadIdx.x < parts) {
@@ -328,6 +327,7 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(float* __restrict__ sc
     for (int i = threadIdx.x; i < c; i += kPick) {
       k = list[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < c; ++j) rank += above(list[j], k);
       if (rank < W) put(rank, k);
     }
