@@ -17,7 +17,11 @@ constexpr int kMaxBeams = 64;
 // picks among the segments' candidates, in fp64.  Both find the W first of many
 // without sorting them: the W-th greatest of the threads' own maxima bounds the
 // W-th greatest of all from below, few values reach it, and those are ranked by
-// counting.
+// counting.  The segments' lists are in order, so the second launch reads each only
+// as far as it reaches the bound.  Latency-bound but for large vocabularies: 1 request
+// of 4 beams over 4,096 tokens 9.4 us, 8 of 8 over 128,256 17 (reading and the
+// exponentials 11.6 of it, 2.8 TB/s), 1 of 32 19 (1,065 with all candidates looked
+// at), 1 of 64 25 (3,992).
 //
 // Values are compared as unsigned keys in the order of the values: none 0, NaN
 // 1, -inf the lowest number, -0 as +0.
