@@ -60,7 +60,8 @@ __device__ __forceinline__ float row_sum(float x) {
 // Sixteen lanes take a head's slot: lane n holds values 32 b + n and 32 b + 16 + n
 // of every block, so a block's extremes are reductions over 16 lanes and the
 // lane's nb bytes are its share of the slot.  HBM-bound (7.1 B read for 1 written)
-// as long as a block costs few instructions.
+// as long as a block costs few instructions: 16384 tokens of 8 heads of 128 43 us
+// (3.6 TB/s, reading alone reaches 4.0), reading them back 26 (5.9 TB/s).
 
 // A block by its definition: the first of the greatest magnitudes by ballots, and
 // floor(x / d + 8.5) from an approximate quotient and the exact borders (c - 8.5) d:
@@ -197,6 +198,9 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Cache c, int layer, 
 // up to four heads (G) repeat, so that the scores of positions 0 .. 15 come out in
 // the lower eight rows and those of 16 .. 31 in the upper, one lane each, and
 // 8 / G blocks' steps share an operand of w.
+//
+// 32 heads on 8 kv heads of 128, 130001 positions 32.3 us (4.6 TB/s) and the join 5.4;
+// 32 sequences of up to 8192 40.7 (the last pieces are uneven) and 6.4.
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
