@@ -88,6 +88,11 @@ int absmax_parts(const XpSpec* specs, int count, const char* prof_name);
 
 // What every entry point over a 4-bit cache checks of it; `fn` names the caller.
 int check_kv4_cache(const fg_kv4_cache* c, const char* fn);
+// fg_kv4_attn.  only_new: a sequence without new tokens takes no part; its output is
+// zeros, its cache is not read and its weights stay (fg_kv4_attn takes it as one
+// that attends to what is stored).
+int kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
+             const int32_t* count, bool only_new);
 
 }  // namespace fg
 

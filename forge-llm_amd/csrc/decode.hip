@@ -1336,7 +1336,8 @@ extern "C" int fg_decode_step_kv4(const fg_decode_model* m, const fg_kv4_cache* 
     if (rc) return rc;
     rc = fg_kv4_append(c, l, k, v, kvD, 1, count);
     if (rc) return rc;
-    rc = fg_kv4_attn(c, l, att, m->q, st.nH, 1.0 / sqrt((double)st.dH), 1, count);
+    // (the query of a sequence that takes no part is NaN: it adds to no weights)
+    rc = fg::kv4_attn(c, l, att, m->q, st.nH, 1.0 / sqrt((double)st.dH), 1, count, true);
     if (rc) return rc;
     rc = step_residual(st, kWoCombined, m->x, att, ly.wo, ly.wo_type, D, D, N);
     if (rc) return rc;

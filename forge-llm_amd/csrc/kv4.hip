@@ -23,6 +23,7 @@ struct Cache {
   int32_t *len, *next;
   float* weight;
   int32_t* pos;
+  bool only_new;  // sequences without new tokens take no part: none of their slots count
 };
 // Slot 0 of (layer, sequence, kv head), as a slot number of the whole arrays.
 __host__ __device__ __forceinline__ int64_t head_slot(const Cache& c, int layer, int s, int h) {
@@ -34,8 +35,8 @@ __device__ __forceinline__ int new_tokens(const int32_t* count, int s, int T) {
 }
 __device__ __forceinline__ int slots_used(const Cache& c, int s) { return min(max(c.len[s], 0), c.maxSeq); }
 __device__ __forceinline__ int slots_after(const Cache& c, const int32_t* count, int s, int T) {
-  const int used = slots_used(c, s);
-  return used + min(new_tokens(count, s, T), c.maxSeq - used);
+  const int used = slots_used(c, s), more = new_tokens(count, s, T);
+  return c.only_new && more == 0 ? 0 : used + min(more, c.maxSeq - used);
 }
 
 // Maximum, minimum and sum over the 16 lanes of a row, by rotation.
@@ -1257,8 +1258,9 @@ int check_layer(const fg_kv4_cache* c, int layer, const char* fn) {
   FG_ARG_CHECK(layer >= 0 && layer < c->nLayers, "%s: layer %d outside [0, %d)", fn, layer, c->nLayers);
   return FG_OK;
 }
-Cache view(const fg_kv4_cache* c) {
-  return {c->nSeq, c->nKvHeads, c->maxSeq, c->k, c->v, (_Float16*)c->kd, (_Float16*)c->vd, c->len, c->next, c->weight, c->pos};
+Cache view(const fg_kv4_cache* c, bool only_new = false) {
+  return {c->nSeq,   c->nKvHeads, c->maxSeq,  c->k,      c->v,    (_Float16*)c->kd, (_Float16*)c->vd,
+          c->len,    c->next,     c->weight,  c->pos,    only_new};
 }
 double slot_bytes(const fg_kv4_cache* c) { return (double)c->nKvHeads * (c->dHead + c->dHead / 8); }
 
@@ -1335,6 +1337,10 @@ extern "C" int fg_kv4_read(const fg_kv4_cache* c, int layer, float* k, float* v,
 
 extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, int nHeads, double scale,
                            int T, const int32_t* count) {
+  return fg::kv4_attn(c, layer, out, q, nHeads, scale, T, count, false);
+}
+int fg::kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
+                 const int32_t* count, bool only_new) {
   KV4_TRY(fg::check_kv4_cache(c, "fg_kv4_attn"));
   KV4_TRY(check_layer(c, layer, "fg_kv4_attn"));
   FG_ARG_CHECK(out && q, "fg_kv4_attn: null argument");
@@ -1382,6 +1388,7 @@ extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const f
   const size_t ml = pieces ? (size_t)grid * G * sizeof(float2) : 0;
   const size_t po = pieces && rounds > 1 ? (size_t)grid * G * c->dHead * sizeof(float) : 0;
   const size_t ps = c->weight ? (size_t)c->nSeq * nHeads * c->maxSeq * sizeof(float) : 0;
+  const Cache cache = view(c, only_new);
   fg::Workspace ws;
   if (ml + po + ps > 0) KV4_TRY(ws.get(ml + po + ps));
   float2* part_ml = (float2*)ws.ptr;
@@ -1389,13 +1396,13 @@ extern "C" int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const f
   float* sc = c->weight ? (float*)((uint8_t*)ws.ptr + ml + po) : nullptr;
 #define KV4_ATTN(GS)                                                                                                   \
   if (whole)                                                                                                           \
-    FG_LAUNCH((kv4_attn_kernel<NB, GS, true>), dim3((unsigned)grid), dim3(64 * kWholeWaves<NB, GS>), 0, view(c), layer, \
+    FG_LAUNCH((kv4_attn_kernel<NB, GS, true>), dim3((unsigned)grid), dim3(64 * kWholeWaves<NB, GS>), 0, cache, layer,   \
               out, q, nHeads, subs, (float)scale, T, count, target, part_ml, part_o, sc);                              \
   else                                                                                                                 \
-    FG_LAUNCH((kv4_attn_kernel<NB, GS, false>), dim3((unsigned)grid), dim3(kThreads), 0, view(c), layer, out, q,       \
+    FG_LAUNCH((kv4_attn_kernel<NB, GS, false>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q,         \
               nHeads, subs, (float)scale, T, count, target, part_ml, part_o, sc)
 #define KV4_JOIN(J)                                                                                               \
-  FG_LAUNCH((kv4_join_kernel<NB, J>), dim3((unsigned)join), dim3(J), 0, view(c), layer, out, nHeads, subs, G, T, count, \
+  FG_LAUNCH((kv4_join_kernel<NB, J>), dim3((unsigned)join), dim3(J), 0, cache, layer, out, nHeads, subs, G, T, count,   \
             target, (const float2*)part_ml, (const float*)part_o, (const float*)sc, (int)chunks)
   KV4_DISPATCH(c->dHead, {
     if (G == 1) {

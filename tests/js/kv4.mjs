@@ -105,6 +105,31 @@ rec("a generation past the cache's size under a budget", () => {
   return { ok, detail: "" };
 });
 
+rec("an idle sequence keeps its weights, and what an eviction keeps goes by them", () => {
+  const { cfg, w } = model(13);
+  const tr = new Transformer(cfg).loadWeights(w);
+  let ok = true;
+  for (const slots of [20, 4000]) {  // a workgroup a head, and pieces
+    const c = cacheFor(cfg, slots, { sequences: 3, trackWeights: true });
+    for (let t = 0; t < 9; t++) tr.forwardAll([t, 3 * t % 90, 2 * t], c);
+    const read = (s) => { const x = []; for (let l = 0; l < cfg.nLayers; l++) for (let h = 0; h < cfg.nKvHeads; h++) x.push(...c.weights(l, s, h)); return x; };
+    const before = [read(0), read(1), read(2)];
+    const logits = tr.forwardAll([5, -1, 900], c);
+    ok = ok && logits.subarray(cfg.vocabSize).every(Number.isNaN) && before.every((x) => x.every((v) => v > 0)) &&
+      same(read(1), before[1]) && same(read(2), before[2]) && !same(read(0).slice(0, 9), before[0].slice(0, 9));
+    c.evict(4, 1);
+    for (let l = 0; l < cfg.nLayers; l++)
+      for (let h = 0; h < cfg.nKvHeads; h++) {
+        const at = (l * cfg.nKvHeads + h) * 9, all = before[1].slice(at, at + 9);
+        const keep = all.slice(0, 8).map((x, i) => [x, i]).sort((a, b) => b[0] - a[0] || a[1] - b[1]).slice(0, 3).map((x) => x[1]).concat([8]).sort((a, b) => a - b);
+        ok = ok && same(Array.from(c.positions(l, 1, h)).sort((a, b) => a - b), keep);
+      }
+    c.free();
+  }
+  tr.release();
+  return { ok, detail: "" };
+});
+
 rec("reorder and reset", () => {
   const r = new RNG(9), c = new KV4Cache(2, 6, 1, 32, { sequences: 4, trackWeights: true });
   for (let l = 0; l < 2; l++) c.append(l, normal(r, 4 * 3 * 32), normal(r, 4 * 3 * 32), 3);
