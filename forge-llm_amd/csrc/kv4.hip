@@ -1251,6 +1251,7 @@ __global__ void kv4_follow_kernel(int32_t* __restrict__ len, int32_t* __restrict
 
 // ── entry points ──────────────────────────────────────────────────────────
 constexpr int kMaxSlots = 1 << 30;
+constexpr int kMoveParts = 65535 / FG_BEAM_STATES, kMoveGroups = 65535;  // of a fg_beam_reorder call
 constexpr int kMaxHeads = 1 << 21;  // heads x sequences x layers: a workgroup of 1024 threads each
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
@@ -1488,20 +1489,30 @@ extern "C" int fg_kv4_reorder(const fg_kv4_cache* c, const int32_t* parent, int 
   FG_ARG_CHECK(W >= 1 && W <= 64 && c->nSeq % W == 0, "fg_kv4_reorder: %d sequences are not groups of %d beams "
                "(1 to 64)", c->nSeq, W);
   FG_REQUIRE_INIT();
-  fg_beam_state st[6];
-  int n = 0;
-  auto add = [&](void* base, int64_t row) {
-    if (!base) return;
-    const int64_t head = c->maxSeq * row, seq = c->nKvHeads * head;
-    st[n++] = {base, seq, c->nLayers, c->nSeq * seq, c->nKvHeads, head, row, c->maxSeq};
-  };
-  add(c->k, c->dHead / 2);
-  add(c->v, c->dHead / 2);
-  add(c->kd, c->dHead / 16);
-  add(c->vd, c->dHead / 16);
-  add(c->weight, 4);
-  add(c->pos, 4);
-  KV4_TRY(fg_beam_reorder(st, n, parent, c->len, c->nSeq / W, W));
+  // a launch takes so many parts (layers x kv heads) and requests: larger caches go in
+  // several, the lengths read by all of them and moved at the end
+  const int heads = c->nKvHeads < kMoveParts ? c->nKvHeads : kMoveParts, layers = kMoveParts / heads;
+  const int groups = c->nSeq / W;
+  for (int r0 = 0; r0 < groups; r0 += kMoveGroups)
+    for (int l0 = 0; l0 < c->nLayers; l0 += layers)
+      for (int h0 = 0; h0 < c->nKvHeads; h0 += heads) {
+        fg_beam_state st[6];
+        int n = 0;
+        auto add = [&](void* base, int64_t row) {
+          if (!base) return;
+          const int64_t head = c->maxSeq * row, seq = c->nKvHeads * head, layer = c->nSeq * seq;
+          st[n++] = {(uint8_t*)base + l0 * layer + (int64_t)r0 * W * seq + h0 * head, seq,
+                     min(layers, c->nLayers - l0), layer, min(heads, c->nKvHeads - h0), head, row, c->maxSeq};
+        };
+        add(c->k, c->dHead / 2);
+        add(c->v, c->dHead / 2);
+        add(c->kd, c->dHead / 16);
+        add(c->vd, c->dHead / 16);
+        add(c->weight, 4);
+        add(c->pos, 4);
+        const int64_t at = (int64_t)r0 * W;
+        KV4_TRY(fg_beam_reorder(st, n, parent + at, c->len + at, min(kMoveGroups, groups - r0), W));
+      }
   FG_LAUNCH(kv4_follow_kernel, dim3(c->nSeq / W), dim3(64), 0, c->len, c->next, parent, W);
   return FG_OK;
 }
