@@ -905,11 +905,23 @@ FN(js_graph_abort) {
 }
 
 // ── decode ──────────────────────────────────────────────────────────────
+constexpr uint32_t kDecodeTag = 0x4647444du;  // decode model
 struct DecodeHolder {
+  uint32_t tag = kDecodeTag;
   fg_decode_model m;
   std::vector<fg_decode_layer> layers;
 };
 void decode_finalize(napi_env, void* data, void*) { delete static_cast<DecodeHolder*>(data); }
+
+const fg_decode_model* model_of(Args& a, size_t i) {
+  void* d = nullptr;
+  if (napi_get_value_external(a.env, a.argv[i], &d) != napi_ok || !d || static_cast<DecodeHolder*>(d)->tag != kDecodeTag) {
+    a.ok = false;
+    throw_err(a.env, "expected a decode model handle");
+    return nullptr;
+  }
+  return &static_cast<DecodeHolder*>(d)->m;
+}
 
 bool get_prop(napi_env env, napi_value obj, const char* k, napi_value* out) {
   bool has = false;
@@ -1053,9 +1065,8 @@ FN(js_decode_part_len) {  // decodePartLen(nHeads, dHead, maxSeq) -> doubles
 FN(js_decode_step) {  // decodeStep(model, kcache, vcache, state, logits)
   Args a(env, info, 5);
   if (!a.ok) return nullptr;
-  void* d = nullptr;
-  if (napi_get_value_external(env, a.argv[0], &d) != napi_ok || !d) return throw_err(env, "decodeStep: bad model");
-  CALL(fg_decode_step(&static_cast<DecodeHolder*>(d)->m, a.f(1), a.f(2), a.i32p(3), a.f(4)), "fg_decode_step");
+  const fg_decode_model* m = model_of(a, 0);
+  CALL(fg_decode_step(m, a.f(1), a.f(2), a.i32p(3), a.f(4)), "fg_decode_step");
 }
 
 // ── 4-bit cache and beam search ─────────────────────────────────────────
@@ -1129,10 +1140,10 @@ FN(js_kv4_reorder) {  // kv4Reorder(cache, parent, W)
 FN(js_decode_step_kv4) {  // decodeStepKv4(model, cache, tokens, logits)
   Args a(env, info, 4);
   if (!a.ok) return nullptr;
-  void* d = nullptr;
-  if (napi_get_value_external(env, a.argv[0], &d) != napi_ok || !d) return throw_err(env, "decodeStepKv4: bad model");
+  const fg_decode_model* m = model_of(a, 0);
+  if (!a.ok) return nullptr;
   const fg_kv4_cache* c = kv4_of(a, 1);
-  CALL(fg_decode_step_kv4(&static_cast<DecodeHolder*>(d)->m, c, a.i32p(2), a.f(3)), "fg_decode_step_kv4");
+  CALL(fg_decode_step_kv4(m, c, a.i32p(2), a.f(3)), "fg_decode_step_kv4");
 }
 // beamSelect(scoreOut, token, parent, doneOut|null, logits, ld, scores, done|null, eos, nReq, W, V)
 FN(js_beam_select) {

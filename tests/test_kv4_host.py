@@ -193,3 +193,23 @@ def test_beam_select_known_answers():
     s, t, p, f = ref.beam_select(x, np.array([0.0, -0.1], np.float32), np.array([0, 1]), 2, 1, 2)
     np.testing.assert_array_equal((t, p, f), ([2, 0], [1, 0], [1, 0]))
     assert s[0] == np.float32(-0.1)
+
+
+def test_handles_of_one_kind_are_not_read_as_another():
+    """The addon's cache handle as a decode model, and things that are no handle at all."""
+    import os
+    import subprocess
+    code = """
+import { addonUninitialised } from './src/L2/device.js';
+const a = addonUninitialised(), no = [null, null, null, null, null, null, null, null];
+const cache = a.kv4Cache(1, 1, 1, 32, 8, ...no), say = (fn) => { try { fn(); return 'nothing'; } catch (e) { return e.message; } };
+for (const x of [cache, {}, null, 7]) {
+  console.log(say(() => a.decodeStep(x, null, null, null, null)));
+  console.log(say(() => a.decodeStepKv4(x, cache, null, null)));
+}
+for (const x of [{}, null, 7]) console.log(say(() => a.kv4Commit(x, 1, null)));
+"""
+    r = subprocess.run(["node", "--input-type=module", "-e", code], cwd=os.path.dirname(os.path.abspath(fh.__file__)),
+                       stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout
+    assert r.stdout.split("\n")[:-1] == ["expected a decode model handle"] * 8 + ["expected a 4-bit cache handle"] * 3, r.stdout
