@@ -66,7 +66,8 @@ export function beamSelect(logits, scores, { beams, vocab, requests = 1, done = 
  * by the sum of their tokens' log probabilities, best first: [{tokens, score, done}].
  * A beam that takes `eos` (the Config's eosId; -1: none) is done and keeps its score.
  * With `budget` the cache holds that many tokens of every head, the newest `recent`
- * among them, and the others by accumulated attention.
+ * among them, and the others by accumulated attention.  The search ends at the Config's
+ * maxSeq positions: its continuations are at most maxSeq - prompt.length + 1 tokens.
  */
 export function beamSearch(transformer, prompt, { beams = 4, maxNew = 32, eos, budget = 0, recent = 0 } = {}) {
   const c = transformer.cfg, V = c.vocabSize;
@@ -75,7 +76,9 @@ export function beamSearch(transformer, prompt, { beams = 4, maxNew = 32, eos, b
   if (!Number.isInteger(beams) || beams < 1 || beams > 64 || beams > V) throw new RangeError(`beamSearch: ${beams} beams`);
   if (!Number.isInteger(maxNew) || maxNew < 1) throw new RangeError(`beamSearch: maxNew ${maxNew}`);
   if (budget && budget < 1) throw new RangeError(`beamSearch: budget ${budget}`);
-  const room = budget ? budget + 1 : prompt.length + maxNew;
+  if (prompt.length > c.maxSeq) throw new RangeError(`beamSearch: a prompt of ${prompt.length} tokens, the model has ${c.maxSeq} positions`);
+  const most = Math.min(maxNew, c.maxSeq - prompt.length + 1);  // the last token taken is not run
+  const room = budget ? budget + 1 : prompt.length + most;
   const cache = new KV4Cache(c.nLayers, room, c.nKvHeads, c.dHead, { sequences: beams, trackWeights: budget > 0 });
   const b = new Beams(1, beams);
   try {
@@ -92,14 +95,14 @@ export function beamSearch(transformer, prompt, { beams = 4, maxNew = 32, eos, b
     cache.reorder(idle.map(() => 0));  // all beams go on from the prompt
     b.set(idle.map((_, i) => (i === 0 ? 0 : -Infinity)), new Int32Array(beams));
     let rows = idle.map(() => ({ tokens: [], done: false }));
-    for (let n = 0; n < maxNew; n++) {
+    for (let n = 0; n < most; n++) {
       b.select(e.logits, V, eos);
       const tokens = b.read(b.token, new Int32Array(beams)), parents = b.read(b.parent, new Int32Array(beams));
       rows = rows.map((_, i) => {
         const p = rows[parents[i]];
         return p.done ? p : { tokens: p.tokens.concat(tokens[i]), done: tokens[i] === eos };
       });
-      if (n + 1 === maxNew || rows.every((r) => r.done)) break;
+      if (n + 1 === most || rows.every((r) => r.done)) break;
       hip().kv4Reorder(cache.handle, b.parent, beams);
       cache._follow(parents, beams);
       step(rows.map((r, i) => (r.done ? -1 : tokens[i])));

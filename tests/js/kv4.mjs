@@ -200,6 +200,22 @@ rec("beamSearch: one beam is greedy, scores are the tokens' log probabilities, f
   return { ok, detail: `rescored ${worst.toExponential(1)}` };
 });
 
+rec("beamSearch up to the model's last position", () => {
+  const { cfg, w } = model(23, { maxSeq: 20 });
+  const tr = new Transformer(cfg).loadWeights(w), prompt = [4, 8, 15, 16, 23];
+  let ok = true;
+  for (const o of [{}, { budget: 6, recent: 2 }]) {
+    const long = beamSearch(tr, prompt, Object.assign({ beams: 3, maxNew: 50, eos: -1 }, o));
+    const just = beamSearch(tr, prompt, Object.assign({ beams: 3, maxNew: 16, eos: -1 }, o));
+    ok = ok && long.every((b, i) => b.tokens.length === 16 && same(b.tokens, just[i].tokens) && b.score === just[i].score);
+  }
+  const full = Array.from({ length: 20 }, (_, i) => i);
+  const last = beamSearch(tr, full, { beams: 2, maxNew: 8, eos: -1 });
+  ok = ok && last.every((b) => b.tokens.length === 1) && throws(() => beamSearch(tr, full.concat(1)), RangeError);
+  tr.release();
+  return { ok, detail: "" };
+});
+
 rec("errors", () => {
   const { cfg, w } = model();
   const tr = new Transformer(cfg).loadWeights(w), c = cacheFor(cfg, 8), c2 = cacheFor(cfg, 8, { sequences: 2 });
