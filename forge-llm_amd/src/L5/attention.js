@@ -57,6 +57,12 @@ export class KVCache {
   }
 }
 
+/** What KV4Cache.evict takes: whole numbers of 32 bits, which the device's call holds. */
+export function checkEviction(budget, recent) {
+  if (!Number.isInteger(budget) || budget < 1 || budget > 0x7FFFFFFF) throw new RangeError(`KV4Cache.evict: budget ${budget}`);
+  if (!Number.isInteger(recent) || recent < 0 || recent > budget) throw new RangeError(`KV4Cache.evict: recent ${recent} outside [0, ${budget}]`);
+}
+
 /**
  * A KV cache in 4-bit blocks (Q4_0: 32 values on one fp16 step, 4.5 bits a
  * value), for one or several sequences: 7.1 times the context of KVCache in the
@@ -126,6 +132,9 @@ export class KV4Cache {
    *  committed ones: q [sequences][nHeads][dHead], the same shape returned. */
   attend(layer, q, nHeads, T = 0, scale = 1 / Math.sqrt(this.dHead)) {
     this._layer(layer); this._room(T);
+    if (!Number.isInteger(nHeads) || nHeads <= 0 || nHeads % this.nKvHeads !== 0)
+      throw new RangeError(`KV4Cache.attend: ${nHeads} query heads for ${this.nKvHeads} kv heads`);
+    if (typeof scale !== "number") throw new TypeError(`KV4Cache.attend: scale ${scale}`);
     const n = this.sequences * nHeads * this.dHead, h = this.handle;
     const qh = f32Slice(q, 0, n, "KV4Cache.attend q"), out = new Float32Array(n);
     this._withBuffers([n, n], (a, [bq, bo]) => {
@@ -148,6 +157,7 @@ export class KV4Cache {
    *  newest `recent` and those of most accumulated attention. */
   evict(budget, recent = 0) {
     if (!this.trackWeights) throw new Error("KV4Cache.evict: the cache was made without trackWeights");
+    checkEviction(budget, recent);
     hip().kv4Evict(this.handle, budget, recent);
     for (let s = 0; s < this.sequences; s++) this.lens[s] = Math.min(this.lens[s], budget);
   }

@@ -5,7 +5,7 @@
  * forge-llm, whose sampling (src/L8/sampling.js) draws one token of one sequence.
  */
 import { hip } from "../L2/device.js";
-import { KV4Cache } from "../L5/attention.js";
+import { KV4Cache, checkEviction } from "../L5/attention.js";
 
 /** The device arrays of a selection of `requests` x `beams`. */
 class Beams {
@@ -45,6 +45,7 @@ export function beamSelect(logits, scores, { beams, vocab, requests = 1, done = 
   const n = requests * beams;
   if (!logits || logits.length < n * vocab) throw new RangeError(`beamSelect: ${n} x ${vocab} logits expected`);
   if (!scores || scores.length < n || (done && done.length < n)) throw new RangeError(`beamSelect: ${n} scores and flags expected`);
+  if (!Number.isInteger(eos) || eos >= vocab) throw new RangeError(`beamSelect: eos ${eos}`);
   if (done && eos < 0) throw new RangeError("beamSelect: done needs eos");
   const a = hip(), b = new Beams(requests, beams), x = a.alloc(n * vocab * 4);
   try {
@@ -75,7 +76,8 @@ export function beamSearch(transformer, prompt, { beams = 4, maxNew = 32, eos, b
   if (!prompt || prompt.length < 1) throw new RangeError("beamSearch: the prompt is empty");
   if (!Number.isInteger(beams) || beams < 1 || beams > 64 || beams > V) throw new RangeError(`beamSearch: ${beams} beams`);
   if (!Number.isInteger(maxNew) || maxNew < 1) throw new RangeError(`beamSearch: maxNew ${maxNew}`);
-  if (budget && budget < 1) throw new RangeError(`beamSearch: budget ${budget}`);
+  if (!Number.isInteger(eos) || eos >= V) throw new RangeError(`beamSearch: eos ${eos}`);
+  if (budget) checkEviction(budget, recent);
   if (prompt.length > c.maxSeq) throw new RangeError(`beamSearch: a prompt of ${prompt.length} tokens, the model has ${c.maxSeq} positions`);
   const most = Math.min(maxNew, c.maxSeq - prompt.length + 1);  // the last token taken is not run
   const room = budget ? budget + 1 : prompt.length + most;

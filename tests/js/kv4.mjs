@@ -241,5 +241,33 @@ rec("errors", () => {
   return { ok: e.every((x) => x), detail: e.map(Number).join("") };
 });
 
+rec("numbers that a call would not take as they are", () => {
+  const { cfg, w } = model();
+  const tr = new Transformer(cfg).loadWeights(w), r = new RNG(6);
+  const c = new KV4Cache(1, 12, 2, 32, { trackWeights: true });
+  c.append(0, normal(r, 9 * 64), normal(r, 9 * 64), 9);
+  c.commit(9);
+  const x = new Float32Array(10), s = [0, 0], q = normal(r, 128);
+  const e = [
+    // 2^32 + 5 is 5 in 32 bits: the device would evict, the lengths here would stay
+    throws(() => c.evict(2 ** 32 + 5), RangeError), throws(() => c.evict(4.5), RangeError), throws(() => c.evict(4, 0.5), RangeError),
+    throws(() => c.evict(), RangeError), throws(() => c.evict(4, 5), RangeError), throws(() => c.evict(4, null), RangeError),
+    throws(() => c.evict(0), RangeError), c.len === 9, c.positions(0).length === 9,
+    throws(() => c.attend(0, q, 4, 0, null), TypeError), throws(() => c.attend(0, q, 4, 0, "0.1"), TypeError),
+    throws(() => c.attend(0, q), RangeError), throws(() => c.attend(0, q, 3), RangeError), throws(() => c.attend(0, q, 0), RangeError),
+    throws(() => beamSelect(x, s, { beams: 2, vocab: 5, eos: 2.5 }), RangeError), throws(() => beamSelect(x, s, { beams: 2, vocab: 5, eos: null }), RangeError),
+    throws(() => beamSelect(x, s, { beams: 2, vocab: 5, eos: NaN }), RangeError), throws(() => beamSelect(x, s, { beams: 2, vocab: 5, eos: 5 }), RangeError),
+    throws(() => beamSearch(tr, [1], { eos: 2.5 }), RangeError), throws(() => beamSearch(tr, [1], { eos: null }), RangeError),
+    throws(() => beamSearch(tr, [1], { eos: cfg.vocabSize }), RangeError), throws(() => beamSearch(tr, [1], { budget: 1.5 }), RangeError),
+    throws(() => beamSearch(tr, [1], { budget: -1 }), RangeError), throws(() => beamSearch(tr, [1], { budget: 4, recent: 5 }), RangeError),
+    beamSearch(tr, [1], { beams: 2, maxNew: 2, eos: -7, budget: 0, recent: 5 }).length === 2,
+    c.attend(0, q, 4).every(Number.isFinite),
+  ];
+  c.evict(4, 1);
+  e.push(c.len === 4);
+  tr.release();
+  return { ok: e.every((v) => v), detail: e.map(Number).join("") };
+});
+
 for (const r of out) console.log(JSON.stringify(r));
 process.exit(out.every((r) => r.ok) ? 0 : 1);
