@@ -96,6 +96,7 @@ export class KV4Cache {
     this.lens = new Int32Array(sequences); this.nexts = new Int32Array(sequences);
   }
   get len() { return this.lens[0]; }
+  get freed() { return !this._bufs; }
   /** The device handle (throws once the cache has been freed). */
   get handle() {
     if (!this._bufs) throw new Error("KV4Cache: the cache has been freed");

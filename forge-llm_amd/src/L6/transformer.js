@@ -108,7 +108,7 @@ export class Transformer {
     const c = this.cfg;
     if (c.dim % c.nHeads !== 0) throw new Error(`Transformer: dim ${c.dim} must be a multiple of nHeads ${c.nHeads}`);
     this.logits = new Float32Array(c.vocabSize);
-    this._w = null; this._model = null; this._graphs = []; this._kv4 = null;
+    this._w = null; this._model = null; this._graphs = []; this._kv4 = [];
   }
 
   loadWeights(w) {
@@ -168,35 +168,49 @@ export class Transformer {
     return this._model;
   }
 
-  // The model over vectors of every sequence of a 4-bit cache, kept for the last
-  // cache used.
+  // The model over vectors of every sequence of a 4-bit cache, and its recorded step,
+  // kept for the last GRAPHS_KEPT caches used.
   _kv4For(cache) {
     const c = this.cfg, W = this._w, a = hip();
-    if (this._kv4 && this._kv4.cache === cache) return this._kv4;
-    this._dropKv4();
+    const known = this._kv4.findIndex((e) => e.cache === cache);
+    if (known >= 0) {
+      this._kv4.push(this._kv4.splice(known, 1)[0]);
+      return this._kv4[this._kv4.length - 1];
+    }
+    for (const e of this._kv4.slice()) if (e.cache.freed) this._dropKv4(e.cache);
+    while (this._kv4.length >= GRAPHS_KEPT) this._dropKv4(this._kv4[0].cache);
     const N = cache.sequences, bufs = [];
     const scratch = (n) => { const h = a.alloc(n * 4); bufs.push(h); return h; };
-    const x = scratch(N * c.dim);
-    const model = a.decodeModel({
-      dim: c.dim, hidden: c.hidden, nLayers: c.nLayers, nHeads: c.nHeads, nKvHeads: c.nKvHeads,
-      vocab: c.vocabSize, maxSeq: c.maxSeq, normEps: c.normEps, tok_emb: W.tok, ln_f: W.ln_f, wcls: W.wcls,
-      emb_type: W.emb_type, cls_type: W.cls_type,
-      rope_cos: W.rope_cos, rope_sin: W.rope_sin, x, q: scratch(N * c.dim), h: scratch(N * c.hidden), attn_part: x,
-      layers: W.layers,
-    });
-    this._kv4 = { cache, model, bufs, tokens: scratch(N), logits: scratch(N * c.vocabSize), graph: null, steps: 0 };
-    return this._kv4;
+    try {
+      const x = scratch(N * c.dim);
+      const model = a.decodeModel({
+        dim: c.dim, hidden: c.hidden, nLayers: c.nLayers, nHeads: c.nHeads, nKvHeads: c.nKvHeads,
+        vocab: c.vocabSize, maxSeq: c.maxSeq, normEps: c.normEps, tok_emb: W.tok, ln_f: W.ln_f, wcls: W.wcls,
+        emb_type: W.emb_type, cls_type: W.cls_type,
+        rope_cos: W.rope_cos, rope_sin: W.rope_sin, x, q: scratch(N * c.dim), h: scratch(N * c.hidden), attn_part: x,
+        layers: W.layers,
+      });
+      const e = { cache, model, bufs, tokens: scratch(N), logits: scratch(N * c.vocabSize), graph: null, steps: 0 };
+      this._kv4.push(e);
+      return e;
+    } catch (err) {
+      for (const h of bufs) a.free(h);
+      throw err;
+    }
   }
-  _dropKv4() {
-    if (!this._kv4) return;
+  // Of one cache, or of all.
+  _dropKv4(cache) {
     const a = hip();
-    if (this._kv4.graph) a.graphDestroy(this._kv4.graph);
-    for (const h of this._kv4.bufs) a.free(h);
-    this._kv4 = null;
+    for (const e of this._kv4) {
+      if (cache && e.cache !== cache) continue;
+      if (e.graph) a.graphDestroy(e.graph);
+      for (const h of e.bufs) a.free(h);
+    }
+    this._kv4 = this._kv4.filter((e) => cache && e.cache !== cache);
   }
 
   /** Queues one token of every sequence of a 4-bit cache (logits stay in device
-   *  memory, `_kv4.logits`); a token outside the vocabulary leaves its sequence idle. */
+   *  memory, `logits` of what it returns); a token outside the vocabulary leaves its sequence idle. */
   _stepAll(tokens, cache) {
     const c = this.cfg, a = hip();
     if (!this._w) throw new Error("Transformer.forward: call loadWeights first");

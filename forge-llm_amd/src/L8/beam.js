@@ -113,7 +113,7 @@ export function beamSearch(transformer, prompt, { beams = 4, maxNew = 32, eos, b
     return rows.map((r, i) => ({ tokens: r.tokens, score: scores[i], done: r.done }));
   } finally {
     b.free();
-    transformer._dropKv4();  // its graph and vectors belong to this cache
+    transformer._dropKv4(cache);  // its graph and vectors belong to this cache
     cache.free();
   }
 }

@@ -1,6 +1,6 @@
 // The 4-bit cache and beam search through the JS API (KV4Cache, Transformer.forward /
 // forwardAll over it, beamSelect, beamSearch).  Prints one JSON line per case.
-import { Config, Transformer, KV4Cache, initWeights, beamSelect, beamSearch, RNG } from "../../forge-llm_amd/src/index.js";
+import { Config, Transformer, KV4Cache, initWeights, beamSelect, beamSearch, RNG, hip } from "../../forge-llm_amd/src/index.js";
 
 const out = [];
 function rec(test, fn) {
@@ -267,6 +267,45 @@ rec("numbers that a call would not take as they are", () => {
   e.push(c.len === 4);
   tr.release();
   return { ok: e.every((v) => v), detail: e.map(Number).join("") };
+});
+
+rec("caches in turn on one Transformer keep their recorded steps, a beam search leaves them", () => {
+  const { cfg, w } = model(31), a = hip(), V = cfg.vocabSize;
+  const calls = {};
+  for (const name of ["decodeStepKv4", "graphEnd", "graphLaunch", "graphDestroy"]) {
+    const f = a[name];
+    calls[name] = { n: 0, restore: () => { a[name] = f; } };
+    a[name] = (...x) => { calls[name].n++; return f(...x); };
+  }
+  let ok = true, detail = "";
+  try {
+    const tr = new Transformer(cfg).loadWeights(w), alone = new Transformer(cfg, { graph: false }).loadWeights(w);
+    const caches = [1, 2, 1, 3].map((n) => cacheFor(cfg, 24, { sequences: n }));
+    const refs = caches.map((c) => cacheFor(cfg, 24, { sequences: c.sequences }));
+    const turn = (i, t) => {
+      const ids = Array.from({ length: caches[i].sequences }, (_, s) => (7 * t + 13 * s + i) % V);
+      return same(tr.forwardAll(ids, caches[i]), alone.forwardAll(ids, refs[i]));
+    };
+    for (let t = 0; t < 8; t++) for (let i = 0; i < 4; i++) ok = ok && turn(i, t);
+    // the first step of a cache runs op by op, the second is recorded (one call each), the others replay
+    ok = ok && calls.graphEnd.n === 4 && calls.graphLaunch.n === 4 * 7 && calls.graphDestroy.n === 0 && calls.decodeStepKv4.n === 4 * 2 + 4 * 8;
+    detail += `${calls.graphEnd.n} ${calls.graphLaunch.n} ${calls.decodeStepKv4.n}`;
+    caches[0].free();
+    beamSearch(tr, [3, 1, 4], { beams: 2, maxNew: 4, eos: -1 });  // takes the freed cache's place
+    const recorded = calls.graphEnd.n;
+    for (let i = 1; i < 4; i++) ok = ok && turn(i, 9);
+    ok = ok && calls.graphEnd.n === recorded;
+    // one more than are kept, in turn
+    caches.push(...[1, 2].map((n) => cacheFor(cfg, 24, { sequences: n })));
+    refs.push(...[1, 2].map((n) => cacheFor(cfg, 24, { sequences: n })));
+    for (let t = 10; t < 14; t++) for (let i = 1; i < 6; i++) ok = ok && turn(i, t);
+    tr.release();
+    ok = ok && calls.graphDestroy.n === calls.graphEnd.n;
+    alone.release();
+  } finally {
+    for (const c of Object.values(calls)) c.restore();
+  }
+  return { ok, detail };
 });
 
 for (const r of out) console.log(JSON.stringify(r));
