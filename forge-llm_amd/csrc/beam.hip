@@ -13,8 +13,9 @@ constexpr int kMaxBeams = 64;
 // ── selection ─────────────────────────────────────────────────────────────
 // Each logit is read once, so the choice is made in two launches: a workgroup
 // per segment of a row leaves the segment's maximum, sum of exponentials and W
-// first candidates, then a workgroup per request forms the rows' log sums and
-// picks among the segments' candidates, in fp64.  Both find the W first of many
+// first candidates, then a workgroup per request adds the segments' sums up and
+// picks among their candidates, in fp64; the exponentials and a segment's sum are
+// fp32, which leaves a row's log sum good to about 2^-20.  Both find the W first of many
 // without sorting them: the W-th greatest of the threads' own maxima bounds the
 // W-th greatest of all from below, few values reach it, and those are ranked by
 // counting.  The segments' lists are in order, so the second launch reads each only

@@ -62,7 +62,7 @@ __device__ __forceinline__ float row_sum(float x) {
 // of every block, so a block's extremes are reductions over 16 lanes and the
 // lane's nb bytes are its share of the slot.  HBM-bound (7.1 B read for 1 written)
 // as long as a block costs few instructions: 16384 tokens of 8 heads of 128 43 us
-// (3.6 TB/s, reading alone reaches 4.0), reading them back 26 (5.9 TB/s).
+// (3.6 TB/s read and written), reading them back 26 (5.9 TB/s).
 
 // A block by its definition: the first of the greatest magnitudes by ballots, and
 // floor(x / d + 8.5) from an approximate quotient and the exact borders (c - 8.5) d:
@@ -931,8 +931,9 @@ __device__ __forceinline__ void find_border(AllKeys all_keys, int budget, Search
 }
 
 // Keys in registers (4 Q a thread), read once.  256 heads of 16384 slots 23.6 us, of
-// which reading is 9 to 10.7, the bins 6.5, the ranks 3.3, the lists 5: a workgroup
-// fills a CU, so they do not overlap.
+// which reading is 9 to 10.7, the bins 6.5, the ranks 3.3, the lists 5.  They do not
+// overlap: 256 heads are one workgroup a CU, and 72 registers would not let a second
+// one in (seven waves a SIMD of the eight that two need).
 template <int Q>
 __global__ void __launch_bounds__(kSelect) evict_select_kernel(int32_t* __restrict__ holes,
                                                                int32_t* __restrict__ movers,
@@ -1355,16 +1356,30 @@ int fg::kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, i
   const int64_t heads = (int64_t)c->nSeq * c->nKvHeads * subs, rounds = (c->maxSeq + kRound - 1) / kRound;
   // Short caches, of more slots the more heads there are to fill the chip: a
   // workgroup a head, no second launch (but where shares of a head's query heads
-  // would add to the same weights).  us, a workgroup a head against pieces:
-  //                     256 slots    1024          2048          4096
-  //   12 heads of 64    4.7  8.1     7.0  8.2      10.0  8.4
-  //    8 heads of 128   5.9  8.8     9.6  9.2      14.6  9.9
-  //    8 heads of 256   9.8 11.5    19.6 11.8
-  //   96 heads of 64    4.7 10.6     7.1 12.0      10.2 16.5     18.2 18.2
-  //   64 heads of 128   6.0 11.4     9.6 12.9      15.9 18.4     26.8 21.7
-  //  256 heads of 128   6.2 14.2    11.5 22.0      17.2 29.7     28.8 39.8
-  // (at 8192 slots 256 heads still take 55 against 64, but only as long as the
-  // sequences are: of all lengths, 55 against 45)
+  // would add to the same weights).  The host knows the slots, not how many are in
+  // use.  us, a workgroup a head against pieces, every sequence full and (in
+  // brackets) sequences of all lengths up to that:
+  //                    up to the limit                     beyond it
+  //    8 heads of 32   1536:  7.3  8.3                     2304:  9.1  8.2
+  //   64 heads of 32   2048:  8.6 12.9 (2900: 10.3 12.9)   4096: 13.3 17.9 (13.2 14.0)
+  //  256 heads of 32   7680: 26.5 30.8 (7600: 25.2 24.5)  11520: 37.3 38.2
+  //    8 heads of 64   1280:  7.5  8.3                     1920:  9.1  8.6
+  //   48 heads of 64   1280:  7.6 11.5 ( 7.4 11.2)         2048:  9.7 12.6 ( 9.7 11.6)
+  //   64 heads of 64   2560: 11.2 16.0 (11.0 12.6)         4096: 15.6 20.1 (15.4 16.3)
+  //  256 heads of 64   6400: 26.4 34.0 (25.6 25.3)         9600: 37.1 42.1
+  //    8 heads of 96    512:  7.5  9.5  1024: 10.8  9.8    1536: 14.3 10.1
+  //   64 heads of 96   2048: 17.7 19.5 (17.6 15.3)         4096: 31.1 22.9 (29.5 22.2)
+  //  256 heads of 96   5120: 39.4 48.2 (37.9 35.5)         8192: 59.5 62.9
+  //    8 heads of 128   896:  8.5  9.3                     1344: 10.8  9.9
+  //   48 heads of 128   896:  8.5 13.0 ( 8.5 11.8)         2048: 14.3 15.2 (14.3 13.8)
+  //   64 heads of 128  1792: 12.9 18.2 (12.9 14.4)         2688: 17.7 22.6 (16.9 18.6)
+  //  256 heads of 128  4480: 30.0 40.2 (28.7 31.0)         8192: 55.3 64.0 (47.8 40.6)
+  //    8 heads of 256   256: 10.1 11.5   384: 13.1 11.7     512: 16.0 11.8
+  //   64 heads of 256   512: 16.2 16.0   768: 21.5 20.0    1152: 31.1 27.2 (1024: 26.7 18.9)
+  //  256 heads of 256  1920: 55.8 61.0 (53.5 50.5)         2880: 91.8 80.2
+  // Three classes of heads are coarse: from 48 to some 100 heads of 32 to 128 a
+  // workgroup a head stays ahead for up to 1.5 times the limit, and heads of 96
+  // and 256 cross a little before it.
   const int few = c->dHead == 32 ? 1536 : c->dHead == 64 ? 1280 : c->dHead == 96 ? 1024 : c->dHead == 128 ? 896 : 384;
   const bool whole = c->maxSeq <= few * (heads < 64 ? 1 : heads < 192 ? 2 : 5) && !(c->weight && subs > 1);
   // One sequence: equal pieces, all resident at once (130001 positions of 8 heads

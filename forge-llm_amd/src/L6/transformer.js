@@ -99,7 +99,8 @@ const GRAPHS_KEPT = 4;
  * memory); `opts.graph = false` issues every step op by op.  `cache` must be
  * this package's device KVCache, or its KV4Cache: `forward` takes one of one
  * sequence, at the sequence's next position, `forwardAll(tokens, cache)` one token
- * of every sequence (fg_decode_step_kv4).
+ * of every sequence (fg_decode_step_kv4).  Recorded steps are kept for the last four
+ * caches of each kind.
  */
 export class Transformer {
   constructor(config, opts = {}) {

@@ -690,7 +690,8 @@ int fg_kv4_read(const fg_kv4_cache* c, int layer, float* k, float* v, int64_t ld
  * latter to 2^-33 of the greatest step at least), sums are fp32. */
 int fg_kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
                 const int32_t* count);
-/* Ends a step: len[s] += T (or count[s]; to maxSeq at most), next[s] += the same. */
+/* Ends a step: len[s] += T (or count[s]; to maxSeq at most), next[s] += T (or
+ * count[s]) whether there were slots for all of them or not. */
 int fg_kv4_commit(const fg_kv4_cache* c, int T, const int32_t* count);
 /* Which cached tokens a bounded cache keeps, by accumulated attention: a head
  * [layer][seq][head] of n = len[seq] > budget slots keeps those whose position is
@@ -715,7 +716,8 @@ int fg_kv4_evict(const fg_kv4_cache* c, int budget, int recent);
  * attended to from the cache, and committed at the end, so nothing else changes
  * from step to step and a recorded graph of one serves them all.  A sequence
  * whose token is outside [0, vocab), whose position is outside the model's RoPE
- * table (m->maxSeq) or whose cache is full gets NaN logits and stays as it was.
+ * table (m->maxSeq) or whose cache is full gets NaN logits and stays as it was, its
+ * weights among the rest (the products run for it all the same).
  * m->x, m->q and m->h hold nSeq vectors each; m->attn_part is not used.  The
  * limits of fg_decode_step on dim and hidden hold, the head size is one of the
  * cache's; nSeq <= 65535. */
@@ -733,8 +735,10 @@ int fg_decode_step_kv4(const fg_decode_model* m, const fg_kv4_cache* c, const in
  * eos < 0: none, done NULL.  Logits of -inf are masked tokens: they come after all
  * others.  A beam of masked tokens alone has V candidates of -inf, one whose score
  * less the log of its sum is otherwise not finite V candidates of that value; NaN
- * comes after all others.  Candidates compare in
- * fp64 across beams, by their logits within one.  logits rows have stride ld;
+ * comes after all others.  Candidates compare in fp64 across beams, by their logits
+ * within one.  A beam's log sum is added up from fp32 exponentials and is good to
+ * about 2^-20: candidates of two beams that are closer than that may come in either
+ * order.  logits rows have stride ld;
  * 1 <= W <= 64, nReq W <= 65535, V <= 2^26; outputs apart from the inputs. */
 int fg_beam_select(float* score_out, int32_t* token, int32_t* parent, int32_t* done_out, const float* logits,
                    int64_t ld, const float* scores, const int32_t* done, int eos, int nReq, int W, int V);
@@ -759,7 +763,7 @@ typedef struct fg_beam_state {
 #define FG_BEAM_STATES 8
 int fg_beam_reorder(const fg_beam_state* states, int count, const int32_t* parent, const int32_t* len, int nReq,
                     int W);
-/* fg_beam_reorder of a whole cache, nSeq = requests x W: codes, steps, weights and
+/* fg_beam_reorder of a whole cache of any size, nSeq = requests x W: codes, steps, weights and
  * positions of the slots in use, len and next. */
 int fg_kv4_reorder(const fg_kv4_cache* c, const int32_t* parent, int W);
 
