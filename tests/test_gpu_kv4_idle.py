@@ -2,6 +2,8 @@
 the vocabulary, a full cache, a position past the RoPE table): every array of theirs
 stays bit for bit, the accumulated weights among them, and a later eviction keeps
 what those weights say."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -63,15 +65,52 @@ def test_idle_full_and_far_sequences_keep_their_weights(fh, name):
     np.testing.assert_array_equal(heads2[0], np.minimum(heads1[0], budget))
 
 
+@pytest.mark.parametrize("N", [1, 3])
 @pytest.mark.parametrize("name", ["short", "pieces"])
-def test_all_sequences_idle(fh, name):
+def test_all_sequences_idle(fh, name, N):
     """A step in which none takes part changes nothing."""
     kw, types, maxSeq = SHAPES[name]
-    m = Model(fh, kw, 4, 3, maxSeq, 20, types=types, track=True)
+    m = Model(fh, kw, 4, N, maxSeq, 20, types=types, track=True)
     for t in range(4):
-        m.step([1, 2, 3 + t])
+        m.step([1, 2, 3 + t][:N])
     before = arrays(m)
-    assert np.isnan(m.step([-1, m.cfg.vocab, -5])).all()
+    assert np.isnan(m.step([-1, m.cfg.vocab, -5][:N])).all()
     for a, b in zip(arrays(m), before):
         for x, y in zip(a, b):
             np.testing.assert_array_equal(x, y)
+
+
+@pytest.mark.parametrize("name", ["short", "pieces"])
+def test_a_recorded_step_with_idle_sequences(fh, name):
+    """A graph of one step, replayed with other sequences idle each time and eager work between, does what the eager steps do."""
+    kw, types, maxSeq = SHAPES[name]
+    N, results = 4, []
+    for graph in (False, True):
+        rng = np.random.default_rng(11)
+        m = Model(fh, kw, 4, N, maxSeq, 20, types=types, track=True)
+        m.step(rng.integers(0, m.cfg.vocab, N))
+        handle, got = ctypes.c_void_p(), []
+        if graph:
+            fh.check(fh.lib.fg_graph_begin(), "begin")
+            fh.check(fh.lib.fg_decode_step_kv4(ctypes.byref(m.dec.m), ctypes.byref(m.cache), m.tokens.ptr, m.logits.ptr), "step")
+            fh.check(fh.lib.fg_graph_end(ctypes.byref(handle)), "end")
+        for _ in range(6):
+            tokens = rng.integers(0, m.cfg.vocab, N).astype(np.int32)
+            tokens[rng.random(N) < 0.5] = -1
+            if graph:
+                m.tokens.upload(tokens)
+                fh.check(fh.lib.fg_graph_launch(handle), "launch")
+                junk = [fh.DeviceArray.from_numpy(np.ones(50000, np.float32)) for _ in range(3)]
+                fh.sync()
+                del junk
+                got.append(m.logits.numpy())
+            else:
+                got.append(m.step(tokens))
+            np.testing.assert_array_equal(np.isnan(got[-1]).all(1), tokens < 0)
+        slots, heads = arrays(m)
+        assert np.isfinite(slots[4]).all()
+        results.append(got + slots + heads)
+        if graph:
+            fh.check(fh.lib.fg_graph_destroy(handle), "destroy")
+    for x, y in zip(*results):
+        np.testing.assert_array_equal(x, y)
