@@ -205,6 +205,11 @@ class Kv4Cache(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("k", "v", "kd", "vd", "len", "next", "weight", "pos")])
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int) for n in ("nLayers", "nSeq", "nKvHeads", "dHead", "pageSize", "nPages", "maxPages", "type")]
+                + [(n, ctypes.c_void_p) for n in ("k", "v", "table", "len")])
+
+
 class BeamState(ctypes.Structure):
     _fields_ = [("base", ctypes.c_void_p), ("beam_stride", ctypes.c_int64), ("outer", ctypes.c_int),
                 ("outer_stride", ctypes.c_int64), ("inner", ctypes.c_int), ("inner_stride", ctypes.c_int64),

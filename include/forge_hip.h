@@ -767,6 +767,92 @@ int fg_beam_reorder(const fg_beam_state* states, int count, const int32_t* paren
  * positions of the slots in use, len and next. */
 int fg_kv4_reorder(const fg_kv4_cache* c, const int32_t* parent, int W);
 
+/* ──────────── paged key-value cache of several sequences ────────────
+ * PagedKVCache (attention.js:157-187) for several sequences that share one pool
+ * of pages.  dHead is 32, 64, 96, 128 or 256; pageSize a power of two up to 1024;
+ * a sequence has room for maxPages pageSize <= 2^30 slots, a slot being one cached
+ * token of position = slot.
+ *
+ * Arrays (device; k and v 16-byte aligned)
+ *   k, v    [nLayers][nPages][nKvHeads][pageSize][dHead] of `type`: 0 F32, or
+ *           1 F16 (values are rounded to the nearest, to even between two; above
+ *           65504 they become infinite)
+ *   table   [nSeq][maxPages]: page p of sequence s holds its slots p pageSize ..
+ *           A number outside [0, nPages) is no page: its slots do not exist,
+ *           nothing is written to them, no query sees them.  Sequences may share
+ *           pages that neither appends to; slots that two of them append to in
+ *           one call hold the values of either
+ *   len     [nSeq] slots in use.  A length outside [0, maxPages pageSize] counts as
+ *           the nearer of the two
+ * A step appends T tokens to the layers, attends, and commits once (to fewer, where
+ * drafted tokens did not stand): until then len stands.  `count` (device, [nSeq], or
+ * NULL) gives each sequence its own number of new tokens, held to 0..T; rows of new
+ * tokens are s T + t, and rows t >= count[s] are neither read nor written.  The
+ * structure itself is host memory, read during the call. */
+typedef struct fg_paged_cache {
+  int nLayers, nSeq, nKvHeads, dHead, pageSize, nPages, maxPages, type;
+  void* k;
+  void* v;
+  const int32_t* table;
+  int32_t* len;
+} fg_paged_cache;
+/* PagedKVCache.append (attention.js:157-187) of T tokens for every sequence with
+ * the rotation of their positions (ropeRows, tensor.js:133-149): rows of q (nHeads
+ * dHead values), k and v (nKvHeads dHead values), all of row stride ld; row s T + t
+ * is the token of position len[s] + t.  The first `rot` values (even, 0..dHead) of
+ * each head of q and k turn by the position's angles, in fp64, in pairs (2 i, 2 i + 1)
+ * or, with `half`, (i, i + rot / 2); cos_tab, sin_tab [npos][rot / 2] as
+ * fg_rope_table(.., rot, theta) gives them; a position from npos on turns to NaN.
+ * Keys and values go to slot len[s] + t of `layer`; queries to q_out
+ * [nSeq T][nHeads dHead], which may be q where ld = nHeads dHead.  q and q_out may
+ * be NULL (together: no queries; nHeads is not used). */
+int fg_paged_append(const fg_paged_cache* c, int layer, float* q_out, const float* q, const float* k, const float* v,
+                    int64_t ld, int nHeads, int T, const int32_t* count, const double* cos_tab, const double* sin_tab,
+                    int npos, int rot, int half);
+/* The values of slots first .. first + T - 1 of every sequence into rows s T + t of k
+ * and v (fp32, row stride ld), whether in use or not; zeros for slots of no page
+ * (0 <= first, first + T <= maxPages pageSize). */
+int fg_paged_read(const fg_paged_cache* c, int layer, float* k, float* v, int64_t ld, int first, int T);
+/* Causal attention (causalAttn, tensor.js:191-229) of T appended tokens of every
+ * sequence over its cache: query row s T + t, of position i = len[s] + t, sees slots
+ * j <= i, and with window > 0 of these the last `window` (j > i - window) and the
+ * first `sinks` (j < sinks):
+ *   out[s T + t][h] = sum_j p_j V_j,  p = softmax_j(scale q[s T + t][h] . K_j),
+ * q and out [nSeq T][nHeads][dHead], query head h on kv head h / (nHeads / nKvHeads);
+ * zeros where no slot is seen.  What is not seen, whatever its value, has no part in
+ * it.  Sums are fp32; with an F32 cache products are fp32, with F16 q and p are
+ * held in two fp16 pieces (22 bits). */
+int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
+                  const int32_t* count, int window, int sinks);
+/* Ends a step: len[s] += T (or count[s]; to maxPages pageSize at most). */
+int fg_paged_commit(const fg_paged_cache* c, int T, const int32_t* count);
+
+/* ──────────── drafted tokens ────────────
+ * No counterpart in the reference (its sampling.js:28-98 draws one token from one row). */
+/* Speculative sampling: which of D drafted tokens of each of nSeq sequences stand, and
+ * the token after them.  logits: the target model's, row s (D + 1) + t what it
+ * gives after draft t - 1 (t = 0: after the token before the drafts), row stride ld;
+ * draft_logits: what draft t was drawn from, row s D + t, row stride ld_draft, or NULL
+ * where drafts are certain (of probability 1).  With p and q the softmax of
+ * logits / temperature and draft_logits / temperature:
+ *   draft x of row t stands if u[s (D + 1) + t] q_t(x) < p_t(x) and all before it stand;
+ *   with n of them standing, the next token is drawn from max(p_n - q_n, 0) (from p_n
+ *   for n = the number of drafts, or where that is nothing): the least whose cumulated
+ *   weight exceeds u[s (D + 1) + D] of the whole.
+ * temperature 0: a draft stands if it is the lowest token of greatest logit, which is
+ * the next one, too (NaN counts below all); draft_logits and u are not used.  Else
+ * temperature >= 1e-30.
+ * token [nSeq][D + 1]: the standing drafts, the next token, then -1; count [nSeq]: how
+ * many those are, n + 1, as fg_paged_commit takes it.  Where a row's probabilities are not
+ * numbers (a NaN, an infinite logit, all -inf), its draft does not stand, and what is
+ * drawn from it is -1.  drafted (device, [nSeq], or NULL: D) is each sequence's number of
+ * drafts, D at most; one below 0 takes no part: tokens -1, count 0.  A draft outside
+ * [0, V) does not stand.  Probabilities and sums are fp64.  u in [0, 1);
+ * D <= 1023, V <= 2^26, nSeq (D + 1) <= 65535 x 16; outputs apart from the inputs. */
+int fg_draft_verify(int32_t* token, int32_t* count, const float* logits, int64_t ld, const float* draft_logits,
+                    int64_t ld_draft, const int32_t* draft, const int32_t* drafted, const float* u, double temperature,
+                    int nSeq, int D, int V);
+
 #ifdef __cplusplus
 }
 #endif
