@@ -157,47 +157,596 @@ __global__ void paged_commit_kernel(Cache c, int T, const int32_t* __restrict__ 
 }
 
 // ── attention ─────────────────────────────────────────────────────────────
-// A wave takes a query of a head, its lanes the head's values.
-template <class KV>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(Cache c, int layer, int dH, float* __restrict__ out,
-                                                              const float* __restrict__ q, int nH, float scale, int T,
-                                                              const int32_t* __restrict__ count, int window, int sinks) {
-  const int64_t item = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  const int64_t row = item / nH;
-  const int h = (int)(item - row * nH), lane = threadIdx.x & 63;
-  const int s = (int)(row / T), t = (int)(row - (int64_t)s * T);
-  if (s >= c.nSeq || t >= new_tokens(count, s, T)) return;
-  const int kvh = h / (nH / c.nKV);
-  const int64_t pos = (int64_t)slots_used(c, s) + t;
-  const int end = (int)min(pos + 1, (int64_t)slots(c));
-  const int64_t begin = window > 0 ? pos + 1 - window : 0;  // first slot of the window
-  constexpr int N = 4;                                       // values of a lane, up to 256 a head
-  float qv[N], o[N] = {}, top = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) qv[i] = lane + 64 * i < dH ? q[item * dH + lane + 64 * i] * scale : 0.f;
-  for (int j = 0; j < end; ++j) {
-    if (j >= sinks && j < begin) j = (int)begin;
-    if (j >= end) break;
-    const int64_t slot = slot_row(c, layer, s, j);
-    if (slot < 0) continue;
-    const KV* key = (const KV*)c.k + (slot + ((int64_t)kvh << c.lg)) * dH;
-    const KV* val = (const KV*)c.v + (slot + ((int64_t)kvh << c.lg)) * dH;
-    float d = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane + 64 * i < dH) d += qv[i] * (float)key[lane + 64 * i];
-    d = fg_wave_sum(d);
-    const float was = top;
-    top = fmaxf(top, d);
-    const float keep = was == -INFINITY ? 0.f : expf(was - top), p = expf(d - top);
-    sum = sum * keep + p;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (lane + 64 * i < dH) o[i] = o[i] * keep + p * (float)val[lane + 64 * i];
+// The rows of a kv head are the queries of its group: row t group + h is query head h
+// of the group of token t.  A wave takes a tile of NT x 16 rows through steps of Keys slots
+// (16 rows and 16 slots a matrix instruction), all in registers, and joins what others
+// of its workgroup and of other workgroups have found of the same rows at the end.
+//
+// Scores are formed slots x rows and the sums values x rows, so that a lane has one
+// row (lane & 15) throughout: its reference, its sum and its factors need no other
+// lane, and the scores that the instruction leaves in a lane, slots 4 g .. 4 g + 3 (g = lane >> 4)
+// of a sixteen, are the second operand of the sums as they are.  The first operand of
+// the sums wants a value of those slots for the lane's d: rows of V come in as runs, E values of
+// every slot a lane, and the instruction's 16 rows are d = E i + e, e by e.
+//
+// fp32 caches multiply in fp32 (16x16x4).  fp16 caches multiply as they are
+// (16x16x32), q and p against them in two fp16 pieces each: 22 bits.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Queries of a call: the sequences' rows, and which slots they see.
+struct Span {
+  int T, group, rows;  // rows of a workgroup
+  int window, sinks, keys;
+  const int32_t* count;
+};
+struct Steps {  // steps of slots that some of the rows of tokens t0 .. t1 see: the first `sink`, then from `low` on
+  int sink, low, total;
+  __device__ __forceinline__ int at(int x) const { return x < sink ? x : x - sink + low; }
+};
+__device__ __forceinline__ Steps steps_of(const Cache& c, const Span& q, int used, int t0, int t1) {
+  const int first = used + t0, end = min(used + t1 + 1, slots(c));  // (slots(c) <= 2^30)
+  Steps s;
+  s.low = q.window > 0 ? min(max(first - q.window + 1, 0), end) / q.keys : 0;
+  s.sink = q.window > 0 ? min((min(q.sinks, end) + q.keys - 1) / q.keys, s.low) : 0;
+  s.total = s.sink + (end + q.keys - 1) / q.keys - s.low;
+  return s;
+}
+
+// Which part of the work a workgroup has.  Sequences are cut into pieces of `per`
+// steps, as many as make about `target` workgroups of all of them, whatever their
+// lengths; every wave finds its own, its lanes sharing the sequences out.
+struct Part {
+  int s, kvh, tile, piece, pieces, per;
+  int64_t first;  // pieces of the sequences before
+};
+__device__ __forceinline__ int tiles_of(const Span& q, int tokens) { return (tokens * q.group + q.rows - 1) / q.rows; }
+// id: a workgroup, or with by_seq a sequence, whose `first`, `pieces` and `per` are found.
+__device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int64_t id, bool by_seq) {
+  const int lane = threadIdx.x & 63, each = (c.nSeq + 63) / 64;
+  const int from = min(lane * each, c.nSeq), to = min(from + each, c.nSeq);
+  auto steps = [&](int s, int tokens) { return steps_of(c, q, slots_used(c, s), 0, tokens - 1).total; };
+  int64_t work = 0;
+  for (int s = from; s < to; ++s) {
+    const int n = new_tokens(q.count, s, q.T);
+    if (n > 0) work += (int64_t)steps(s, n) * tiles_of(q, n);
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (lane + 64 * i < dH) out[item * dH + lane + 64 * i] = sum == 0.f ? 0.f : o[i] / sum;
+  for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
+  const int64_t per = (work * c.nKV + target - 1) / target;
+  p.per = ((int)min(max(per, (int64_t)1), (int64_t)1 << 28) + kWaves - 1) / kWaves * kWaves;
+  auto groups = [&](int s, int& pieces) -> int64_t {
+    const int n = new_tokens(q.count, s, q.T);
+    pieces = n > 0 ? (steps(s, n) + p.per - 1) / p.per : 0;
+    return (int64_t)pieces * tiles_of(q, n) * c.nKV;
+  };
+  int64_t mine = 0;
+  for (int s = from, pieces; s < to; ++s) mine += groups(s, pieces);
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t below = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += below;
+  }
+  const uint64_t has = __ballot(by_seq ? id >= from && id < to : id < upto);
+  if (has == 0) return false;
+  const int owner = __builtin_ctzll(has);
+  p.first = __shfl(upto - mine, owner, 64);
+  for (p.s = owner * each;; ++p.s) {
+    const int64_t here = groups(p.s, p.pieces);
+    if (by_seq ? p.s == id : id < p.first + here) break;
+    p.first += here;
+  }
+  if (by_seq) return true;
+  const int in_seq = (int)(id - p.first), n = new_tokens(q.count, p.s, q.T), tiles = tiles_of(q, n);
+  p.piece = in_seq % p.pieces;
+  p.tile = in_seq / p.pieces % tiles;
+  p.kvh = in_seq / p.pieces / tiles;
+  return true;
+}
+
+// Slots of a step as a lane holds them: keys of slot i (and 16 + i), 8 (fp32: 4) values of every 32 (16) from 8 g (4 g) on;
+// values of slots 4 g .. 4 g + 3 (and 16 more on), runs of E.
+template <class KV, int DH>
+struct Step;
+template <int DH>
+struct Step<_Float16, DH> {
+  static constexpr int Keys = 32, Sub = 2, E = DH == 32 ? 2 : DH == 64 ? 4 : DH == 96 ? 6 : 8, Runs = DH / (16 * E);
+  static constexpr float kOver = 11.f;  // p is held as 2^11 p: up to 2^4 above the reference it is below 2^15
+  f16x8 k[Sub][DH / 32];
+  uint32_t v[4 * Sub][Runs][E / 2];
+  __device__ __forceinline__ void load_k(const _Float16* (&row)[Sub]) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int u = 0; u < Sub; ++u)
+#pragma unroll
+      for (int b = 0; b < DH / 32; ++b) k[u][b] = *reinterpret_cast<const f16x8*>(row[u] + 32 * b + 8 * g);
+  }
+  __device__ __forceinline__ void load_v(const _Float16* (&row)[Sub]) {
+    const int i = threadIdx.x & 15;
+#pragma unroll
+    for (int j = 0; j < 4 * Sub; ++j)
+#pragma unroll
+      for (int r = 0; r < Runs; ++r)
+        __builtin_memcpy(v[j][r], __builtin_assume_aligned(row[j / 4] + (j % 4) * DH + r * 16 * E + i * E, E == 6 ? 4 : 2 * E), 2 * E);
+  }
+  __device__ __forceinline__ void clear(int j) {
+#pragma unroll
+    for (int r = 0; r < Runs; ++r)
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) v[j][r][e] = 0;
+  }
+  __device__ __forceinline__ bool finite() const {
+    bool ok = true;
+#pragma unroll
+    for (int j = 0; j < 4 * Sub; ++j)
+#pragma unroll
+      for (int r = 0; r < Runs; ++r)
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) ok &= (v[j][r][e] & 0x7C00u) != 0x7C00u && (v[j][r][e] & 0x7C000000u) != 0x7C000000u;
+    return ok;
+  }
+  // q's operand of a tile: two pieces of q 2^e, its greatest value just below 2^15
+  static constexpr int kQ = DH / 32 * 2;  // 16-byte words a lane
+  static __device__ __forceinline__ float pack_q(u32x4 (*to)[64], const float* q, float factor, bool on) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    float x[DH / 32][8], m = 0.f;
+#pragma unroll
+    for (int b = 0; b < DH / 32; ++b)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[b][j] = on ? q[32 * b + 8 * g + j] * factor : 0.f;
+        m = fmaxf(m, fabsf(x[b][j]));
+      }
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const int e = m > 0.f && m < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
+#pragma unroll
+    for (int b = 0; b < DH / 32; ++b) {
+      f16x8 hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = __builtin_amdgcn_ldexpf(x[b][j], e);
+        hi[j] = (_Float16)y;
+        lo[j] = (_Float16)(y - (float)hi[j]);
+      }
+      to[2 * b][lane] = __builtin_bit_cast(u32x4, hi);
+      to[2 * b + 1][lane] = __builtin_bit_cast(u32x4, lo);
+    }
+    return __builtin_amdgcn_ldexpf(1.f, -e);
+  }
+  __device__ __forceinline__ void scores(f32x4 (&s)[Sub], const u32x4 (*q)[64]) const {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < Sub; ++u) s[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < DH / 32; ++b) {
+      const f16x8 hi = __builtin_bit_cast(f16x8, q[2 * b][lane]), lo = __builtin_bit_cast(f16x8, q[2 * b + 1][lane]);
+#pragma unroll
+      for (int u = 0; u < Sub; ++u) {
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[u][b], lo, s[u], 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[u][b], hi, s[u], 0, 0, 0);
+      }
+    }
+  }
+  // o += V^T p for NT tiles of rows
+  template <int NT>
+  __device__ __forceinline__ void sums(f32x4 (&o)[NT][DH / 16], const f32x4 (&p)[NT][Sub]) const {
+    f16x8 hi[NT], lo[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) hi[n][j] = (_Float16)p[n][j / 4][j % 4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lo[n][j] = (_Float16)(p[n][j / 4][j % 4] - (float)hi[n][j]);
+    }
+#pragma unroll
+    for (int r = 0; r < Runs; ++r)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          w[j] = __builtin_amdgcn_perm(v[2 * j + 1][r][e / 2], v[2 * j][r][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+        const f16x8 a = __builtin_bit_cast(f16x8, w);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          o[n][r * E + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo[n], o[n][r * E + e], 0, 0, 0);
+          o[n][r * E + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[n], o[n][r * E + e], 0, 0, 0);
+        }
+      }
+  }
+};
+template <int DH>
+struct Step<float, DH> {
+  static constexpr int Keys = 16, Sub = 1, E = DH == 32 || DH == 96 ? 2 : 4, Runs = DH / (16 * E);
+  static constexpr float kOver = 0.f;
+  f32x4 k[Sub][DH / 16];
+  float v[4][Runs][E];
+  __device__ __forceinline__ void load_k(const float* (&row)[Sub]) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int b = 0; b < DH / 16; ++b) k[0][b] = *reinterpret_cast<const f32x4*>(row[0] + 16 * b + 4 * g);
+  }
+  __device__ __forceinline__ void load_v(const float* (&row)[Sub]) {
+    const int i = threadIdx.x & 15;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < Runs; ++r)
+        __builtin_memcpy(v[j][r], __builtin_assume_aligned(row[0] + j * DH + r * 16 * E + i * E, 4 * E), 4 * E);
+  }
+  __device__ __forceinline__ void clear(int j) {
+#pragma unroll
+    for (int r = 0; r < Runs; ++r)
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[j][r][e] = 0.f;
+  }
+  __device__ __forceinline__ bool finite() const {
+    bool ok = true;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < Runs; ++r)
+#pragma unroll
+        for (int e = 0; e < E; ++e) ok &= fabsf(v[j][r][e]) < INFINITY;
+    return ok;
+  }
+  static constexpr int kQ = DH / 16;
+  static __device__ __forceinline__ float pack_q(u32x4 (*to)[64], const float* q, float factor, bool on) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < DH / 16; ++b) {
+      f32x4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = on ? q[16 * b + 4 * g + j] * factor : 0.f;
+      to[b][lane] = __builtin_bit_cast(u32x4, x);
+    }
+    return 1.f;
+  }
+  __device__ __forceinline__ void scores(f32x4 (&s)[Sub], const u32x4 (*q)[64]) const {
+    const int lane = threadIdx.x & 63;
+    s[0] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < DH / 16; ++b) {
+      const f32x4 x = __builtin_bit_cast(f32x4, q[b][lane]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0][b][j], x[j], s[0], 0, 0, 0);
+    }
+  }
+  template <int NT>
+  __device__ __forceinline__ void sums(f32x4 (&o)[NT][DH / 16], const f32x4 (&p)[NT][Sub]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < Runs; ++r)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            o[n][r * E + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j][r][e], p[n][0][j], o[n][r * E + e], 0, 0, 0);
+  }
+};
+
+// Scores are in units of log 2, references are scores; a tile's reference moves where a
+// score is more than kRise above it.
+constexpr float kRise = 4.f;
+__device__ __forceinline__ float over_groups_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float over_groups_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// part_ml, part_o: references and sums, and values of the pieces, a workgroup's rows
+// each; null: every sequence is one piece.
+template <class KV, int DH, int NT>
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(Cache c, int layer, float* __restrict__ out,
+                                                              const float* __restrict__ q, int nH, float factor, Span span,
+                                                              int target, float2* __restrict__ part_ml,
+                                                              float* __restrict__ part_o) {
+  using S = Step<KV, DH>;
+  constexpr int Keys = S::Keys, Sub = S::Sub, E = S::E, Runs = S::Runs, M = DH / 16, kRow = DH + 4;
+  constexpr int kShared = NT * S::kQ * 64 * 16 > kWaves * 16 * kRow * 4 ? NT * S::kQ * 64 * 16 : kWaves * 16 * kRow * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t shared[kShared];  // q's operand, and the waves' values at the end
+  __shared__ float2 wave_ml[kWaves][NT * 16];
+  u32x4(*const qs)[64] = reinterpret_cast<u32x4(*)[64]>(shared);  // [NT kQ]
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Part p;
+  if (part_ml) {
+    if (!part_of(p, c, span, target, blockIdx.x, false)) return;
+  } else {
+    const int tiles = tiles_of(span, span.T);
+    p.tile = blockIdx.x % tiles;
+    p.kvh = blockIdx.x / tiles % c.nKV;
+    p.s = blockIdx.x / tiles / c.nKV;
+    p.piece = 0;
+    p.pieces = 1;
+    p.per = INT32_MAX;
+  }
+  const int s = __builtin_amdgcn_readfirstlane(p.s), kvh = __builtin_amdgcn_readfirstlane(p.kvh);
+  const int row0 = __builtin_amdgcn_readfirstlane(p.tile) * (16 * NT), pieces = __builtin_amdgcn_readfirstlane(p.pieces);
+  const int tokens = new_tokens(span.count, s, span.T), rows = min(tokens * span.group - row0, 16 * NT);
+  if (rows <= 0) return;
+  const int used = slots_used(c, s), t0 = row0 / span.group, t1 = (row0 + rows - 1) / span.group;
+  const Steps steps = steps_of(c, span, used, t0, t1);
+  const int per = __builtin_amdgcn_readfirstlane(p.per);
+  const int begin = min((int64_t)__builtin_amdgcn_readfirstlane(p.piece) * per, (int64_t)steps.total);
+  const int end = min((int64_t)begin + per, (int64_t)steps.total);
+
+  // Pages of the step's slots that this lane reads: of its keys and its values.
+  const int32_t* table = c.table + (int64_t)s * c.maxPages;
+  struct Pages {
+    int k[Sub], v[Sub];
+  };
+  auto find = [&](int x) {
+    Pages pg;
+    const int j = steps.at(min(x, steps.total - 1)) * Keys;
+#pragma unroll
+    for (int u = 0; u < Sub; ++u) {
+      const int pk = (j + 16 * u + i) >> c.lg, pv = (j + 16 * u + 4 * g) >> c.lg;
+      pg.k[u] = pk < c.maxPages ? table[pk] : -1;
+      pg.v[u] = pv < c.maxPages ? table[pv] : -1;
+    }
+    return pg;
+  };
+  // Row of a slot in a layer's pages; slots of no page are read from the first page and not seen.
+  const KV* const kbase = (const KV*)c.k + ((((int64_t)layer * c.nPages) * c.nKV + kvh) << c.lg) * DH;
+  const KV* const vbase = (const KV*)c.v + ((((int64_t)layer * c.nPages) * c.nKV + kvh) << c.lg) * DH;
+  const uint32_t inside = (1u << c.lg) - 1;
+  auto row_at = [&](const KV* base, int page, int j) {
+    const uint32_t there = (uint32_t)page < (uint32_t)c.nPages ? (uint32_t)page : 0u;
+    return base + (((uint64_t)there * (uint32_t)c.nKV << c.lg) + ((uint32_t)j & inside)) * DH;
+  };
+  auto key_rows = [&](const Pages& pg, int x, const KV* (&r)[Sub]) {
+    const int j = steps.at(x) * Keys;
+#pragma unroll
+    for (int u = 0; u < Sub; ++u) r[u] = row_at(kbase, pg.k[u], j + 16 * u + i);
+  };
+  auto value_rows = [&](const Pages& pg, int x, const KV* (&r)[Sub]) {
+    const int j = steps.at(x) * Keys;
+#pragma unroll
+    for (int u = 0; u < Sub; ++u) r[u] = row_at(vbase, pg.v[u], j + 16 * u + 4 * g);
+  };
+
+  S step;
+  Pages now, next;
+  int x = begin + wave;
+  if (x < end) {
+    now = find(x);
+    next = find(x + kWaves);
+    const KV* r[Sub];
+    key_rows(now, x, r);
+    step.load_k(r);
+    value_rows(now, x, r);
+    step.load_v(r);
+  }
+
+  // q's operand, a wave every fourth tile of rows, and each tile's factor to the lanes
+  __shared__ float unscale[NT * 16];
+  for (int n = wave; n < NT; n += kWaves) {
+    const int row = n * 16 + i, r = row0 + min(row, rows - 1), t = r / span.group, h = r - t * span.group;
+    const float f = S::pack_q(qs + n * S::kQ, q + (((int64_t)s * span.T + t) * nH + kvh * span.group + h) * DH, factor, row < rows);
+    if (g == 0) unscale[row] = f;
+  }
+  __syncthreads();
+  float back[NT], ref[NT], sum[NT];
+  int pos[NT];
+  f32x4 o[NT][M];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    back[n] = unscale[n * 16 + i];
+    pos[n] = used + (row0 + min(n * 16 + i, rows - 1)) / span.group;
+    ref[n] = -INFINITY;
+    sum[n] = 0.f;
+#pragma unroll
+    for (int m = 0; m < M; ++m) o[n][m] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  const int first_pos = used + t0, last_pos = used + t1;
+  const int window = span.window > 0 ? span.window : INT32_MAX;
+
+  for (; x < end; x += kWaves) {
+    const int j0 = steps.at(x) * Keys;
+    f32x4 sc[NT][Sub];
+    int again = 0;
+    asm volatile("" : "+s"(again));  // q's operand is read anew each step: kept, it would fill the registers
+#pragma unroll
+    for (int n = 0; n < NT; ++n) step.scores(sc[n], qs + n * S::kQ + again);
+    const Pages here = now;
+    const bool more = x + kWaves < end;
+    if (more) {
+      const KV* r[Sub];
+      key_rows(next, x + kWaves, r);
+      step.load_k(r);
+      now = next;
+      next = find(x + 2 * kWaves);
+    }
+    bool pages = true;
+#pragma unroll
+    for (int u = 0; u < Sub; ++u) pages &= (uint32_t)here.v[u] < (uint32_t)c.nPages;
+    // every row sees every slot of the step
+    const bool whole = j0 + Keys - 1 <= first_pos && (j0 > last_pos - window || j0 + Keys <= span.sinks) && __all(pages);
+    bool slow = false;
+    if (!whole) {
+      bool seen[4 * Sub];  // by some row
+#pragma unroll
+      for (int j = 0; j < 4 * Sub; ++j) {
+        const int at = j0 + 16 * (j / 4) + 4 * g + j % 4;
+        const bool there = (uint32_t)here.v[j / 4] < (uint32_t)c.nPages;
+        seen[j] = there && at <= last_pos && (at > first_pos - window || at < span.sinks);
+        if (!seen[j]) step.clear(j);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          if (!(there && at <= pos[n] && (at > pos[n] - window || at < span.sinks))) sc[n][j / 4][j % 4] = -INFINITY;
+      }
+      slow = !__all(step.finite());
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4 * Sub; ++j) {
+        sc[n][j / 4][j % 4] *= back[n];
+        top = fmaxf(top, sc[n][j / 4][j % 4]);
+      }
+      if (__any(top > ref[n] + kRise)) {
+        const float was = ref[n];
+        ref[n] = fmaxf(was, over_groups_max(top));
+        const float keep = ref[n] == was ? 1.f : __builtin_amdgcn_exp2f(was - ref[n]);
+        sum[n] *= keep;
+#pragma unroll
+        for (int m = 0; m < M; ++m) o[n][m] *= keep;
+      }
+      const float base = S::kOver - ref[n];
+#pragma unroll
+      for (int j = 0; j < 4 * Sub; ++j) {
+        const float y = sc[n][j / 4][j % 4];
+        float e = __builtin_amdgcn_exp2f(y + base);
+        if (!whole) {
+          const int at = j0 + 16 * (j / 4) + 4 * g + j % 4;
+          const bool there = (uint32_t)here.v[j / 4] < (uint32_t)c.nPages;
+          if (!(there && at <= pos[n] && (at > pos[n] - window || at < span.sinks))) e = 0.f;
+        }
+        sum[n] += e;
+        sc[n][j / 4][j % 4] = e;
+      }
+    }
+    if (!slow) {
+      step.template sums<NT>(o, sc);
+    } else {
+      // a value that is seen is not finite: it must not reach the rows that do not see it
+      for (int j = 0; j < Keys; ++j) {
+        const int at = j0 + j, page = (at >> c.lg) < c.maxPages ? table[at >> c.lg] : -1;
+        if ((uint32_t)page >= (uint32_t)c.nPages) continue;
+        const KV* row = row_at(vbase, page, at);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const bool mine = at <= pos[n] && (at > pos[n] - window || at < span.sinks);
+          float e = 0.f;
+#pragma unroll
+          for (int u = 0; u < Sub; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float y = __shfl(sc[n][u][r], i + 16 * ((j & 15) >> 2), 64);
+              if (j >> 4 == u && (j & 3) == r) e = y;
+            }
+          if (mine) {
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[n][m][r] += e * (float)row[(m / E) * 16 * E + (4 * g + r) * E + m % E];
+          }
+        }
+      }
+    }
+    if (more) {
+      const KV* r[Sub];
+      value_rows(now, x + kWaves, r);
+      step.load_v(r);
+    }
+  }
+
+  // the waves' parts joined
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    sum[n] = over_groups_sum(sum[n]);
+    if (g == 0) wave_ml[wave][n * 16 + i] = make_float2(ref[n], sum[n]);
+  }
+  float* const vals = reinterpret_cast<float*>(shared);  // [kWaves][16][kRow]
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_ml[w][n * 16 + i].x);
+    const float f = ref[n] == top ? 1.f : __builtin_amdgcn_exp2f(ref[n] - top);
+#pragma unroll
+    for (int r = 0; r < Runs; ++r)
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+#pragma unroll
+        for (int e = 0; e < E; ++e) vals[(wave * 16 + i) * kRow + r * 16 * E + (4 * g + z) * E + e] = o[n][r * E + e][z] * f;
+    __syncthreads();
+    constexpr int kQuads = DH / 4;
+    for (int at = threadIdx.x; at < 16 * kQuads; at += kThreads) {
+      const int row = at / kQuads, d = (at - row * kQuads) * 4;
+      if (n * 16 + row >= rows) break;
+      float most = -INFINITY, all = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) most = fmaxf(most, wave_ml[w][n * 16 + row].x);
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float2 ml = wave_ml[w][n * 16 + row];
+        all += ml.y * (ml.x == most ? 1.f : __builtin_amdgcn_exp2f(ml.x - most));
+        y += *reinterpret_cast<const f32x4*>(vals + (w * 16 + row) * kRow + d);
+      }
+      if (pieces > 1) {
+        const int64_t part = (int64_t)blockIdx.x * (16 * NT) + n * 16 + row;
+        *reinterpret_cast<f32x4*>(part_o + part * DH + d) = y;
+        if (d == 0) part_ml[part] = make_float2(most, all);
+      } else {
+        const int r = row0 + n * 16 + row, t = r / span.group, h = r - t * span.group;
+        float* to = out + (((int64_t)s * span.T + t) * nH + kvh * span.group + h) * DH + d;
+        const float f = all == 0.f ? 0.f : 1.f / all;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) to[z] = y[z] * f;
+      }
+    }
+  }
+}
+
+// A workgroup joins the pieces of a row.
+template <int DH>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(Cache c, float* __restrict__ out, int nH, Span span, int target,
+                                                              const float2* __restrict__ part_ml,
+                                                              const float* __restrict__ part_o) {
+  constexpr int kQuads = DH / 4, kSets = kThreads / kQuads;
+  __shared__ f32x4 vals[kSets][kQuads];
+  __shared__ float sums[kSets];
+  const int t = blockIdx.x / nH % span.T, h = blockIdx.x % nH, s = blockIdx.x / nH / span.T;
+  const int tokens = new_tokens(span.count, s, span.T);
+  if (t >= tokens) return;
+  Part p;
+  if (!part_of(p, c, span, target, s, true) || p.pieces <= 1) return;
+  const int kvh = h / span.group, row = t * span.group + (h - kvh * span.group), tile = row / span.rows;
+  const int64_t first = (p.first + ((int64_t)kvh * tiles_of(span, tokens) + tile) * p.pieces) * span.rows + (row - tile * span.rows);
+  float top = -INFINITY;
+  for (int x = threadIdx.x & 63; x < p.pieces; x += 64) top = fmaxf(top, part_ml[first + (int64_t)x * span.rows].x);
+  top = fg_wave_max(top);
+  const int set = threadIdx.x / kQuads, quad = threadIdx.x - set * kQuads;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  float all = 0.f;
+  if (set < kSets) {
+    for (int x = set; x < p.pieces; x += kSets) {
+      const int64_t at = first + (int64_t)x * span.rows;
+      const float2 ml = part_ml[at];
+      const float f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+      all += ml.y * f;
+      y += *reinterpret_cast<const f32x4*>(part_o + at * DH + 4 * quad) * f;
+    }
+    vals[set][quad] = y;
+    if (quad == 0) sums[set] = all;
+  }
+  __syncthreads();
+  if (threadIdx.x >= kQuads) return;
+  y = vals[0][quad];
+  all = sums[0];
+#pragma unroll
+  for (int x = 1; x < kSets; ++x) {
+    y += vals[x][quad];
+    all += sums[x];
+  }
+  const float f = all == 0.f ? 0.f : 1.f / all;
+  float* to = out + ((int64_t)s * span.T * nH + (int64_t)t * nH + h) * DH + 4 * quad;
+#pragma unroll
+  for (int z = 0; z < 4; ++z) to[z] = y[z] * f;
 }
 
 // ── entry points' checks ──────────────────────────────────────────────────
@@ -210,7 +759,7 @@ int check_cache(const fg_paged_cache* c, const char* fn) {
   const int d = c->dHead, p = c->pageSize;
   FG_ARG_CHECK(d == 32 || d == 64 || d == 96 || d == 128 || d == 256,
                "%s: head size %d is not one of 32, 64, 96, 128, 256", fn, d);
-  FG_ARG_CHECK(p > 0 && p <= 1024 && (p & (p - 1)) == 0, "%s: page size %d is not a power of two up to 1024", fn, p);
+  FG_ARG_CHECK(p >= 4 && p <= 1024 && (p & (p - 1)) == 0, "%s: page size %d is not a power of two from 4 to 1024", fn, p);
   FG_ARG_CHECK((int64_t)c->maxPages * p <= 1 << 30, "%s: %d pages of %d slots a sequence are above 2^30", fn,
                c->maxPages, p);
   FG_ARG_CHECK(c->nKvHeads <= 1 << 16 && (int64_t)c->nLayers * c->nPages < (int64_t)1 << 36,
@@ -313,13 +862,54 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   FG_REQUIRE_INIT();
   if (T == 0) return FG_OK;
   fg::KProfScope prof("paged_attn", 0.0, (double)c->nSeq * c->maxPages * c->pageSize * 2 * row_bytes(c));
-  const dim3 grid((unsigned)((items + kWaves - 1) / kWaves));
-  if (c->type == 0)
-    FG_LAUNCH(paged_attn_kernel<float>, grid, dim3(kThreads), 0, view(c), layer, c->dHead, out, q, nHeads, (float)scale,
-              T, count, window, sinks);
-  else
-    FG_LAUNCH(paged_attn_kernel<_Float16>, grid, dim3(kThreads), 0, view(c), layer, c->dHead, out, q, nHeads,
-              (float)scale, T, count, window, sinks);
+  const int group = nHeads / c->nKvHeads, all = T * group;
+  int tiles = all <= 16 ? 1 : all <= 32 || c->dHead == 256 ? 2 : 4;
+  Span span{T, group, 16 * tiles, window, sinks, c->type ? 32 : 16, count};
+  const int64_t heads = (int64_t)c->nSeq * c->nKvHeads * ((all + span.rows - 1) / span.rows);
+  const int64_t room = (int64_t)c->maxPages * c->pageSize;
+  int64_t seen = room;  // by a workgroup's rows, at most
+  if (window > 0 && (int64_t)window + T + sinks + 2 * span.keys < room) seen = (int64_t)window + T + sinks + 2 * span.keys;
+  const int64_t rounds = (seen + span.keys * kWaves - 1) / (span.keys * kWaves);
+  const int cus = fg::device_cu_count() > 0 ? fg::device_cu_count() : 256;
+  const int target = 2 * cus;
+  const bool whole = rounds <= 4 || heads >= 4 * target;
+  const int64_t grid = whole ? heads : heads + target;
+  fg::Workspace ws;
+  float2* part_ml = nullptr;
+  float* part_o = nullptr;
+  if (!whole) {
+    const size_t rows = (size_t)grid * span.rows;
+    PAGED_TRY(ws.get(rows * (sizeof(float2) + c->dHead * sizeof(float))));
+    part_o = (float*)ws.ptr;
+    part_ml = (float2*)(part_o + rows * c->dHead);
+  }
+  const float factor = (float)(scale * M_LOG2E);
+  const Cache cache = view(c);
+#define PAGED_ATTN(KV, DH, NT)                                                                                        \
+  FG_LAUNCH((paged_attn_kernel<KV, DH, NT>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q, nHeads,   \
+            factor, span, target, part_ml, part_o)
+#define PAGED_TILES(KV, DH)                          \
+  if (tiles == 1) PAGED_ATTN(KV, DH, 1);             \
+  else if (tiles == 2) PAGED_ATTN(KV, DH, 2);        \
+  else PAGED_ATTN(KV, (DH == 256 ? 128 : DH), 4) /* heads of 256 have no tiles of 4 */
+#define PAGED_HEAD(DH)                               \
+  do {                                               \
+    if (c->type == 0) {                              \
+      PAGED_TILES(float, DH);                        \
+    } else {                                         \
+      PAGED_TILES(_Float16, DH);                     \
+    }                                                \
+    if (!whole)                                      \
+      FG_LAUNCH(paged_join_kernel<DH>, dim3((unsigned)items), dim3(kThreads), 0, cache, out, nHeads, span, target, \
+                (const float2*)part_ml, (const float*)part_o);                                                     \
+  } while (0)
+  switch (c->dHead) {
+    case 32: PAGED_HEAD(32); break;
+    case 64: PAGED_HEAD(64); break;
+    case 96: PAGED_HEAD(96); break;
+    case 128: PAGED_HEAD(128); break;
+    default: PAGED_HEAD(256); break;
+  }
   return FG_OK;
 }
 

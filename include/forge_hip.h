@@ -769,7 +769,7 @@ int fg_kv4_reorder(const fg_kv4_cache* c, const int32_t* parent, int W);
 
 /* ──────────── paged key-value cache of several sequences ────────────
  * PagedKVCache (attention.js:157-187) for several sequences that share one pool
- * of pages.  dHead is 32, 64, 96, 128 or 256; pageSize a power of two up to 1024;
+ * of pages.  dHead is 32, 64, 96, 128 or 256; pageSize a power of two from 4 to 1024;
  * a sequence has room for maxPages pageSize <= 2^30 slots, a slot being one cached
  * token of position = slot.
  *

@@ -113,7 +113,7 @@ def check_attention(fh, c, rng, layer, nH, T, counts, window=0, sinks=0, scale=N
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("dH,rot,half", [(32, 32, 0), (64, 32, 1), (96, 96, 1), (128, 128, 0), (256, 64, 1), (64, 0, 0), (32, 6, 0),
                                          (96, 50, 1), (128, 2, 1)])
-@pytest.mark.parametrize("nSeq,nH,nKV,T,P,pad", [(1, 1, 1, 1, 1, 0), (3, 6, 2, 5, 4, 4), (4, 5, 5, 3, 16, 1), (2, 12, 3, 40, 8, 0)])
+@pytest.mark.parametrize("nSeq,nH,nKV,T,P,pad", [(1, 1, 1, 1, 4, 0), (3, 6, 2, 5, 4, 4), (4, 5, 5, 3, 16, 1), (2, 12, 3, 40, 8, 0)])
 def test_append(fh, kind, dH, rot, half, nSeq, nH, nKV, T, P, pad):
     rng = np.random.default_rng(dH + rot + nSeq)
     maxPages = -(-(T + 9) // P)
@@ -237,7 +237,7 @@ def test_commit(fh):
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("dH", HEADS)
 @pytest.mark.parametrize("nKV,group,T,P,lens", [
-    (1, 1, 1, 1, [0]), (2, 3, 1, 16, [40, 0, 7, 31]), (1, 8, 5, 8, [3, 64, 129]), (3, 4, 2, 32, [1, 95, 500, 0]), (2, 1, 33, 16, [0, 17]),
+    (1, 1, 1, 4, [0]), (2, 3, 1, 16, [40, 0, 7, 31]), (1, 8, 5, 8, [3, 64, 129]), (3, 4, 2, 32, [1, 95, 500, 0]), (2, 1, 33, 16, [0, 17]),
     (1, 5, 70, 64, [50, 0, 3]), (1, 12, 1, 128, [1300])])
 def test_attention(fh, kind, dH, nKV, group, T, P, lens):
     rng = np.random.default_rng(dH + nKV + T)
