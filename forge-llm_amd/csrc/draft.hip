@@ -4,12 +4,13 @@
 // What decides are two numbers of a row, p(x) and q(x) at its draft, but each needs its row's
 // sum, so the first launch reads every logit of both models once, in chunks, and leaves a
 // greatest logit and a sum of exponentials for each.  The second finds the row that the next
-// token is drawn from, a chunk a workgroup, and sums its weights max(p - q, 0); the third finds the
-// chunk and in it the token that the given number falls on.
+// token is drawn from and sums its weights max(p - q, 0), a piece a wave; the third finds the
+// piece, and in it the token, that the given number falls on (the second does where a workgroup has the
+// whole row.  Letting the last of a sequence's workgroups draw, instead of a launch, needs their sums to be
+// written back between the dies' caches first: 48 us against 12 and 8).
 //
 // Everything from the exponentials on is fp64: an fp32 sum is off by 1e-7 of itself, which among the
-// 1e5 borders between tokens would give another token once in a few thousand draws.  The
-// exponentials take about as long as reading the logits does, and mostly beside it.
+// 1e5 borders between tokens would give another token once in a few thousand draws.
 #include "common.h"
 
 #include <math.h>
@@ -18,9 +19,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kEach = 16, kChunk = kThreads * kEach;  // logits of a thread, of a workgroup
-constexpr int kLast = 1024;                           // threads of the last launch, 4 logits each
-static_assert(kLast * 4 == kChunk, "the last launch takes a chunk");
+constexpr int kEach = 16, kChunk = kThreads * kEach;  // logits of a thread, of a workgroup of the first launch
+constexpr int kDrawWaves = 16;               // of a workgroup of the launches that draw
 
 __device__ __forceinline__ double wave_sum(double x) { return fg_wave_sum_d(x); }
 __device__ __forceinline__ int wave_min(int x) {
@@ -58,38 +58,60 @@ __device__ __forceinline__ const float* target_row(const Args& a, int s, int t) 
 __device__ __forceinline__ const float* draft_row(const Args& a, int s, int t) {
   return a.draft_logits + ((int64_t)s * a.D + t) * a.ld_draft;
 }
-// Logits of chunk c as a thread has them; -inf behind the last.
-__device__ __forceinline__ void load_chunk(float (&x)[kEach], const float* row, int c, int V, bool fours) {
-  const int from = c * kChunk;
-  if (fours && from + kChunk <= V) {
+// N logits a thread from `from` on, a wave's neighbours; -inf behind the last.  Runs of four where rows are aligned.
+template <int N>
+__device__ __forceinline__ void load_logits(float (&x)[N], const float* row, int from, int V, bool fours) {
+  const int lane = threadIdx.x & 63;
+  if (fours && from + 64 * N <= V) {
 #pragma unroll
-    for (int k = 0; k < kEach / 4; ++k) {
-      const float4 y = *reinterpret_cast<const float4*>(row + from + (k * kThreads + threadIdx.x) * 4);
+    for (int k = 0; k < N / 4; ++k) {
+      const float4 y = *reinterpret_cast<const float4*>(row + from + (k * 64 + lane) * 4);
       x[4 * k] = y.x, x[4 * k + 1] = y.y, x[4 * k + 2] = y.z, x[4 * k + 3] = y.w;
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int v = from + k * kThreads + threadIdx.x;
+    for (int k = 0; k < N; ++k) {
+      const int v = from + k * 64 + lane;
       x[k] = v < V ? row[v] : -INFINITY;
     }
   }
 }
-// Where element k of load_chunk stands.
-__device__ __forceinline__ int token_of(int k, int c, int V, bool fours) {
-  const int from = c * kChunk;
-  return fours && from + kChunk <= V ? from + (k / 4 * kThreads + threadIdx.x) * 4 + k % 4 : from + k * kThreads + threadIdx.x;
+// Where element k of load_logits stands.
+template <int N>
+__device__ __forceinline__ int token_of(int k, int from, int V, bool fours) {
+  const int lane = threadIdx.x & 63;
+  return fours && from + 64 * N <= V ? from + (k / 4 * 64 + lane) * 4 + k % 4 : from + k * 64 + lane;
 }
 __device__ __forceinline__ double power(float x, float top, double inv) {
   return x == -INFINITY ? 0.0 : exp(((double)x - (double)top) * inv);
 }
 
+// exp((x - top) inv) for the sums, where about 1e-11 of each is enough (their errors have both
+// signs): t = (x - top) inv log2 e in 1/256ths, its whole part from a table and the exponent, the rest, up to
+// 1/512, by a polynomial in fp32.  19 instructions; exp takes 30, and 16 sequences of 9 rows of
+// 128256 logits then 18 us instead of 27 (13 with fp32 exponentials).
+constexpr int kSteps = 256;
+struct Quick {
+  const double* table;  // 2^(j / kSteps), LDS
+  double top, k;
+  __device__ __forceinline__ double at(float x) const {
+    // below 2^-1000 all the same; NaN is the caller's
+    const double t = fmax(((double)x - top) * k, -1000.0 * kSteps), whole = t + 0x1.8p52;
+    const int n = __double2loint(whole);
+    const float f = (float)(t - (whole - 0x1.8p52)) * (float)(M_LN2 / kSteps);
+    const float c = f * fmaf(f, fmaf(f, 1.f / 6, 0.5f), 1.f);
+    const double base = table[n & (kSteps - 1)], y = fma(base, (double)c, base);
+    return __hiloint2double(__double2hiint(y) + (n >> 8 << 20), __double2loint(y));
+  }
+};
+
 // A workgroup takes a chunk of a row: rows of the target model first, then the draft model's.
 template <bool Greedy>
 __global__ void __launch_bounds__(kThreads) draft_sums_kernel(Sum* __restrict__ sums, Args a, int nSeq) {
   __shared__ float tops[kWaves];
-  __shared__ double parts[kWaves];
+  __shared__ double parts[kWaves], table[kSteps];
   __shared__ int ats[kWaves];
+  static_assert(kSteps == kThreads, "a thread an entry");
   const int64_t row = blockIdx.x / a.chunks;
   const int c = blockIdx.x - (int)row * a.chunks;
   const int64_t targets = (int64_t)nSeq * (a.D + 1);
@@ -99,7 +121,9 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(Sum* __restrict__ 
   if (t > drafts_of(a, s) - second) return;
   const bool fours = second ? a.draft_fours : a.fours;
   float x[kEach];
-  load_chunk(x, second ? draft_row(a, s, t) : target_row(a, s, t), c, a.V, fours);
+  const int from = c * kChunk + (int)(threadIdx.x >> 6) * (64 * kEach);
+  load_logits(x, second ? draft_row(a, s, t) : target_row(a, s, t), from, a.V, fours);
+  if constexpr (!Greedy) table[threadIdx.x] = exp2(threadIdx.x * (1.0 / kSteps));
   float top = x[0];
 #pragma unroll
   for (int k = 1; k < kEach; ++k) top = fmaxf(top, x[k]);
@@ -114,7 +138,7 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(Sum* __restrict__ 
     int at = INT32_MAX;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      const int v = token_of(k, c, a.V, fours);
+      const int v = token_of<kEach>(k, from, a.V, fours);
       if (x[k] == top && v < a.V) at = min(at, v);
     }
     at = wave_min(at);
@@ -126,10 +150,16 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(Sum* __restrict__ 
       sums[blockIdx.x] = Sum{0.0, top, at};
     }
   } else {
-    double sum = 0;
+    bool number = top < INFINITY;  // all of them below infinity
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) sum += power(x[k], top, a.inv);
-    sum = wave_sum(sum);
+    for (int k = 0; k < kEach; ++k) number &= x[k] == x[k];
+    double sum = 0;
+    if (top > -INFINITY) {
+      const Quick quick{table, top, a.inv * (M_LOG2E * kSteps)};
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) sum += quick.at(x[k]);
+    }
+    sum = wave_sum(number ? sum : (double)NAN);
     if (lane == 0) parts[wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -156,69 +186,42 @@ __device__ __forceinline__ void row_sum(const Sum* sums, const Args& a, float& t
   back = m == -INFINITY ? (double)NAN : 1.0 / sum;
 }
 
-// How many drafts of sequence s stand, by the workgroup: a wave a row, kWaves rows at a time.
+// How many drafts of sequence s stand, by the workgroup: a wave a row, kDrawWaves rows at a time.
 __device__ Next next_of(const Sum* sums, const Args& a, int s, int nSeq, int n) {
-  __shared__ Next rows[kWaves];
-  __shared__ int stands[kWaves];
+  __shared__ Next rows[kDrawWaves];
+  __shared__ int stands[kDrawWaves];
   const int wave = threadIdx.x >> 6;
-  for (int t0 = 0;; t0 += kWaves) {
+  for (int t0 = 0;; t0 += kDrawWaves) {
     const int t = t0 + wave;
     if (t <= n) {
       Next r{t, t < n ? a.draft[(int64_t)s * a.D + t] : -1, 0.f, 0.f, 0.0, 0.0};
+      const bool in = t < n && (uint32_t)r.draft < (uint32_t)a.V, two = t < n && a.draft_logits;
+      // (asked for before the sums are)
+      const float x = in ? target_row(a, s, t)[r.draft] : 0.f, y = in && two ? draft_row(a, s, t)[r.draft] : 0.f;
+      const float u = t < n ? a.u[(int64_t)s * (a.D + 1) + t] : 0.f;
       row_sum(sums + ((int64_t)s * (a.D + 1) + t) * a.chunks, a, r.ptop, r.pback);
-      const bool in = (uint32_t)r.draft < (uint32_t)a.V;
-      bool ok = false;
-      double q = 1.0;  // of a draft that was certain
-      if (t < n && a.draft_logits) {
-        row_sum(sums + ((int64_t)nSeq * (a.D + 1) + (int64_t)s * a.D + t) * a.chunks, a, r.qtop, r.qback);
-        if (in) q = power(draft_row(a, s, t)[r.draft], r.qtop, a.inv) * r.qback;
-      }
-      if (t < n && in) ok = (double)a.u[(int64_t)s * (a.D + 1) + t] * q < power(target_row(a, s, t)[r.draft], r.ptop, a.inv) * r.pback;
+      if (two) row_sum(sums + ((int64_t)nSeq * (a.D + 1) + (int64_t)s * a.D + t) * a.chunks, a, r.qtop, r.qback);
+      const double q = two ? power(y, r.qtop, a.inv) * r.qback : 1.0;  // 1: of a draft that was certain
+      const bool ok = in && (double)u * q < power(x, r.ptop, a.inv) * r.pback;
       if ((threadIdx.x & 63) == 0) {
         rows[wave] = r;
         stands[wave] = ok;
       }
     }
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w)
+    for (int w = 0; w < kDrawWaves; ++w)
       if (!stands[w]) return rows[w];  // at t = n at the latest
     __syncthreads();
   }
 }
-// max(p - q, 0) of a token, or p where `less` is not set.  Each product is rounded before
-// the subtraction: where p and q are equal nothing is left, in every launch.
-__device__ __forceinline__ double weight(const Next& r, const Args& a, float x, float y, int v, bool less) {
+// p of a token, and max(p - q, 0) where `less` is set.  Each product is rounded before
+// the subtraction: where p and q are equal nothing is left, wherever this is computed.
+__device__ __forceinline__ double weight(const Next& r, const Args& a, float x, float y, int v, bool less, double& p) {
 #pragma clang fp contract(off)
-  const double p = power(x, r.ptop, a.inv) * r.pback;
+  p = power(x, r.ptop, a.inv) * r.pback;
   if (!less) return p;
   const double q = a.draft_logits ? power(y, r.qtop, a.inv) * r.qback : v == r.draft ? 1.0 : 0.0;
   return fmax(p - q, 0.0);
-}
-
-// A workgroup takes a chunk of the row that a sequence's next token is drawn from.
-__global__ void __launch_bounds__(kThreads) draft_weights_kernel(double* __restrict__ weights, Next* __restrict__ nexts,
-                                                                 const Sum* __restrict__ sums, Args a, int nSeq) {
-  __shared__ double parts[kWaves];
-  const int s = blockIdx.x / a.chunks, c = blockIdx.x - s * a.chunks, n = drafts_of(a, s);
-  if (n < 0) return;
-  const Next r = next_of(sums, a, s, nSeq, n);
-  if (c == 0 && threadIdx.x == 0) nexts[s] = r;
-  if (r.taken == n) return;  // no weights but the probabilities
-  float x[kEach], y[kEach] = {};
-  const bool fours = a.fours && (!a.draft_logits || a.draft_fours);
-  load_chunk(x, target_row(a, s, r.taken), c, a.V, fours);
-  if (a.draft_logits) load_chunk(y, draft_row(a, s, r.taken), c, a.V, fours);
-  double sum = 0;
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) sum += weight(r, a, x[k], y[k], token_of(k, c, a.V, fours), true);
-  sum = wave_sum(sum);
-  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) sum += parts[w];
-    weights[blockIdx.x] = sum;
-  }
 }
 
 __device__ __forceinline__ void write_tokens(int32_t* token, int32_t* count, const Args& a, int s, int taken, int last) {
@@ -227,118 +230,139 @@ __device__ __forceinline__ void write_tokens(int32_t* token, int32_t* count, con
   if (threadIdx.x == 0) count[s] = taken + 1;
 }
 
+// The inclusive sums of 64 lanes' x.
+__device__ __forceinline__ double lanes_upto(double x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double below = __shfl_up(x, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) x += below;
+  }
+  return x;
+}
+
+// The token of a sequence's row r that its number falls on, by the workgroup; weights[piece]: the
+// weights' sums (both kinds, max(p - q, 0) and p, where drafts are left).
+template <int E>
+__device__ int draw(const double* weights, const Next& r, const Args& a, int s, bool less) {
+  __shared__ double parts[E], shared_start, shared_goal;  // E waves take a piece
+  __shared__ int found[E], ends[E], shared_at, shared_less;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pieces = (a.V + (64 * E) - 1) / (64 * E);
+  const float u = a.u[(int64_t)s * (a.D + 1) + a.D];
+  if (wave == 0) {  // the piece: neighbours a lane
+    const int each = (pieces + 63) / 64, from = min(lane * each, pieces), to = min(from + each, pieces);
+    double mine, upto, all;
+    for (;; less = false) {
+      mine = 0;
+      for (int z = from; z < to; ++z) mine += weights[2 * z + !less];
+      upto = lanes_upto(mine);
+      all = __shfl(upto, 63, 64);
+      if (all > 0 || !less) break;
+    }
+    const double goal = (double)u * all;
+    const uint64_t some = __ballot(mine > 0), over = __ballot(mine > 0 && upto > goal);
+    const int who = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
+    if (lane == (all > 0 ? who : 0)) {
+      int at = -1;
+      double reach = upto - mine, before = 0;
+      if (all > 0)
+        for (int z = from; z < to; ++z) {
+          const double w = weights[2 * z + !less];
+          if (w > 0) at = z, before = reach;  // the last of any weight where none reaches the goal
+          reach += w;
+          if (w > 0 && reach > goal) break;
+        }
+      shared_at = at;
+      shared_start = before;
+      shared_goal = goal;
+      shared_less = less;
+    }
+  }
+  __syncthreads();
+  if (shared_at < 0) return -1;
+  less = shared_less != 0;
+  // the token: one a thread, of the first waves
+  const int v = shared_at * (64 * E) + threadIdx.x;
+  const bool in = threadIdx.x < (64 * E) && v < a.V;
+  double p, w = 0;
+  if (in) w = weight(r, a, target_row(a, s, r.taken)[v], less && a.draft_logits ? draft_row(a, s, r.taken)[v] : 0.f, v, less, p);
+  const double upto = lanes_upto(w);
+  if (lane == 63 && wave < E) parts[wave] = upto;
+  __syncthreads();
+  double reach = shared_start;
+#pragma unroll
+  for (int z = 0; z < E; ++z) reach += z < wave ? parts[z] : 0.0;
+  reach += upto;
+  const uint64_t some = __ballot(w > 0), over = __ballot(w > 0 && reach > shared_goal);
+  if (lane == 0 && wave < E) {
+    found[wave] = over ? v + __builtin_ctzll(over) : INT32_MAX;
+    ends[wave] = some ? v + 63 - __builtin_clzll(some) : -1;
+  }
+  __syncthreads();
+  int at = INT32_MAX, end = -1;  // the token, and the last of any weight
+#pragma unroll
+  for (int z = 0; z < E; ++z) {
+    at = min(at, found[z]);
+    end = max(end, ends[z]);
+  }
+  return at != INT32_MAX ? at : end;
+}
+
+// A workgroup takes pieces of the row that a sequence's next token is drawn from, a wave one of 64 E logits.
+// Alone: it has all of them, and draws.
+template <int E, bool Alone>
+__global__ void __launch_bounds__(64 * kDrawWaves) draft_weights_kernel(int32_t* __restrict__ token,
+                                                                        int32_t* __restrict__ count, double* weights,
+                                                                        Next* __restrict__ nexts,
+                                                                        const Sum* __restrict__ sums, Args a, int nSeq,
+                                                                        int groups) {
+  const int s = blockIdx.x / groups, c = blockIdx.x - s * groups, n = drafts_of(a, s);
+  if (n < 0) {
+    if (Alone) write_tokens(token, count, a, s, -1, -1);
+    return;
+  }
+  const Next r = next_of(sums, a, s, nSeq, n);
+  const bool less = r.taken < n;  // else there are no weights but the probabilities
+  float x[E], y[E] = {};
+  const bool two = less && a.draft_logits, fours = a.fours && (!two || a.draft_fours);
+  const int piece = c * kDrawWaves + (threadIdx.x >> 6), pieces = (a.V + (64 * E) - 1) / (64 * E);
+  if (piece >= pieces && !Alone) return;
+  load_logits(x, target_row(a, s, r.taken), piece * (64 * E), a.V, fours);
+  if (two) load_logits(y, draft_row(a, s, r.taken), piece * (64 * E), a.V, fours);
+  double sum = 0, whole = 0;
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    double p;
+    sum += weight(r, a, x[k], y[k], token_of<E>(k, piece * (64 * E), a.V, fours), less, p);
+    whole += p;
+  }
+  sum = wave_sum(sum);
+  whole = wave_sum(whole);
+  __shared__ double own[2 * kDrawWaves];
+  double* const mine = Alone ? own : weights + (int64_t)s * 2 * pieces;
+  if ((threadIdx.x & 63) == 0 && piece < pieces) {
+    mine[2 * piece] = sum;
+    mine[2 * piece + 1] = whole;
+  }
+  if constexpr (Alone) {
+    __syncthreads();
+    write_tokens(token, count, a, s, r.taken, draw<E>(own, r, a, s, less));
+  } else {
+    if (c == 0 && threadIdx.x == 0) nexts[s] = r;
+  }
+}
 // A workgroup draws a sequence's next token.
-__global__ void __launch_bounds__(kLast) draft_draw_kernel(int32_t* __restrict__ token, int32_t* __restrict__ count,
-                                                           const double* __restrict__ weights,
-                                                           const Next* __restrict__ nexts, const Sum* __restrict__ sums,
-                                                           Args a) {
-  constexpr int kLastWaves = kLast / 64;
-  __shared__ double parts[kLastWaves];
-  __shared__ int found[kLastWaves], ends[kLastWaves];
-  __shared__ double start, goal_at;
-  __shared__ int chunk_at;
-  const int s = blockIdx.x, n = drafts_of(a, s), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <int E>
+__global__ void __launch_bounds__(64 * kDrawWaves) draft_draw_kernel(int32_t* __restrict__ token,
+                                                                     int32_t* __restrict__ count,
+                                                                     const double* __restrict__ weights,
+                                                                     const Next* __restrict__ nexts, Args a) {
+  const int s = blockIdx.x, n = drafts_of(a, s), pieces = (a.V + (64 * E) - 1) / (64 * E);
   if (n < 0) {
     write_tokens(token, count, a, s, -1, -1);
     return;
   }
   const Next r = nexts[s];
-  const Sum* mine = sums + ((int64_t)s * (a.D + 1) + r.taken) * a.chunks;
-  // the chunk: one wave, 64 chunks at a time
-  bool less = r.taken < n;
-  if (wave == 0) {
-    auto chunk_weight = [&](int c) {
-      return c >= a.chunks ? 0.0 : less ? weights[(int64_t)s * a.chunks + c] : mine[c].sum * power(mine[c].top, r.ptop, a.inv) * r.pback;
-    };
-    double all = 0;
-    for (;; less = false) {
-      all = 0;
-      for (int c = lane; c < a.chunks; c += 64) all += chunk_weight(c);
-      all = wave_sum(all);
-      if (all > 0 || !less) break;
-    }
-    const double goal = (double)a.u[(int64_t)s * (a.D + 1) + a.D] * all;
-    int at = -1;
-    double before = 0, run = 0;
-    if (all > 0 && r.pback == r.pback) {
-      for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-        const double w = chunk_weight(c0 + lane);
-        double upto = w;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const double below = __shfl_up(upto, o, 64);
-          if (lane >= o) upto += below;
-        }
-        upto += run;
-        const uint64_t some = __ballot(w > 0), over = __ballot(w > 0 && upto > goal);
-        const int who = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
-        if (who >= 0) {
-          at = c0 + who;
-          before = __shfl(upto - w, who, 64);
-        }
-        run = __shfl(upto, 63, 64);
-        if (over) break;
-      }
-    }
-    if (lane == 0) {
-      chunk_at = at;
-      start = before;
-      goal_at = goal;
-      ends[0] = less;
-    }
-  }
-  __syncthreads();
-  const int c = chunk_at;
-  less = ends[0] != 0;
-  const double goal = goal_at;
-  if (c < 0) {
-    write_tokens(token, count, a, s, r.taken, -1);
-    return;
-  }
-  // the token: four neighbours a thread
-  const int v0 = c * kChunk + threadIdx.x * 4;
-  const float *x = target_row(a, s, r.taken), *y = less && a.draft_logits ? draft_row(a, s, r.taken) : nullptr;
-  double w[4], sum = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int v = v0 + k;
-    w[k] = v < a.V ? weight(r, a, x[v], y ? y[v] : 0.f, v, less) : 0.0;
-    sum += w[k];
-  }
-  double upto = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double below = __shfl_up(upto, o, 64);
-    if (lane >= o) upto += below;
-  }
-  if (lane == 63) parts[wave] = upto;
-  __syncthreads();
-  double reach = start;
-  for (int v = 0; v < wave; ++v) reach += parts[v];
-  reach += upto - sum;
-  int at = INT32_MAX, end = -1;  // the token, and the last of any weight
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    reach += w[k];
-    if (w[k] > 0) {
-      end = v0 + k;
-      if (reach > goal) at = min(at, v0 + k);
-    }
-  }
-  at = wave_min(at);
-  end = -wave_min(-end);
-  __syncthreads();
-  if (lane == 0) {
-    found[wave] = at;
-    ends[wave] = end;
-  }
-  __syncthreads();
-  at = INT32_MAX, end = -1;
-  for (int v = 0; v < kLastWaves; ++v) {
-    at = min(at, found[v]);
-    end = max(end, ends[v]);
-  }
-  write_tokens(token, count, a, s, r.taken, at != INT32_MAX ? at : end);
+  write_tokens(token, count, a, s, r.taken, draw<E>(weights + (int64_t)s * 2 * pieces, r, a, s, r.taken < n));
 }
 
 // Temperature 0: a workgroup takes a sequence, a wave a row.
@@ -398,23 +422,41 @@ extern "C" int fg_draft_verify(int32_t* token, int32_t* count, const float* logi
   fg::KProfScope prof("draft_verify", 0.0, 4.0 * V * rows);
   const Args a{logits, drawn ? draft_logits : nullptr, ld, ld_draft, draft, drafted, u, temperature == 0 ? 0.0 : 1.0 / temperature,
                D, V, chunks, ld % 4 == 0 && aligned16(logits), drawn && ld_draft % 4 == 0 && aligned16(draft_logits)};
+  // Logits of a thread of the second launch.  Few, where there are workgroups for all of them at once: each first finds
+  // the row that is drawn from, 5 us, and 16 logits take 5 more (7 rows of 32000: 4 a thread 6.8 us, 16 11.9; 16 rows of
+  // 128256: 4 a thread, two rounds of workgroups, 15 us, 8 12).
+  const int cus = fg::device_cu_count() > 0 ? fg::device_cu_count() : 256;
+  auto groups_of = [&](int each) { return (V + 64 * kDrawWaves * each - 1) / (64 * kDrawWaves * each); };
+  const int each = (int64_t)nSeq * groups_of(4) <= cus ? 4 : (int64_t)nSeq * groups_of(8) <= cus ? 8 : 16;
+  const int groups = groups_of(each), pieces = (V + 64 * each - 1) / (64 * each);
   const size_t sums_bytes = (size_t)rows * chunks * sizeof(Sum), next_bytes = (size_t)nSeq * sizeof(Next);
-  const size_t weight_bytes = (size_t)nSeq * chunks * sizeof(double);
+  const size_t weight_bytes = (size_t)nSeq * 2 * pieces * sizeof(double);
   fg::Workspace ws;
   const int rc = ws.get(sums_bytes + next_bytes + weight_bytes);
   if (rc != FG_OK) return rc;
   Sum* sums = (Sum*)ws.ptr;
   double* weights = (double*)((uint8_t*)ws.ptr + sums_bytes);
   Next* nexts = (Next*)((uint8_t*)ws.ptr + sums_bytes + weight_bytes);
-  const dim3 all((unsigned)(rows * chunks)), row((unsigned)(nSeq * chunks)), seq((unsigned)nSeq);
+  const dim3 all((unsigned)(rows * chunks)), row((unsigned)(nSeq * groups)), block(64 * kDrawWaves);
   if (temperature == 0) {
     FG_LAUNCH(draft_sums_kernel<true>, all, dim3(kThreads), 0, sums, a, nSeq);
-    FG_LAUNCH(draft_greedy_kernel, seq, dim3(kThreads), 0, token, count, (const Sum*)sums, a);
+    FG_LAUNCH(draft_greedy_kernel, dim3(nSeq), dim3(kThreads), 0, token, count, (const Sum*)sums, a);
     return FG_OK;
   }
   FG_LAUNCH(draft_sums_kernel<false>, all, dim3(kThreads), 0, sums, a, nSeq);
-  FG_LAUNCH(draft_weights_kernel, row, dim3(kThreads), 0, weights, nexts, (const Sum*)sums, a, nSeq);
-  FG_LAUNCH(draft_draw_kernel, seq, dim3(kLast), 0, token, count, (const double*)weights, (const Next*)nexts,
-            (const Sum*)sums, a);
+#define DRAFT_DRAW(E)                                                                                                  \
+  do {                                                                                                                 \
+    if (groups == 1) {                                                                                                 \
+      FG_LAUNCH((draft_weights_kernel<E, true>), row, block, 0, token, count, weights, nexts, (const Sum*)sums, a,     \
+                nSeq, groups);                                                                                         \
+    } else {                                                                                                           \
+      FG_LAUNCH((draft_weights_kernel<E, false>), row, block, 0, token, count, weights, nexts, (const Sum*)sums, a,    \
+                nSeq, groups);                                                                                         \
+      FG_LAUNCH(draft_draw_kernel<E>, dim3(nSeq), block, 0, token, count, (const double*)weights, (const Next*)nexts, a); \
+    }                                                                                                                  \
+  } while (0)
+  if (each == 4) DRAFT_DRAW(4);
+  else if (each == 8) DRAFT_DRAW(8);
+  else DRAFT_DRAW(16);
   return FG_OK;
 }
