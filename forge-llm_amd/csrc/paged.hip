@@ -201,11 +201,15 @@ __device__ __forceinline__ Steps steps_of(const Cache& c, const Span& q, int use
 // lengths; every wave finds its own, its lanes sharing the sequences out.
 struct Part {
   int s, kvh, tile, piece, pieces, per;
-  int64_t first;  // pieces of the sequences before
+  int64_t first;  // workgroups of the sequences before
+};
+// What the workgroups leave of a sequence for the joining launch.
+struct Pieces {
+  int64_t first;
+  int count;
 };
 __device__ __forceinline__ int tiles_of(const Span& q, int tokens) { return (tokens * q.group + q.rows - 1) / q.rows; }
-// id: a workgroup, or with by_seq a sequence, whose `first`, `pieces` and `per` are found.
-__device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int64_t id, bool by_seq) {
+__device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int64_t id) {
   const int lane = threadIdx.x & 63, each = (c.nSeq + 63) / 64;
   const int from = min(lane * each, c.nSeq), to = min(from + each, c.nSeq);
   auto steps = [&](int s, int tokens) { return steps_of(c, q, slots_used(c, s), 0, tokens - 1).total; };
@@ -231,16 +235,15 @@ __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int6
     const int64_t below = __shfl_up(upto, o, 64);
     if (lane >= o) upto += below;
   }
-  const uint64_t has = __ballot(by_seq ? id >= from && id < to : id < upto);
+  const uint64_t has = __ballot(id < upto);
   if (has == 0) return false;
   const int owner = __builtin_ctzll(has);
   p.first = __shfl(upto - mine, owner, 64);
   for (p.s = owner * each;; ++p.s) {
     const int64_t here = groups(p.s, p.pieces);
-    if (by_seq ? p.s == id : id < p.first + here) break;
+    if (id < p.first + here) break;
     p.first += here;
   }
-  if (by_seq) return true;
   const int in_seq = (int)(id - p.first), n = new_tokens(q.count, p.s, q.T), tiles = tiles_of(q, n);
   p.piece = in_seq % p.pieces;
   p.tile = in_seq / p.pieces % tiles;
@@ -443,13 +446,13 @@ __device__ __forceinline__ float over_groups_sum(float x) {
   return x + __shfl_xor(x, 32, 64);
 }
 
-// part_ml, part_o: references and sums, and values of the pieces, a workgroup's rows
-// each; null: every sequence is one piece.
+// plan, part_ml, part_o: the sequences' pieces, the pieces' references and sums, and
+// values, a workgroup's rows each; null: every sequence is one piece.
 template <class KV, int DH, int NT>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(Cache c, int layer, float* __restrict__ out,
+__global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) paged_attn_kernel(Cache c, int layer, float* __restrict__ out,
                                                               const float* __restrict__ q, int nH, float factor, Span span,
-                                                              int target, float2* __restrict__ part_ml,
-                                                              float* __restrict__ part_o) {
+                                                              int target, Pieces* __restrict__ plan,
+                                                              float2* __restrict__ part_ml, float* __restrict__ part_o) {
   using S = Step<KV, DH>;
   constexpr int Keys = S::Keys, Sub = S::Sub, E = S::E, Runs = S::Runs, M = DH / 16, kRow = DH + 4;
   constexpr int kShared = NT * S::kQ * 64 * 16 > kWaves * 16 * kRow * 4 ? NT * S::kQ * 64 * 16 : kWaves * 16 * kRow * 4;
@@ -460,7 +463,8 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(Cache c, int layer
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Part p;
   if (part_ml) {
-    if (!part_of(p, c, span, target, blockIdx.x, false)) return;
+    if (!part_of(p, c, span, target, blockIdx.x)) return;
+    if (p.first == blockIdx.x && threadIdx.x == 0) plan[p.s] = Pieces{p.first, p.pieces};
   } else {
     const int tiles = tiles_of(span, span.T);
     p.tile = blockIdx.x % tiles;
@@ -702,51 +706,60 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(Cache c, int layer
   }
 }
 
-// A workgroup joins the pieces of a row.
+// A workgroup joins the pieces of R rows of a kv head: its threads share out quads of a row's
+// values, rows and (1 / sets of) the pieces.
 template <int DH>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(Cache c, float* __restrict__ out, int nH, Span span, int target,
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(Cache c, float* __restrict__ out, int nH, Span span, int R,
+                                                              const Pieces* __restrict__ plan,
                                                               const float2* __restrict__ part_ml,
                                                               const float* __restrict__ part_o) {
-  constexpr int kQuads = DH / 4, kSets = kThreads / kQuads;
-  __shared__ f32x4 vals[kSets][kQuads];
-  __shared__ float sums[kSets];
-  const int t = blockIdx.x / nH % span.T, h = blockIdx.x % nH, s = blockIdx.x / nH / span.T;
-  const int tokens = new_tokens(span.count, s, span.T);
-  if (t >= tokens) return;
-  Part p;
-  if (!part_of(p, c, span, target, s, true) || p.pieces <= 1) return;
-  const int kvh = h / span.group, row = t * span.group + (h - kvh * span.group), tile = row / span.rows;
-  const int64_t first = (p.first + ((int64_t)kvh * tiles_of(span, tokens) + tile) * p.pieces) * span.rows + (row - tile * span.rows);
-  float top = -INFINITY;
-  for (int x = threadIdx.x & 63; x < p.pieces; x += 64) top = fmaxf(top, part_ml[first + (int64_t)x * span.rows].x);
-  top = fg_wave_max(top);
-  const int set = threadIdx.x / kQuads, quad = threadIdx.x - set * kQuads;
-  f32x4 y = {0.f, 0.f, 0.f, 0.f};
-  float all = 0.f;
-  if (set < kSets) {
-    for (int x = set; x < p.pieces; x += kSets) {
-      const int64_t at = first + (int64_t)x * span.rows;
-      const float2 ml = part_ml[at];
-      const float f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
-      all += ml.y * f;
-      y += *reinterpret_cast<const f32x4*>(part_o + at * DH + 4 * quad) * f;
+  constexpr int kQuads = DH / 4, kLanes = kThreads / kQuads;
+  __shared__ f32x4 vals[kLanes][kQuads];
+  __shared__ float sums[kLanes];
+  const int blocks = (span.T * span.group + R - 1) / R;
+  const int s = blockIdx.x / blocks / c.nKV, kvh = blockIdx.x / blocks % c.nKV, row0 = blockIdx.x % blocks * R;
+  const Pieces p = plan[s];  // (of no tokens: whatever was there, and not used)
+  const int tokens = new_tokens(span.count, s, span.T), rows = min(tokens * span.group - row0, R);
+  if (rows <= 0 || p.count <= 1) return;
+  const int at_once = min(R, kLanes), sets = kLanes / at_once;  // rows at a time, threads that share one
+  const int lane = threadIdx.x / kQuads, quad = threadIdx.x - lane * kQuads, set = lane / at_once, tiles = tiles_of(span, tokens);
+  for (int r0 = 0; r0 < rows; r0 += at_once) {
+    const int mine = r0 + (lane - set * at_once), row = row0 + mine, tile = row / span.rows;
+    const bool on = lane < kLanes && set < sets && mine < rows;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float all = 0.f;
+    if (on) {
+      const int64_t first = (p.first + ((int64_t)kvh * tiles + tile) * p.count) * span.rows + (row - tile * span.rows);
+      float top = -INFINITY;
+      for (int x = 0; x < p.count; ++x) top = fmaxf(top, part_ml[first + (int64_t)x * span.rows].x);
+      for (int x = set; x < p.count; x += sets) {
+        const int64_t at = first + (int64_t)x * span.rows;
+        const float2 ml = part_ml[at];
+        const float f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+        all += ml.y * f;
+        y += *reinterpret_cast<const f32x4*>(part_o + at * DH + 4 * quad) * f;
+      }
     }
-    vals[set][quad] = y;
-    if (quad == 0) sums[set] = all;
-  }
-  __syncthreads();
-  if (threadIdx.x >= kQuads) return;
-  y = vals[0][quad];
-  all = sums[0];
+    if (sets > 1) {
+      __syncthreads();
+      if (lane < kLanes) {
+        vals[lane][quad] = y;
+        if (quad == 0) sums[lane] = all;
+      }
+      __syncthreads();
+      for (int x = 1; x < sets && set == 0 && on; ++x) {
+        y += vals[lane + x * at_once][quad];
+        all += sums[lane + x * at_once];
+      }
+    }
+    if (on && set == 0) {
+      const int t = row / span.group, h = kvh * span.group + (row - t * span.group);
+      const float f = all == 0.f ? 0.f : 1.f / all;
+      float* to = out + (((int64_t)s * span.T + t) * nH + h) * DH + 4 * quad;
 #pragma unroll
-  for (int x = 1; x < kSets; ++x) {
-    y += vals[x][quad];
-    all += sums[x];
+      for (int z = 0; z < 4; ++z) to[z] = y[z] * f;
+    }
   }
-  const float f = all == 0.f ? 0.f : 1.f / all;
-  float* to = out + ((int64_t)s * span.T * nH + (int64_t)t * nH + h) * DH + 4 * quad;
-#pragma unroll
-  for (int z = 0; z < 4; ++z) to[z] = y[z] * f;
 }
 
 // ── entry points' checks ──────────────────────────────────────────────────
@@ -877,17 +890,22 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   fg::Workspace ws;
   float2* part_ml = nullptr;
   float* part_o = nullptr;
+  Pieces* plan = nullptr;
+  int R = 1;
   if (!whole) {
     const size_t rows = (size_t)grid * span.rows;
-    PAGED_TRY(ws.get(rows * (sizeof(float2) + c->dHead * sizeof(float))));
+    PAGED_TRY(ws.get(rows * (sizeof(float2) + c->dHead * sizeof(float)) + c->nSeq * sizeof(Pieces)));
     part_o = (float*)ws.ptr;
     part_ml = (float2*)(part_o + rows * c->dHead);
+    plan = (Pieces*)(part_ml + rows);
+    while (R < 16 && items / R > 4 * cus) R *= 2;
   }
+  const int64_t joins = (int64_t)c->nSeq * c->nKvHeads * ((all + R - 1) / R);
   const float factor = (float)(scale * M_LOG2E);
   const Cache cache = view(c);
 #define PAGED_ATTN(KV, DH, NT)                                                                                        \
   FG_LAUNCH((paged_attn_kernel<KV, DH, NT>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q, nHeads,   \
-            factor, span, target, part_ml, part_o)
+            factor, span, target, plan, part_ml, part_o)
 #define PAGED_TILES(KV, DH)                          \
   if (tiles == 1) PAGED_ATTN(KV, DH, 1);             \
   else if (tiles == 2) PAGED_ATTN(KV, DH, 2);        \
@@ -900,8 +918,8 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
       PAGED_TILES(_Float16, DH);                     \
     }                                                \
     if (!whole)                                      \
-      FG_LAUNCH(paged_join_kernel<DH>, dim3((unsigned)items), dim3(kThreads), 0, cache, out, nHeads, span, target, \
-                (const float2*)part_ml, (const float*)part_o);                                                     \
+      FG_LAUNCH(paged_join_kernel<DH>, dim3((unsigned)joins), dim3(kThreads), 0, cache, out, nHeads, span, R, \
+                (const Pieces*)plan, (const float2*)part_ml, (const float*)part_o);                          \
   } while (0)
   switch (c->dHead) {
     case 32: PAGED_HEAD(32); break;
