@@ -175,12 +175,14 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Queries of a call: the sequences' rows, and which slots they see.
 struct Span {
   int T, group, rows;  // rows of a workgroup
-  int window, sinks, keys;
+  int window, sinks;
+  int keys, waves;  // slots of a step, and waves that share steps out
   const int32_t* count;
 };
 struct Steps {  // steps of slots that some of the rows of tokens t0 .. t1 see: the first `sink`, then from `low` on
@@ -221,7 +223,7 @@ __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int6
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
   const int64_t per = (work * c.nKV + target - 1) / target;
-  p.per = ((int)min(max(per, (int64_t)1), (int64_t)1 << 28) + kWaves - 1) / kWaves * kWaves;
+  p.per = ((int)min(max(per, (int64_t)1), (int64_t)1 << 28) + q.waves - 1) / q.waves * q.waves;
   auto groups = [&](int s, int& pieces) -> int64_t {
     const int n = new_tokens(q.count, s, q.T);
     pieces = n > 0 ? (steps(s, n) + p.per - 1) / p.per : 0;
@@ -706,6 +708,407 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
   }
 }
 
+// ── attention of many rows ────────────────────────────────────────────────
+// Where a kv head's queries fill more than a few tiles the products bound: a workgroup takes
+// 128 rows, a wave 32 of them, and its waves share steps of 64 slots (fp32: 32) through LDS,
+// fetched a step ahead.  32x32 instructions (16 and 2 values deep), scores slots x rows as above: a lane has
+// row lane & 31 and slots 8 a + 4 h + b (h = lane >> 5; a, b < 4) of every 32, which again is the order that the sums want p in.
+//
+// In LDS, in words of 16 bytes:
+//   K  row by row, word w of slot j at w ^ (j's swizzle): 16 slots' same word lie in different banks;
+//      copied there straight from memory
+//   V  the values of d at eight slots (fp32: four) that a lane's operand takes, [e][8 groups of slots][i] for d = E i + e:
+//      turned around on the way, four rows of a run of E values a lane
+template <class KV, int DH>
+struct Wide;
+template <int DH>
+struct Wide<_Float16, DH> {
+  static constexpr int Keys = 64, Sub = 2, Words = DH / 8, Quads = 2;  // quads of rows a lane turns around
+  static constexpr int Lanes = DH % 64 == 0 ? 32 : 16, E = DH / Lanes, M = DH / 32;
+  static constexpr float kOver = 11.f;
+  f16x8 qh[DH / 16], ql[DH / 16];
+  _Float16 v[8][E];
+  // slots of the quads that lane `lane` of wave `wave` turns around, and their group
+  static __device__ __forceinline__ int group_at(int wave, int lane) { return Lanes == 32 ? 2 * wave + (lane >> 5) : 4 * wave + (lane >> 4); }
+  static __device__ __forceinline__ int slot_at(int group, int quad) { return 16 * (group >> 1) + 8 * quad + 4 * (group & 1); }
+  static __device__ __forceinline__ bool turns(int wave) { return Lanes == 32 || wave < 2; }
+  __device__ __forceinline__ float load_q(const float* q, float factor, bool on) {
+    const int h = (threadIdx.x & 63) >> 5;
+    float m = 0.f;
+    f32x4 x[DH / 16][2];
+#pragma unroll
+    for (int b = 0; b < DH / 16; ++b)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = on ? q[16 * b + 8 * h + j] * factor : 0.f;
+        x[b][j / 4][j % 4] = y;
+        m = fmaxf(m, fabsf(y));
+      }
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const int e = m > 0.f && m < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
+#pragma unroll
+    for (int b = 0; b < DH / 16; ++b)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = __builtin_amdgcn_ldexpf(x[b][j / 4][j % 4], e);
+        qh[b][j] = (_Float16)y;
+        ql[b][j] = (_Float16)(y - (float)qh[b][j]);
+      }
+    return __builtin_amdgcn_ldexpf(1.f, -e);
+  }
+  // the scores of slots 32 u .. from the rows' words
+  __device__ __forceinline__ void product(f32x16& s, int b, u32x4 word) const {
+    const f16x8 k = __builtin_bit_cast(f16x8, word);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[b], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[b], s, 0, 0, 0);
+  }
+  struct Probs {
+    f16x8 hi[2 * Sub], lo[2 * Sub];
+    __device__ __forceinline__ void take(const f32x16 (&p)[Sub]) {
+#pragma unroll
+      for (int z = 0; z < 2 * Sub; ++z)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float y = p[z / 2][8 * (z & 1) + j];
+          hi[z][j] = (_Float16)y;
+          lo[z][j] = (_Float16)(y - (float)hi[z][j]);
+        }
+    }
+    // o += the word's slots (group 2 z + h)
+    __device__ __forceinline__ void sum(f32x16& o, int z, u32x4 word) const {
+      const f16x8 a = __builtin_bit_cast(f16x8, word);
+      o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, lo[z], o, 0, 0, 0);
+      o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, hi[z], o, 0, 0, 0);
+    }
+  };
+  static constexpr int Z = 2 * Sub;
+  __device__ __forceinline__ u32x4 turned(int e) const {
+    f16x8 w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = v[j][e];
+    return __builtin_bit_cast(u32x4, w);
+  }
+  static __device__ __forceinline__ bool number(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00) != 0x7C00; }
+  // where slot j's value stands in its group's word
+  static __device__ __forceinline__ int group_of(int j) { return 2 * (j >> 4) + (j >> 2 & 1); }
+  static __device__ __forceinline__ int place_of(int j) { return (j >> 3 & 1) * 4 + (j & 3); }
+};
+template <int DH>
+struct Wide<float, DH> {
+  static constexpr int Keys = 32, Sub = 1, Words = DH / 4, Quads = 1;
+  static constexpr int Lanes = 32, E = DH / 32, M = DH / 32;
+  static constexpr float kOver = 0.f;
+  f32x4 q4[DH / 8];
+  float v[4][E];
+  static __device__ __forceinline__ int group_at(int wave, int lane) { return 2 * wave + (lane >> 5); }
+  static __device__ __forceinline__ int slot_at(int group, int) { return 4 * group; }
+  static __device__ __forceinline__ bool turns(int) { return true; }
+  __device__ __forceinline__ float load_q(const float* q, float factor, bool on) {
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int b = 0; b < DH / 8; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q4[b][j] = on ? q[8 * b + 4 * h + j] * factor : 0.f;
+    return 1.f;
+  }
+  __device__ __forceinline__ void product(f32x16& s, int b, u32x4 word) const {
+    const f32x4 k = __builtin_bit_cast(f32x4, word);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q4[b][j], s, 0, 0, 0);
+  }
+  struct Probs {
+    f32x16 p;
+    __device__ __forceinline__ void take(const f32x16 (&x)[Sub]) { p = x[0]; }
+    __device__ __forceinline__ void sum(f32x16& o, int z, u32x4 word) const {
+      const f32x4 a = __builtin_bit_cast(f32x4, word);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], p[4 * z + j], o, 0, 0, 0);
+    }
+  };
+  static constexpr int Z = 4;
+  __device__ __forceinline__ u32x4 turned(int e) const {
+    const f32x4 w = {v[0][e], v[1][e], v[2][e], v[3][e]};
+    return __builtin_bit_cast(u32x4, w);
+  }
+  static __device__ __forceinline__ bool number(float x) { return fabsf(x) < INFINITY; }
+  static __device__ __forceinline__ int group_of(int j) { return j >> 2; }
+  static __device__ __forceinline__ int place_of(int j) { return j & 3; }
+};
+
+// 16 bytes a lane from `from` to LDS at `lds` + 16 lane; waited for by hand (the compiler does not count
+// it, which makes its own waits longer, never shorter).  m0 is given back: it cannot be named as changed.
+__device__ __forceinline__ void load_to_lds(uint32_t lds, const void* from) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0)
+               : "s"(lds), "v"(from)
+               : "memory");
+}
+
+constexpr int kWideRows = 32 * kWaves;
+template <class KV, int DH>
+__global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kernel(
+    Cache c, int layer, float* __restrict__ out, const float* __restrict__ q, int nH, float factor, Span span, int target,
+    Pieces* __restrict__ plan, float2* __restrict__ part_ml, float* __restrict__ part_o) {
+  using W = Wide<KV, DH>;
+  constexpr int Keys = W::Keys, Sub = W::Sub, Words = W::Words, E = W::E, M = W::M, Z = W::Z, Lanes = W::Lanes;
+  constexpr int kTile = Keys * Words;  // words of a step's K, and of its V
+  // slot j's swizzle: the words of 16 neighbouring slots in 16 different places of 256 bytes
+  constexpr int kShift = Words % 16 == 0 ? 0 : Words % 8 == 0 ? 1 : 2, kMask = Words % 16 == 0 ? 15 : Words % 8 == 0 ? 7 : 3;
+  __shared__ __attribute__((aligned(16))) u32x4 lds[4 * kTile];  // [2][K, V][kTile]
+  // Of a step's quads of slots: their pages, -1 for none, and whether all have one; of its V: whether
+  // what a wave has turned around holds infinities or NaN.  Pages are read up to the end of their step, and
+  // those of the next but one are written in it.
+  __shared__ int pages[3][Keys / 4], all_pages[3], odd[2][kWaves];
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+  const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Part p;
+  if (part_ml) {
+    if (!part_of(p, c, span, target, blockIdx.x)) return;
+    if (p.first == blockIdx.x && threadIdx.x == 0) plan[p.s] = Pieces{p.first, p.pieces};
+  } else {
+    const int tiles = tiles_of(span, span.T);
+    p.tile = tiles - 1 - blockIdx.x % tiles;  // the longest first
+    p.kvh = blockIdx.x / tiles % c.nKV;
+    p.s = blockIdx.x / tiles / c.nKV;
+    p.piece = 0;
+    p.pieces = 1;
+    p.per = INT32_MAX;
+  }
+  const int s = __builtin_amdgcn_readfirstlane(p.s), kvh = __builtin_amdgcn_readfirstlane(p.kvh);
+  const int row0 = __builtin_amdgcn_readfirstlane(p.tile) * kWideRows, pieces = __builtin_amdgcn_readfirstlane(p.pieces);
+  const int tokens = new_tokens(span.count, s, span.T), rows = min(tokens * span.group - row0, kWideRows);
+  if (rows <= 0) return;
+  const int used = slots_used(c, s), t0 = row0 / span.group, t1 = (row0 + rows - 1) / span.group;
+  const Steps steps = steps_of(c, span, used, t0, t1);
+  const int per = __builtin_amdgcn_readfirstlane(p.per);
+  const int begin = min((int64_t)__builtin_amdgcn_readfirstlane(p.piece) * per, (int64_t)steps.total);
+  const int end = min((int64_t)begin + per, (int64_t)steps.total);
+  const int first_pos = used + t0, last_pos = used + t1;
+  const int window = span.window > 0 ? span.window : INT32_MAX;
+
+  const int32_t* table = c.table + (int64_t)s * c.maxPages;
+  const KV* const kbase = (const KV*)c.k + ((((int64_t)layer * c.nPages) * c.nKV + kvh) << c.lg) * DH;
+  const KV* const vbase = (const KV*)c.v + ((((int64_t)layer * c.nPages) * c.nKV + kvh) << c.lg) * DH;
+  const uint32_t inside = (1u << c.lg) - 1;
+  auto row_at = [&](const KV* base, int page, int j) {
+    const uint32_t there = page < 0 ? 0u : (uint32_t)page;
+    return base + (((uint64_t)there * (uint32_t)c.nKV << c.lg) + ((uint32_t)j & inside)) * DH;
+  };
+  auto page_at = [&](int x) {  // of quad threadIdx.x of step x
+    const int at = (steps.at(x) * Keys + 4 * (int)threadIdx.x) >> c.lg, page = at < c.maxPages ? table[at] : -1;
+    return (uint32_t)page < (uint32_t)c.nPages ? page : -1;
+  };
+  auto put_pages = [&](int page, int b) {
+    if (threadIdx.x < Keys / 4) {
+      pages[b][threadIdx.x] = page;
+      const uint64_t there = __ballot(page >= 0);
+      if (threadIdx.x == 0) all_pages[b] = __builtin_popcountll(there) == Keys / 4;
+    }
+  };
+  W w;
+  auto fetch_k = [&](int x, int b, int pb) {  // straight to LDS, a wave 64 words at a time
+    const int j0 = steps.at(x) * Keys;
+#pragma unroll
+    for (int z = 0; z < kTile / kThreads; ++z) {
+      const int first = (z * kWaves + wave) * 64, word = first + lane, j = word / Words;
+      const int at = (word - j * Words) ^ (j >> kShift & kMask);
+      const KV* from = row_at(kbase, pages[pb][j / 4], j0 + j) + at * (16 / sizeof(KV));
+      load_to_lds(lds_at + (2 * b * kTile + first) * 16, from);
+    }
+  };
+  const int group = W::group_at(wave, lane), run = lane & (Lanes - 1);
+  auto fetch_v = [&](int x, int pb) {
+    if (!W::turns(wave)) return;
+    const int j0 = steps.at(x) * Keys;
+#pragma unroll
+    for (int u = 0; u < W::Quads; ++u) {
+      const int j = W::slot_at(group, u);
+      const KV* from = row_at(vbase, pages[pb][j / 4], j0 + j) + run * E;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) __builtin_memcpy(w.v[4 * u + r], __builtin_assume_aligned(from + r * DH, E * sizeof(KV) % 16 == 0 ? 16 : E * sizeof(KV) % 8 == 0 ? 8 : 4), E * sizeof(KV));
+    }
+  };
+  // Whether every row of the workgroup sees every slot of step x.
+  auto is_whole = [&](int x, int pb) {
+    const int j0 = steps.at(x) * Keys;
+    return j0 + Keys - 1 <= first_pos && (j0 > last_pos - window || j0 + Keys <= span.sinks) && all_pages[pb] != 0;
+  };
+  auto put_v = [&](int x, int b, int pb) {
+    if (!W::turns(wave)) {
+      if (lane == 0) odd[b][wave] = 0;
+      return;
+    }
+    bool ok = true;
+    if (!is_whole(x, pb)) {
+      // slots that no row sees are zeros; of the others infinities and NaN are told of
+      const int j0 = steps.at(x) * Keys;
+#pragma unroll
+      for (int u = 0; u < W::Quads; ++u) {
+        const int j = W::slot_at(group, u);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int at = j0 + j + r;
+          const bool seen = pages[pb][j / 4] >= 0 && at <= last_pos && (at > first_pos - window || at < span.sinks);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            if (!seen) w.v[4 * u + r][e] = (KV)0;
+            ok &= W::number(w.v[4 * u + r][e]);
+          }
+        }
+      }
+    }
+    const bool all = __all(ok);
+    if (lane == 0) odd[b][wave] = !all;
+    u32x4* to = lds + (2 * b + 1) * kTile + group * Lanes + run;
+#pragma unroll
+    for (int e = 0; e < E; ++e) to[e * 8 * Lanes] = w.turned(e);
+  };
+
+  if (begin < end) {
+    put_pages(threadIdx.x < Keys / 4 ? page_at(begin) : -1, 0);
+    __syncthreads();
+    fetch_k(begin, 0, 0);
+    fetch_v(begin, 0);
+    if (begin + 1 < end) put_pages(threadIdx.x < Keys / 4 ? page_at(begin + 1) : -1, 1);
+  }
+  // the wave's rows; a wave without any computes nothing
+  const int mine = min(rows - 32 * wave, 32);
+  const int row = row0 + 32 * wave + min(r32, max(mine, 1) - 1);
+  const int t = min(row / span.group, tokens - 1), head = kvh * span.group + (row - row / span.group * span.group);
+  const int pos = used + t, wave_first = used + (row0 + 32 * wave) / span.group, wave_last = used + (row0 + 32 * wave + max(mine, 1) - 1) / span.group;
+  const float back = w.load_q(q + (((int64_t)s * span.T + t) * nH + head) * DH, factor, mine > 0 && r32 < mine);
+  float ref = -INFINITY, sum = 0.f;
+  f32x16 o[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int z = 0; z < 16; ++z) o[m][z] = 0.f;
+  if (begin < end) put_v(begin, 0, 0);
+
+  int this_page = 0;
+  for (int x = begin; x < end; ++x) {
+    const int b = (x - begin) & 1, j0 = steps.at(x) * Keys;
+    const int next_page = this_page == 2 ? 0 : this_page + 1, free_page = 3 - this_page - next_page;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int page = -1;
+    if (x + 1 < end) {
+      fetch_k(x + 1, b ^ 1, next_page);
+      fetch_v(x + 1, next_page);
+      if (x + 2 < end && threadIdx.x < Keys / 4) page = page_at(x + 2);
+    }
+    const bool whole = all_pages[this_page] != 0 && j0 + Keys - 1 <= wave_first && (j0 > wave_last - window || j0 + Keys <= span.sinks);
+    const bool some = mine > 0 && j0 <= wave_last && (j0 + Keys - 1 > wave_first - window || j0 < span.sinks);
+    if (some) {
+      const u32x4 *kt = lds + 2 * b * kTile, *vt = kt + kTile;
+      f32x16 sc[Sub];
+#pragma unroll
+      for (int u = 0; u < Sub; ++u) {
+#pragma unroll
+        for (int z = 0; z < 16; ++z) sc[u][z] = 0.f;
+        const int j = 32 * u + r32, swizzle = j >> kShift & kMask;
+#pragma unroll
+        for (int k = 0; k < Words / 2; ++k) w.product(sc[u], k, kt[j * Words + ((2 * k + h) ^ swizzle)]);
+      }
+      uint32_t seen[Sub];  // this lane's scores
+      if (!whole) {
+#pragma unroll
+        for (int u = 0; u < Sub; ++u) {
+          seen[u] = 0;
+#pragma unroll
+          for (int z = 0; z < 16; ++z) {
+            const int j = 32 * u + 8 * (z / 4) + 4 * h + z % 4, at = j0 + j;
+            if (pages[this_page][j / 4] >= 0 && at <= pos && (at > pos - window || at < span.sinks)) seen[u] |= 1u << z;
+            else sc[u][z] = -INFINITY;
+          }
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < Sub; ++u)
+#pragma unroll
+        for (int z = 0; z < 16; ++z) top = fmaxf(top, sc[u][z]);
+      top *= back;
+      if (__any(top > ref + kRise)) {
+        const float was = ref;
+        ref = fmaxf(was, fmaxf(top, __shfl_xor(top, 32, 64)));
+        const float keep = ref == was ? 1.f : __builtin_amdgcn_exp2f(was - ref);
+        sum *= keep;
+#pragma unroll
+        for (int m = 0; m < M; ++m) o[m] *= keep;
+      }
+      const float base = W::kOver - ref;
+#pragma unroll
+      for (int u = 0; u < Sub; ++u)
+#pragma unroll
+        for (int z = 0; z < 16; ++z) {
+          float e = __builtin_amdgcn_exp2f(fmaf(sc[u][z], back, base));
+          if (!whole && !(seen[u] >> z & 1)) e = 0.f;
+          sum += e;
+          sc[u][z] = e;
+        }
+      bool slow = false;
+      if (!whole)
+#pragma unroll
+        for (int z = 0; z < kWaves; ++z) slow |= odd[b][z] != 0;
+      if (!slow) {
+        typename W::Probs pr;
+        pr.take(sc);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int z = 0; z < Z; ++z) {
+            const int at = Lanes == 32 ? (m * 8 + 2 * z + h) * 32 + r32 : ((2 * m + (r32 >> 4)) * 8 + 2 * z + h) * 16 + (r32 & 15);
+            pr.sum(o[m], z, vt[at]);
+          }
+      } else {
+        // a value that is seen is not finite: it must not reach the rows that do not see it
+        for (int j = 0; j < Keys; ++j) {
+          const int at = j0 + j;
+          const bool is = pages[this_page][j / 4] >= 0 && at <= pos && (at > pos - window || at < span.sinks);
+          float e = 0.f;
+#pragma unroll
+          for (int u = 0; u < Sub; ++u)
+#pragma unroll
+            for (int z = 0; z < 16; ++z) {
+              const float y = __shfl(sc[u][z], r32 + 32 * (j >> 2 & 1), 64);
+              if (j >> 5 == u && (j >> 3 & 3) == z / 4 && (j & 3) == z % 4) e = y;
+            }
+          if (is) {
+            const KV* const flat = reinterpret_cast<const KV*>(vt);
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+              for (int z = 0; z < 16; ++z) {
+                const int r = 8 * (z / 4) + 4 * h + z % 4, i = Lanes == 32 ? r : r & 15, run_e = Lanes == 32 ? m : 2 * m + (r >> 4);
+                o[m][z] += e * (float)flat[((run_e * 8 + W::group_of(j)) * Lanes + i) * (16 / (int)sizeof(KV)) + W::place_of(j)];
+              }
+          }
+        }
+      }
+    }
+    if (x + 1 < end) {
+      put_v(x + 1, b ^ 1, next_page);
+      if (x + 2 < end) put_pages(page, free_page);
+    }
+    this_page = next_page;
+  }
+  if (mine <= 0 || r32 >= mine) return;
+  sum += __shfl_xor(sum, 32, 64);
+  const int64_t part = (int64_t)blockIdx.x * kWideRows + 32 * wave + r32;
+  const float f = pieces > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+  float* const to = pieces > 1 ? part_o + part * DH : out + (((int64_t)s * span.T + t) * nH + head) * DH;
+  if (pieces > 1 && h == 0) part_ml[part] = make_float2(ref, sum);
+#pragma unroll
+  for (int z = 0; z < 16; ++z) {
+    const int r = 8 * (z / 4) + 4 * h + z % 4;
+#pragma unroll
+    for (int m = 0; m < M; ++m) to[Lanes == 32 ? r * E + m : (r & 15) * E + 2 * m + (r >> 4)] = o[m][z] * f;
+  }
+}
+
 // A workgroup joins the pieces of R rows of a kv head: its threads share out quads of a row's
 // values, rows and (1 / sets of) the pieces.
 template <int DH>
@@ -876,13 +1279,15 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   if (T == 0) return FG_OK;
   fg::KProfScope prof("paged_attn", 0.0, (double)c->nSeq * c->maxPages * c->pageSize * 2 * row_bytes(c));
   const int group = nHeads / c->nKvHeads, all = T * group;
-  int tiles = all <= 16 ? 1 : all <= 32 || c->dHead == 256 ? 2 : 4;
-  Span span{T, group, 16 * tiles, window, sinks, c->type ? 32 : 16, count};
+  const bool wide = all > 64;
+  const int tiles = all <= 16 ? 1 : all <= 32 || c->dHead == 256 ? 2 : 4;
+  const Span span{T, group, wide ? kWideRows : 16 * tiles, window, sinks, (c->type ? 32 : 16) * (wide ? 2 : 1),
+                  wide ? 1 : kWaves, count};
   const int64_t heads = (int64_t)c->nSeq * c->nKvHeads * ((all + span.rows - 1) / span.rows);
   const int64_t room = (int64_t)c->maxPages * c->pageSize;
   int64_t seen = room;  // by a workgroup's rows, at most
   if (window > 0 && (int64_t)window + T + sinks + 2 * span.keys < room) seen = (int64_t)window + T + sinks + 2 * span.keys;
-  const int64_t rounds = (seen + span.keys * kWaves - 1) / (span.keys * kWaves);
+  const int64_t rounds = (seen + span.keys * span.waves - 1) / (span.keys * span.waves);
   const int cus = fg::device_cu_count() > 0 ? fg::device_cu_count() : 256;
   const int target = 2 * cus;
   const bool whole = rounds <= 4 || heads >= 4 * target;
@@ -907,7 +1312,10 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   FG_LAUNCH((paged_attn_kernel<KV, DH, NT>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q, nHeads,   \
             factor, span, target, plan, part_ml, part_o)
 #define PAGED_TILES(KV, DH)                          \
-  if (tiles == 1) PAGED_ATTN(KV, DH, 1);             \
+  if (wide)                                          \
+    FG_LAUNCH((paged_wide_kernel<KV, DH>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q, nHeads,     \
+              factor, span, target, plan, part_ml, part_o);                                                          \
+  else if (tiles == 1) PAGED_ATTN(KV, DH, 1);             \
   else if (tiles == 2) PAGED_ATTN(KV, DH, 2);        \
   else PAGED_ATTN(KV, (DH == 256 ? 128 : DH), 4) /* heads of 256 have no tiles of 4 */
 #define PAGED_HEAD(DH)                               \
