@@ -727,7 +727,7 @@ struct Wide<_Float16, DH> {
   static constexpr int Lanes = DH % 64 == 0 ? 32 : 16, E = DH / Lanes, M = DH / 32;
   static constexpr float kOver = 11.f;
   f16x8 qh[DH / 16], ql[DH / 16];
-  _Float16 v[8][E];
+  uint32_t v[8][E / 2];
   // slots of the quads that lane `lane` of wave `wave` turns around, and their group
   static __device__ __forceinline__ int group_at(int wave, int lane) { return Lanes == 32 ? 2 * wave + (lane >> 5) : 4 * wave + (lane >> 4); }
   static __device__ __forceinline__ int slot_at(int group, int quad) { return 16 * (group >> 1) + 8 * quad + 4 * (group & 1); }
@@ -763,32 +763,42 @@ struct Wide<_Float16, DH> {
     s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[b], s, 0, 0, 0);
   }
   struct Probs {
-    f16x8 hi[2 * Sub], lo[2 * Sub];
-    __device__ __forceinline__ void take(const f32x16 (&p)[Sub]) {
+    f16x8 hi[2], lo[2];
+    __device__ __forceinline__ void take(const f32x16& p) {
 #pragma unroll
-      for (int z = 0; z < 2 * Sub; ++z)
+      for (int z = 0; z < 2; ++z)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = p[z / 2][8 * (z & 1) + j];
+          const float y = p[8 * z + j];
           hi[z][j] = (_Float16)y;
           lo[z][j] = (_Float16)(y - (float)hi[z][j]);
         }
     }
-    // o += the word's slots (group 2 z + h)
+    // o += the word's slots
     __device__ __forceinline__ void sum(f32x16& o, int z, u32x4 word) const {
       const f16x8 a = __builtin_bit_cast(f16x8, word);
       o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, lo[z], o, 0, 0, 0);
       o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, hi[z], o, 0, 0, 0);
     }
   };
-  static constexpr int Z = 2 * Sub;
+  static constexpr int Z = 2;  // words of 32 slots that a lane's operand takes
   __device__ __forceinline__ u32x4 turned(int e) const {
-    f16x8 w;
+    u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = v[j][e];
-    return __builtin_bit_cast(u32x4, w);
+    for (int j = 0; j < 4; ++j)
+      w[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+    return w;
   }
-  static __device__ __forceinline__ bool number(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7C00) != 0x7C00; }
+  // row j's run kept, or made zeros; whether it holds numbers alone
+  __device__ __forceinline__ bool keep(int j, bool seen) {
+    bool ok = true;
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      v[j][e] = seen ? v[j][e] : 0u;
+      ok &= (v[j][e] & 0x7C00u) != 0x7C00u & (v[j][e] & 0x7C000000u) != 0x7C000000u;
+    }
+    return ok;
+  }
   // where slot j's value stands in its group's word
   static __device__ __forceinline__ int group_of(int j) { return 2 * (j >> 4) + (j >> 2 & 1); }
   static __device__ __forceinline__ int place_of(int j) { return (j >> 3 & 1) * 4 + (j & 3); }
@@ -818,7 +828,7 @@ struct Wide<float, DH> {
   }
   struct Probs {
     f32x16 p;
-    __device__ __forceinline__ void take(const f32x16 (&x)[Sub]) { p = x[0]; }
+    __device__ __forceinline__ void take(const f32x16& x) { p = x; }
     __device__ __forceinline__ void sum(f32x16& o, int z, u32x4 word) const {
       const f32x4 a = __builtin_bit_cast(f32x4, word);
 #pragma unroll
@@ -830,18 +840,30 @@ struct Wide<float, DH> {
     const f32x4 w = {v[0][e], v[1][e], v[2][e], v[3][e]};
     return __builtin_bit_cast(u32x4, w);
   }
-  static __device__ __forceinline__ bool number(float x) { return fabsf(x) < INFINITY; }
+  __device__ __forceinline__ bool keep(int j, bool seen) {
+    bool ok = true;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      v[j][e] = seen ? v[j][e] : 0.f;
+      ok &= fabsf(v[j][e]) < INFINITY;
+    }
+    return ok;
+  }
   static __device__ __forceinline__ int group_of(int j) { return j >> 2; }
   static __device__ __forceinline__ int place_of(int j) { return j & 3; }
 };
 
-// 16 bytes a lane from `from` to LDS at `lds` + 16 lane; waited for by hand (the compiler does not count
-// it, which makes its own waits longer, never shorter).  m0 is given back: it cannot be named as changed.
-__device__ __forceinline__ void load_to_lds(uint32_t lds, const void* from) {
+// 16 bytes a lane from `from` + `offset` to LDS at `lds` + 16 lane; waited for by hand (the compiler does not count
+// it, which makes its own waits longer, never shorter).  m0 is given back: it cannot be named as changed; the
+// scalar registers may come from a vector instruction just before, which a load has to follow by five.
+__device__ __forceinline__ void load_to_lds(uint32_t lds, const void* from, uint32_t offset) {
+  const uint64_t at = (uint64_t)from;
+  const uint32_t high = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)), low = __builtin_amdgcn_readfirstlane((uint32_t)at);
+  const uint64_t base = (uint64_t)high << 32 | low;
   uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
                : "=&s"(m0)
-               : "s"(lds), "v"(from)
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(offset), "s"(base)
                : "memory");
 }
 
@@ -860,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   // what a wave has turned around holds infinities or NaN.  Pages are read up to the end of their step, and
   // those of the next but one are written in it.
   __shared__ int pages[3][Keys / 4], all_pages[3], odd[2][kWaves];
-  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+  const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
   const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Part p;
@@ -908,15 +930,30 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     }
   };
   W w;
-  auto fetch_k = [&](int x, int b, int pb) {  // straight to LDS, a wave 64 words at a time
+  // Where a wave's 64 words are whole slots of a quad their page is the wave's, and they are copied straight to
+  // LDS; smaller heads go through registers.
+  constexpr bool kStraight = Words % 16 == 0;
+  constexpr int kFetch = kTile / kThreads;
+  u32x4 kw[kStraight ? 1 : kFetch];
+  auto fetch_k = [&](int x, int b, int pb) {
     const int j0 = steps.at(x) * Keys;
 #pragma unroll
-    for (int z = 0; z < kTile / kThreads; ++z) {
+    for (int z = 0; z < kFetch; ++z) {
       const int first = (z * kWaves + wave) * 64, word = first + lane, j = word / Words;
       const int at = (word - j * Words) ^ (j >> kShift & kMask);
-      const KV* from = row_at(kbase, pages[pb][j / 4], j0 + j) + at * (16 / sizeof(KV));
-      load_to_lds(lds_at + (2 * b * kTile + first) * 16, from);
+      if constexpr (kStraight) {
+        const int jw = first / Words;  // the wave's first slot
+        const KV* from = row_at(kbase, __builtin_amdgcn_readfirstlane(pages[pb][jw / 4]), j0 + jw);
+        load_to_lds(lds_at + (2 * b * kTile + first) * 16, from, (uint32_t)((j - jw) * Words + at) * 16);
+      } else {
+        kw[z] = *reinterpret_cast<const u32x4*>(row_at(kbase, pages[pb][j / 4], j0 + j) + at * (16 / sizeof(KV)));
+      }
     }
+  };
+  auto put_k = [&](int b) {
+    if constexpr (!kStraight)
+#pragma unroll
+      for (int z = 0; z < kFetch; ++z) lds[2 * b * kTile + (z * kWaves + wave) * 64 + lane] = kw[z];
   };
   const int group = W::group_at(wave, lane), run = lane & (Lanes - 1);
   auto fetch_v = [&](int x, int pb) {
@@ -950,12 +987,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int at = j0 + j + r;
-          const bool seen = pages[pb][j / 4] >= 0 && at <= last_pos && (at > first_pos - window || at < span.sinks);
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            if (!seen) w.v[4 * u + r][e] = (KV)0;
-            ok &= W::number(w.v[4 * u + r][e]);
-          }
+          ok &= w.keep(4 * u + r, (pages[pb][j / 4] >= 0) & (at <= last_pos) & ((at > first_pos - window) | (at < span.sinks)));
         }
       }
     }
@@ -985,7 +1017,10 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   for (int m = 0; m < M; ++m)
 #pragma unroll
     for (int z = 0; z < 16; ++z) o[m][z] = 0.f;
-  if (begin < end) put_v(begin, 0, 0);
+  if (begin < end) {
+    put_k(0);
+    put_v(begin, 0, 0);
+  }
 
   int this_page = 0;
   for (int x = begin; x < end; ++x) {
@@ -1003,93 +1038,101 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     const bool some = mine > 0 && j0 <= wave_last && (j0 + Keys - 1 > wave_first - window || j0 < span.sinks);
     if (some) {
       const u32x4 *kt = lds + 2 * b * kTile, *vt = kt + kTile;
-      f32x16 sc[Sub];
-#pragma unroll
-      for (int u = 0; u < Sub; ++u) {
-#pragma unroll
-        for (int z = 0; z < 16; ++z) sc[u][z] = 0.f;
-        const int j = 32 * u + r32, swizzle = j >> kShift & kMask;
-#pragma unroll
-        for (int k = 0; k < Words / 2; ++k) w.product(sc[u], k, kt[j * Words + ((2 * k + h) ^ swizzle)]);
-      }
-      uint32_t seen[Sub];  // this lane's scores
-      if (!whole) {
-#pragma unroll
-        for (int u = 0; u < Sub; ++u) {
-          seen[u] = 0;
-#pragma unroll
-          for (int z = 0; z < 16; ++z) {
-            const int j = 32 * u + 8 * (z / 4) + 4 * h + z % 4, at = j0 + j;
-            if (pages[this_page][j / 4] >= 0 && at <= pos && (at > pos - window || at < span.sinks)) seen[u] |= 1u << z;
-            else sc[u][z] = -INFINITY;
-          }
-        }
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < Sub; ++u)
-#pragma unroll
-        for (int z = 0; z < 16; ++z) top = fmaxf(top, sc[u][z]);
-      top *= back;
-      if (__any(top > ref + kRise)) {
-        const float was = ref;
-        ref = fmaxf(was, fmaxf(top, __shfl_xor(top, 32, 64)));
-        const float keep = ref == was ? 1.f : __builtin_amdgcn_exp2f(was - ref);
-        sum *= keep;
-#pragma unroll
-        for (int m = 0; m < M; ++m) o[m] *= keep;
-      }
-      const float base = W::kOver - ref;
-#pragma unroll
-      for (int u = 0; u < Sub; ++u)
-#pragma unroll
-        for (int z = 0; z < 16; ++z) {
-          float e = __builtin_amdgcn_exp2f(fmaf(sc[u][z], back, base));
-          if (!whole && !(seen[u] >> z & 1)) e = 0.f;
-          sum += e;
-          sc[u][z] = e;
-        }
       bool slow = false;
       if (!whole)
 #pragma unroll
         for (int z = 0; z < kWaves; ++z) slow |= odd[b][z] != 0;
-      if (!slow) {
-        typename W::Probs pr;
-        pr.take(sc);
+      // 32 slots at a time: their scores and p are all that a wave holds
 #pragma unroll
-        for (int m = 0; m < M; ++m)
+      for (int u = 0; u < Sub; ++u) {
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 sc;
 #pragma unroll
-          for (int z = 0; z < Z; ++z) {
-            const int at = Lanes == 32 ? (m * 8 + 2 * z + h) * 32 + r32 : ((2 * m + (r32 >> 4)) * 8 + 2 * z + h) * 16 + (r32 & 15);
-            pr.sum(o[m], z, vt[at]);
+        for (int z = 0; z < 16; ++z) sc[z] = 0.f;
+        // word 2 k + h at its swizzle: that of k = 0 with k's bits turned (computed here: kept, these would fill the registers)
+        const int j = 32 * u + r32;
+        int word = j * Words + (h ^ (j >> kShift & kMask));
+        asm volatile("" : "+v"(word));
+#pragma unroll
+        for (int k = 0; k < Words / 2; ++k) {
+          constexpr int kTurn = kMask & ~1;
+          w.product(sc, k, kt[(word ^ (2 * k & kTurn)) + (2 * k & ~kTurn)]);
+        }
+        uint32_t seen = 0;  // this lane's scores
+        if (!whole) {
+          asm volatile("");  // (a branch: most steps go past it)
+#pragma unroll
+          for (int z = 0; z < 16; ++z) {
+            const int j = 32 * u + 8 * (z / 4) + 4 * h + z % 4, at = j0 + j;
+            const bool is = (pages[this_page][j / 4] >= 0) & (at <= pos) & ((at > pos - window) | (at < span.sinks));
+            seen |= is ? 1u << z : 0u;
+            sc[z] = is ? sc[z] : -INFINITY;
           }
-      } else {
-        // a value that is seen is not finite: it must not reach the rows that do not see it
-        for (int j = 0; j < Keys; ++j) {
-          const int at = j0 + j;
-          const bool is = pages[this_page][j / 4] >= 0 && at <= pos && (at > pos - window || at < span.sinks);
-          float e = 0.f;
+        }
+        float top = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < Sub; ++u)
+        for (int z = 0; z < 16; ++z) top = fmaxf(top, sc[z]);
+        top *= back;
+        if (__any(top > ref + kRise)) {
+          const float was = ref;
+          ref = fmaxf(was, fmaxf(top, __shfl_xor(top, 32, 64)));
+          const float keep = ref == was ? 1.f : __builtin_amdgcn_exp2f(was - ref);
+          sum *= keep;
+#pragma unroll
+          for (int m = 0; m < M; ++m) o[m] *= keep;
+        }
+        const float base = W::kOver - ref;
+#pragma unroll
+        for (int z = 0; z < 16; ++z) {
+          sc[z] = __builtin_amdgcn_exp2f(fmaf(sc[z], back, base));
+        }
+        if (!whole) {
+          asm volatile("");
+#pragma unroll
+          for (int z = 0; z < 16; ++z) sc[z] = seen >> z & 1 ? sc[z] : 0.f;
+        }
+#pragma unroll
+        for (int z = 0; z < 16; ++z) sum += sc[z];
+        if (!slow) {
+          typename W::Probs pr;
+          pr.take(sc);
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int z = 0; z < Z; ++z) {
+              const int g8 = 2 * (Z * u + z) + h;
+              const int at = Lanes == 32 ? (m * 8 + g8) * 32 + r32 : ((2 * m + (r32 >> 4)) * 8 + g8) * 16 + (r32 & 15);
+              pr.sum(o[m], z, vt[at]);
+            }
+        } else {
+          // a value that is seen is not finite: it must not reach the rows that do not see it
+          for (int j = 32 * u; j < 32 * u + 32; ++j) {
+            const int at = j0 + j;
+            const bool is = pages[this_page][j / 4] >= 0 && at <= pos && (at > pos - window || at < span.sinks);
+            float e = 0.f;
 #pragma unroll
             for (int z = 0; z < 16; ++z) {
-              const float y = __shfl(sc[u][z], r32 + 32 * (j >> 2 & 1), 64);
-              if (j >> 5 == u && (j >> 3 & 3) == z / 4 && (j & 3) == z % 4) e = y;
+              const float y = __shfl(sc[z], r32 + 32 * (j >> 2 & 1), 64);
+              if ((j >> 3 & 3) == z / 4 && (j & 3) == z % 4) e = y;
+              __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the other path)
             }
-          if (is) {
-            const KV* const flat = reinterpret_cast<const KV*>(vt);
+            if (is) {
+              const KV* const flat = reinterpret_cast<const KV*>(vt);
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+              for (int m = 0; m < M; ++m)
 #pragma unroll
-              for (int z = 0; z < 16; ++z) {
-                const int r = 8 * (z / 4) + 4 * h + z % 4, i = Lanes == 32 ? r : r & 15, run_e = Lanes == 32 ? m : 2 * m + (r >> 4);
-                o[m][z] += e * (float)flat[((run_e * 8 + W::group_of(j)) * Lanes + i) * (16 / (int)sizeof(KV)) + W::place_of(j)];
-              }
+                for (int z = 0; z < 16; ++z) {
+                  const int r = 8 * (z / 4) + 4 * h + z % 4, i = Lanes == 32 ? r : r & 15, run_e = Lanes == 32 ? m : 2 * m + (r >> 4);
+                  o[m][z] += e * (float)flat[((run_e * 8 + W::group_of(j)) * Lanes + i) * (16 / (int)sizeof(KV)) + W::place_of(j)];
+                  if (z % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
           }
         }
       }
     }
     if (x + 1 < end) {
+      put_k(b ^ 1);
       put_v(x + 1, b ^ 1, next_page);
       if (x + 2 < end) put_pages(page, free_page);
     }
