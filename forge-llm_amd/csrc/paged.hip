@@ -253,6 +253,30 @@ __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int6
   return true;
 }
 
+// Zeros for what is not finite; whether all was.
+template <int N>
+__device__ __forceinline__ bool tame_halves(uint32_t (&v)[N]) {
+  bool ok = true;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const bool low = (v[e] & 0x7C00u) != 0x7C00u, high = (v[e] & 0x7C000000u) != 0x7C000000u;
+    ok &= low & high;
+    v[e] &= (low ? 0xFFFFu : 0u) | (high ? 0xFFFF0000u : 0u);
+  }
+  return ok;
+}
+template <int N>
+__device__ __forceinline__ bool tame_floats(float (&v)[N]) {
+  bool ok = true;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const bool is = fabsf(v[e]) < INFINITY;
+    ok &= is;
+    v[e] = is ? v[e] : 0.f;
+  }
+  return ok;
+}
+
 // Slots of a step as a lane holds them: keys of slot i (and 16 + i), 8 (fp32: 4) values of every 32 (16) from 8 g (4 g) on;
 // values of slots 4 g .. 4 g + 3 (and 16 more on), runs of E.
 template <class KV, int DH>
@@ -278,20 +302,11 @@ struct Step<_Float16, DH> {
       for (int r = 0; r < Runs; ++r)
         __builtin_memcpy(v[j][r], __builtin_assume_aligned(row[j / 4] + (j % 4) * DH + r * 16 * E + i * E, E == 6 ? 4 : 2 * E), 2 * E);
   }
-  __device__ __forceinline__ void clear(int j) {
-#pragma unroll
-    for (int r = 0; r < Runs; ++r)
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) v[j][r][e] = 0;
-  }
-  __device__ __forceinline__ bool finite() const {
+  // Slot j's values with zeros for what is not finite; whether all of them were.
+  __device__ __forceinline__ bool tame(int j) {
     bool ok = true;
 #pragma unroll
-    for (int j = 0; j < 4 * Sub; ++j)
-#pragma unroll
-      for (int r = 0; r < Runs; ++r)
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) ok &= (v[j][r][e] & 0x7C00u) != 0x7C00u && (v[j][r][e] & 0x7C000000u) != 0x7C000000u;
+    for (int r = 0; r < Runs; ++r) ok &= tame_halves<E / 2>(v[j][r]);
     return ok;
   }
   // q's operand of a tile: two pieces of q 2^e, its greatest value just below 2^15
@@ -303,7 +318,8 @@ struct Step<_Float16, DH> {
     for (int b = 0; b < DH / 32; ++b)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        x[b][j] = on ? q[32 * b + 8 * g + j] * factor : 0.f;
+        const float y = q[32 * b + 8 * g + j];  // (loaded in any case: a branch a value would wait for each)
+        x[b][j] = on ? y * factor : 0.f;
         m = fmaxf(m, fabsf(x[b][j]));
       }
     m = fmaxf(m, __shfl_xor(m, 16, 64));
@@ -384,20 +400,10 @@ struct Step<float, DH> {
       for (int r = 0; r < Runs; ++r)
         __builtin_memcpy(v[j][r], __builtin_assume_aligned(row[0] + j * DH + r * 16 * E + i * E, 4 * E), 4 * E);
   }
-  __device__ __forceinline__ void clear(int j) {
-#pragma unroll
-    for (int r = 0; r < Runs; ++r)
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[j][r][e] = 0.f;
-  }
-  __device__ __forceinline__ bool finite() const {
+  __device__ __forceinline__ bool tame(int j) {
     bool ok = true;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int r = 0; r < Runs; ++r)
-#pragma unroll
-        for (int e = 0; e < E; ++e) ok &= fabsf(v[j][r][e]) < INFINITY;
+    for (int r = 0; r < Runs; ++r) ok &= tame_floats<E>(v[j][r]);
     return ok;
   }
   static constexpr int kQ = DH / 16;
@@ -407,7 +413,10 @@ struct Step<float, DH> {
     for (int b = 0; b < DH / 16; ++b) {
       f32x4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = on ? q[16 * b + 4 * g + j] * factor : 0.f;
+      for (int j = 0; j < 4; ++j) {
+        const float y = q[16 * b + 4 * g + j];
+        x[j] = on ? y * factor : 0.f;
+      }
       to[b][lane] = __builtin_bit_cast(u32x4, x);
     }
     return 1.f;
@@ -578,20 +587,22 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
     for (int u = 0; u < Sub; ++u) pages &= (uint32_t)here.v[u] < (uint32_t)c.nPages;
     // every row sees every slot of the step
     const bool whole = j0 + Keys - 1 <= first_pos && (j0 > last_pos - window || j0 + Keys <= span.sinks) && __all(pages);
-    bool slow = false;
+    bool odd = false;  // a value that some row sees is not finite; it is left out of the product
     if (!whole) {
-      bool seen[4 * Sub];  // by some row
+      asm volatile("");  // (a branch: most steps go past it)
+      bool ok = true;
 #pragma unroll
       for (int j = 0; j < 4 * Sub; ++j) {
         const int at = j0 + 16 * (j / 4) + 4 * g + j % 4;
         const bool there = (uint32_t)here.v[j / 4] < (uint32_t)c.nPages;
-        seen[j] = there && at <= last_pos && (at > first_pos - window || at < span.sinks);
-        if (!seen[j]) step.clear(j);
+        ok &= step.tame(j) | !(there & (at <= last_pos) & ((at > first_pos - window) | (at < span.sinks)));
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          if (!(there && at <= pos[n] && (at > pos[n] - window || at < span.sinks))) sc[n][j / 4][j % 4] = -INFINITY;
+        for (int n = 0; n < NT; ++n) {
+          const bool is = there & (at <= pos[n]) & ((at > pos[n] - window) | (at < span.sinks));
+          sc[n][j / 4][j % 4] = is ? sc[n][j / 4][j % 4] : -INFINITY;
+        }
       }
-      slow = !__all(step.finite());
+      odd = !__all(ok);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -617,23 +628,21 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
         if (!whole) {
           const int at = j0 + 16 * (j / 4) + 4 * g + j % 4;
           const bool there = (uint32_t)here.v[j / 4] < (uint32_t)c.nPages;
-          if (!(there && at <= pos[n] && (at > pos[n] - window || at < span.sinks))) e = 0.f;
+          e = there & (at <= pos[n]) & ((at > pos[n] - window) | (at < span.sinks)) ? e : 0.f;
         }
         sum[n] += e;
         sc[n][j / 4][j % 4] = e;
       }
     }
-    if (!slow) {
-      step.template sums<NT>(o, sc);
-    } else {
-      // a value that is seen is not finite: it must not reach the rows that do not see it
+    step.template sums<NT>(o, sc);
+    if (odd) {
       for (int j = 0; j < Keys; ++j) {
         const int at = j0 + j, page = (at >> c.lg) < c.maxPages ? table[at >> c.lg] : -1;
         if ((uint32_t)page >= (uint32_t)c.nPages) continue;
-        const KV* row = row_at(vbase, page, at);
+        const KV* from = row_at(vbase, page, at);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const bool mine = at <= pos[n] && (at > pos[n] - window || at < span.sinks);
+          const bool is = (at <= pos[n]) & ((at > pos[n] - window) | (at < span.sinks));
           float e = 0.f;
 #pragma unroll
           for (int u = 0; u < Sub; ++u)
@@ -641,13 +650,16 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
             for (int r = 0; r < 4; ++r) {
               const float y = __shfl(sc[n][u][r], i + 16 * ((j & 15) >> 2), 64);
               if (j >> 4 == u && (j & 3) == r) e = y;
+              __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the common path)
             }
-          if (mine) {
 #pragma unroll
-            for (int m = 0; m < M; ++m)
+          for (int m = 0; m < M; ++m)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) o[n][m][r] += e * (float)row[(m / E) * 16 * E + (4 * g + r) * E + m % E];
-          }
+            for (int r = 0; r < 4; ++r) {
+              const float y = (float)from[(m / E) * 16 * E + (4 * g + r) * E + m % E];
+              o[n][m][r] += is && !(fabsf(y) < INFINITY) ? e * y : 0.f;
+              if (r == 3) __builtin_amdgcn_sched_barrier(0);
+            }
         }
       }
     }
@@ -740,7 +752,7 @@ struct Wide<_Float16, DH> {
     for (int b = 0; b < DH / 16; ++b)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float y = on ? q[16 * b + 8 * h + j] * factor : 0.f;
+        const float z = q[16 * b + 8 * h + j], y = on ? z * factor : 0.f;
         x[b][j / 4][j % 4] = y;
         m = fmaxf(m, fabsf(y));
       }
@@ -789,16 +801,8 @@ struct Wide<_Float16, DH> {
       w[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
     return w;
   }
-  // row j's run kept, or made zeros; whether it holds numbers alone
-  __device__ __forceinline__ bool keep(int j, bool seen) {
-    bool ok = true;
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      v[j][e] = seen ? v[j][e] : 0u;
-      ok &= (v[j][e] & 0x7C00u) != 0x7C00u & (v[j][e] & 0x7C000000u) != 0x7C000000u;
-    }
-    return ok;
-  }
+  // Row j's run with zeros for what is not finite; whether all of it was.
+  __device__ __forceinline__ bool tame(int j) { return tame_halves<E / 2>(v[j]); }
   // where slot j's value stands in its group's word
   static __device__ __forceinline__ int group_of(int j) { return 2 * (j >> 4) + (j >> 2 & 1); }
   static __device__ __forceinline__ int place_of(int j) { return (j >> 3 & 1) * 4 + (j & 3); }
@@ -818,7 +822,10 @@ struct Wide<float, DH> {
 #pragma unroll
     for (int b = 0; b < DH / 8; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) q4[b][j] = on ? q[8 * b + 4 * h + j] * factor : 0.f;
+      for (int j = 0; j < 4; ++j) {
+        const float y = q[8 * b + 4 * h + j];
+        q4[b][j] = on ? y * factor : 0.f;
+      }
     return 1.f;
   }
   __device__ __forceinline__ void product(f32x16& s, int b, u32x4 word) const {
@@ -840,15 +847,7 @@ struct Wide<float, DH> {
     const f32x4 w = {v[0][e], v[1][e], v[2][e], v[3][e]};
     return __builtin_bit_cast(u32x4, w);
   }
-  __device__ __forceinline__ bool keep(int j, bool seen) {
-    bool ok = true;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      v[j][e] = seen ? v[j][e] : 0.f;
-      ok &= fabsf(v[j][e]) < INFINITY;
-    }
-    return ok;
-  }
+  __device__ __forceinline__ bool tame(int j) { return tame_floats<E>(v[j]); }
   static __device__ __forceinline__ int group_of(int j) { return j >> 2; }
   static __device__ __forceinline__ int place_of(int j) { return j & 3; }
 };
@@ -879,9 +878,10 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   constexpr int kShift = Words % 16 == 0 ? 0 : Words % 8 == 0 ? 1 : 2, kMask = Words % 16 == 0 ? 15 : Words % 8 == 0 ? 7 : 3;
   __shared__ __attribute__((aligned(16))) u32x4 lds[4 * kTile];  // [2][K, V][kTile]
   // Of a step's quads of slots: their pages, -1 for none, and whether all have one; of its V: whether
-  // what a wave has turned around holds infinities or NaN.  Pages are read up to the end of their step, and
+  // what a wave has turned around held infinities or NaN.  Pages are read up to the end of their step, and
   // those of the next but one are written in it.
-  __shared__ int pages[3][Keys / 4], all_pages[3], odd[2][kWaves];
+  __shared__ int pages[3][Keys / 4], all_pages[3];
+  __shared__ __attribute__((aligned(4))) uint8_t odd[2][kWaves];
   const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
   const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -979,7 +979,8 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     }
     bool ok = true;
     if (!is_whole(x, pb)) {
-      // slots that no row sees are zeros; of the others infinities and NaN are told of
+      // Not every row sees all of it: what is not finite would reach, times a p of zero, rows that do not.  It becomes
+      // zeros and, if any row sees it, is told of.
       const int j0 = steps.at(x) * Keys;
 #pragma unroll
       for (int u = 0; u < W::Quads; ++u) {
@@ -987,7 +988,8 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int at = j0 + j + r;
-          ok &= w.keep(4 * u + r, (pages[pb][j / 4] >= 0) & (at <= last_pos) & ((at > first_pos - window) | (at < span.sinks)));
+          const bool seen = (pages[pb][j / 4] >= 0) & (at <= last_pos) & ((at > first_pos - window) | (at < span.sinks));
+          ok &= w.tame(4 * u + r) | !seen;
         }
       }
     }
@@ -1038,10 +1040,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     const bool some = mine > 0 && j0 <= wave_last && (j0 + Keys - 1 > wave_first - window || j0 < span.sinks);
     if (some) {
       const u32x4 *kt = lds + 2 * b * kTile, *vt = kt + kTile;
-      bool slow = false;
-      if (!whole)
-#pragma unroll
-        for (int z = 0; z < kWaves; ++z) slow |= odd[b][z] != 0;
+      const bool odd_step = *reinterpret_cast<const uint32_t*>(odd[b]) != 0;
       // 32 slots at a time: their scores and p are all that a wave holds
 #pragma unroll
       for (int u = 0; u < Sub; ++u) {
@@ -1093,40 +1092,38 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
         }
 #pragma unroll
         for (int z = 0; z < 16; ++z) sum += sc[z];
-        if (!slow) {
-          typename W::Probs pr;
-          pr.take(sc);
+        typename W::Probs pr;
+        pr.take(sc);
 #pragma unroll
-          for (int m = 0; m < M; ++m)
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-            for (int z = 0; z < Z; ++z) {
-              const int g8 = 2 * (Z * u + z) + h;
-              const int at = Lanes == 32 ? (m * 8 + g8) * 32 + r32 : ((2 * m + (r32 >> 4)) * 8 + g8) * 16 + (r32 & 15);
-              pr.sum(o[m], z, vt[at]);
-            }
-        } else {
-          // a value that is seen is not finite: it must not reach the rows that do not see it
+          for (int z = 0; z < Z; ++z) {
+            const int g8 = 2 * (Z * u + z) + h;
+            const int at = Lanes == 32 ? (m * 8 + g8) * 32 + r32 : ((2 * m + (r32 >> 4)) * 8 + g8) * 16 + (r32 & 15);
+            pr.sum(o[m], z, vt[at]);
+          }
+        if (odd_step) {
+          // infinities and NaN, zeros so far, for the rows that see them
           for (int j = 32 * u; j < 32 * u + 32; ++j) {
-            const int at = j0 + j;
-            const bool is = pages[this_page][j / 4] >= 0 && at <= pos && (at > pos - window || at < span.sinks);
+            const int at = j0 + j, page = pages[this_page][j / 4];
+            const bool is = (page >= 0) & (at <= pos) & ((at > pos - window) | (at < span.sinks));
+            const KV* const from = row_at(vbase, page, at);
             float e = 0.f;
 #pragma unroll
             for (int z = 0; z < 16; ++z) {
               const float y = __shfl(sc[z], r32 + 32 * (j >> 2 & 1), 64);
               if ((j >> 3 & 3) == z / 4 && (j & 3) == z % 4) e = y;
-              __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the other path)
+              __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the common path)
             }
-            if (is) {
-              const KV* const flat = reinterpret_cast<const KV*>(vt);
 #pragma unroll
-              for (int m = 0; m < M; ++m)
+            for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int z = 0; z < 16; ++z) {
-                  const int r = 8 * (z / 4) + 4 * h + z % 4, i = Lanes == 32 ? r : r & 15, run_e = Lanes == 32 ? m : 2 * m + (r >> 4);
-                  o[m][z] += e * (float)flat[((run_e * 8 + W::group_of(j)) * Lanes + i) * (16 / (int)sizeof(KV)) + W::place_of(j)];
-                  if (z % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                }
-            }
+              for (int z = 0; z < 16; ++z) {
+                const int r = 8 * (z / 4) + 4 * h + z % 4;
+                const float y = (float)from[Lanes == 32 ? r * E + m : (r & 15) * E + 2 * m + (r >> 4)];
+                o[m][z] += is && !(fabsf(y) < INFINITY) ? e * y : 0.f;
+                if (z % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+              }
           }
         }
       }
