@@ -253,6 +253,13 @@ __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int6
   return true;
 }
 
+// y - h, exactly, as one instruction that takes an fp16 operand (v_fma_mix; a subtraction would convert first).
+__device__ __forceinline__ float rest_of(float y, _Float16 h) {
+  float minus = -1.f;
+  asm("" : "+s"(minus));
+  return __builtin_fmaf((float)h, minus, y);
+}
+
 // Zeros for what is not finite; whether all was.
 template <int N>
 __device__ __forceinline__ bool tame_halves(uint32_t (&v)[N]) {
@@ -362,7 +369,7 @@ struct Step<_Float16, DH> {
 #pragma unroll
       for (int j = 0; j < 8; ++j) hi[n][j] = (_Float16)p[n][j / 4][j % 4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) lo[n][j] = (_Float16)(p[n][j / 4][j % 4] - (float)hi[n][j]);
+      for (int j = 0; j < 8; ++j) lo[n][j] = (_Float16)rest_of(p[n][j / 4][j % 4], hi[n][j]);
     }
 #pragma unroll
     for (int r = 0; r < Runs; ++r)
@@ -783,7 +790,7 @@ struct Wide<_Float16, DH> {
         for (int j = 0; j < 8; ++j) {
           const float y = p[8 * z + j];
           hi[z][j] = (_Float16)y;
-          lo[z][j] = (_Float16)(y - (float)hi[z][j]);
+          lo[z][j] = (_Float16)rest_of(y, hi[z][j]);
         }
     }
     // o += the word's slots
@@ -937,15 +944,22 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   u32x4 kw[kStraight ? 1 : kFetch];
   auto fetch_k = [&](int x, int b, int pb) {
     const int j0 = steps.at(x) * Keys;
+    if constexpr (kStraight) {
+      // kRows slots a load; the swizzle's bits from a load's number and a lane's part do not meet
+      constexpr int kRows = 64 / Words;
+      const int j = lane / Words;
+      uint32_t offset = (j * Words + (lane - j * Words ^ (wave * kRows + j))) * 16;
+      asm volatile("" : "+v"(offset));  // (one register, not one a load)
 #pragma unroll
-    for (int z = 0; z < kFetch; ++z) {
-      const int first = (z * kWaves + wave) * 64, word = first + lane, j = word / Words;
-      const int at = (word - j * Words) ^ (j >> kShift & kMask);
-      if constexpr (kStraight) {
-        const int jw = first / Words;  // the wave's first slot
+      for (int z = 0; z < kFetch; ++z) {
+        const int jw = (z * kWaves + wave) * kRows;  // the wave's first slot
         const KV* from = row_at(kbase, __builtin_amdgcn_readfirstlane(pages[pb][jw / 4]), j0 + jw);
-        load_to_lds(lds_at + (2 * b * kTile + first) * 16, from, (uint32_t)((j - jw) * Words + at) * 16);
-      } else {
+        load_to_lds(lds_at + (2 * b * kTile + (z * kWaves + wave) * 64) * 16, from, offset ^ (z * kWaves * kRows & 15) * 16);
+      }
+    } else {
+#pragma unroll
+      for (int z = 0; z < kFetch; ++z) {
+        const int word = (z * kWaves + wave) * 64 + lane, j = word / Words, at = (word - j * Words) ^ (j >> kShift & kMask);
         kw[z] = *reinterpret_cast<const u32x4*>(row_at(kbase, pages[pb][j / 4], j0 + j) + at * (16 / sizeof(KV)));
       }
     }
@@ -1135,15 +1149,20 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     }
     this_page = next_page;
   }
-  if (mine <= 0 || r32 >= mine) return;
+  // (found again rather than kept through the loop)
+  int me = threadIdx.x;
+  asm volatile("" : "+v"(me));
+  const int my_row = me & 31, my_h = me >> 5 & 1, at_row = row0 + 32 * wave + my_row;
+  if (my_row >= mine) return;
   sum += __shfl_xor(sum, 32, 64);
-  const int64_t part = (int64_t)blockIdx.x * kWideRows + 32 * wave + r32;
+  const int64_t part = (int64_t)blockIdx.x * kWideRows + 32 * wave + my_row;
   const float f = pieces > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
-  float* const to = pieces > 1 ? part_o + part * DH : out + (((int64_t)s * span.T + t) * nH + head) * DH;
-  if (pieces > 1 && h == 0) part_ml[part] = make_float2(ref, sum);
+  const int my_t = at_row / span.group, my_head = kvh * span.group + (at_row - my_t * span.group);
+  float* const to = pieces > 1 ? part_o + part * DH : out + (((int64_t)s * span.T + my_t) * nH + my_head) * DH;
+  if (pieces > 1 && my_h == 0) part_ml[part] = make_float2(ref, sum);
 #pragma unroll
   for (int z = 0; z < 16; ++z) {
-    const int r = 8 * (z / 4) + 4 * h + z % 4;
+    const int r = 8 * (z / 4) + 4 * my_h + z % 4;
 #pragma unroll
     for (int m = 0; m < M; ++m) to[Lanes == 32 ? r * E + m : (r & 15) * E + 2 * m + (r >> 4)] = o[m][z] * f;
   }
