@@ -253,11 +253,26 @@ __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int6
   return true;
 }
 
-// y - h, exactly, as one instruction that takes an fp16 operand (v_fma_mix; a subtraction would convert first).
-__device__ __forceinline__ float rest_of(float y, _Float16 h) {
+// The two fp16 pieces of eight values, pair by pair.  The first pieces are one conversion a pair, the remainders,
+// exact before they are rounded, one mixed product each (v_fma_mix takes and gives fp16) of those very halves: the
+// compiler, left alone, would convert each value a second time.
+__device__ __forceinline__ void two_pieces(const float (&x)[8], f16x8& hi, f16x8& lo) {
   float minus = -1.f;
   asm("" : "+s"(minus));
-  return __builtin_fmaf((float)h, minus, y);
+  u32x4 h, l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x[2 * j], x[2 * j + 1]}, f16x2));
+    asm("" : "+v"(pair));
+    const f16x2 y = __builtin_bit_cast(f16x2, pair);
+    f16x2 rest;
+    rest[0] = (_Float16)__builtin_fmaf((float)y[0], minus, x[2 * j]);
+    rest[1] = (_Float16)__builtin_fmaf((float)y[1], minus, x[2 * j + 1]);
+    h[j] = pair;
+    l[j] = __builtin_bit_cast(uint32_t, rest);
+  }
+  hi = __builtin_bit_cast(f16x8, h);
+  lo = __builtin_bit_cast(f16x8, l);
 }
 
 // Zeros for what is not finite; whether all was.
@@ -336,11 +351,8 @@ struct Step<_Float16, DH> {
     for (int b = 0; b < DH / 32; ++b) {
       f16x8 hi, lo;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = __builtin_amdgcn_ldexpf(x[b][j], e);
-        hi[j] = (_Float16)y;
-        lo[j] = (_Float16)(y - (float)hi[j]);
-      }
+      for (int j = 0; j < 8; ++j) x[b][j] = __builtin_amdgcn_ldexpf(x[b][j], e);
+      two_pieces(x[b], hi, lo);
       to[2 * b][lane] = __builtin_bit_cast(u32x4, hi);
       to[2 * b + 1][lane] = __builtin_bit_cast(u32x4, lo);
     }
@@ -366,10 +378,10 @@ struct Step<_Float16, DH> {
     f16x8 hi[NT], lo[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) hi[n][j] = (_Float16)p[n][j / 4][j % 4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) lo[n][j] = (_Float16)rest_of(p[n][j / 4][j % 4], hi[n][j]);
+      for (int j = 0; j < 8; ++j) x[j] = p[n][j / 4][j % 4];
+      two_pieces(x, hi[n], lo[n]);
     }
 #pragma unroll
     for (int r = 0; r < Runs; ++r)
@@ -664,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float y = (float)from[(m / E) * 16 * E + (4 * g + r) * E + m % E];
-              o[n][m][r] += is && !(fabsf(y) < INFINITY) ? e * y : 0.f;
+              o[n][m][r] += is & !(fabsf(y) < INFINITY) ? e * y : 0.f;
               if (r == 3) __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -754,25 +766,23 @@ struct Wide<_Float16, DH> {
   __device__ __forceinline__ float load_q(const float* q, float factor, bool on) {
     const int h = (threadIdx.x & 63) >> 5;
     float m = 0.f;
-    f32x4 x[DH / 16][2];
+    float x[DH / 16][8];
 #pragma unroll
     for (int b = 0; b < DH / 16; ++b)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float z = q[16 * b + 8 * h + j], y = on ? z * factor : 0.f;
-        x[b][j / 4][j % 4] = y;
-        m = fmaxf(m, fabsf(y));
+        const float y = q[16 * b + 8 * h + j];
+        x[b][j] = on ? y * factor : 0.f;
+        m = fmaxf(m, fabsf(x[b][j]));
       }
     m = fmaxf(m, __shfl_xor(m, 32, 64));
     const int e = m > 0.f && m < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
 #pragma unroll
-    for (int b = 0; b < DH / 16; ++b)
+    for (int b = 0; b < DH / 16; ++b) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = __builtin_amdgcn_ldexpf(x[b][j / 4][j % 4], e);
-        qh[b][j] = (_Float16)y;
-        ql[b][j] = (_Float16)(y - (float)qh[b][j]);
-      }
+      for (int j = 0; j < 8; ++j) x[b][j] = __builtin_amdgcn_ldexpf(x[b][j], e);
+      two_pieces(x[b], qh[b], ql[b]);
+    }
     return __builtin_amdgcn_ldexpf(1.f, -e);
   }
   // the scores of slots 32 u .. from the rows' words
@@ -785,14 +795,15 @@ struct Wide<_Float16, DH> {
     f16x8 hi[2], lo[2];
     __device__ __forceinline__ void take(const f32x16& p) {
 #pragma unroll
-      for (int z = 0; z < 2; ++z)
+      for (int z = 0; z < 2; ++z) {
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float y = p[8 * z + j];
-          hi[z][j] = (_Float16)y;
-          lo[z][j] = (_Float16)rest_of(y, hi[z][j]);
-        }
+        for (int j = 0; j < 8; ++j) x[j] = p[8 * z + j];
+        two_pieces(x, hi[z], lo[z]);
+        asm("" : "+v"(lo[z]));  // (what the rare path takes from here are these, not more registers)
+      }
     }
+    __device__ __forceinline__ float at(int z) const { return (float)hi[z / 8][z % 8] + (float)lo[z / 8][z % 8]; }
     // o += the word's slots
     __device__ __forceinline__ void sum(f32x16& o, int z, u32x4 word) const {
       const f16x8 a = __builtin_bit_cast(f16x8, word);
@@ -843,6 +854,7 @@ struct Wide<float, DH> {
   struct Probs {
     f32x16 p;
     __device__ __forceinline__ void take(const f32x16& x) { p = x; }
+    __device__ __forceinline__ float at(int z) const { return p[z]; }
     __device__ __forceinline__ void sum(f32x16& o, int z, u32x4 word) const {
       const f32x4 a = __builtin_bit_cast(f32x4, word);
 #pragma unroll
@@ -950,10 +962,13 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
       const int j = lane / Words;
       uint32_t offset = (j * Words + (lane - j * Words ^ (wave * kRows + j))) * 16;
       asm volatile("" : "+v"(offset));  // (one register, not one a load)
+      int page[kFetch];
+#pragma unroll
+      for (int z = 0; z < kFetch; ++z) page[z] = pages[pb][(z * kWaves + wave) * kRows / 4];
 #pragma unroll
       for (int z = 0; z < kFetch; ++z) {
         const int jw = (z * kWaves + wave) * kRows;  // the wave's first slot
-        const KV* from = row_at(kbase, __builtin_amdgcn_readfirstlane(pages[pb][jw / 4]), j0 + jw);
+        const KV* from = row_at(kbase, __builtin_amdgcn_readfirstlane(page[z]), j0 + jw);
         load_to_lds(lds_at + (2 * b * kTile + (z * kWaves + wave) * 64) * 16, from, offset ^ (z * kWaves * kRows & 15) * 16);
       }
     } else {
@@ -1055,22 +1070,43 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     if (some) {
       const u32x4 *kt = lds + 2 * b * kTile, *vt = kt + kTile;
       const bool odd_step = *reinterpret_cast<const uint32_t*>(odd[b]) != 0;
-      // 32 slots at a time: their scores and p are all that a wave holds
+      // 32 slots at a time: their scores and p are all that a wave holds.  Words of K are read while the slots before
+      // them are summed, the first words of V while p is formed (read when they are wanted, the waits took a third
+      // of the time; all of them ahead would not fit the registers).
+      constexpr int kKeyWords = Words / 2, kAhead = kKeyWords < 4 ? kKeyWords : 4;
+      // word 2 k + h of slot 32 u + r32 at its swizzle: that of k = 0 with k's bits turned
+      auto first_key = [&](int u) {
+        const int j = 32 * u + r32;
+        int word = j * Words + (h ^ (j >> kShift & kMask));
+        asm volatile("" : "+v"(word));  // (the others are computed where they are read: kept, they would fill the registers)
+        return word;
+      };
+      auto key_word = [&](int word, int k) {
+        constexpr int kTurn = kMask & ~1;
+        return kt[(word ^ (2 * k & kTurn)) + (2 * k & ~kTurn)];
+      };
+      auto value_word = [&](int u, int i) {  // of o[i % M]
+        const int m = i % M, g8 = 2 * (Z * u + i / M) + h;
+        return vt[Lanes == 32 ? (m * 8 + g8) * 32 + r32 : ((2 * m + (r32 >> 4)) * 8 + g8) * 16 + (r32 & 15)];
+      };
+      u32x4 ks[kAhead], vs[M];
 #pragma unroll
       for (int u = 0; u < Sub; ++u) {
         __builtin_amdgcn_sched_barrier(0);
+        const int first = first_key(u);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) ks[k] = key_word(first, k);
         f32x16 sc;
 #pragma unroll
         for (int z = 0; z < 16; ++z) sc[z] = 0.f;
-        // word 2 k + h at its swizzle: that of k = 0 with k's bits turned (computed here: kept, these would fill the registers)
-        const int j = 32 * u + r32;
-        int word = j * Words + (h ^ (j >> kShift & kMask));
-        asm volatile("" : "+v"(word));
 #pragma unroll
-        for (int k = 0; k < Words / 2; ++k) {
-          constexpr int kTurn = kMask & ~1;
-          w.product(sc, k, kt[(word ^ (2 * k & kTurn)) + (2 * k & ~kTurn)]);
+        for (int k = 0; k < kKeyWords; ++k) {
+          w.product(sc, k, ks[k % kAhead]);
+          if (k + kAhead < kKeyWords) ks[k % kAhead] = key_word(first, k + kAhead);
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int m = 0; m < M; ++m) vs[m] = value_word(u, m);
         uint32_t seen = 0;  // this lane's scores
         if (!whole) {
           asm volatile("");  // (a branch: most steps go past it)
@@ -1108,14 +1144,12 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
         for (int z = 0; z < 16; ++z) sum += sc[z];
         typename W::Probs pr;
         pr.take(sc);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int m = 0; m < M; ++m)
-#pragma unroll
-          for (int z = 0; z < Z; ++z) {
-            const int g8 = 2 * (Z * u + z) + h;
-            const int at = Lanes == 32 ? (m * 8 + g8) * 32 + r32 : ((2 * m + (r32 >> 4)) * 8 + g8) * 16 + (r32 & 15);
-            pr.sum(o[m], z, vt[at]);
-          }
+        for (int i = 0; i < M * Z; ++i) {
+          pr.sum(o[i % M], i / M, vs[i % M]);
+          if (i + M < M * Z) vs[i % M] = value_word(u, i + M);
+        }
         if (odd_step) {
           // infinities and NaN, zeros so far, for the rows that see them
           for (int j = 32 * u; j < 32 * u + 32; ++j) {
@@ -1125,7 +1159,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
             float e = 0.f;
 #pragma unroll
             for (int z = 0; z < 16; ++z) {
-              const float y = __shfl(sc[z], r32 + 32 * (j >> 2 & 1), 64);
+              const float y = __shfl(pr.at(z), r32 + 32 * (j >> 2 & 1), 64);
               if ((j >> 3 & 3) == z / 4 && (j & 3) == z % 4) e = y;
               __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the common path)
             }
@@ -1135,7 +1169,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
               for (int z = 0; z < 16; ++z) {
                 const int r = 8 * (z / 4) + 4 * h + z % 4;
                 const float y = (float)from[Lanes == 32 ? r * E + m : (r & 15) * E + 2 * m + (r >> 4)];
-                o[m][z] += is && !(fabsf(y) < INFINITY) ? e * y : 0.f;
+                o[m][z] += is & !(fabsf(y) < INFINITY) ? e * y : 0.f;
                 if (z % 4 == 3) __builtin_amdgcn_sched_barrier(0);
               }
           }
