@@ -203,6 +203,7 @@ __device__ __forceinline__ Steps steps_of(const Cache& c, const Span& q, int use
 // lengths; every wave finds its own, its lanes sharing the sequences out.
 struct Part {
   int s, kvh, tile, piece, pieces, per;
+  int id;         // its number; neighbours read the same slots
   int64_t first;  // workgroups of the sequences before
 };
 // What the workgroups leave of a sequence for the joining launch.
@@ -211,7 +212,12 @@ struct Pieces {
   int count;
 };
 __device__ __forceinline__ int tiles_of(const Span& q, int tokens) { return (tokens * q.group + q.rows - 1) / q.rows; }
-__device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int64_t id) {
+// Workgroups go to the eight dies in turn, each with a cache of its own: `id` of `total` such that a die has a run of them.
+__device__ __forceinline__ int64_t by_die(int id, int64_t total) {
+  const int64_t run = (total + 7) / 8;
+  return id / 8 < run ? id % 8 * run + id / 8 : total;
+}
+__device__ bool part_of(Part& p, const Cache& c, const Span& q, int target) {
   const int lane = threadIdx.x & 63, each = (c.nSeq + 63) / 64;
   const int from = min(lane * each, c.nSeq), to = min(from + each, c.nSeq);
   auto steps = [&](int s, int tokens) { return steps_of(c, q, slots_used(c, s), 0, tokens - 1).total; };
@@ -237,6 +243,7 @@ __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int6
     const int64_t below = __shfl_up(upto, o, 64);
     if (lane >= o) upto += below;
   }
+  const int64_t id = by_die(blockIdx.x, __shfl(upto, 63, 64));
   const uint64_t has = __ballot(id < upto);
   if (has == 0) return false;
   const int owner = __builtin_ctzll(has);
@@ -247,6 +254,7 @@ __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target, int6
     p.first += here;
   }
   const int in_seq = (int)(id - p.first), n = new_tokens(q.count, p.s, q.T), tiles = tiles_of(q, n);
+  p.id = (int)id;
   p.piece = in_seq % p.pieces;
   p.tile = in_seq / p.pieces % tiles;
   p.kvh = in_seq / p.pieces / tiles;
@@ -493,13 +501,15 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Part p;
   if (part_ml) {
-    if (!part_of(p, c, span, target, blockIdx.x)) return;
-    if (p.first == blockIdx.x && threadIdx.x == 0) plan[p.s] = Pieces{p.first, p.pieces};
+    if (!part_of(p, c, span, target)) return;
+    if (p.first == p.id && threadIdx.x == 0) plan[p.s] = Pieces{p.first, p.pieces};
   } else {
     const int tiles = tiles_of(span, span.T);
+    p.id = blockIdx.x;
     p.tile = blockIdx.x % tiles;
     p.kvh = blockIdx.x / tiles % c.nKV;
     p.s = blockIdx.x / tiles / c.nKV;
+    if (p.s >= c.nSeq) return;
     p.piece = 0;
     p.pieces = 1;
     p.per = INT32_MAX;
@@ -725,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
         y += *reinterpret_cast<const f32x4*>(vals + (w * 16 + row) * kRow + d);
       }
       if (pieces > 1) {
-        const int64_t part = (int64_t)blockIdx.x * (16 * NT) + n * 16 + row;
+        const int64_t part = (int64_t)p.id * (16 * NT) + n * 16 + row;
         *reinterpret_cast<f32x4*>(part_o + part * DH + d) = y;
         if (d == 0) part_ml[part] = make_float2(most, all);
       } else {
@@ -906,18 +916,22 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Part p;
   if (part_ml) {
-    if (!part_of(p, c, span, target, blockIdx.x)) return;
-    if (p.first == blockIdx.x && threadIdx.x == 0) plan[p.s] = Pieces{p.first, p.pieces};
+    if (!part_of(p, c, span, target)) return;
+    if (p.first == p.id && threadIdx.x == 0) plan[p.s] = Pieces{p.first, p.pieces};
   } else {
     const int tiles = tiles_of(span, span.T);
-    p.tile = tiles - 1 - blockIdx.x % tiles;  // the longest first
-    p.kvh = blockIdx.x / tiles % c.nKV;
-    p.s = blockIdx.x / tiles / c.nKV;
+    const int64_t id = by_die(blockIdx.x, (int64_t)c.nSeq * c.nKV * tiles);
+    p.id = (int)id;
+    p.tile = tiles - 1 - p.id % tiles;  // the longest first
+    p.kvh = p.id / tiles % c.nKV;
+    p.s = p.id / tiles / c.nKV;
+    if (p.s >= c.nSeq) return;
     p.piece = 0;
     p.pieces = 1;
     p.per = INT32_MAX;
   }
   const int s = __builtin_amdgcn_readfirstlane(p.s), kvh = __builtin_amdgcn_readfirstlane(p.kvh);
+  const int part_id = __builtin_amdgcn_readfirstlane(p.id);
   const int row0 = __builtin_amdgcn_readfirstlane(p.tile) * kWideRows, pieces = __builtin_amdgcn_readfirstlane(p.pieces);
   const int tokens = new_tokens(span.count, s, span.T), rows = min(tokens * span.group - row0, kWideRows);
   if (rows <= 0) return;
@@ -1090,12 +1104,12 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
         return vt[Lanes == 32 ? (m * 8 + g8) * 32 + r32 : ((2 * m + (r32 >> 4)) * 8 + g8) * 16 + (r32 & 15)];
       };
       u32x4 ks[kAhead], vs[M];
+      int first = first_key(0);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) ks[k] = key_word(first, k);
 #pragma unroll
       for (int u = 0; u < Sub; ++u) {
         __builtin_amdgcn_sched_barrier(0);
-        const int first = first_key(u);
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) ks[k] = key_word(first, k);
         f32x16 sc;
 #pragma unroll
         for (int z = 0; z < 16; ++z) sc[z] = 0.f;
@@ -1145,6 +1159,11 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
         typename W::Probs pr;
         pr.take(sc);
         __builtin_amdgcn_sched_barrier(0);
+        if (u + 1 < Sub) {
+          first = first_key(u + 1);
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) ks[k] = key_word(first, k);
+        }
 #pragma unroll
         for (int i = 0; i < M * Z; ++i) {
           pr.sum(o[i % M], i / M, vs[i % M]);
@@ -1189,7 +1208,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   const int my_row = me & 31, my_h = me >> 5 & 1, at_row = row0 + 32 * wave + my_row;
   if (my_row >= mine) return;
   sum += __shfl_xor(sum, 32, 64);
-  const int64_t part = (int64_t)blockIdx.x * kWideRows + 32 * wave + my_row;
+  const int64_t part = (int64_t)part_id * kWideRows + 32 * wave + my_row;
   const float f = pieces > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
   const int my_t = at_row / span.group, my_head = kvh * span.group + (at_row - my_t * span.group);
   float* const to = pieces > 1 ? part_o + part * DH : out + (((int64_t)s * span.T + my_t) * nH + my_head) * DH;
@@ -1202,60 +1221,65 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   }
 }
 
-// A workgroup joins the pieces of R rows of a kv head: its threads share out quads of a row's
-// values, rows and (1 / sets of) the pieces.
+// A workgroup joins the pieces of R rows of a kv head, R <= kThreads / (DH / 4): its threads share out quads of a
+// row's values, the rows, and (a set of threads each) the pieces, four pieces in flight.
 template <int DH>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(Cache c, float* __restrict__ out, int nH, Span span, int R,
                                                               const Pieces* __restrict__ plan,
                                                               const float2* __restrict__ part_ml,
                                                               const float* __restrict__ part_o) {
-  constexpr int kQuads = DH / 4, kLanes = kThreads / kQuads;
+  constexpr int kQuads = DH / 4, kLanes = kThreads / kQuads, kAtOnce = 4;
   __shared__ f32x4 vals[kLanes][kQuads];
-  __shared__ float sums[kLanes];
+  __shared__ float2 mls[kLanes];
   const int blocks = (span.T * span.group + R - 1) / R;
   const int s = blockIdx.x / blocks / c.nKV, kvh = blockIdx.x / blocks % c.nKV, row0 = blockIdx.x % blocks * R;
   const Pieces p = plan[s];  // (of no tokens: whatever was there, and not used)
   const int tokens = new_tokens(span.count, s, span.T), rows = min(tokens * span.group - row0, R);
   if (rows <= 0 || p.count <= 1) return;
-  const int at_once = min(R, kLanes), sets = kLanes / at_once;  // rows at a time, threads that share one
-  const int lane = threadIdx.x / kQuads, quad = threadIdx.x - lane * kQuads, set = lane / at_once, tiles = tiles_of(span, tokens);
-  for (int r0 = 0; r0 < rows; r0 += at_once) {
-    const int mine = r0 + (lane - set * at_once), row = row0 + mine, tile = row / span.rows;
-    const bool on = lane < kLanes && set < sets && mine < rows;
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    float all = 0.f;
-    if (on) {
-      const int64_t first = (p.first + ((int64_t)kvh * tiles + tile) * p.count) * span.rows + (row - tile * span.rows);
-      float top = -INFINITY;
-      for (int x = 0; x < p.count; ++x) top = fmaxf(top, part_ml[first + (int64_t)x * span.rows].x);
-      for (int x = set; x < p.count; x += sets) {
-        const int64_t at = first + (int64_t)x * span.rows;
-        const float2 ml = part_ml[at];
-        const float f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
-        all += ml.y * f;
-        y += *reinterpret_cast<const f32x4*>(part_o + at * DH + 4 * quad) * f;
-      }
-    }
-    if (sets > 1) {
-      __syncthreads();
-      if (lane < kLanes) {
-        vals[lane][quad] = y;
-        if (quad == 0) sums[lane] = all;
-      }
-      __syncthreads();
-      for (int x = 1; x < sets && set == 0 && on; ++x) {
-        y += vals[lane + x * at_once][quad];
-        all += sums[lane + x * at_once];
-      }
-    }
-    if (on && set == 0) {
-      const int t = row / span.group, h = kvh * span.group + (row - t * span.group);
-      const float f = all == 0.f ? 0.f : 1.f / all;
-      float* to = out + (((int64_t)s * span.T + t) * nH + h) * DH + 4 * quad;
+  const int sets = kLanes / R, lane = threadIdx.x / kQuads, quad = threadIdx.x - lane * kQuads, set = lane / R;
+  const int mine = lane - set * R, row = row0 + mine, tile = row / span.rows;
+  const bool on = lane < kLanes && set < sets && mine < rows;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, all = 0.f;
+  // what a piece adds, its reference brought to the greatest so far
+  auto add = [&](float2 ml, f32x4 v) {
+    const float was = top;
+    top = fmaxf(top, ml.x);
+    const float keep = was == top ? 1.f : __builtin_amdgcn_exp2f(was - top), f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+    all = all * keep + ml.y * f;
+    y = y * keep + v * f;
+  };
+  if (on) {
+    const int64_t first = (p.first + ((int64_t)kvh * tiles_of(span, tokens) + tile) * p.count) * span.rows + (row - tile * span.rows);
+    for (int x0 = set; x0 < p.count; x0 += kAtOnce * sets) {
+      float2 ml[kAtOnce];
+      f32x4 v[kAtOnce];
 #pragma unroll
-      for (int z = 0; z < 4; ++z) to[z] = y[z] * f;
+      for (int z = 0; z < kAtOnce; ++z) {
+        const int64_t at = first + (int64_t)min(x0 + z * sets, p.count - 1) * span.rows;
+        ml[z] = part_ml[at];
+        v[z] = *reinterpret_cast<const f32x4*>(part_o + at * DH + 4 * quad);
+      }
+#pragma unroll
+      for (int z = 0; z < kAtOnce; ++z)
+        if (x0 + z * sets < p.count) add(ml[z], v[z]);
     }
   }
+  if (sets > 1) {
+    if (lane < kLanes) {
+      vals[lane][quad] = y;
+      if (quad == 0) mls[lane] = make_float2(top, all);
+    }
+    __syncthreads();
+    if (set == 0 && on)
+      for (int x = 1; x < sets; ++x) add(mls[lane + x * R], vals[lane + x * R][quad]);
+  }
+  if (!on || set != 0) return;
+  const int t = row / span.group, h = kvh * span.group + (row - t * span.group);
+  const float f = all == 0.f ? 0.f : 1.f / all;
+  float* to = out + (((int64_t)s * span.T + t) * nH + h) * DH + 4 * quad;
+#pragma unroll
+  for (int z = 0; z < 4; ++z) to[z] = y[z] * f;
 }
 
 // ── entry points' checks ──────────────────────────────────────────────────
@@ -1384,7 +1408,7 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   const int cus = fg::device_cu_count() > 0 ? fg::device_cu_count() : 256;
   const int target = 2 * cus;
   const bool whole = rounds <= 4 || heads >= 4 * target;
-  const int64_t grid = whole ? heads : heads + target;
+  const int64_t grid = (whole ? heads : heads + target) + 8;  // (by_die: a die's run may end beyond the last)
   fg::Workspace ws;
   float2* part_ml = nullptr;
   float* part_o = nullptr;
@@ -1396,7 +1420,7 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
     part_o = (float*)ws.ptr;
     part_ml = (float2*)(part_o + rows * c->dHead);
     plan = (Pieces*)(part_ml + rows);
-    while (R < 16 && items / R > 4 * cus) R *= 2;
+    while (2 * R <= kThreads / (c->dHead / 4) && items / R > 4 * cus) R *= 2;
   }
   const int64_t joins = (int64_t)c->nSeq * c->nKvHeads * ((all + R - 1) / R);
   const float factor = (float)(scale * M_LOG2E);
