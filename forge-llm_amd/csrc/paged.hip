@@ -220,23 +220,37 @@ __device__ __forceinline__ int64_t by_die(int id, int64_t total) {
 __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target) {
   const int lane = threadIdx.x & 63, each = (c.nSeq + 63) / 64;
   const int from = min(lane * each, c.nSeq), to = min(from + each, c.nSeq);
-  auto steps = [&](int s, int tokens) { return steps_of(c, q, slots_used(c, s), 0, tokens - 1).total; };
-  int64_t work = 0;
-  for (int s = from; s < to; ++s) {
-    const int n = new_tokens(q.count, s, q.T);
-    if (n > 0) work += (int64_t)steps(s, n) * tiles_of(q, n);
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
-  const int64_t per = (work * c.nKV + target - 1) / target;
-  p.per = ((int)min(max(per, (int64_t)1), (int64_t)1 << 28) + q.waves - 1) / q.waves * q.waves;
-  auto groups = [&](int s, int& pieces) -> int64_t {
-    const int n = new_tokens(q.count, s, q.T);
-    pieces = n > 0 ? (steps(s, n) + p.per - 1) / p.per : 0;
-    return (int64_t)pieces * tiles_of(q, n) * c.nKV;
+  struct Load {
+    int steps, tiles;
   };
-  int64_t mine = 0;
-  for (int s = from, pieces; s < to; ++s) mine += groups(s, pieces);
+  auto load = [&](int s) {
+    const int n = new_tokens(q.count, s, q.T);
+    return n > 0 ? Load{steps_of(c, q, slots_used(c, s), 0, n - 1).total, tiles_of(q, n)} : Load{0, 0};
+  };
+  const Load first = from < to ? load(from) : Load{0, 0};  // (of up to 64 sequences there are no others)
+  auto sum = [&](auto what) {
+    int64_t all = from < to ? what(first) : 0;
+    for (int s = from + 1; s < to; ++s) all += what(load(s));
+    return all;
+  };
+  auto of_wave = [](int64_t x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    return x;
+  };
+  const int64_t work = of_wave(sum([](Load l) { return (int64_t)l.steps * l.tiles; })) * c.nKV;
+  // The fewest steps that keep the workgroups, of which the last of each sequence's has fewer, to `target`: all of
+  // them at once.  (A few left over for a second round: 16 sequences up to 8192 82 us, 61 so.)
+  int64_t per = max((work + target - 1) / target, (int64_t)1), mine;
+  auto pieces = [&](Load l) { return l.steps ? (l.steps + p.per - 1) / p.per : 0; };
+  for (int turn = 0;; ++turn) {
+    p.per = ((int)min(per, (int64_t)1 << 28) + q.waves - 1) / q.waves * q.waves;
+    mine = sum([&](Load l) { return (int64_t)pieces(l) * l.tiles; }) * c.nKV;
+    if (turn == 6) break;
+    const int64_t all = of_wave(mine);
+    if (all <= target || p.per >= 1 << 28) break;
+    per = max(p.per * all / target, (int64_t)p.per + 1);
+  }
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -249,7 +263,9 @@ __device__ bool part_of(Part& p, const Cache& c, const Span& q, int target) {
   const int owner = __builtin_ctzll(has);
   p.first = __shfl(upto - mine, owner, 64);
   for (p.s = owner * each;; ++p.s) {
-    const int64_t here = groups(p.s, p.pieces);
+    const Load l = load(p.s);
+    p.pieces = pieces(l);
+    const int64_t here = (int64_t)p.pieces * l.tiles * c.nKV;
     if (id < p.first + here) break;
     p.first += here;
   }
@@ -686,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float y = (float)from[(m / E) * 16 * E + (4 * g + r) * E + m % E];
-              o[n][m][r] += is & !(fabsf(y) < INFINITY) ? e * y : 0.f;
+              o[n][m][r] += (is & !(fabsf(y) < INFINITY)) ? e * y : 0.f;
               if (r == 3) __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -922,7 +938,10 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     const int tiles = tiles_of(span, span.T);
     const int64_t id = by_die(blockIdx.x, (int64_t)c.nSeq * c.nKV * tiles);
     p.id = (int)id;
-    p.tile = tiles - 1 - p.id % tiles;  // the longest first
+    // the longest first, and beside them, as the second of a CU, the shortest: 2048 tokens of 8 heads, none before them,
+    // 105 us (cut into equal pieces 139)
+    const int at = p.id % tiles, half = (tiles + 1) / 2;
+    p.tile = at < half ? tiles - 1 - at : at - half;
     p.kvh = p.id / tiles % c.nKV;
     p.s = p.id / tiles / c.nKV;
     if (p.s >= c.nSeq) return;
@@ -1188,7 +1207,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
               for (int z = 0; z < 16; ++z) {
                 const int r = 8 * (z / 4) + 4 * h + z % 4;
                 const float y = (float)from[Lanes == 32 ? r * E + m : (r & 15) * E + 2 * m + (r >> 4)];
-                o[m][z] += is & !(fabsf(y) < INFINITY) ? e * y : 0.f;
+                o[m][z] += (is & !(fabsf(y) < INFINITY)) ? e * y : 0.f;
                 if (z % 4 == 3) __builtin_amdgcn_sched_barrier(0);
               }
           }
@@ -1396,7 +1415,13 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   if (T == 0) return FG_OK;
   fg::KProfScope prof("paged_attn", 0.0, (double)c->nSeq * c->maxPages * c->pageSize * 2 * row_bytes(c));
   const int group = nHeads / c->nKvHeads, all = T * group;
-  const bool wide = all > 64;
+  // Many rows share steps through LDS, few take them in registers.  us, shared against registers:
+  //   fp16  24 rows of 128, 8 sequences of 8000   64  53     48 rows   76  95     96 rows   86 154
+  //         24 rows of 64                        104  48     48 rows  109 122     96 rows  115 189
+  //   fp32  48 rows of 128, 8 sequences of 8000  289 212     64 rows  290 215     96 rows  293 382
+  //         48 rows of 64                        252 241     64 rows  253 231     96 rows  337 360
+  // Heads of 256 leave a wave of 32 rows no registers: 256 rows 116 (two tiles of 16: 65), 1024 rows 261 (152).
+  const bool wide = c->dHead < 256 && all > (c->type ? 32 : 64);
   const int tiles = all <= 16 ? 1 : all <= 32 || c->dHead == 256 ? 2 : 4;
   const Span span{T, group, wide ? kWideRows : 16 * tiles, window, sinks, (c->type ? 32 : 16) * (wide ? 2 : 1),
                   wide ? 1 : kWaves, count};
@@ -1405,10 +1430,28 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   int64_t seen = room;  // by a workgroup's rows, at most
   if (window > 0 && (int64_t)window + T + sinks + 2 * span.keys < room) seen = (int64_t)window + T + sinks + 2 * span.keys;
   const int64_t rounds = (seen + span.keys * span.waves - 1) / (span.keys * span.waves);
+  // Workgroups that the chip holds at once, and, where a workgroup's time is mostly its reads, as many of them as give
+  // every head two.
   const int cus = fg::device_cu_count() > 0 ? fg::device_cu_count() : 256;
-  const int target = 2 * cus;
-  const bool whole = rounds <= 4 || heads >= 4 * target;
+  const int64_t held = (int64_t)cus * (wide || (tiles < 4 && c->dHead < 256) ? 2 : 1);
+  const int64_t target = wide ? held : held * ((2 * heads + held - 1) / held);
+  // Short caches, of more slots where there are heads enough to fill the chip: a workgroup a head and tile, no second
+  // launch.  A round of it takes about 0.6 us and 0.07 for each KB that a wave reads; pieces and their joining take
+  // 6 us more than a round.  us, a workgroup a head against pieces:
+  //                        up to the limit              beyond it
+  //    8 heads of 128 fp16   512: 12.0 12.0              1024: 19.1 12.1
+  //    8 heads of 64 fp16    512:  9.2 11.2              1024: 14.3 11.0
+  //    4 heads of 32 fp32    512: 10.3 11.2              1024: 17.5 11.3
+  //   48 heads of 64 fp32    256:  8.4 11.2               512: 12.4 12.5
+  //    4 heads of 256 fp16   256: 12.1 14.1               512: 18.8 14.3
+  //    8 heads, 20 rows      256: 12.4 15.4               512: 17.5 15.5
+  //  256 heads of 32 fp32   1024: 23.6 25.3              2048: 42.8 36.6
+  //  512 heads of 128 fp16  2048: 95.5 99.5
+  const int64_t kb = span.keys * c->dHead * (c->type ? 2 : 4) * 2 / 1024;
+  const int64_t limit = (wide ? 2 : tiles > 1 ? 64 / (8 + kb) : 98 / (8 + kb)) * (heads >= cus ? 4 : 1);
+  const bool whole = rounds <= (limit > 1 ? limit : 1) || heads >= (wide ? held : 4 * held);
   const int64_t grid = (whole ? heads : heads + target) + 8;  // (by_die: a die's run may end beyond the last)
+  FG_ARG_CHECK(grid <= INT32_MAX / kThreads, "%s: %d sequences x %d tokens x %d heads are too many", fn, c->nSeq, T, nHeads);
   fg::Workspace ws;
   float2* part_ml = nullptr;
   float* part_o = nullptr;
@@ -1427,21 +1470,32 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   const Cache cache = view(c);
 #define PAGED_ATTN(KV, DH, NT)                                                                                        \
   FG_LAUNCH((paged_attn_kernel<KV, DH, NT>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q, nHeads,   \
-            factor, span, target, plan, part_ml, part_o)
-#define PAGED_TILES(KV, DH)                          \
-  if (wide)                                          \
-    FG_LAUNCH((paged_wide_kernel<KV, DH>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q, nHeads,     \
-              factor, span, target, plan, part_ml, part_o);                                                          \
-  else if (tiles == 1) PAGED_ATTN(KV, DH, 1);             \
-  else if (tiles == 2) PAGED_ATTN(KV, DH, 2);        \
-  else PAGED_ATTN(KV, (DH == 256 ? 128 : DH), 4) /* heads of 256 have no tiles of 4 */
+            factor, span, (int)target, plan, part_ml, part_o)
+#define PAGED_TILES(KV, DH)                                                                                           \
+  if constexpr (DH < 256) {                                                                                           \
+    if (wide) {                                                                                                       \
+      FG_LAUNCH((paged_wide_kernel<KV, DH>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q, nHeads,   \
+                factor, span, (int)target, plan, part_ml, part_o);                                                    \
+      break;                                                                                                          \
+    }                                                                                                                 \
+    if constexpr (sizeof(KV) == 4) { /* fp16 rows beyond two tiles are wide */                                        \
+      if (tiles == 4) {                                                                                               \
+        PAGED_ATTN(KV, DH, 4);                                                                                        \
+        break;                                                                                                        \
+      }                                                                                                               \
+    }                                                                                                                 \
+  }                                                                                                                   \
+  if (tiles == 1) PAGED_ATTN(KV, DH, 1);                                                                              \
+  else PAGED_ATTN(KV, DH, 2)
 #define PAGED_HEAD(DH)                               \
   do {                                               \
-    if (c->type == 0) {                              \
-      PAGED_TILES(float, DH);                        \
-    } else {                                         \
-      PAGED_TILES(_Float16, DH);                     \
-    }                                                \
+    do {                                             \
+      if (c->type == 0) {                            \
+        PAGED_TILES(float, DH);                      \
+      } else {                                       \
+        PAGED_TILES(_Float16, DH);                   \
+      }                                              \
+    } while (0);                                     \
     if (!whole)                                      \
       FG_LAUNCH(paged_join_kernel<DH>, dim3((unsigned)joins), dim3(kThreads), 0, cache, out, nHeads, span, R, \
                 (const Pieces*)plan, (const float2*)part_ml, (const float*)part_o);                          \
