@@ -93,6 +93,8 @@ int check_kv4_cache(const fg_kv4_cache* c, const char* fn);
 // that attends to what is stored).
 int kv4_attn(const fg_kv4_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
              const int32_t* count, bool only_new);
+// What every entry point over a paged cache checks of it.
+int check_paged_cache(const fg_paged_cache* c, const char* fn);
 
 }  // namespace fg
 

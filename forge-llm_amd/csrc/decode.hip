@@ -1202,6 +1202,34 @@ __global__ void kv4_states_kernel(int32_t* __restrict__ state, int32_t* __restri
   count[s] = on;
 }
 
+// T tokens a sequence of a paged cache: {token, position} of each row, and how many of a
+// sequence's count[s] (NULL: T) take part: the first ones of them that are tokens of the vocabulary at
+// positions of the RoPE table with a page to go to.  The other rows' are {-1, 0}.  A wave takes a sequence.
+__global__ void __launch_bounds__(64) paged_states_kernel(int32_t* __restrict__ state, int32_t* __restrict__ taken,
+                                                          const int32_t* __restrict__ tokens,
+                                                          const int32_t* __restrict__ count, fg_paged_cache c, int T,
+                                                          int V, int maxPos) {
+  const int s = blockIdx.x, lane = threadIdx.x, room = c.maxPages * c.pageSize;
+  const int n = count ? min(max(count[s], 0), T) : T, len = min(max(c.len[s], 0), room);
+  int first = n;  // that does not take part
+  for (int t0 = 0; t0 < T; t0 += 64) {
+    const int t = t0 + lane;
+    const int64_t row = (int64_t)s * T + t, pos = (int64_t)len + t;
+    int token = -1;
+    if (t < first && pos < room && pos < maxPos) {
+      const int page = c.table[(int64_t)s * c.maxPages + pos / c.pageSize];
+      if (page >= 0 && page < c.nPages) token = tokens[row];
+    }
+    const uint64_t out = __ballot(t < first && (token < 0 || token >= V));
+    if (out) first = t0 + __builtin_ctzll(out);
+    if (t < T) {
+      state[2 * row] = t < first ? token : -1;
+      state[2 * row + 1] = t < first ? (int)pos : 0;
+    }
+  }
+  if (lane == 0) taken[s] = first;
+}
+
 template <int LP, int C = 1>
 int launch_attn(const fg_decode_model* m, float* kcache, float* vcache, const int32_t* state, int dH,
                 int64_t layer_off, double scale, int S) {
@@ -1347,6 +1375,57 @@ extern "C" int fg_decode_step_kv4(const fg_decode_model* m, const fg_kv4_cache* 
   rc = step_head(st, logits, m->x, N);
   if (rc) return rc;
   return fg_kv4_commit(c, 1, count);
+}
+
+extern "C" int fg_decode_step_paged(const fg_decode_model* m, const fg_paged_cache* c, const int32_t* tokens, int T,
+                                    const int32_t* count, int window, int sinks, int commit, float* logits) {
+  const char* fn = "fg_decode_step_paged";
+  FG_ARG_CHECK(tokens && logits, "%s: null argument", fn);
+  Step st;
+  double wbytes;
+  int rc = check_model(m, fn, st, wbytes);
+  if (rc) return rc;
+  rc = fg::check_paged_cache(c, fn);
+  if (rc) return rc;
+  FG_ARG_CHECK(c->nLayers == m->nLayers && c->nKvHeads == m->nKvHeads && c->dHead == st.dH,
+               "%s: a cache of %d layers, %d kv heads of %d for a model of %d, %d of %d", fn, c->nLayers, c->nKvHeads,
+               c->dHead, m->nLayers, m->nKvHeads, st.dH);
+  FG_ARG_CHECK(T > 0 && (int64_t)c->nSeq * T <= 65535, "%s: %d sequences x %d tokens: 1 to 65535 in all", fn, c->nSeq, T);
+  FG_ARG_CHECK(window >= 0 && sinks >= 0, "%s: window %d, sinks %d", fn, window, sinks);
+  const int D = st.D, kvD = st.kvD, N = c->nSeq * T;
+  FG_ARG_CHECK(st.lds_qkv <= 64 * 1024 && (size_t)st.H * sizeof(float) <= 64 * 1024,
+               "%s: dim %d / hidden %d exceed the 64 KiB LDS of a launch", fn, D, st.H);
+  FG_REQUIRE_INIT();
+  fg::KProfScope prof("decode_step_paged", 0.0, wbytes);
+  st.vec = aligned16(m->x) && aligned16(m->q) && aligned16(m->h) && aligned16(m->tok_emb) && aligned16(m->ln_f) &&
+           D % 4 == 0 && st.H % 4 == 0;
+  // new keys and values, attention, states, and how many tokens of a sequence take part
+  fg::Workspace ws;
+  rc = ws.get((size_t)N * ((2 * (size_t)kvD + D) * sizeof(float) + 2 * sizeof(int32_t)) + c->nSeq * sizeof(int32_t));
+  if (rc) return rc;
+  float *k = (float*)ws.ptr, *v = k + (int64_t)N * kvD, *att = v + (int64_t)N * kvD;
+  int32_t *state = (int32_t*)(att + (int64_t)N * D), *taken = state + 2 * (int64_t)N;
+  FG_LAUNCH(paged_states_kernel, dim3(c->nSeq), dim3(64), 0, state, taken, tokens, count, *c, T, st.V, m->maxSeq);
+  rc = step_embed(st, m->x, state, N);
+  if (rc) return rc;
+  for (int l = 0; l < m->nLayers; ++l) {
+    const fg_decode_layer& ly = m->layers[l];
+    rc = step_qkv(st, l, m->x, m->q, k, v, state, 0, 0, N);
+    if (rc) return rc;
+    // (turned already, by the model's table)
+    rc = fg_paged_append(c, l, nullptr, nullptr, k, v, kvD, 0, T, taken, nullptr, nullptr, 0, 0, 0);
+    if (rc) return rc;
+    // (rows that take no part are NaN from the embedding on, whatever is in their place here)
+    rc = fg_paged_attn(c, l, att, m->q, st.nH, 1.0 / sqrt((double)st.dH), T, taken, window, sinks);
+    if (rc) return rc;
+    rc = step_residual(st, kWoCombined, m->x, att, ly.wo, ly.wo_type, D, D, N);
+    if (rc) return rc;
+    rc = step_ffn(st, l, m->x, m->h, N);
+    if (rc) return rc;
+  }
+  rc = step_head(st, logits, m->x, N);
+  if (rc) return rc;
+  return commit ? fg_paged_commit(c, T, taken) : FG_OK;
 }
 
 extern "C" int fg_decode_part_len(int nHeads, int dHead, int maxSeq, int64_t* doubles) {

@@ -1153,6 +1153,83 @@ FN(js_beam_select) {
                       a.i32(10), a.i32(11)), "fg_beam_select");
 }
 
+// ── paged cache and drafted tokens ──────────────────────────────────────
+constexpr uint32_t kPagedTag = 0x46475047u;  // paged cache
+struct PagedHolder {
+  uint32_t tag;
+  fg_paged_cache c;
+};
+void paged_finalize(napi_env, void* data, void*) { delete static_cast<PagedHolder*>(data); }
+const fg_paged_cache* paged_of(Args& a, size_t i) {
+  void* d = nullptr;
+  if (napi_get_value_external(a.env, a.argv[i], &d) != napi_ok || !d || static_cast<PagedHolder*>(d)->tag != kPagedTag) {
+    a.ok = false;
+    throw_err(a.env, "expected a paged cache handle");
+    return nullptr;
+  }
+  return &static_cast<PagedHolder*>(d)->c;
+}
+// pagedCache(nLayers, nSeq, nKvHeads, dHead, pageSize, nPages, maxPages, type, k, v, table, len) -> handle
+// (the caller keeps the buffers for as long as the handle is used)
+FN(js_paged_cache) {
+  Args a(env, info, 12);
+  if (!a.ok) return nullptr;
+  PagedHolder* h = new PagedHolder();
+  h->tag = kPagedTag;
+  h->c = {a.i32(0), a.i32(1), a.i32(2), a.i32(3), a.i32(4), a.i32(5), a.i32(6), a.i32(7),
+          a.ptr(8), a.ptr(9), a.i32p(10), a.i32p(11)};
+  napi_value ext;
+  if (!a.ok || napi_create_external(env, h, paged_finalize, nullptr, &ext) != napi_ok) {
+    delete h;
+    return a.ok ? throw_err(env, "napi_create_external failed") : nullptr;
+  }
+  return ext;
+}
+// pagedAppend(cache, layer, qOut|null, q|null, k, v, ld, nHeads, T, count|null, cos|null, sin|null, npos, rot, half)
+FN(js_paged_append) {
+  Args a(env, info, 15);
+  if (!a.ok) return nullptr;
+  const fg_paged_cache* c = paged_of(a, 0);
+  CALL(fg_paged_append(c, a.i32(1), a.f(2), a.f(3), a.f(4), a.f(5), a.i64(6), a.i32(7), a.i32(8), a.i32p(9), a.dp(10),
+                       a.dp(11), a.i32(12), a.i32(13), a.i32(14)), "fg_paged_append");
+}
+FN(js_paged_read) {  // pagedRead(cache, layer, k, v, ld, first, T)
+  Args a(env, info, 7);
+  if (!a.ok) return nullptr;
+  const fg_paged_cache* c = paged_of(a, 0);
+  CALL(fg_paged_read(c, a.i32(1), a.f(2), a.f(3), a.i64(4), a.i32(5), a.i32(6)), "fg_paged_read");
+}
+FN(js_paged_attn) {  // pagedAttn(cache, layer, out, q, nHeads, scale, T, count|null, window, sinks)
+  Args a(env, info, 10);
+  if (!a.ok) return nullptr;
+  const fg_paged_cache* c = paged_of(a, 0);
+  CALL(fg_paged_attn(c, a.i32(1), a.f(2), a.f(3), a.i32(4), a.f64(5), a.i32(6), a.i32p(7), a.i32(8), a.i32(9)),
+       "fg_paged_attn");
+}
+FN(js_paged_commit) {  // pagedCommit(cache, T, count|null)
+  Args a(env, info, 3);
+  if (!a.ok) return nullptr;
+  const fg_paged_cache* c = paged_of(a, 0);
+  CALL(fg_paged_commit(c, a.i32(1), a.i32p(2)), "fg_paged_commit");
+}
+// decodeStepPaged(model, cache, tokens, T, count|null, window, sinks, commit, logits)
+FN(js_decode_step_paged) {
+  Args a(env, info, 9);
+  if (!a.ok) return nullptr;
+  const fg_decode_model* m = model_of(a, 0);
+  if (!a.ok) return nullptr;
+  const fg_paged_cache* c = paged_of(a, 1);
+  CALL(fg_decode_step_paged(m, c, a.i32p(2), a.i32(3), a.i32p(4), a.i32(5), a.i32(6), a.i32(7), a.f(8)),
+       "fg_decode_step_paged");
+}
+// draftVerify(token, count, logits, ld, draftLogits|null, ldDraft, draft|null, drafted|null, u|null, temperature, nSeq, D, V)
+FN(js_draft_verify) {
+  Args a(env, info, 13);
+  if (!a.ok) return nullptr;
+  CALL(fg_draft_verify(a.i32p(0), a.i32p(1), a.f(2), a.i64(3), a.f(4), a.i64(5), a.i32p(6), a.i32p(7), a.f(8), a.f64(9),
+                       a.i32(10), a.i32(11), a.i32(12)), "fg_draft_verify");
+}
+
 napi_value Init(napi_env env, napi_value exports) {
   struct {
     const char* name;
@@ -1194,6 +1271,9 @@ napi_value Init(napi_env env, napi_value exports) {
       {"kv4Cache", js_kv4_cache}, {"kv4Append", js_kv4_append}, {"kv4Read", js_kv4_read}, {"kv4Attn", js_kv4_attn},
       {"kv4Commit", js_kv4_commit}, {"kv4Evict", js_kv4_evict}, {"kv4Reorder", js_kv4_reorder},
       {"decodeStepKv4", js_decode_step_kv4}, {"beamSelect", js_beam_select},
+      {"pagedCache", js_paged_cache}, {"pagedAppend", js_paged_append}, {"pagedRead", js_paged_read},
+      {"pagedAttn", js_paged_attn}, {"pagedCommit", js_paged_commit}, {"decodeStepPaged", js_decode_step_paged},
+      {"draftVerify", js_draft_verify},
   };
   for (auto& f : fns) {
     napi_value fn;

@@ -1303,7 +1303,20 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(Cache c, float* __
 
 // ── entry points' checks ──────────────────────────────────────────────────
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-int check_cache(const fg_paged_cache* c, const char* fn) {
+int check_step(const fg_paged_cache* c, int layer, int T, const char* fn) {
+  FG_ARG_CHECK(layer >= 0 && layer < c->nLayers, "%s: layer %d outside [0, %d)", fn, layer, c->nLayers);
+  FG_ARG_CHECK(T >= 0, "%s: T %d is negative", fn, T);
+  FG_ARG_CHECK((int64_t)c->nSeq * T <= INT32_MAX / kThreads, "%s: %d sequences x %d tokens are too many", fn, c->nSeq, T);
+  return FG_OK;
+}
+Cache view(const fg_paged_cache* c) {
+  return {c->nSeq, c->nKvHeads, __builtin_ctz(c->pageSize), c->nPages, c->maxPages, c->k, c->v, c->table, c->len};
+}
+double row_bytes(const fg_paged_cache* c) { return (double)c->nKvHeads * c->dHead * (c->type ? 2 : 4); }
+
+}  // namespace
+
+int fg::check_paged_cache(const fg_paged_cache* c, const char* fn) {
   FG_ARG_CHECK(c, "%s: null cache", fn);
   FG_ARG_CHECK(c->nLayers > 0 && c->nSeq > 0 && c->nKvHeads > 0 && c->nPages > 0 && c->maxPages > 0,
                "%s: bad dimensions: %d layers, %d sequences, %d kv heads, %d pages, %d a sequence", fn, c->nLayers,
@@ -1321,18 +1334,6 @@ int check_cache(const fg_paged_cache* c, const char* fn) {
   FG_ARG_CHECK(aligned16(c->k) && aligned16(c->v), "%s: the cache's pages must be 16-byte aligned", fn);
   return FG_OK;
 }
-int check_step(const fg_paged_cache* c, int layer, int T, const char* fn) {
-  FG_ARG_CHECK(layer >= 0 && layer < c->nLayers, "%s: layer %d outside [0, %d)", fn, layer, c->nLayers);
-  FG_ARG_CHECK(T >= 0, "%s: T %d is negative", fn, T);
-  FG_ARG_CHECK((int64_t)c->nSeq * T <= INT32_MAX / kThreads, "%s: %d sequences x %d tokens are too many", fn, c->nSeq, T);
-  return FG_OK;
-}
-Cache view(const fg_paged_cache* c) {
-  return {c->nSeq, c->nKvHeads, __builtin_ctz(c->pageSize), c->nPages, c->maxPages, c->k, c->v, c->table, c->len};
-}
-double row_bytes(const fg_paged_cache* c) { return (double)c->nKvHeads * c->dHead * (c->type ? 2 : 4); }
-
-}  // namespace
 
 #define PAGED_TRY(expr)               \
   do {                                \
@@ -1344,7 +1345,7 @@ extern "C" int fg_paged_append(const fg_paged_cache* c, int layer, float* q_out,
                                const float* v, int64_t ld, int nHeads, int T, const int32_t* count,
                                const double* cos_tab, const double* sin_tab, int npos, int rot, int half) {
   const char* fn = "fg_paged_append";
-  PAGED_TRY(check_cache(c, fn));
+  PAGED_TRY(fg::check_paged_cache(c, fn));
   PAGED_TRY(check_step(c, layer, T, fn));
   FG_ARG_CHECK(T == 0 || (k && v), "%s: null argument", fn);
   FG_ARG_CHECK(!q == !q_out, "%s: q and q_out are given together", fn);
@@ -1375,7 +1376,7 @@ extern "C" int fg_paged_append(const fg_paged_cache* c, int layer, float* q_out,
 
 extern "C" int fg_paged_read(const fg_paged_cache* c, int layer, float* k, float* v, int64_t ld, int first, int T) {
   const char* fn = "fg_paged_read";
-  PAGED_TRY(check_cache(c, fn));
+  PAGED_TRY(fg::check_paged_cache(c, fn));
   PAGED_TRY(check_step(c, layer, T, fn));
   FG_ARG_CHECK(first >= 0 && (int64_t)first + T <= (int64_t)c->maxPages * c->pageSize,
                "%s: slots [%d, %lld) outside [0, %lld)", fn, first, (long long)first + T,
@@ -1404,7 +1405,7 @@ extern "C" int fg_paged_read(const fg_paged_cache* c, int layer, float* k, float
 extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, const float* q, int nHeads, double scale,
                              int T, const int32_t* count, int window, int sinks) {
   const char* fn = "fg_paged_attn";
-  PAGED_TRY(check_cache(c, fn));
+  PAGED_TRY(fg::check_paged_cache(c, fn));
   PAGED_TRY(check_step(c, layer, T, fn));
   FG_ARG_CHECK(T == 0 || (out && q), "%s: null argument", fn);
   FG_ARG_CHECK(nHeads > 0 && nHeads % c->nKvHeads == 0, "%s: %d query heads for %d kv heads", fn, nHeads, c->nKvHeads);
@@ -1511,7 +1512,7 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
 }
 
 extern "C" int fg_paged_commit(const fg_paged_cache* c, int T, const int32_t* count) {
-  PAGED_TRY(check_cache(c, "fg_paged_commit"));
+  PAGED_TRY(fg::check_paged_cache(c, "fg_paged_commit"));
   FG_ARG_CHECK(T >= 0, "fg_paged_commit: T %d is negative", T);
   FG_REQUIRE_INIT();
   if (T == 0) return FG_OK;

@@ -6,6 +6,7 @@
  */
 import { hip } from "../L2/device.js";
 import { KVCache, KV4Cache } from "../L5/attention.js";
+import { PagedKVCache } from "../L5/paged.js";
 import { info, rowBytes } from "../L3/quant.js";
 
 function pick(o, k, d) { return o[k] === undefined || o[k] === null ? d : o[k]; }
@@ -100,7 +101,8 @@ const GRAPHS_KEPT = 4;
  * this package's device KVCache, or its KV4Cache: `forward` takes one of one
  * sequence, at the sequence's next position, `forwardAll(tokens, cache)` one token
  * of every sequence (fg_decode_step_kv4).  Recorded steps are kept for the last four
- * caches of each kind.
+ * caches of each kind.  `forwardChunk(tokens, cache)` takes several tokens of every
+ * sequence of a PagedKVCache in one step (fg_decode_step_paged), op by op.
  */
 export class Transformer {
   constructor(config, opts = {}) {
@@ -109,7 +111,7 @@ export class Transformer {
     const c = this.cfg;
     if (c.dim % c.nHeads !== 0) throw new Error(`Transformer: dim ${c.dim} must be a multiple of nHeads ${c.nHeads}`);
     this.logits = new Float32Array(c.vocabSize);
-    this._w = null; this._model = null; this._graphs = []; this._kv4 = [];
+    this._w = null; this._model = null; this._graphs = []; this._kv4 = []; this._paged = [];
   }
 
   loadWeights(w) {
@@ -208,6 +210,87 @@ export class Transformer {
       for (const h of e.bufs) a.free(h);
     }
     this._kv4 = this._kv4.filter((e) => cache && e.cache !== cache);
+  }
+
+  // The model over the vectors of `rows` tokens for a paged cache, kept for the last GRAPHS_KEPT caches used.
+  _pagedFor(cache, rows) {
+    const c = this.cfg, W = this._w, a = hip();
+    const known = this._paged.findIndex((e) => e.cache === cache);
+    if (known >= 0 && this._paged[known].rows >= rows) {
+      this._paged.push(this._paged.splice(known, 1)[0]);
+      return this._paged[this._paged.length - 1];
+    }
+    this._dropPaged(cache);
+    for (const e of this._paged.slice()) if (e.cache.freed) this._dropPaged(e.cache);
+    while (this._paged.length >= GRAPHS_KEPT) this._dropPaged(this._paged[0].cache);
+    const bufs = [];
+    const scratch = (n) => { const h = a.alloc(n * 4); bufs.push(h); return h; };
+    try {
+      const x = scratch(rows * c.dim);
+      const model = a.decodeModel({
+        dim: c.dim, hidden: c.hidden, nLayers: c.nLayers, nHeads: c.nHeads, nKvHeads: c.nKvHeads,
+        vocab: c.vocabSize, maxSeq: c.maxSeq, normEps: c.normEps, tok_emb: W.tok, ln_f: W.ln_f, wcls: W.wcls,
+        emb_type: W.emb_type, cls_type: W.cls_type,
+        rope_cos: W.rope_cos, rope_sin: W.rope_sin, x, q: scratch(rows * c.dim), h: scratch(rows * c.hidden), attn_part: x,
+        layers: W.layers,
+      });
+      const e = { cache, rows, model, bufs, tokens: scratch(rows), count: scratch(cache.sequences), logits: scratch(rows * c.vocabSize) };
+      this._paged.push(e);
+      return e;
+    } catch (err) {
+      for (const h of bufs) a.free(h);
+      throw err;
+    }
+  }
+  // Of one cache, or of all.
+  _dropPaged(cache) {
+    const a = hip();
+    for (const e of this._paged)
+      if (!cache || e.cache === cache) for (const h of e.bufs) a.free(h);
+    this._paged = this._paged.filter((e) => cache && e.cache !== cache);
+  }
+
+  /** Queues tokens[s] (arrays) of every sequence of a paged cache; rows [sequences][T] of logits stay in device
+   *  memory (`logits` of what it returns), T being the most tokens of a sequence. */
+  _chunk(tokens, cache, opts = {}) {
+    const c = this.cfg, a = hip(), { window = 0, sinks = 0, commit = true } = opts;
+    if (!this._w) throw new Error("Transformer.forwardChunk: call loadWeights first");
+    if (!(cache instanceof PagedKVCache)) throw new TypeError("Transformer.forwardChunk: cache must be a PagedKVCache");
+    const handle = cache.handle, S = cache.sequences;
+    if (cache.nLayers !== c.nLayers || cache.nKvHeads !== c.nKvHeads || cache.dHead !== c.dHead)
+      throw new RangeError("Transformer.forwardChunk: cache shape does not match the Config");
+    if (!tokens || tokens.length !== S || !Array.from(tokens).every((t) => t && t.length !== undefined))
+      throw new RangeError(`Transformer.forwardChunk: tokens of ${S} sequences expected`);
+    for (const [k, v] of [["window", window], ["sinks", sinks]])
+      if (!Number.isInteger(v) || v < 0 || v > 0x7FFFFFFF) throw new RangeError(`Transformer.forwardChunk: ${k} ${v}`);
+    const counts = Int32Array.from(tokens, (t) => t.length), T = Math.max.apply(null, Array.from(counts));
+    if (T < 1 || S * T > 65535) throw new RangeError(`Transformer.forwardChunk: ${S} sequences of ${T} tokens`);
+    const ids = new Int32Array(S * T).fill(-1);
+    for (let s = 0; s < S; s++) {
+      for (let t = 0; t < counts[s]; t++) {
+        const id = tokens[s][t];
+        if (!(Number.isInteger(id) && id >= 0 && id < c.vocabSize)) throw new RangeError(`Transformer.forwardChunk: token ${id}`);
+        ids[s * T + t] = id;
+      }
+      if (cache.lens[s] + counts[s] > c.maxSeq) throw new RangeError(`Transformer.forwardChunk: sequence ${s} runs past position ${c.maxSeq}`);
+    }
+    cache.reserve(counts);
+    const e = this._pagedFor(cache, S * T);
+    a.h2d(e.tokens, ids); a.h2d(e.count, counts);
+    a.decodeStepPaged(e.model, handle, e.tokens, T, e.count, window, sinks, commit ? 1 : 0, e.logits);
+    if (commit) cache._advance(counts);
+    return e;
+  }
+
+  /** Several tokens of every sequence of a PagedKVCache (tokens[s]: an array, empty for none): logits
+   *  [sequences][T][vocabSize], T being the most tokens of a sequence, NaN for rows behind a sequence's tokens.
+   *  opts.window: the tokens see the last so many positions alone, and the first opts.sinks; opts.commit false: they
+   *  are stored, but do not count until cache.commit takes as many of them as stand. */
+  forwardChunk(tokens, cache, opts = {}) {
+    const e = this._chunk(tokens, cache, opts), T = Math.max.apply(null, Array.from(tokens, (t) => t.length));
+    const out = new Float32Array(cache.sequences * T * this.cfg.vocabSize);
+    hip().d2h(e.logits, out);
+    return out;
   }
 
   /** Queues one token of every sequence of a 4-bit cache (logits stay in device
@@ -319,6 +402,7 @@ export class Transformer {
     const a = hip();
     this._dropGraphs();
     this._dropKv4();
+    this._dropPaged();
     for (const h of this._w.bufs) a.free(h);
     if (this._w.part) a.free(this._w.part);
     this._w = null; this._model = null;

@@ -15,7 +15,9 @@ export {
 } from "./L2/tensor.js";
 export { Config, Transformer } from "./L6/transformer.js";
 export { KVCache, KV4Cache, attentionDecode, attentionNaive, flashAttention } from "./L5/attention.js";
+export { PagedKVCache } from "./L5/paged.js";
 export { beamSelect, beamSearch } from "./L8/beam.js";
+export { verifyDrafts, speculate } from "./L8/speculate.js";
 export { TrainableTransformer, initWeights, toParams, train, DeviceTrainLoop } from "./L6/train.js";
 export { hip } from "./L2/device.js";
 export {

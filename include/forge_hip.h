@@ -826,6 +826,19 @@ int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, const float* q
                   const int32_t* count, int window, int sinks);
 /* Ends a step: len[s] += T (or count[s]; to maxPages pageSize at most). */
 int fg_paged_commit(const fg_paged_cache* c, int T, const int32_t* count);
+/* Transformer.forward (transformer.js:134-184) of T tokens for every sequence of a paged
+ * cache (a prompt's chunk, drafted tokens, or one): tokens [nSeq][T] (device), logits
+ * [nSeq][T][vocab].  Token t of sequence s stands at position len[s] + t; its keys and
+ * values are appended to every layer and attended to (window and sinks as in
+ * fg_paged_attn).  With `commit` the tokens that took part count at the end; without,
+ * len stands, and fg_paged_commit takes as many of them as stand.  Of a sequence's
+ * count[s] (NULL: T) tokens those take part that come before the first one that is outside [0,
+ * vocab), at a position outside the model's RoPE table (m->maxSeq), or without a page;
+ * the logits of other rows are NaN.  m->x, m->q and m->h hold nSeq T vectors each;
+ * m->attn_part is not used.  The limits of fg_decode_step on dim and hidden hold, the
+ * head size is one of the cache's; nSeq T <= 65535. */
+int fg_decode_step_paged(const fg_decode_model* m, const fg_paged_cache* c, const int32_t* tokens, int T,
+                         const int32_t* count, int window, int sinks, int commit, float* logits);
 
 /* ──────────── drafted tokens ────────────
  * No counterpart in the reference (its sampling.js:28-98 draws one token from one row). */

@@ -133,6 +133,25 @@ def test_good_arguments_need_a_device():
     assert fh.lib.fg_draft_verify(A, A, A, 100, None, 0, None, None, None, 0.0, 4, 0, 100) == -4
 
 
+def test_handles_of_one_kind_are_not_read_as_another():
+    """The addon's paged cache handle as a decode model or a 4-bit cache, and things that are no handle at all."""
+    import os
+    import subprocess
+    code = """
+import { addonUninitialised } from './src/L2/device.js';
+const a = addonUninitialised(), no = [null, null, null, null, null, null, null, null];
+const paged = a.pagedCache(1, 1, 1, 32, 16, 4, 4, 0, null, null, null, null), kv4 = a.kv4Cache(1, 1, 1, 32, 8, ...no);
+const say = (fn) => { try { fn(); return 'nothing'; } catch (e) { return e.message; } };
+for (const x of [paged, kv4, {}, null, 7]) console.log(say(() => a.decodeStepPaged(x, paged, null, 1, null, 0, 0, 1, null)));
+for (const x of [kv4, {}, null, 7]) console.log(say(() => a.pagedCommit(x, 1, null)));
+console.log(say(() => a.kv4Commit(paged, 1, null)));
+"""
+    r = subprocess.run(["node", "--input-type=module", "-e", code], cwd=os.path.dirname(os.path.abspath(fh.__file__)),
+                       stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout
+    assert r.stdout.split("\n")[:-1] == ["expected a decode model handle"] * 5 + ["expected a paged cache handle"] * 4 + ["expected a 4-bit cache handle"], r.stdout
+
+
 # ── the plain forms ───────────────────────────────────────────────────────
 def test_rotation_by_hand():
     cos, sin = np.array([[1.0, 1.0], [0.0, 0.6]]), np.array([[0.0, 0.0], [1.0, 0.8]])
