@@ -1,5 +1,8 @@
 // Paged key-value cache (fg_paged_*): storing rows with their positions' rotation,
 // reading them back, and causal attention of one or more new tokens a sequence.
+//
+// A page holds a head's slots next to each other, so a head's slots of a page are one run of memory,
+// and four neighbouring slots (pages have at least four, at multiples of four) always are.
 #include "common.h"
 
 #include <math.h>
@@ -70,7 +73,9 @@ __device__ __forceinline__ void get(float* x, const _Float16* p) {
 
 // A workgroup takes a token.  A thread takes P pairs (4, or 1 where rows are not
 // aligned or pairs do not come in fours) of every so many heads, so that it reads
-// their angles once.
+// their angles once (fp64, 64 bytes for four pairs, where a head's share of a row is 32).
+// HBM-bound: 8191 tokens of 32 query heads and 8 kv heads of 128 74 us (5.0 TB/s read and
+// written); a token of four sequences 2.3.
 template <class KV, int P>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(Cache c, int layer, int dH, float* q_out,
                                                                 const float* q, const float* __restrict__ k,
@@ -171,6 +176,12 @@ __global__ void paged_commit_kernel(Cache c, int T, const int32_t* __restrict__ 
 //
 // fp32 caches multiply in fp32 (16x16x4).  fp16 caches multiply as they are
 // (16x16x32), q and p against them in two fp16 pieces each: 22 bits.
+//
+// Bound by reading the cache: each value of K and V is read once a workgroup's rows, the products
+// of 32 rows take a third of the time that 16 KB of a wave's slots take to come.  A step's loads
+// are issued as soon as the registers of the one before are free.  One token after 130001 (32 query
+// heads on 8 of 128, fp16) 97 us, 5.5 TB/s; five of 16 sequences up to 8192 45 us (5.2 TB/s); of
+// what is left the joining launch is 5 to 6.
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -194,13 +205,15 @@ __device__ __forceinline__ Steps steps_of(const Cache& c, const Span& q, int use
   Steps s;
   s.low = q.window > 0 ? min(max(first - q.window + 1, 0), end) / q.keys : 0;
   s.sink = q.window > 0 ? min((min(q.sinks, end) + q.keys - 1) / q.keys, s.low) : 0;
-  s.total = s.sink + (end + q.keys - 1) / q.keys - s.low;
+  // (one at least, whose slots do not exist, for windows wholly behind the room's end)
+  s.total = max(s.sink + (end + q.keys - 1) / q.keys - s.low, 1);
   return s;
 }
 
 // Which part of the work a workgroup has.  Sequences are cut into pieces of `per`
 // steps, as many as make about `target` workgroups of all of them, whatever their
-// lengths; every wave finds its own, its lanes sharing the sequences out.
+// lengths (which are known on the device alone, so that a recorded step serves all of
+// them); every wave finds its own, its lanes sharing the sequences out.
 struct Part {
   int s, kvh, tile, piece, pieces, per;
   int id;         // its number; neighbours read the same slots
@@ -776,6 +789,11 @@ __global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) page
 //      copied there straight from memory
 //   V  the values of d at eight slots (fp32: four) that a lane's operand takes, [e][8 groups of slots][i] for d = E i + e:
 //      turned around on the way, four rows of a run of E values a lane
+//
+// Bound by the matrix pipes: 512 tokens after 8192 (32 query heads on 8 of 128, fp16) 150 us for 142 GFLOP of fp16 products
+// (two pieces each), 0.95 PFLOP/s where a large library product of fp16 matrices reaches 1.15.  Two workgroups of a
+// CU take turns at scores and exponentials (46% of the cycles have a matrix instruction running, 40% a vector
+// one); registers (255) leave no room to interleave the two in one wave.  Every spill cost a wait for all loads: 12 of them 40 us.
 template <class KV, int DH>
 struct Wide;
 template <int DH>
@@ -1408,6 +1426,7 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   PAGED_TRY(fg::check_paged_cache(c, fn));
   PAGED_TRY(check_step(c, layer, T, fn));
   FG_ARG_CHECK(T == 0 || (out && q), "%s: null argument", fn);
+  FG_ARG_CHECK(T == 0 || out != q, "%s: out in place of q", fn);
   FG_ARG_CHECK(nHeads > 0 && nHeads % c->nKvHeads == 0, "%s: %d query heads for %d kv heads", fn, nHeads, c->nKvHeads);
   FG_ARG_CHECK(window >= 0 && sinks >= 0, "%s: window %d, sinks %d", fn, window, sinks);
   const int64_t items = (int64_t)c->nSeq * T * nHeads;

@@ -71,6 +71,19 @@ def test_long_vocabulary(fh):
         compare(run(fh, logits, y, draft, u, 1.0), logits, y, draft, u, 1.0)
 
 
+@pytest.mark.parametrize("nSeq,D,V", [(2, 40, 64), (1, 1023, 8), (300, 2, 4500), (20, 1, 9000), (70, 1, 20000)])
+def test_many_rows(fh, nSeq, D, V):
+    """Long drafts, most of which stand, and more sequences than there are units: every share of a row that a thread may have."""
+    rng = np.random.default_rng(nSeq + D)
+    logits, draft_logits, _, u = case(rng, nSeq, D, V, noise=0.05)
+    draft = np.array([[ref.draw(ref.softmax(draft_logits[s, t], 1.0), rng.random()) for t in range(D)] for s in range(nSeq)], np.int32)
+    u[:, :D] *= 0.9
+    got = run(fh, logits, draft_logits, draft, u, 1.0)
+    compare(got, logits, draft_logits, draft, u, 1.0)
+    compare(run(fh, logits, None, draft, u, 1.0), logits, None, draft, u, 1.0)
+    assert D < 40 or got[1].max() > 20
+
+
 def test_own_numbers_of_drafts(fh):
     rng = np.random.default_rng(4)
     logits, draft_logits, draft, u = case(rng, 8, 5, 500, noise=0.05)

@@ -17,11 +17,14 @@ TYPES = {"f32": (0, np.float32, 2.0 ** -24), "f16": (1, np.float16, 2.0 ** -11)}
 class Cache:
     """A cache on the device whose slots all hold NaN and whose pages are handed out shuffled."""
 
-    def __init__(self, fh, rng, nLayers, nSeq, nKV, dH, P, maxPages, kind, lens, spare=3):
+    def __init__(self, fh, rng, nLayers, nSeq, nKV, dH, P, maxPages, kind, lens, spare=3, upto=None):
         self.fh, self.nLayers, self.nSeq, self.nKV, self.dH, self.P, self.maxPages = fh, nLayers, nSeq, nKV, dH, P, maxPages
         self.type, self.dtype, self.half_step = TYPES[kind]
-        self.nPages = nSeq * maxPages + spare
-        self.table_host = rng.permutation(self.nPages)[:nSeq * maxPages].reshape(nSeq, maxPages).astype(np.int32)
+        # pages for the first upto[s] slots of a sequence, or for all of them
+        need = [maxPages if upto is None else -(-int(n) // P) for n in (upto if upto is not None else [0] * nSeq)]
+        self.nPages = sum(need) + spare
+        order = iter(rng.permutation(self.nPages))
+        self.table_host = np.array([[next(order) if p < n else -1 for p in range(maxPages)] for n in need], np.int32)
         shape = (nLayers, self.nPages, nKV, P, dH)
         up = fh.DeviceArray.from_numpy
         self.k, self.v = (up(np.full(shape, np.nan, self.dtype)) for _ in range(2))
@@ -281,6 +284,19 @@ def test_missing_pages_and_odd_lengths(fh, kind, T):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("T,group", [(3, 2), (50, 1), (40, 4)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (2, 5), (30, 0)])
+def test_windows_behind_the_end_of_the_room(fh, kind, T, group, window, sinks):
+    """Queries of positions that the cache has no room for see what there is of their window, in caches that are cut into pieces."""
+    rng = np.random.default_rng(T + window)
+    c = Cache(fh, rng, 1, 3, 2, 64, 16, 70, kind, [1120, 1118, 600])
+    c.fill(rng, 0, [1120, 1120, 600 + T])
+    got = check_attention(fh, c, rng, 0, 2 * group, T, [T] * 3, window, sinks, given=False)
+    if window and not sinks:
+        assert (got[0, window:] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("dH,group,T,window", [(64, 1, 12, 0), (128, 4, 5, 0), (32, 2, 80, 0), (96, 3, 20, 9), (256, 1, 40, 30)])
 def test_unseen_values_have_no_part(fh, kind, dH, group, T, window):
     """Infinities and NaN in later tokens' slots, behind the window and in unused slots leave what a query sees alone;
@@ -356,6 +372,23 @@ def test_large_and_small_scores(fh, kind, dH, T):
     c.k.upload(k)
     for scale in (1.0, -1.0, 0.0, 1e-3):
         check_attention(fh, c, rng, 0, 4, T, [T, T], scale=scale)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("dH,group,T", [(64, 2, 1), (128, 4, 5), (32, 1, 40), (128, 4, 40), (256, 2, 3), (96, 3, 30)])
+@pytest.mark.parametrize("nSeq", [1, 70, 200])
+def test_pieces_of_many_sequences(fh, kind, dH, group, T, nSeq):
+    """Caches that are cut into pieces, of lengths from nothing to long ones, more sequences than a wave has lanes, windows for some."""
+    rng = np.random.default_rng(nSeq + T)
+    longest = 2600 if nSeq == 1 else 700
+    lens = [longest if s == 0 else int(longest * rng.random() ** 4) for s in range(nSeq)]
+    counts = [T if s == 0 else int(rng.integers(0, T + 1)) for s in range(nSeq)]
+    upto = [n + t for n, t in zip(lens, counts)]
+    c = Cache(fh, rng, 1, nSeq, 1, dH, 16, -(-(2600 + T) // 16), kind, lens, upto=upto)
+    c.fill(rng, 0, upto)
+    check_attention(fh, c, rng, 0, group, T, counts)
+    if nSeq < 100:
+        check_attention(fh, c, rng, 0, group, T, counts, window=300, sinks=3)
 
 
 def test_a_long_cache(fh):

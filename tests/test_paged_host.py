@@ -36,7 +36,7 @@ def test_structure_matches_the_header():
 CALLS = {
     "paged_append": lambda c: (c, 0, A, A, A, A, 512, 4, 1, None, A, A, 9, 64, 0),
     "paged_read": lambda c: (c, 0, A, A, 128, 0, 1),
-    "paged_attn": lambda c: (c, 0, A, A, 4, 1.0, 1, None, 0, 0),
+    "paged_attn": lambda c: (c, 0, A, 2 * A, 4, 1.0, 1, None, 0, 0),
     "paged_commit": lambda c: (c, 1, None),
 }
 
@@ -104,6 +104,7 @@ def test_bad_steps_are_refused():
     ok = CALLS["paged_attn"](c)
     for i in ("_2", "_3"):
         refused("paged_attn", *but(ok, **{i: None}), says="null")
+    refused("paged_attn", *but(ok, _3=A), says="in place")
     for h in (0, 3, -2):
         refused("paged_attn", *but(ok, _4=h), says="heads")
     for i in ("_8", "_9"):
