@@ -224,10 +224,15 @@ __device__ __forceinline__ double weight(const Next& r, const Args& a, float x, 
   return fmax(p - q, 0.0);
 }
 
-__device__ __forceinline__ void write_tokens(int32_t* token, int32_t* count, const Args& a, int s, int taken, int last) {
-  for (int t = threadIdx.x; t <= a.D; t += blockDim.x)
-    token[(int64_t)s * (a.D + 1) + t] = t < taken ? a.draft[(int64_t)s * a.D + t] : t == taken ? last : -1;
-  if (threadIdx.x == 0) count[s] = taken + 1;
+// Thread t's draft (up to 1023 drafts, a thread each), asked for before it is known whether it stands.
+static_assert(64 * kDrawWaves >= 1024, "a thread a draft");
+__device__ __forceinline__ int own_draft(const Args& a, int s) {
+  return (int)threadIdx.x < a.D ? a.draft[(int64_t)s * a.D + threadIdx.x] : -1;
+}
+__device__ __forceinline__ void write_tokens(int32_t* token, int32_t* count, const Args& a, int s, int taken, int last, int own) {
+  const int t = threadIdx.x;
+  if (t <= a.D) token[(int64_t)s * (a.D + 1) + t] = t < taken ? own : t == taken ? last : -1;
+  if (t == 0) count[s] = taken + 1;
 }
 
 // The inclusive sums of 64 lanes' x.
@@ -241,13 +246,13 @@ __device__ __forceinline__ double lanes_upto(double x) {
 }
 
 // The token of a sequence's row r that its number falls on, by the workgroup; weights[piece]: the
-// weights' sums (both kinds, max(p - q, 0) and p, where drafts are left).
+// weights' sums (both kinds, max(p - q, 0) and p, where drafts are left).  Weights of 2^-40 in all at most are
+// what roundings leave of equal rows, summed in other orders.
 template <int E>
-__device__ int draw(const double* weights, const Next& r, const Args& a, int s, bool less) {
+__device__ int draw(const double* weights, const Next& r, const Args& a, int s, bool less, float u) {
   __shared__ double parts[E], shared_start, shared_goal;  // E waves take a piece
   __shared__ int found[E], ends[E], shared_at, shared_less;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pieces = (a.V + (64 * E) - 1) / (64 * E);
-  const float u = a.u[(int64_t)s * (a.D + 1) + a.D];
   if (wave == 0) {  // the piece: neighbours a lane
     const int each = (pieces + 63) / 64, from = min(lane * each, pieces), to = min(from + each, pieces);
     double mine, upto, all;
@@ -256,7 +261,7 @@ __device__ int draw(const double* weights, const Next& r, const Args& a, int s, 
       for (int z = from; z < to; ++z) mine += weights[2 * z + !less];
       upto = lanes_upto(mine);
       all = __shfl(upto, 63, 64);
-      if (all > 0 || !less) break;
+      if (all > 0x1p-40 || !less) break;
     }
     const double goal = (double)u * all;
     const uint64_t some = __ballot(mine > 0), over = __ballot(mine > 0 && upto > goal);
@@ -317,9 +322,11 @@ __global__ void __launch_bounds__(64 * kDrawWaves) draft_weights_kernel(int32_t*
                                                                         int groups) {
   const int s = blockIdx.x / groups, c = blockIdx.x - s * groups, n = drafts_of(a, s);
   if (n < 0) {
-    if (Alone) write_tokens(token, count, a, s, -1, -1);
+    if (Alone) write_tokens(token, count, a, s, -1, -1, -1);
     return;
   }
+  const int own = Alone ? own_draft(a, s) : -1;
+  const float u = Alone ? a.u[(int64_t)s * (a.D + 1) + a.D] : 0.f;
   const Next r = next_of(sums, a, s, nSeq, n);
   const bool less = r.taken < n;  // else there are no weights but the probabilities
   float x[E], y[E] = {};
@@ -337,15 +344,15 @@ __global__ void __launch_bounds__(64 * kDrawWaves) draft_weights_kernel(int32_t*
   }
   sum = wave_sum(sum);
   whole = wave_sum(whole);
-  __shared__ double own[2 * kDrawWaves];
-  double* const mine = Alone ? own : weights + (int64_t)s * 2 * pieces;
+  __shared__ double here[2 * kDrawWaves];
+  double* const mine = Alone ? here : weights + (int64_t)s * 2 * pieces;
   if ((threadIdx.x & 63) == 0 && piece < pieces) {
     mine[2 * piece] = sum;
     mine[2 * piece + 1] = whole;
   }
   if constexpr (Alone) {
     __syncthreads();
-    write_tokens(token, count, a, s, r.taken, draw<E>(own, r, a, s, less));
+    write_tokens(token, count, a, s, r.taken, draw<E>(here, r, a, s, less, u), own);
   } else {
     if (c == 0 && threadIdx.x == 0) nexts[s] = r;
   }
@@ -358,23 +365,27 @@ __global__ void __launch_bounds__(64 * kDrawWaves) draft_draw_kernel(int32_t* __
                                                                      const Next* __restrict__ nexts, Args a) {
   const int s = blockIdx.x, n = drafts_of(a, s), pieces = (a.V + (64 * E) - 1) / (64 * E);
   if (n < 0) {
-    write_tokens(token, count, a, s, -1, -1);
+    write_tokens(token, count, a, s, -1, -1, -1);
     return;
   }
+  const int own = own_draft(a, s);
+  const float u = a.u[(int64_t)s * (a.D + 1) + a.D];
   const Next r = nexts[s];
-  write_tokens(token, count, a, s, r.taken, draw<E>(weights + (int64_t)s * 2 * pieces, r, a, s, r.taken < n));
+  write_tokens(token, count, a, s, r.taken, draw<E>(weights + (int64_t)s * 2 * pieces, r, a, s, r.taken < n, u), own);
 }
 
 // Temperature 0: a workgroup takes a sequence, a wave a row.
-__global__ void __launch_bounds__(kThreads) draft_greedy_kernel(int32_t* __restrict__ token, int32_t* __restrict__ count,
-                                                                const Sum* __restrict__ sums, Args a) {
-  __shared__ int best[kWaves];
+__global__ void __launch_bounds__(64 * kDrawWaves) draft_greedy_kernel(int32_t* __restrict__ token,
+                                                                       int32_t* __restrict__ count,
+                                                                       const Sum* __restrict__ sums, Args a) {
+  __shared__ int best[kDrawWaves];
   const int s = blockIdx.x, n = drafts_of(a, s), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (n < 0) {
-    write_tokens(token, count, a, s, -1, -1);
+    write_tokens(token, count, a, s, -1, -1, -1);
     return;
   }
-  for (int t0 = 0;; t0 += kWaves) {
+  const int own = own_draft(a, s);
+  for (int t0 = 0;; t0 += kDrawWaves) {
     const int t = t0 + wave;
     if (t <= n) {
       const Sum* mine = sums + ((int64_t)s * (a.D + 1) + t) * a.chunks;
@@ -388,10 +399,10 @@ __global__ void __launch_bounds__(kThreads) draft_greedy_kernel(int32_t* __restr
       if (lane == 0) best[wave] = at == INT32_MAX ? -1 : at;
     }
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kDrawWaves; ++w) {
       const int b = best[w];
       if (t0 + w == n || b < 0 || a.draft[(int64_t)s * a.D + t0 + w] != b) {
-        write_tokens(token, count, a, s, t0 + w, b);
+        write_tokens(token, count, a, s, t0 + w, b, own);
         return;
       }
     }
@@ -440,7 +451,7 @@ extern "C" int fg_draft_verify(int32_t* token, int32_t* count, const float* logi
   const dim3 all((unsigned)(rows * chunks)), row((unsigned)(nSeq * groups)), block(64 * kDrawWaves);
   if (temperature == 0) {
     FG_LAUNCH(draft_sums_kernel<true>, all, dim3(kThreads), 0, sums, a, nSeq);
-    FG_LAUNCH(draft_greedy_kernel, dim3(nSeq), dim3(kThreads), 0, token, count, (const Sum*)sums, a);
+    FG_LAUNCH(draft_greedy_kernel, dim3(nSeq), block, 0, token, count, (const Sum*)sums, a);
     return FG_OK;
   }
   FG_LAUNCH(draft_sums_kernel<false>, all, dim3(kThreads), 0, sums, a, nSeq);

@@ -850,8 +850,8 @@ int fg_decode_step_paged(const fg_decode_model* m, const fg_paged_cache* c, cons
  * logits / temperature and draft_logits / temperature:
  *   draft x of row t stands if u[s (D + 1) + t] q_t(x) < p_t(x) and all before it stand;
  *   with n of them standing, the next token is drawn from max(p_n - q_n, 0) (from p_n
- *   for n = the number of drafts, or where that is nothing): the least whose cumulated
- *   weight exceeds u[s (D + 1) + D] of the whole.
+ *   for n = the number of drafts, or where that is nothing, 2^-40 in all at most): the
+ *   least whose cumulated weight exceeds u[s (D + 1) + D] of the whole.
  * temperature 0: a draft stands if it is the lowest token of greatest logit, which is
  * the next one, too (NaN counts below all); draft_logits and u are not used.  Else
  * temperature >= 1e-30.

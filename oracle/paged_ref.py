@@ -110,7 +110,7 @@ def verify(logits, draft_logits, draft, u, temperature, n):
                 last = -1
                 if not np.isnan(p).any():
                     w = np.fmax(p - q, 0.0)
-                    last = draw(w if w.sum() > 0 else p, float(u[D]))
+                    last = draw(w if w.sum() > 2.0 ** -40 else p, float(u[D]))
         if not stands:
             token[t] = last
             return token, t + 1

@@ -133,6 +133,21 @@ def test_drafts_outside_the_vocabulary(fh):
     compare(run(fh, logits, None, draft, None, 0.0), logits, None, draft, None, 0.0)
 
 
+@pytest.mark.parametrize("V,pad,pad_draft", [(1000, 0, 1), (1000, 3, 2), (4099, 1, 0), (40000, 0, 3)])
+def test_equal_rows(fh, V, pad, pad_draft):
+    """Rows of one distribution that lie apart and are shifted, so that they are summed in other orders: a draft outside the
+    vocabulary leaves no weight, and the next token is drawn from the target's own row."""
+    rng = np.random.default_rng(V + pad)
+    logits = (np.round(rng.standard_normal((6, 3, V)) * 16) / 8).astype(np.float32)
+    draft_logits = logits[:, :2] + np.float32(4)  # exact: no bit is lost
+    draft = np.array([[V, 0], [-1, 0], [V + 5, V]] * 2, np.int32)
+    u = rng.random((6, 3)).astype(np.float32)
+    u[0, 2], u[1, 2] = 0, np.float32(1 - 2.0 ** -24)
+    got = run(fh, logits, draft_logits, draft, u, 1.0, pad=pad, pad_draft=pad_draft)
+    assert (got[1] == 1).all()
+    compare(got, logits, draft_logits, draft, u, 1.0)
+
+
 def test_numbers_at_the_ends(fh):
     """u of 0 takes the first token of any weight, one of nearly 1 the last that it reaches; equal rows leave no rest and every draft stands."""
     rng = np.random.default_rng(14)
