@@ -42,6 +42,7 @@ export class PagedKVCache {
       this._table = alloc(sequences * maxPages * 4); this._len = alloc(sequences * 4); this._count = alloc(sequences * 4);
       this._handle = a.pagedCache(nLayers, sequences, nKvHeads, dHead, pageSize, pages, maxPages, TYPES[type], k, v, this._table, this._len);
       this.table = new Int32Array(sequences * maxPages).fill(-1); this.lens = new Int32Array(sequences);
+      this._least = new Int32Array(sequences);  // the shortest that truncate may leave, after forget
       this._free = Array.from({ length: pages }, (_, i) => pages - 1 - i);  // the next one last
       this._rope = null;
       a.h2d(this._table, this.table);
@@ -195,12 +196,16 @@ export class PagedKVCache {
     this._advance(n);
   }
   _advance(counts) { for (let s = 0; s < this.sequences; s++) this.lens[s] += counts[s]; }
-  /** Keeps the first `length` tokens of a sequence; the pages behind them come back. */
+  /** Keeps the first `length` tokens of a sequence; the pages behind them come back.  After `forget`, a length whose
+   *  window reaches back to what was forgotten throws (0, a new start, does not). */
   truncate(seq, length) {
     this._seq(seq);
     if (!Number.isInteger(length) || length < 0 || length > this.lens[seq]) throw new RangeError(`PagedKVCache.truncate: ${length} of ${this.lens[seq]} tokens`);
+    if (length > 0 && length < this._least[seq])
+      throw new RangeError(`PagedKVCache.truncate: ${length} tokens, of which the window needs forgotten ones (${this._least[seq]} at least, or 0)`);
     this.handle;
     this.lens[seq] = length;
+    if (length === 0) this._least[seq] = 0;
     hip().h2d(this._len, this.lens);
     this._giveBack((s, p) => s === seq && p * this.pageSize >= length);
   }
@@ -208,7 +213,11 @@ export class PagedKVCache {
   forget(window, sinks = 0) {
     whole(window, "window", 1); whole(sinks, "sinks", 0);
     this.handle;
-    this._giveBack((s, p) => p * this.pageSize >= sinks && (p + 1) * this.pageSize <= this.lens[s] + 1 - window);
+    this._giveBack((s, p) => {
+      const end = (p + 1) * this.pageSize, unseen = p * this.pageSize >= sinks && end <= this.lens[s] + 1 - window;
+      if (unseen) this._least[s] = Math.max(this._least[s], end - 1 + window);
+      return unseen;
+    });
   }
   _view(layer, upto, seq, which) {
     this._layer(layer); this._seq(seq);

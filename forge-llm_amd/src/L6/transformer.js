@@ -102,7 +102,8 @@ const GRAPHS_KEPT = 4;
  * sequence, at the sequence's next position, `forwardAll(tokens, cache)` one token
  * of every sequence (fg_decode_step_kv4).  Recorded steps are kept for the last four
  * caches of each kind.  `forwardChunk(tokens, cache)` takes several tokens of every
- * sequence of a PagedKVCache in one step (fg_decode_step_paged), op by op.
+ * sequence of a PagedKVCache in one step (fg_decode_step_paged), op by op; `forward` takes
+ * one of one sequence, at the sequence's next position.
  */
 export class Transformer {
   constructor(config, opts = {}) {
@@ -344,6 +345,12 @@ export class Transformer {
       if (cache.sequences !== 1) throw new TypeError("Transformer.forward: a cache of several sequences goes to forwardAll");
       if (pos !== cache.nexts[0]) throw new RangeError(`Transformer.forward: position ${pos}, the 4-bit cache is at ${cache.nexts[0]}`);
       hip().d2h(this._stepAll([token], cache).logits, this.logits);
+      return this.logits;
+    }
+    if (cache instanceof PagedKVCache) {
+      if (cache.sequences !== 1) throw new TypeError("Transformer.forward: a cache of several sequences goes to forwardChunk");
+      if (pos !== cache.len) throw new RangeError(`Transformer.forward: position ${pos}, the cache is at ${cache.len}`);
+      hip().d2h(this._chunk([[token]], cache).logits, this.logits);
       return this.logits;
     }
     this._step(token, pos, cache);

@@ -62,6 +62,21 @@ rec("append, views, attention, commit and truncate of several sequences", () => 
   return { ok, detail: `attention ${worst.toExponential(1)}` };
 });
 
+rec("truncate after forget", () => {
+  // 20 tokens in pages of 4, a window of 6: slots 0..11 of pages 0 to 2 are behind it for good, and 17 tokens see slot 12 on.
+  const r = new RNG(5), kvD = 32, c = new PagedKVCache(1, 8, 1, 32, { pageSize: 4 }), k = normal(r, 20 * kvD);
+  c.append(0, k, k, 20); c.commit(20); c.forget(6);
+  let ok = c.freePages === 8 - 2 && c.lens[0] === 20;
+  c.truncate(0, 17);
+  ok = ok && throws(() => c.truncate(0, 16), RangeError) && c.lens[0] === 17 && same(c.kView(0, 17).subarray(12 * kvD), k.subarray(12 * kvD, 17 * kvD));
+  c.truncate(0, 0);
+  ok = ok && c.freePages === 8;
+  c.append(0, k, k, 3); c.commit(3); c.truncate(0, 1);
+  ok = ok && same(c.kView(0, 1), k.subarray(0, kvD));
+  c.free();
+  return { ok };
+});
+
 rec("rotation on the way into the pages", () => {
   const r = new RNG(9), T = 5, nKV = 1, dH = 64, nH = 3, theta = 1e4, c = new PagedKVCache(1, 8, nKV, dH, { type: "f16" });
   const k = normal(r, T * dH), v = normal(r, T * dH), q = normal(r, T * nH * dH);
@@ -115,6 +130,16 @@ rec("forwardChunk == token by token, whatever the chunks; uncommitted tokens do 
   c.free(); one.free(); M.release();
   // fp32 products and sums of the same terms in another order, through two layers
   return { ok: ok && worst < 1e-5, detail: worst.toExponential(1) };
+});
+
+rec("forward of one token at the cache's next position", () => {
+  const { cfg, w } = model(), V = cfg.vocabSize, M = new Transformer(cfg).loadWeights(w), ids = [3, 50, 89];
+  const c = paged(cfg, 4), d = paged(cfg, 4), two = paged(cfg, 4, { sequences: 2 });
+  let ok = throws(() => M.forward(1, 1, c), RangeError) && throws(() => M.forward(V, 0, c), RangeError) && throws(() => M.forward(1, 0, two), TypeError) && c.len === 0;
+  ids.forEach((id, t) => { ok = ok && same(M.forward(id, t, c), M.forwardChunk([[id]], d)) && c.len === t + 1; });
+  for (const x of [c, d, two]) x.free();
+  M.release();
+  return { ok };
 });
 
 rec("a window with sinks, and pages given back behind it", () => {
