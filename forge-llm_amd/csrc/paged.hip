@@ -1371,7 +1371,7 @@ extern "C" int fg_paged_append(const fg_paged_cache* c, int layer, float* q_out,
   FG_ARG_CHECK(!q || (nHeads > 0 && nHeads <= 1 << 20), "%s: %d query heads", fn, nHeads);
   const int64_t wide = (int64_t)(nH > c->nKvHeads ? nH : c->nKvHeads) * c->dHead;
   FG_ARG_CHECK(ld >= wide, "%s: row stride %lld is below %lld", fn, (long long)ld, (long long)wide);
-  FG_ARG_CHECK(q != q_out || !q || ld == wide, "%s: q in place needs rows of %d x %d", fn, nH, c->dHead);
+  FG_ARG_CHECK(q != q_out || !q || ld == (int64_t)nH * c->dHead, "%s: q in place needs rows of %d x %d", fn, nH, c->dHead);
   FG_ARG_CHECK(rot >= 0 && rot <= c->dHead && rot % 2 == 0, "%s: %d rotated values of %d", fn, rot, c->dHead);
   FG_ARG_CHECK(rot == 0 || (cos_tab && sin_tab && npos > 0), "%s: no table of angles", fn);
   FG_REQUIRE_INIT();

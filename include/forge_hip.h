@@ -804,8 +804,8 @@ typedef struct fg_paged_cache {
  * or, with `half`, (i, i + rot / 2); cos_tab, sin_tab [npos][rot / 2] as
  * fg_rope_table(.., rot, theta) gives them; a position from npos on turns to NaN.
  * Keys and values go to slot len[s] + t of `layer`; queries to q_out
- * [nSeq T][nHeads dHead], which may be q where ld = nHeads dHead, else is apart from the rows.  q and q_out may
- * be NULL (together: no queries; nHeads is not used). */
+ * [nSeq T][nHeads dHead], which may be q where ld = nHeads dHead, else is apart from
+ * the rows.  q and q_out may be NULL (together: no queries; nHeads is not used). */
 int fg_paged_append(const fg_paged_cache* c, int layer, float* q_out, const float* q, const float* k, const float* v,
                     int64_t ld, int nHeads, int T, const int32_t* count, const double* cos_tab, const double* sin_tab,
                     int npos, int rot, int half);
@@ -821,7 +821,7 @@ int fg_paged_read(const fg_paged_cache* c, int layer, float* k, float* v, int64_
  * q and out [nSeq T][nHeads][dHead], query head h on kv head h / (nHeads / nKvHeads);
  * out apart from q; zeros where no slot is seen.  What is not seen, whatever its value, has no
  * part in it.  Sums are fp32; with an F32 cache products are fp32, with F16 q and p are
- * held in two fp16 pieces (22 bits). */
+ * held in two fp16 pieces (22 bits), and an infinite key that a row sees may make it NaN. */
 int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
                   const int32_t* count, int window, int sinks);
 /* Ends a step: len[s] += T (or count[s]; to maxPages pageSize at most). */

@@ -90,6 +90,7 @@ def test_bad_steps_are_refused():
     refused("paged_append", *but(ok, _6=255), says="stride")
     refused("paged_append", *but(ok, _2=None, _3=None, _6=127), says="stride")
     refused("paged_append", *ok, says="in place")
+    refused("paged_append", *but(ok, _6=128, _7=1), says="in place")  # rows of two kv heads, one query head
     ok = but(ok, _2=2 * A)
     for rot in (-2, 3, 66):
         refused("paged_append", *but(ok, _13=rot), says="rotated")
