@@ -170,18 +170,21 @@ __global__ void __launch_bounds__(kThreads) draft_sums_kernel(Sum* __restrict__ 
   }
 }
 
-// A row's greatest logit and 1 / sum, by a wave.
-__device__ __forceinline__ void row_sum(const Sum* sums, const Args& a, float& top, double& back) {
+// A lane's share of a row's chunks, its own numbers asked for at once where there are up to 64, and, of a wave's
+// lanes, the row's greatest logit and 1 / sum.
+__device__ __forceinline__ Sum lanes_chunk(const Sum* sums, const Args& a) {
   const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, sums[c].top);
-  m = fg_wave_max(m);
-  double sum = 0;
-  for (int c = lane; c < a.chunks; c += 64) {
-    const Sum p = sums[c];
-    sum += p.sum * power(p.top, m, a.inv);
+  return lane < a.chunks ? sums[lane] : Sum{0.0, -INFINITY, 0};
+}
+__device__ __forceinline__ void row_sum(Sum p, const Sum* sums, const Args& a, float& top, double& back) {
+  for (int c = (threadIdx.x & 63) + 64; c < a.chunks; c += 64) {
+    const Sum z = sums[c];
+    const float m = fmaxf(p.top, z.top);
+    p.sum = p.sum * power(p.top, m, a.inv) + z.sum * power(z.top, m, a.inv);
+    p.top = m;
   }
-  sum = wave_sum(sum);
+  const float m = fg_wave_max(p.top);
+  const double sum = wave_sum(p.sum * power(p.top, m, a.inv));
   top = m;
   back = m == -INFINITY ? (double)NAN : 1.0 / sum;
 }
@@ -194,15 +197,19 @@ __device__ Next next_of(const Sum* sums, const Args& a, int s, int nSeq, int n) 
   for (int t0 = 0;; t0 += kDrawWaves) {
     const int t = t0 + wave;
     if (t <= n) {
+      const bool two = t < n && a.draft_logits;
+      const Sum* const ps = sums + ((int64_t)s * (a.D + 1) + t) * a.chunks;
+      const Sum* const qs = sums + ((int64_t)nSeq * (a.D + 1) + (int64_t)s * a.D + t) * a.chunks;
+      // (the draft first, whose logits are asked for when it is there, before the sums are waited for)
       Next r{t, t < n ? a.draft[(int64_t)s * a.D + t] : -1, 0.f, 0.f, 0.0, 0.0};
-      const bool in = t < n && (uint32_t)r.draft < (uint32_t)a.V, two = t < n && a.draft_logits;
-      // (asked for before the sums are)
-      const float x = in ? target_row(a, s, t)[r.draft] : 0.f, y = in && two ? draft_row(a, s, t)[r.draft] : 0.f;
       const float u = t < n ? a.u[(int64_t)s * (a.D + 1) + t] : 0.f;
-      row_sum(sums + ((int64_t)s * (a.D + 1) + t) * a.chunks, a, r.ptop, r.pback);
-      if (two) row_sum(sums + ((int64_t)nSeq * (a.D + 1) + (int64_t)s * a.D + t) * a.chunks, a, r.qtop, r.qback);
-      const double q = two ? power(y, r.qtop, a.inv) * r.qback : 1.0;  // 1: of a draft that was certain
-      const bool ok = in && (double)u * q < power(x, r.ptop, a.inv) * r.pback;
+      const Sum p = lanes_chunk(ps, a), q = two ? lanes_chunk(qs, a) : Sum{};
+      const bool in = t < n && (uint32_t)r.draft < (uint32_t)a.V;
+      const float x = in ? target_row(a, s, t)[r.draft] : 0.f, y = in && two ? draft_row(a, s, t)[r.draft] : 0.f;
+      row_sum(p, ps, a, r.ptop, r.pback);
+      if (two) row_sum(q, qs, a, r.qtop, r.qback);
+      const double share = two ? power(y, r.qtop, a.inv) * r.qback : 1.0;  // 1: of a draft that was certain
+      const bool ok = in && (double)u * share < power(x, r.ptop, a.inv) * r.pback;
       if ((threadIdx.x & 63) == 0) {
         rows[wave] = r;
         stands[wave] = ok;

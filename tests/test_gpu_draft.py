@@ -71,6 +71,22 @@ def test_long_vocabulary(fh):
         compare(run(fh, logits, y, draft, u, 1.0), logits, y, draft, u, 1.0)
 
 
+@pytest.mark.parametrize("V", [262145, 700001])
+def test_more_chunks_than_lanes(fh, V):
+    """A lane adds up more than one of a row's chunks, whose greatest logits differ; a masked one, and one that is no number."""
+    rng = np.random.default_rng(V)
+    logits, draft_logits, draft, u = case(rng, 3, 2, V)
+    logits[:, :, 262144:] += 8
+    logits[1, :, 4096:8192] = -np.inf
+    for y in (draft_logits, None):
+        compare(run(fh, logits, y, draft, u, 1.0), logits, y, draft, u, 1.0)
+    logits[2, 0, V - 1] = np.nan
+    got = run(fh, logits, draft_logits, draft, u, 1.0)
+    compare(got, logits, draft_logits, draft, u, 1.0)
+    assert got[1][2] == 1 and got[0][2, 0] == -1
+    compare(run(fh, logits, None, draft, None, 0.0), logits, None, draft, None, 0.0)
+
+
 @pytest.mark.parametrize("nSeq,D,V", [(2, 40, 64), (1, 1023, 8), (300, 2, 4500), (20, 1, 9000), (70, 1, 20000)])
 def test_many_rows(fh, nSeq, D, V):
     """Long drafts, most of which stand, and more sequences than there are units: every share of a row that a thread may have."""
