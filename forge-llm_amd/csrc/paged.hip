@@ -516,7 +516,7 @@ __device__ __forceinline__ float over_groups_sum(float x) {
 // plan, part_ml, part_o: the sequences' pieces, the pieces' references and sums, and
 // values, a workgroup's rows each; null: every sequence is one piece.
 template <class KV, int DH, int NT>
-__global__ void __launch_bounds__(kThreads, (NT == 4 || DH == 256 ? 1 : 2)) paged_attn_kernel(Cache c, int layer, float* __restrict__ out,
+__global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kernel(Cache c, int layer, float* __restrict__ out,
                                                               const float* __restrict__ q, int nH, float factor, Span span,
                                                               int target, Pieces* __restrict__ plan,
                                                               float2* __restrict__ part_ml, float* __restrict__ part_o) {
@@ -954,7 +954,10 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     if (p.first == p.id && threadIdx.x == 0) plan[p.s] = Pieces{p.first, p.pieces};
   } else {
     const int tiles = tiles_of(span, span.T);
-    const int64_t id = by_die(blockIdx.x, (int64_t)c.nSeq * c.nKV * tiles);
+    // A head's tiles, which read the same slots, on one die; many heads go to the dies in turn, since sequences differ: 28
+    // of up to 164 tokens, 36 heads on 12 of 128, 77 us, 91 with neighbours on a die.
+    const int64_t id = c.nSeq * c.nKV >= 64 ? (blockIdx.x / 8 / tiles * 8 + blockIdx.x % 8) * tiles + blockIdx.x / 8 % tiles
+                                             : by_die(blockIdx.x, (int64_t)c.nSeq * c.nKV * tiles);
     p.id = (int)id;
     // the longest first, and beside them, as the second of a CU, the shortest: 2048 tokens of 8 heads, none before them,
     // 105 us (cut into equal pieces 139)
@@ -1438,11 +1441,12 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   // Many rows share steps through LDS, few take them in registers.  us, shared against registers:
   //   fp16  24 rows of 128, 8 sequences of 8000   64  53     48 rows   76  95     96 rows   86 154
   //         24 rows of 64                        104  48     48 rows  109 122     96 rows  115 189
-  //   fp32  48 rows of 128, 8 sequences of 8000  289 212     64 rows  290 215     96 rows  293 382
-  //         48 rows of 64                        252 241     64 rows  253 231     96 rows  337 360
+  //   fp32  64 rows of 128, 8 sequences up to 8000 164 108    96 rows  172 175   128 rows  174 222
+  //         64 rows of 64                           94  66    96 rows   96 106   128 rows   98 133
+  // (A tile of 64 rows in registers leaves a CU one workgroup: 64 rows of 128 fp32 120, of 64 73.)
   // Heads of 256 leave a wave of 32 rows no registers: 256 rows 116 (two tiles of 16: 65), 1024 rows 261 (152).
   const bool wide = c->dHead < 256 && all > (c->type ? 32 : 64);
-  const int tiles = all <= 16 ? 1 : all <= 32 || c->dHead == 256 ? 2 : 4;
+  const int tiles = all <= 16 ? 1 : 2;
   const Span span{T, group, wide ? kWideRows : 16 * tiles, window, sinks, (c->type ? 32 : 16) * (wide ? 2 : 1),
                   wide ? 1 : kWaves, count};
   const int64_t heads = (int64_t)c->nSeq * c->nKvHeads * ((all + span.rows - 1) / span.rows);
@@ -1453,7 +1457,7 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   // Workgroups that the chip holds at once, and, where a workgroup's time is mostly its reads, as many of them as give
   // every head two.
   const int cus = fg::device_cu_count() > 0 ? fg::device_cu_count() : 256;
-  const int64_t held = (int64_t)cus * (wide || (tiles < 4 && c->dHead < 256) ? 2 : 1);
+  const int64_t held = (int64_t)cus * (wide || c->dHead < 256 ? 2 : 1);
   const int64_t target = wide ? held : held * ((2 * heads + held - 1) / held);
   // Short caches, of more slots where there are heads enough to fill the chip: a workgroup a head and tile, no second
   // launch.  A round of it takes about 0.6 us and 0.07 for each KB that a wave reads; pieces and their joining take
@@ -1470,7 +1474,7 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
   const int64_t kb = span.keys * c->dHead * (c->type ? 2 : 4) * 2 / 1024;
   const int64_t limit = (wide ? 2 : tiles > 1 ? 64 / (8 + kb) : 98 / (8 + kb)) * (heads >= cus ? 4 : 1);
   const bool whole = rounds <= (limit > 1 ? limit : 1) || heads >= (wide ? held : 4 * held);
-  const int64_t grid = (whole ? heads : heads + target) + 8;  // (by_die: a die's run may end beyond the last)
+  const int64_t grid = (whole ? heads : heads + target) + 8 * (whole ? (all + span.rows - 1) / span.rows : 1);  // (by_die: a die's run may end beyond the last)
   FG_ARG_CHECK(grid <= INT32_MAX / kThreads, "%s: %d sequences x %d tokens x %d heads are too many", fn, c->nSeq, T, nHeads);
   fg::Workspace ws;
   float2* part_ml = nullptr;
@@ -1497,12 +1501,6 @@ extern "C" int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, con
       FG_LAUNCH((paged_wide_kernel<KV, DH>), dim3((unsigned)grid), dim3(kThreads), 0, cache, layer, out, q, nHeads,   \
                 factor, span, (int)target, plan, part_ml, part_o);                                                    \
       break;                                                                                                          \
-    }                                                                                                                 \
-    if constexpr (sizeof(KV) == 4) { /* fp16 rows beyond two tiles are wide */                                        \
-      if (tiles == 4) {                                                                                               \
-        PAGED_ATTN(KV, DH, 4);                                                                                        \
-        break;                                                                                                        \
-      }                                                                                                               \
     }                                                                                                                 \
   }                                                                                                                   \
   if (tiles == 1) PAGED_ATTN(KV, DH, 1);                                                                              \

@@ -391,6 +391,20 @@ def test_pieces_of_many_sequences(fh, kind, dH, group, T, nSeq):
         check_attention(fh, c, rng, 0, group, T, counts, window=300, sinks=3)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("nSeq,nKV,group,T,dH", [(9, 8, 2, 70, 64), (43, 6, 2, 130, 64), (23, 3, 3, 90, 32), (64, 1, 5, 60, 128), (21, 3, 1, 200, 96)])
+def test_many_heads_of_short_sequences(fh, kind, nSeq, nKV, group, T, dH):
+    """A workgroup a head and tile, heads of sequences of all numbers of tokens on the dies in turn, numbers of heads that are no
+    multiple of eight and some below the 64 that it takes."""
+    rng = np.random.default_rng(nSeq + T)
+    lens = [int(rng.integers(0, 40)) for _ in range(nSeq)]
+    counts = [T if s == 0 else int(rng.integers(0, T + 1)) for s in range(nSeq)]
+    upto = [n + t for n, t in zip(lens, counts)]
+    c = Cache(fh, rng, 1, nSeq, nKV, dH, 16, -(-(40 + T) // 16), kind, lens, upto=upto)
+    c.fill(rng, 0, upto)
+    check_attention(fh, c, rng, 0, nKV * group, T, counts, window=5, sinks=2)
+
+
 def test_a_long_cache(fh):
     """Offsets that pass 2^31 elements within a layer, the last slots of the room in use."""
     rng = np.random.default_rng(2)
