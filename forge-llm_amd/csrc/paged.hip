@@ -75,7 +75,7 @@ __device__ __forceinline__ void get(float* x, const _Float16* p) {
 // aligned or pairs do not come in fours) of every so many heads, so that it reads
 // their angles once (fp64, 64 bytes for four pairs, where a head's share of a row is 32).
 // HBM-bound: 8191 tokens of 32 query heads and 8 kv heads of 128 74 us (5.0 TB/s read and
-// written); a token of four sequences 2.3.
+// written); a token of four sequences 3.3.
 template <class KV, int P>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(Cache c, int layer, int dH, float* q_out,
                                                                 const float* q, const float* __restrict__ k,
