@@ -5,6 +5,7 @@
 // and four neighbouring slots (pages have at least four, at multiples of four) always are.
 #include "common.h"
 
+#include <float.h>
 #include <math.h>
 
 namespace {
@@ -502,8 +503,9 @@ struct Step<float, DH> {
 };
 
 // Scores are in units of log 2, references are scores; a tile's reference moves where a
-// score is more than kRise above it.
-constexpr float kRise = 4.f;
+// score is more than kRise above it.  It starts at the lowest finite number: scores of -inf (an infinite key) are
+// p = 0 against it, where -inf - -inf would be NaN.
+constexpr float kRise = 4.f, kNoScore = -FLT_MAX;
 __device__ __forceinline__ float over_groups_max(float x) {
   x = fmaxf(x, __shfl_xor(x, 16, 64));
   return fmaxf(x, __shfl_xor(x, 32, 64));
@@ -511,6 +513,20 @@ __device__ __forceinline__ float over_groups_max(float x) {
 __device__ __forceinline__ float over_groups_sum(float x) {
   x += __shfl_xor(x, 16, 64);
   return x + __shfl_xor(x, 32, 64);
+}
+// Whether a query of position pos of sequence s sees a slot.
+__device__ __forceinline__ bool sees_some(const Cache& c, const Span& q, int s, int pos) {
+  const int end = min(pos + 1, slots(c)), low = q.window > 0 ? max(pos - q.window + 1, 0) : 0;
+  for (int j = 0;; j = ((j >> c.lg) + 1) << c.lg) {
+    if (j >= q.sinks) j = max(j, low);
+    if (j >= end) return false;
+    if (slot_row(c, 0, s, j) >= 0) return true;
+  }
+}
+// What a row's values are multiplied with at the end.  Without a sum it has seen nothing, and is zeros, or scores of
+// -inf alone, of which no p is a number.
+__device__ __forceinline__ float one_by(float sum, const Cache& c, const Span& q, int s, int t) {
+  return sum != 0.f ? 1.f / sum : sees_some(c, q, s, slots_used(c, s) + t) ? NAN : 0.f;
 }
 
 // plan, part_ml, part_o: the sequences' pieces, the pieces' references and sums, and
@@ -616,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
   for (int n = 0; n < NT; ++n) {
     back[n] = unscale[n * 16 + i];
     pos[n] = used + (row0 + min(n * 16 + i, rows - 1)) / span.group;
-    ref[n] = -INFINITY;
+    ref[n] = kNoScore;
     sum[n] = 0.f;
 #pragma unroll
     for (int m = 0; m < M; ++m) o[n][m] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -770,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
       } else {
         const int r = row0 + n * 16 + row, t = r / span.group, h = r - t * span.group;
         float* to = out + (((int64_t)s * span.T + t) * nH + kvh * span.group + h) * DH + d;
-        const float f = all == 0.f ? 0.f : 1.f / all;
+        const float f = one_by(all, c, span, s, t);
 #pragma unroll
         for (int z = 0; z < 4; ++z) to[z] = y[z] * f;
       }
@@ -1096,7 +1112,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   const int t = min(row / span.group, tokens - 1), head = kvh * span.group + (row - row / span.group * span.group);
   const int pos = used + t, wave_first = used + (row0 + 32 * wave) / span.group, wave_last = used + (row0 + 32 * wave + max(mine, 1) - 1) / span.group;
   const float back = w.load_q(q + (((int64_t)s * span.T + t) * nH + head) * DH, factor, mine > 0 && r32 < mine);
-  float ref = -INFINITY, sum = 0.f;
+  float ref = kNoScore, sum = 0.f;
   f32x16 o[M];
 #pragma unroll
   for (int m = 0; m < M; ++m)
@@ -1249,8 +1265,8 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   if (my_row >= mine) return;
   sum += __shfl_xor(sum, 32, 64);
   const int64_t part = (int64_t)part_id * kWideRows + 32 * wave + my_row;
-  const float f = pieces > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
   const int my_t = at_row / span.group, my_head = kvh * span.group + (at_row - my_t * span.group);
+  const float f = pieces > 1 ? 1.f : one_by(sum, c, span, s, my_t);
   float* const to = pieces > 1 ? part_o + part * DH : out + (((int64_t)s * span.T + my_t) * nH + my_head) * DH;
   if (pieces > 1 && my_h == 0) part_ml[part] = make_float2(ref, sum);
 #pragma unroll
@@ -1316,7 +1332,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(Cache c, float* __
   }
   if (!on || set != 0) return;
   const int t = row / span.group, h = kvh * span.group + (row - t * span.group);
-  const float f = all == 0.f ? 0.f : 1.f / all;
+  const float f = one_by(all, c, span, s, t);
   float* to = out + (((int64_t)s * span.T + t) * nH + h) * DH + 4 * quad;
 #pragma unroll
   for (int z = 0; z < 4; ++z) to[z] = y[z] * f;
