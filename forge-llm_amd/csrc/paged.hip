@@ -526,7 +526,32 @@ __device__ __forceinline__ bool sees_some(const Cache& c, const Span& q, int s, 
 // What a row's values are multiplied with at the end.  Without a sum it has seen nothing, and is zeros, or scores of
 // -inf alone, of which no p is a number.
 __device__ __forceinline__ float one_by(float sum, const Cache& c, const Span& q, int s, int t) {
-  return sum != 0.f ? 1.f / sum : sees_some(c, q, s, slots_used(c, s) + t) ? NAN : 0.f;
+  if (__builtin_expect(sum != 0.f, 1)) return 1.f / sum;
+  return sees_some(c, q, s, slots_used(c, s) + t) ? NAN : 0.f;
+}
+
+// Infinities and NaN among the values that a row sees.  A step's products spoil them: in two pieces of p inf times the second
+// is NaN or of the other sign, a p that underflows gives inf 0, and what is seen by some rows alone is
+// left out.  Where that has been so (a step said it, or a sum is NaN though the p are numbers) a wave goes
+// over its values once more, for the rows whose p are numbers, and adds them to their sums as they are: inf p = inf for any
+// p > 0.  NaN sums are set to kLost, which swallows no infinity, and are NaN again if none came.
+constexpr float kLost = FLT_MAX;
+// Factors that bring sums to another reference: not zero, which would make NaN of an infinite sum.
+__device__ __forceinline__ float factor_of(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), FLT_MIN); }
+template <class KV, int DH>
+__device__ __forceinline__ bool any_odd(const KV* from) {  // of a slot's values, by the wave
+  bool odd = false;
+#pragma unroll
+  for (int d = threadIdx.x & 63; d < DH; d += 64) odd |= !(fabsf((float)from[d]) < INFINITY);
+  return __any(odd);
+}
+// What to multiply a value that is not finite with: 1, or NaN for a p of exactly zero (a score of -inf).
+template <class KV, int DH>
+__device__ __forceinline__ float weight_of_odd(const float* q, float factor, const KV* key) {
+  float x = 0.f;
+#pragma unroll 8
+  for (int d = 0; d < DH; ++d) x = fmaf(q[d] * factor, (float)key[d], x);
+  return x == -INFINITY ? NAN : 1.f;
 }
 
 // plan, part_ml, part_o: the sequences' pieces, the pieces' references and sums, and
@@ -639,6 +664,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
   }
   const int first_pos = used + t0, last_pos = used + t1;
   const int window = span.window > 0 ? span.window : INT32_MAX;
+  bool odd = false;  // values that some row sees were not finite and left out of a product
 
   for (; x < end; x += kWaves) {
     const int j0 = steps.at(x) * Keys;
@@ -661,7 +687,6 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
     for (int u = 0; u < Sub; ++u) pages &= (uint32_t)here.v[u] < (uint32_t)c.nPages;
     // every row sees every slot of the step
     const bool whole = j0 + Keys - 1 <= first_pos && (j0 > last_pos - window || j0 + Keys <= span.sinks) && __all(pages);
-    bool odd = false;  // a value that some row sees is not finite; it is left out of the product
     if (!whole) {
       asm volatile("");  // (a branch: most steps go past it)
       bool ok = true;
@@ -676,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
           sc[n][j / 4][j % 4] = is ? sc[n][j / 4][j % 4] : -INFINITY;
         }
       }
-      odd = !__all(ok);
+      odd |= !__all(ok);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -709,34 +734,6 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
       }
     }
     step.template sums<NT>(o, sc);
-    if (odd) {
-      for (int j = 0; j < Keys; ++j) {
-        const int at = j0 + j, page = (at >> c.lg) < c.maxPages ? table[at >> c.lg] : -1;
-        if ((uint32_t)page >= (uint32_t)c.nPages) continue;
-        const KV* from = row_at(vbase, page, at);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const bool is = (at <= pos[n]) & ((at > pos[n] - window) | (at < span.sinks));
-          float e = 0.f;
-#pragma unroll
-          for (int u = 0; u < Sub; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float y = __shfl(sc[n][u][r], i + 16 * ((j & 15) >> 2), 64);
-              if (j >> 4 == u && (j & 3) == r) e = y;
-              __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the common path)
-            }
-#pragma unroll
-          for (int m = 0; m < M; ++m)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float y = (float)from[(m / E) * 16 * E + (4 * g + r) * E + m % E];
-              o[n][m][r] += (is & !(fabsf(y) < INFINITY)) ? e * y : 0.f;
-              if (r == 3) __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-      }
-    }
     if (more) {
       const KV* r[Sub];
       value_rows(now, x + kWaves, r);
@@ -744,10 +741,59 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
     }
   }
 
-  // the waves' parts joined
+  bool number[NT], lost = false;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     sum[n] = over_groups_sum(sum[n]);
+    number[n] = (n * 16 + i < rows) & (sum[n] == sum[n]);
+    bool nan = odd;
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) nan |= o[n][m][r] != o[n][m][r];
+    lost |= number[n] & nan;
+  }
+  if (__builtin_expect(__any(lost), 0)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[n][m][r] = o[n][m][r] == o[n][m][r] ? o[n][m][r] : kLost;
+    for (x = begin + wave; x < end; x += kWaves) {
+      for (int j = 0; j < Keys; ++j) {
+        const int at = steps.at(x) * Keys + j, page = (at >> c.lg) < c.maxPages ? table[at >> c.lg] : -1;
+        if ((uint32_t)page >= (uint32_t)c.nPages) continue;
+        const KV* from = row_at(vbase, page, at);
+        if (!any_odd<KV, DH>(from)) continue;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const bool is = number[n] & (at <= pos[n]) & ((at > pos[n] - window) | (at < span.sinks));
+          if (!__any(is)) continue;
+          const int row = row0 + min(n * 16 + i, rows - 1), t = row / span.group, h = row - t * span.group;
+          const float e = weight_of_odd<KV, DH>(q + (((int64_t)s * span.T + t) * nH + kvh * span.group + h) * DH, factor, row_at(kbase, page, at));
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float y = (float)from[(m / E) * 16 * E + (4 * g + r) * E + m % E];
+              o[n][m][r] += (is & !(fabsf(y) < INFINITY)) ? e * y : 0.f;
+              if (r == 3) __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the common path)
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[n][m][r] = o[n][m][r] == kLost ? NAN : o[n][m][r];
+  }
+
+  // the waves' parts joined
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
     if (g == 0) wave_ml[wave][n * 16 + i] = make_float2(ref[n], sum[n]);
   }
   float* const vals = reinterpret_cast<float*>(shared);  // [kWaves][16][kRow]
@@ -757,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_ml[w][n * 16 + i].x);
-    const float f = ref[n] == top ? 1.f : __builtin_amdgcn_exp2f(ref[n] - top);
+    const float f = ref[n] == top ? 1.f : factor_of(ref[n] - top);
 #pragma unroll
     for (int r = 0; r < Runs; ++r)
 #pragma unroll
@@ -860,10 +906,8 @@ struct Wide<_Float16, DH> {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = p[8 * z + j];
         two_pieces(x, hi[z], lo[z]);
-        asm("" : "+v"(lo[z]));  // (what the rare path takes from here are these, not more registers)
       }
     }
-    __device__ __forceinline__ float at(int z) const { return (float)hi[z / 8][z % 8] + (float)lo[z / 8][z % 8]; }
     // o += the word's slots
     __device__ __forceinline__ void sum(f32x16& o, int z, u32x4 word) const {
       const f16x8 a = __builtin_bit_cast(f16x8, word);
@@ -881,9 +925,6 @@ struct Wide<_Float16, DH> {
   }
   // Row j's run with zeros for what is not finite; whether all of it was.
   __device__ __forceinline__ bool tame(int j) { return tame_halves<E / 2>(v[j]); }
-  // where slot j's value stands in its group's word
-  static __device__ __forceinline__ int group_of(int j) { return 2 * (j >> 4) + (j >> 2 & 1); }
-  static __device__ __forceinline__ int place_of(int j) { return (j >> 3 & 1) * 4 + (j & 3); }
 };
 template <int DH>
 struct Wide<float, DH> {
@@ -914,7 +955,6 @@ struct Wide<float, DH> {
   struct Probs {
     f32x16 p;
     __device__ __forceinline__ void take(const f32x16& x) { p = x; }
-    __device__ __forceinline__ float at(int z) const { return p[z]; }
     __device__ __forceinline__ void sum(f32x16& o, int z, u32x4 word) const {
       const f32x4 a = __builtin_bit_cast(f32x4, word);
 #pragma unroll
@@ -927,8 +967,6 @@ struct Wide<float, DH> {
     return __builtin_bit_cast(u32x4, w);
   }
   __device__ __forceinline__ bool tame(int j) { return tame_floats<E>(v[j]); }
-  static __device__ __forceinline__ int group_of(int j) { return j >> 2; }
-  static __device__ __forceinline__ int place_of(int j) { return j & 3; }
 };
 
 // 16 bytes a lane from `from` + `offset` to LDS at `lds` + 16 lane; waited for by hand (the compiler does not count
@@ -956,11 +994,10 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   // slot j's swizzle: the words of 16 neighbouring slots in 16 different places of 256 bytes
   constexpr int kShift = Words % 16 == 0 ? 0 : Words % 8 == 0 ? 1 : 2, kMask = Words % 16 == 0 ? 15 : Words % 8 == 0 ? 7 : 3;
   __shared__ __attribute__((aligned(16))) u32x4 lds[4 * kTile];  // [2][K, V][kTile]
-  // Of a step's quads of slots: their pages, -1 for none, and whether all have one; of its V: whether
-  // what a wave has turned around held infinities or NaN.  Pages are read up to the end of their step, and
-  // those of the next but one are written in it.
+  // Of a step's quads of slots: their pages, -1 for none, and whether all have one.  Pages are read up to the
+  // end of their step, and those of the next but one are written in it.
   __shared__ int pages[3][Keys / 4], all_pages[3];
-  __shared__ __attribute__((aligned(4))) uint8_t odd[2][kWaves];
+  __shared__ int odd_values;  // values that some row sees were not finite and left out of a product
   const uint32_t lds_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
   const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1072,14 +1109,11 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     return j0 + Keys - 1 <= first_pos && (j0 > last_pos - window || j0 + Keys <= span.sinks) && all_pages[pb] != 0;
   };
   auto put_v = [&](int x, int b, int pb) {
-    if (!W::turns(wave)) {
-      if (lane == 0) odd[b][wave] = 0;
-      return;
-    }
-    bool ok = true;
+    if (!W::turns(wave)) return;
     if (!is_whole(x, pb)) {
       // Not every row sees all of it: what is not finite would reach, times a p of zero, rows that do not.  It becomes
       // zeros and, if any row sees it, is told of.
+      bool ok = true;
       const int j0 = steps.at(x) * Keys;
 #pragma unroll
       for (int u = 0; u < W::Quads; ++u) {
@@ -1091,14 +1125,14 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
           ok &= w.tame(4 * u + r) | !seen;
         }
       }
+      if (!ok) odd_values = 1;
     }
-    const bool all = __all(ok);
-    if (lane == 0) odd[b][wave] = !all;
     u32x4* to = lds + (2 * b + 1) * kTile + group * Lanes + run;
 #pragma unroll
     for (int e = 0; e < E; ++e) to[e * 8 * Lanes] = w.turned(e);
   };
 
+  if (threadIdx.x == 0) odd_values = 0;
   if (begin < end) {
     put_pages(threadIdx.x < Keys / 4 ? page_at(begin) : -1, 0);
     __syncthreads();
@@ -1139,7 +1173,6 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
     const bool some = mine > 0 && j0 <= wave_last && (j0 + Keys - 1 > wave_first - window || j0 < span.sinks);
     if (some) {
       const u32x4 *kt = lds + 2 * b * kTile, *vt = kt + kTile;
-      const bool odd_step = *reinterpret_cast<const uint32_t*>(odd[b]) != 0;
       // 32 slots at a time: their scores and p are all that a wave holds.  Words of K are read while the slots before
       // them are summed, the first words of V while p is formed (read when they are wanted, the waits took a third
       // of the time; all of them ahead would not fit the registers).
@@ -1225,30 +1258,6 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
           pr.sum(o[i % M], i / M, vs[i % M]);
           if (i + M < M * Z) vs[i % M] = value_word(u, i + M);
         }
-        if (odd_step) {
-          // infinities and NaN, zeros so far, for the rows that see them
-          for (int j = 32 * u; j < 32 * u + 32; ++j) {
-            const int at = j0 + j, page = pages[this_page][j / 4];
-            const bool is = (page >= 0) & (at <= pos) & ((at > pos - window) | (at < span.sinks));
-            const KV* const from = row_at(vbase, page, at);
-            float e = 0.f;
-#pragma unroll
-            for (int z = 0; z < 16; ++z) {
-              const float y = __shfl(pr.at(z), r32 + 32 * (j >> 2 & 1), 64);
-              if ((j >> 3 & 3) == z / 4 && (j & 3) == z % 4) e = y;
-              __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the common path)
-            }
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-#pragma unroll
-              for (int z = 0; z < 16; ++z) {
-                const int r = 8 * (z / 4) + 4 * h + z % 4;
-                const float y = (float)from[Lanes == 32 ? r * E + m : (r & 15) * E + 2 * m + (r >> 4)];
-                o[m][z] += (is & !(fabsf(y) < INFINITY)) ? e * y : 0.f;
-                if (z % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-              }
-          }
-        }
       }
     }
     if (x + 1 < end) {
@@ -1262,19 +1271,57 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_wide_kern
   int me = threadIdx.x;
   asm volatile("" : "+v"(me));
   const int my_row = me & 31, my_h = me >> 5 & 1, at_row = row0 + 32 * wave + my_row;
-  if (my_row >= mine) return;
   sum += __shfl_xor(sum, 32, 64);
+  auto column = [&](int m, int z) {  // of o[m][z]
+    const int r = 8 * (z / 4) + 4 * my_h + z % 4;
+    return Lanes == 32 ? r * E + m : (r & 15) * E + 2 * m + (r >> 4);
+  };
+  const bool number = (my_row < mine) & (sum == sum);
+  bool lost = begin < end && odd_values != 0;  // (last written before the last step's barrier)
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int z = 0; z < 16; ++z) lost |= o[m][z] != o[m][z];
+  if (__builtin_expect(__any(number & lost), 0)) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int z = 0; z < 16; ++z) o[m][z] = o[m][z] == o[m][z] ? o[m][z] : kLost;
+    const int r = row0 + 32 * wave + min(my_row, mine - 1), t = r / span.group, at_pos = used + t;
+    const float* const q_row = q + (((int64_t)s * span.T + t) * nH + kvh * span.group + (r - t * span.group)) * DH;
+    for (int x = begin; x < end; ++x)
+      for (int j = 0; j < Keys; ++j) {
+        const int at = steps.at(x) * Keys + j, page = (at >> c.lg) < c.maxPages ? table[at >> c.lg] : -1;
+        if ((uint32_t)page >= (uint32_t)c.nPages) continue;
+        const KV* from = row_at(vbase, page, at);
+        if (!any_odd<KV, DH>(from)) continue;
+        const bool is = number & (at <= at_pos) & ((at > at_pos - window) | (at < span.sinks));
+        if (!__any(is)) continue;
+        const float e = weight_of_odd<KV, DH>(q_row, factor, row_at(kbase, page, at));
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int z = 0; z < 16; ++z) {
+            const float y = (float)from[column(m, z)];
+            o[m][z] += (is & !(fabsf(y) < INFINITY)) ? e * y : 0.f;
+            if (z % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (many at once would take registers from the common path)
+          }
+      }
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int z = 0; z < 16; ++z) o[m][z] = o[m][z] == kLost ? NAN : o[m][z];
+  }
+  if (my_row >= mine) return;
   const int64_t part = (int64_t)part_id * kWideRows + 32 * wave + my_row;
   const int my_t = at_row / span.group, my_head = kvh * span.group + (at_row - my_t * span.group);
   const float f = pieces > 1 ? 1.f : one_by(sum, c, span, s, my_t);
   float* const to = pieces > 1 ? part_o + part * DH : out + (((int64_t)s * span.T + my_t) * nH + my_head) * DH;
   if (pieces > 1 && my_h == 0) part_ml[part] = make_float2(ref, sum);
 #pragma unroll
-  for (int z = 0; z < 16; ++z) {
-    const int r = 8 * (z / 4) + 4 * my_h + z % 4;
+  for (int z = 0; z < 16; ++z)
 #pragma unroll
-    for (int m = 0; m < M; ++m) to[Lanes == 32 ? r * E + m : (r & 15) * E + 2 * m + (r >> 4)] = o[m][z] * f;
-  }
+    for (int m = 0; m < M; ++m) to[column(m, z)] = o[m][z] * f;
 }
 
 // A workgroup joins the pieces of R rows of a kv head, R <= kThreads / (DH / 4): its threads share out quads of a
@@ -1301,7 +1348,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(Cache c, float* __
   auto add = [&](float2 ml, f32x4 v) {
     const float was = top;
     top = fmaxf(top, ml.x);
-    const float keep = was == top ? 1.f : __builtin_amdgcn_exp2f(was - top), f = ml.x == top ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+    const float keep = was == top ? 1.f : factor_of(was - top), f = ml.x == top ? 1.f : factor_of(ml.x - top);
     all = all * keep + ml.y * f;
     y = y * keep + v * f;
   };

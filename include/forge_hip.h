@@ -821,7 +821,9 @@ int fg_paged_read(const fg_paged_cache* c, int layer, float* k, float* v, int64_
  * q and out [nSeq T][nHeads][dHead], query head h on kv head h / (nHeads / nKvHeads);
  * out apart from q; zeros where no slot is seen.  What is not seen, whatever its value, has no
  * part in it.  Sums are fp32; with an F32 cache products are fp32, with F16 q and p are
- * held in two fp16 pieces (22 bits), and an infinite key that a row sees may make it NaN. */
+ * held in two fp16 pieces (22 bits), and an infinite key that a row sees may make it NaN.
+ * A score of -inf is p = 0; infinite values make infinities and NaN where the formula has
+ * them, however small their p.  Finite values above 2^100 may overflow the sums. */
 int fg_paged_attn(const fg_paged_cache* c, int layer, float* out, const float* q, int nHeads, double scale, int T,
                   const int32_t* count, int window, int sinks);
 /* Ends a step: len[s] += T (or count[s]; to maxPages pageSize at most). */

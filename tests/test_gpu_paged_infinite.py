@@ -102,3 +102,70 @@ def test_nothing_but_infinite_keys(fh, group, T):
     check(fh, c, q, k, v, 0.125)
     check(fh, c, q, k, v, 0.125, window=5)
     assert check(fh, c, q, k, v, 0.125, window=5, sinks=3) > 0
+
+
+def odd_values(c, v, s, slots):
+    """Infinities of either sign and NaN at slots a < b < e of a sequence, in a column alone and two of them in one."""
+    (pa, ia), (pb, ib), (pe, ie) = (c.at(s, j) for j in slots)
+    v[0, pa, :, ia, :4] = [np.inf, -np.inf, np.inf, np.inf]
+    v[0, pb, :, ib, 4:6] = [-np.inf, np.nan]
+    v[0, pb, :, ib, c.dH - 1] = np.inf
+    v[0, pe, :, ie, 2:4] = [-np.inf, np.inf]
+    v[0, pe, :, ie, 6:9] = [np.inf, -np.inf, np.nan]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("spread", [1.0, 80.0])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 4)])
+@pytest.mark.parametrize("dH,nKV,group,T,upto", SHAPES)
+def test_infinite_values(fh, kind, dH, nKV, group, T, upto, window, sinks, spread):
+    """An infinite value makes its column infinite, one of either sign NaN, in steps that all rows see and in others, and where
+    its probability is below what fp32 holds (scores 80 apart on the average; 2^-800 in fp64)."""
+    rng = np.random.default_rng(dH + T + upto)
+    n = upto + T
+    c = Cache(fh, rng, 1, 2, nKV, dH, 16, -(-n // 16), kind, [upto, upto // 2])
+    k, v = c.fill(rng, 0, [n, upto // 2 + T])
+    odd_values(c, v, 0, (min(3, n - 3), max(n // 2, min(3, n - 3) + 1), n - 1))
+    m = upto // 2 + T
+    if m > 4:
+        odd_values(c, v, 1, (1, 2, m - 1 - T // 2))
+    # (values of K are of e^-1 .. e^1: 1.8 in their squares' mean)
+    scale = spread / math.sqrt(1.8 * dH)
+    assert check(fh, c, queries(rng, 2, T, nKV * group, dH), k, v, scale, window, sinks) > 0
+
+
+@pytest.mark.parametrize("dH,nKV,group,T,upto", SHAPES)
+def test_infinite_values_of_no_weight(fh, dH, nKV, group, T, upto):
+    """A probability of exactly zero (a score of -inf) times an infinite value is NaN, beside slots where it is not."""
+    rng = np.random.default_rng(dH + T + upto)
+    n = upto + T
+    c = Cache(fh, rng, 1, 1, nKV, dH, 16, -(-n // 16), "f32", [upto])
+    k, v = c.fill(rng, 0, [n])
+    for j, column in ((1, 3), (n - 1, 4), (n // 2, 5)):
+        p, i = c.at(0, j)
+        k[0, p, :, i, 0] = -np.inf
+        v[0, p, :, i, column] = np.inf
+    p, i = c.at(0, 2)
+    v[0, p, :, i, 2:5] = np.inf
+    assert check(fh, c, queries(rng, 1, T, nKV * group, dH), k, v, dH ** -0.5) > 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("group,T", [(1, 1), (2, 60)])
+def test_large_values_and_unseen_infinities(fh, kind, group, T):
+    """Values at the end of what the sums take (2^100; fp16: 65504), beside an infinite one in another column; infinities
+    in slots behind the last token, which nothing sees."""
+    rng = np.random.default_rng(T)
+    c = Cache(fh, rng, 1, 2, 1, 64, 16, 10, kind, [70, 90])
+    k, v = c.fill(rng, 0, [70 + T, 90 + T])
+    for j in range(30):
+        p, i = c.at(0, j)
+        v[0, p, 0, i, 9] = (2.0 ** 100 if kind == "f32" else 65504) * (-1) ** j
+    for s, j in ((0, 70 + T), (1, 90 + T), (1, 91 + T)):
+        p, i = c.at(s, j)
+        v[0, p, 0, i] = np.inf
+        k[0, p, 0, i] = np.nan
+    assert check(fh, c, queries(rng, 2, T, group, 64), k, v, 0.125) == 0
+    p, i = c.at(0, 40)
+    v[0, p, 0, i, 8] = np.inf
+    assert check(fh, c, queries(rng, 2, T, group, 64), k, v, 0.125) > 0
