@@ -87,6 +87,9 @@ function matWeights(w, N, K, what) {
 const DEVICE_TYPES = new Set([0, 1, 2, 6, 8, 12, 13, 14]);
 
 const GRAPHS_KEPT = 4;
+// Vectors of a paged cache's steps are kept from one to the next up to this many bytes; what a long chunk took beyond it
+// (8192 rows of 32000 logits: 1 GB) goes back when the chunk is done.
+const VECTORS_KEPT = 64 << 20;
 
 /**
  * Inference model (transformer.js:69-184) on the device: `loadWeights(w)`
@@ -291,6 +294,7 @@ export class Transformer {
     const e = this._chunk(tokens, cache, opts), T = Math.max.apply(null, Array.from(tokens, (t) => t.length));
     const out = new Float32Array(cache.sequences * T * this.cfg.vocabSize);
     hip().d2h(e.logits, out);
+    if (e.rows * (2 * this.cfg.dim + this.cfg.hidden + this.cfg.vocabSize) * 4 > VECTORS_KEPT) this._dropPaged(cache);
     return out;
   }
 
