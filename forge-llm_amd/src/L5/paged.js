@@ -76,7 +76,7 @@ export class PagedKVCache {
   /** Gives every sequence the pages of `counts` more tokens (a number, or one each); throws, and changes nothing, where there are none left. */
   reserve(counts) {
     this.handle;
-    if (!(counts && counts.length !== undefined)) counts = new Int32Array(this.sequences).fill(whole(counts, "tokens", 0));
+    counts = counts && counts.length !== undefined ? this._counts(counts, 0x7FFFFFFF) : new Int32Array(this.sequences).fill(whole(counts, "tokens", 0));
     const want = [];
     counts.forEach((n, s) => {
       const end = this.lens[s] + n;
