@@ -29,12 +29,16 @@ export function verifyDrafts(logits, drafts, u, { vocab, draftLogits = null, dra
   if (temperature > 0) need(u, S * (D + 1), "random numbers");
   if (draftLogits) need(draftLogits, S * D * V, "logits of the drafts");
   if (drafted) need(drafted, S, "numbers of drafts");
+  // (an Int32Array would take 2^32 + 1 as 1)
+  const whole = (x, what) => { for (const v of x) if (v !== (v | 0)) throw new RangeError(`verifyDrafts: ${what} ${v}`); };
+  for (const d of drafts) whole(d, "draft");
+  if (drafted) whole(Array.prototype.slice.call(drafted, 0, S), "number of drafts");
   const a = hip(), held = [];
   const up = (x) => { const h = a.alloc(Math.max(4, x.byteLength)); held.push(h); if (x.length) a.h2d(h, x); return h; };
   const f32 = (x, n) => (x instanceof Float32Array ? x.subarray(0, n) : Float32Array.from(Array.prototype.slice.call(x, 0, n)));
   try {
     const x = up(f32(logits, S * (D + 1) * V)), y = draftLogits && D ? up(f32(draftLogits, S * D * V)) : null;
-    const d = up(Int32Array.from([].concat(...drafts.map((r) => Array.from(r))))), n = drafted ? up(Int32Array.from(drafted)) : null;
+    const d = up(Int32Array.from([].concat(...drafts.map((r) => Array.from(r))))), n = drafted ? up(Int32Array.from(Array.prototype.slice.call(drafted, 0, S))) : null;
     const r = temperature > 0 ? up(f32(u, S * (D + 1))) : null;
     const token = new Int32Array(S * (D + 1)), count = new Int32Array(S), bt = up(token), bc = up(count);
     a.draftVerify(bt, bc, x, V, y, V, d, n, r, temperature, S, D, V);

@@ -18,5 +18,11 @@ rec("reserve: a number for every sequence, whole and not below zero", () => {
   return ok;
 });
 
+rec("verifyDrafts: drafts and their numbers are whole and fit 32 bits", () => {
+  const p = [0.5, 0.25, 0.25, 0.1, 0.1, 0.8].map(Math.log), go = (d, n) => verifyDrafts(p, [[d]], [0, 0.5], { vocab: 3, drafted: n });
+  return refused([2 ** 32 + 1, 0.5, NaN, "1", undefined].map((d) => () => go(d, null)).concat([[2 ** 32], [0.5], [NaN]].map((n) => () => go(0, n)))) &&
+    go(0, [1]).counts[0] === 2 && go(-1, null).counts[0] === 1 && go(2 ** 31 - 1, null).counts[0] === 1 && go(0, Int32Array.of(-1, 7)).counts[0] === 0;
+});
+
 for (const o of out) console.log(JSON.stringify(o));
 process.exit(out.every((o) => o.ok) ? 0 : 1);
