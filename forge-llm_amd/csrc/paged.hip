@@ -181,7 +181,7 @@ __global__ void paged_commit_kernel(Cache c, int T, const int32_t* __restrict__ 
 // Bound by reading the cache: each value of K and V is read once a workgroup's rows, the products
 // of 32 rows take a third of the time that 16 KB of a wave's slots take to come.  A step's loads
 // are issued as soon as the registers of the one before are free.  One token after 130001 (32 query
-// heads on 8 of 128, fp16) 97 us, 5.5 TB/s; five of 16 sequences up to 8192 45 us (5.2 TB/s); of
+// heads on 8 of 128, fp16) 97 us, 5.5 TB/s; five of 16 sequences up to 8192 46 us (5.2 TB/s); of
 // what is left the joining launch is 5 to 6.
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -534,7 +534,8 @@ __device__ __forceinline__ float one_by(float sum, const Cache& c, const Span& q
 // is NaN or of the other sign, a p that underflows gives inf 0, and what is seen by some rows alone is
 // left out.  Where that has been so (a step said it, or a sum is NaN though the p are numbers) a wave goes
 // over its values once more, for the rows whose p are numbers, and adds them to their sums as they are: inf p = inf for any
-// p > 0.  NaN sums are set to kLost, which swallows no infinity, and are NaN again if none came.
+// p > 0.  NaN sums are set to kLost, which swallows no infinity, and are NaN again if none came.  512 tokens after 8192
+// (as below) take 1.1 ms with an infinite row of V in every 16 slots, 5.1 with nothing but them, 0.16 without.
 constexpr float kLost = FLT_MAX;
 // Factors that bring sums to another reference: not zero, which would make NaN of an infinite sum.
 __device__ __forceinline__ float factor_of(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), FLT_MIN); }
@@ -545,9 +546,10 @@ __device__ __forceinline__ bool any_odd(const KV* from) {  // of a slot's values
   for (int d = threadIdx.x & 63; d < DH; d += 64) odd |= !(fabsf((float)from[d]) < INFINITY);
   return __any(odd);
 }
-// What to multiply a value that is not finite with: 1, or NaN for a p of exactly zero (a score of -inf).
+// What to multiply a value that is not finite with: 1, or NaN for a p of exactly zero (a score of -inf, of an infinite key).
 template <class KV, int DH>
 __device__ __forceinline__ float weight_of_odd(const float* q, float factor, const KV* key) {
+  if (!any_odd<KV, DH>(key)) return 1.f;
   float x = 0.f;
 #pragma unroll 8
   for (int d = 0; d < DH; ++d) x = fmaf(q[d] * factor, (float)key[d], x);
@@ -852,10 +854,11 @@ __global__ void __launch_bounds__(kThreads, (DH == 256 ? 1 : 2)) paged_attn_kern
 //   V  the values of d at eight slots (fp32: four) that a lane's operand takes, [e][8 groups of slots][i] for d = E i + e:
 //      turned around on the way, four rows of a run of E values a lane
 //
-// Bound by the matrix pipes: 512 tokens after 8192 (32 query heads on 8 of 128, fp16) 150 us for 142 GFLOP of fp16 products
-// (two pieces each), 0.95 PFLOP/s where a large library product of fp16 matrices reaches 1.15.  Two workgroups of a
+// Bound by the matrix pipes: 512 tokens after 8192 (32 query heads on 8 of 128, fp16) 154 to 162 us back to back, the joining
+// launch (8) among them, for 142 GFLOP of fp16 products (two pieces each): 0.9 PFLOP/s where a large library product of fp16
+// matrices reaches 1.15.  (160 to 172 a launch under the tracer, where the clock settles lower.)  Two workgroups of a
 // CU take turns at scores and exponentials (46% of the cycles have a matrix instruction running, 40% a vector
-// one); registers (255) leave no room to interleave the two in one wave.  Every spill cost a wait for all loads: 12 of them 40 us.
+// one); registers (244) leave no room to interleave the two in one wave.  Every spill cost a wait for all loads: 12 of them 40 us.
 template <class KV, int DH>
 struct Wide;
 template <int DH>
