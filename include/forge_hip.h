@@ -788,7 +788,9 @@ int fg_kv4_reorder(const fg_kv4_cache* c, const int32_t* parent, int W);
  * drafted tokens did not stand): until then len stands.  `count` (device, [nSeq], or
  * NULL) gives each sequence its own number of new tokens, held to 0..T; rows of new
  * tokens are s T + t, and rows t >= count[s] are neither read nor written.  The
- * structure itself is host memory, read during the call. */
+ * structure itself is host memory, read during the call.
+ * A call takes up to 2^23 - 1 rows (nSeq T), attention up to 2^23 - 9 of a query
+ * head (nSeq T nHeads); longer ones are refused. */
 typedef struct fg_paged_cache {
   int nLayers, nSeq, nKvHeads, dHead, pageSize, nPages, maxPages, type;
   void* k;
@@ -862,8 +864,10 @@ int fg_decode_step_paged(const fg_decode_model* m, const fg_paged_cache* c, cons
  * numbers (a NaN, an infinite logit, all -inf), its draft does not stand, and what is
  * drawn from it is -1.  drafted (device, [nSeq], or NULL: D) is each sequence's number of
  * drafts, D at most; one below 0 takes no part: tokens -1, count 0.  A draft outside
- * [0, V) does not stand.  Probabilities and sums are fp64.  u in [0, 1);
- * D <= 1023, V <= 2^26, nSeq (D + 1) <= 65535 x 16; outputs apart from the inputs. */
+ * [0, V) does not stand.  Probabilities and sums are fp64, the sums of exponentials good to
+ * 2.2e-10 of themselves; a number that lies as near to a border may fall on its other side.  u in [0, 1);
+ * D <= 1023, V <= 2^26, nSeq (D + 1) <= 65535 x 16, and rows of both models (nSeq (2 D + 1)) x
+ * ceil(V / 4096) < 2^23; outputs apart from the inputs. */
 int fg_draft_verify(int32_t* token, int32_t* count, const float* logits, int64_t ld, const float* draft_logits,
                     int64_t ld_draft, const int32_t* draft, const int32_t* drafted, const float* u, double temperature,
                     int nSeq, int D, int V);
